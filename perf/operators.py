@@ -486,7 +486,7 @@ def run(state):
         p, f = A.make_scored_params(
             q=s["q"], k=s["k"], v=s["v"], k_cache=s["k_cache"], v_cache=s["v_cache"], out=s["out"], scratch=s["scratch"], act_scale=s["act"],
             q_w_scale=s["qw"], k_w_scale=s["kw"], v_w_scale=s["vw"], freq_cis=s["table"], softcap=c["softcap"], alibi_slopes=s["slopes"],
-            key_begin=s["begin"], **more)
+            key_begin=s["begin"], scratch_zeroed=c["op"] == "decode", **more)
         A.forward_scored(p, f)
         return s["out"], s["k_cache"], s["v_cache"]
     cache = kv8.Cache(s["k_codes"], s["v_codes"], s["k_scale"], s["v_scale"], row_pos=s["row_pos"])
@@ -497,7 +497,7 @@ def run(state):
     if c["op"] == "decode8":
         kv8.decode(cache, s["q"], s["k"], s["v"], s["out"], past_lens=s["past"], max_past_len=c["most"], act_scale=s["act"], q_w_scale=s["qw"],
                    k_w_scale=s["kw"], v_w_scale=s["vw"], freq_cis=s["table"], softcap=c["softcap"], alibi_slopes=s["slopes"], key_begin=s["begin"],
-                   weight_in=s.get("w_in"), weight_out=s.get("w_out"), scratch=s["scratch"])
+                   weight_in=s.get("w_in"), weight_out=s.get("w_out"), scratch=s["scratch"], scratch_zeroed=True)
         r = [s["out"], s["k_codes"], s["k_scale"], s["v_codes"], s["v_scale"]]
         return r + [s["w_out"]] if c["weights"] else r
     kv8.evict(cache, past_lens=s["past"], len_out=s["len_out"], budget=c["budget"], recent=c["recent"], sinks=c["sinks"], next_pos=s["next"],
