@@ -314,9 +314,9 @@ def _round(y, code):
     return y.round().clamp(-127, 127).to(torch.int8) if code == "int8" else y.clamp(-448, 448).to(torch.float8_e4m3fn)
 
 
-def _merge(codes, scale, x, new, fresh, code):
-    """Rows x where `new` into blocks: codes, x [B,h,n,block,d], scale, fresh [B,h,n], new [B,h,n,block]. The scale of a block grows to
-    hold its new rows, and the codes it held are brought to the new scale."""
+def _merge(codes, scale, x, new, live, fresh, code):
+    """Rows x where `new` into blocks: codes, x [B,h,n,block,d], scale, fresh [B,h,n], new, live [B,h,n,block]. The scale of a block
+    grows to hold its new rows, and the codes of the live rows it held are brought to the new scale."""
     amax = torch.where(new[..., None], x, torch.zeros_like(x)).abs().amax((-1, -2))
     need = amax / torch.full_like(amax, _top(code))
     old = torch.where(fresh, torch.zeros_like(scale), scale)
@@ -324,7 +324,7 @@ def _merge(codes, scale, x, new, fresh, code):
     touched = new.any(-1)
     grown = touched & (s > old) & ~fresh
     ratio = torch.where(grown, old / s, torch.ones_like(s))[..., None, None]
-    held = torch.where(grown[..., None, None], _round(codes.float() * ratio, code).float(), codes.float())
+    held = torch.where(grown[..., None, None] & live[..., None], _round(codes.float() * ratio, code).float(), codes.float())
     put = torch.where(new[..., None], _encode(x, s[..., None, None], code).float(), held)
     return put.to(codes.dtype), torch.where(touched, s, scale)
 
@@ -344,7 +344,8 @@ def _append_one(codes, scale, x, past, count, block, code):
     window = torch.gather(codes.view(torch.int8), 2, at).view(codes.dtype)
     shape = (B, h, W // block, block)
     fresh = sat * block >= past.long()[:, None, None]
-    c, s = _merge(window.view(*shape, d), torch.gather(scale, 2, sat), x.view(*shape, d), new.reshape(shape), fresh, code)
+    c, s = _merge(window.view(*shape, d), torch.gather(scale, 2, sat), x.view(*shape, d), new.reshape(shape),
+                  (j < 0)[:, None].expand(B, h, W).reshape(shape), fresh, code)
     codes.view(torch.int8).scatter_(2, at, c.view(B, h, W, d).view(torch.int8))
     scale.scatter_(2, sat, s)
     return rows, new
@@ -458,7 +459,7 @@ def _plain_evict(s):
     for which in ("k", "v"):
         codes, scale = s[which + "_codes"], s[which + "_scale"]
         x = torch.gather(_decoded(codes, scale, block), 2, at)
-        a, b = _merge(codes.view(*shape, d), scale, x.view(*shape, d), hole.view(shape), no, c["code"])
+        a, b = _merge(codes.view(*shape, d), scale, x.view(*shape, d), hole.view(shape), (row < m).view(shape), no, c["code"])
         codes.copy_(a.view(B, Hkv, T, d))
         scale.copy_(b)
     s["w_out"].copy_(torch.where(row < m, torch.gather(w, 2, source), s["w_out"]))
