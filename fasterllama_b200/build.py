@@ -15,11 +15,12 @@ LIB_PATH = os.path.join(PKG_DIR, "libflb_attn.so")
 ORACLE_DIR = os.path.join(ROOT, "oracle")
 ORACLE_LIB = os.path.join(ORACLE_DIR, "libflb_oracle.so")
 
-CUDA_SOURCES = ["decode_attn.cu", "prefill_attn.cu", "launch.cu", "static_scratch.cu", "peer_exchange.cu"]
+CUDA_SOURCES = ["decode_attn.cu", "prefill_attn.cu", "launch.cu", "static_scratch.cu", "peer_exchange.cu",
+                "kv8_append.cu", "kv8_decode.cu", "kv8_evict.cu", "kv8_launch.cu"]
 NVCC_FLAGS = [
     "-std=c++17", "-O3", "-lineinfo",
     "-gencode", "arch=compute_100a,code=sm_100a",
-    "-Xcompiler", "-fPIC", "-shared", "-cudart", "shared",
+    "-Xcompiler", "-fPIC", "-shared", "-cudart", "shared", "-t", "0",
 ]
 
 
@@ -40,7 +41,7 @@ def _newer(target: str, sources: list[str]) -> bool:
 def build_cuda(force: bool = False, verbose: bool = False) -> str:
     srcs = [os.path.join(CSRC, s) for s in CUDA_SOURCES]
     deps = srcs + [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cuh", ".h"))]
-    deps.append(os.path.join(ROOT, "include", "flb_attn.h"))
+    deps += [os.path.join(ROOT, "include", f) for f in ("flb_attn.h", "flb_kv8.h")]
     if not force and _newer(LIB_PATH, deps):
         return LIB_PATH
     cmd = [_nvcc(), *NVCC_FLAGS, *(["-Xptxas", "-v"] if verbose else []), "-o", LIB_PATH, *srcs]

@@ -1,0 +1,213 @@
+// kv8.cuh — what the kernels of the 8-bit K/V cache share: the argument blocks, input loads, the RoPE rotation and the
+// coding rule (include/flb_kv8.h).
+#pragma once
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace flb {
+
+enum : unsigned { kKv8BadLen = 4u, kKv8BadPos = 32u };
+
+struct Kv8Cache {
+    int B, H, T;        // H: K/V heads
+    int block_shift;    // log2(block_len)
+    int nblk;           // blocks per slab
+    uint8_t *codes[2];  // K, V
+    float *scale[2];
+    int *row_pos;
+};
+
+struct Kv8Input { // q, k or v rows as the projections leave them
+    const void *p;
+    const float *w_scale;
+    int row_stride;
+};
+
+struct Kv8AppendArgs {
+    Kv8Cache c;
+    int S, nwin; // tokens; blocks that a sequence's tokens can touch
+    int start_pos;
+    const int *past_lens, *new_lens, *token_pos;
+    Kv8Input in[2]; // k, v
+    const float *act_scale;
+    const float *freq_cis;
+    int freq_rows;
+    unsigned *status;
+};
+
+struct Kv8DecodeArgs {
+    Kv8Cache c;
+    int input_mode;
+    int Hq, G, nchunk; // q heads, q heads per K/V head, CTAs that share a K/V head's q heads out among themselves
+    int start_pos;
+    const int *past_lens, *token_pos;
+    Kv8Input in[3]; // q, k, v
+    const float *act_scale;
+    const float *freq_cis;
+    int freq_rows;
+    float scale_log2e, cap_log2e; // softmax_scale, softcap in units of log2
+    const float *slopes;
+    const int *key_begin;
+    float *scores; // [B,Hq,T] log2-domain scores, when weights are accumulated
+    float *ml;     // [B,Hq,2] final maximum and sum, likewise
+    const float *weight_in;
+    float *weight_out;
+    void *out;
+    int out_f16;
+    int append; // the attention kernel stores the new token itself (one CTA per K/V head and split)
+    int nsplit_max, split_len;
+    unsigned *status, *counters;
+    float *part_o, *part_ml;
+};
+
+struct Kv8EvictArgs {
+    Kv8Cache c;
+    int start_pos;
+    const int *past_lens;
+    int *len_out;
+    int budget, recent, sinks;
+    const int *next_pos;
+    const float *weight;
+    float *weight_out;
+    int *pos_out;
+    unsigned *status;
+    int *moves;    // [B*H][T / 2] sources: the i-th kept row at or behind m
+    int *holes;    // [B*H][T / 2] holes below m, rising
+    float *edge_scale; // [B*H][2] scales of the block that row m lies in, as they were
+    int *hole_off; // [B*H][nblk + 1] holes in front of each block
+};
+
+cudaError_t launch_kv8_append(const Kv8AppendArgs &a, int d, int code, int input_mode, cudaStream_t stream);
+cudaError_t launch_kv8_decode(const Kv8DecodeArgs &a, int d, int code, int nt, cudaStream_t stream);
+cudaError_t launch_kv8_evict(const Kv8EvictArgs &a, int d, int code, cudaStream_t stream);
+
+// ---- inputs --------------------------------------------------------------------------------------
+// Eight consecutive values of a row.  MODE 0: float(acc) * act_scale * w_scale, in this order; 1: fp32; 2: fp16.
+template <int MODE> __device__ __forceinline__ void kv8_load8(const Kv8Input &in, const float *act_scale, size_t token, int col, float (&x)[8]) {
+    const size_t off = token * in.row_stride + col;
+    if (MODE == 2) {
+        const uint4 u = __ldg(reinterpret_cast<const uint4 *>((const __half *)in.p + off));
+        const __half2 *h = reinterpret_cast<const __half2 *>(&u);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = __half22float2(h[i]);
+            x[2 * i] = f.x;
+            x[2 * i + 1] = f.y;
+        }
+    } else {
+        const uint4 *p = reinterpret_cast<const uint4 *>((const uint32_t *)in.p + off);
+        const uint4 a = __ldg(p), b = __ldg(p + 1);
+        const uint32_t r[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        if (MODE == 1) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(r[i]);
+        } else {
+            const float as = __ldg(act_scale + token);
+            const float4 *w = reinterpret_cast<const float4 *>(in.w_scale + col);
+            const float4 w0 = __ldg(w), w1 = __ldg(w + 1);
+            const float ws[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(__fmul_rn((float)(int)r[i], as), ws[i]);
+        }
+    }
+}
+
+// Rotation of the pairs (2i, 2i+1) of eight values by a table row (its entries at the same columns).  Every product is
+// rounded before the sum, so that the stored codes do not depend on where a compiler fuses.
+__device__ __forceinline__ void kv8_rotate8(const float *row, float (&x)[8]) {
+    const float4 f0 = __ldg(reinterpret_cast<const float4 *>(row)), f1 = __ldg(reinterpret_cast<const float4 *>(row) + 1);
+    const float cs[8] = {f0.x, f0.y, f0.z, f0.w, f1.x, f1.y, f1.z, f1.w};
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        const float a = x[i], b = x[i + 1];
+        x[i] = __fsub_rn(__fmul_rn(a, cs[i]), __fmul_rn(b, cs[i + 1]));
+        x[i + 1] = __fadd_rn(__fmul_rn(b, cs[i]), __fmul_rn(a, cs[i + 1]));
+    }
+}
+
+// table row of a position; one outside the table is flagged and the nearest row taken
+__device__ __forceinline__ int kv8_table_row(int pos, int rows, unsigned *status) {
+    if (pos >= 0 && pos < rows) return pos;
+    if (status) atomicOr(status, kKv8BadPos);
+    return pos < 0 ? 0 : rows - 1;
+}
+
+// ---- the coding rule -------------------------------------------------------------------------------
+constexpr int kCodeI8 = 0, kCodeE4M3 = 1;
+template <int CODE> __device__ __forceinline__ constexpr float kv8_top() { return CODE == kCodeI8 ? 127.0f : 448.0f; }
+
+// magnitude bits: ordered like the magnitude, NaN above infinity
+__device__ __forceinline__ uint32_t kv8_abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+// scale of a block whose incoming rows reach amax (as magnitude bits); `old` = 0 for a block that starts with them
+template <int CODE> __device__ __forceinline__ float kv8_new_scale(uint32_t amax_bits, float old) {
+    const float need = __fdiv_rn(__uint_as_float(amax_bits), kv8_top<CODE>());
+    return (old != old || need <= old) ? old : need; // NaN on either side stays NaN
+}
+
+// four values to four codes (values of finite size; a scale of 0, infinity or NaN gives codes 0)
+template <int CODE> __device__ __forceinline__ uint32_t kv8_pack4(const float (&y)[4]) {
+    uint32_t r = 0;
+    if (CODE == kCodeI8) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            int q;
+            asm("cvt.rni.sat.s8.f32 %0, %1;" : "=r"(q) : "f"(fmaxf(y[i], -127.0f)));
+            r |= (uint32_t)(q & 0xff) << (8 * i);
+        }
+    } else {
+        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3);
+        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3);
+        r = lo | (hi << 16);
+    }
+    return r;
+}
+template <int CODE> __device__ __forceinline__ uint2 kv8_encode8(const float (&x)[8], float scale) {
+    const bool ok = scale > 0.f && scale <= 3.402823466e38f;
+    float y[2][4];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i >> 2][i & 3] = ok ? __fdiv_rn(x[i], scale) : 0.f;
+    return make_uint2(kv8_pack4<CODE>(y[0]), kv8_pack4<CODE>(y[1]));
+}
+template <int CODE> __device__ __forceinline__ void kv8_decode4(uint32_t w, float (&x)[4]) {
+    if (CODE == kCodeI8) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = (float)(int8_t)(w >> (8 * i));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> (16 * i)), __NV_E4M3);
+            const float2 f = __half22float2(__half2(h));
+            x[2 * i] = f.x;
+            x[2 * i + 1] = f.y;
+        }
+    }
+}
+// codes of a block that a larger scale takes over: ratio = old / new
+template <int CODE> __device__ __forceinline__ uint2 kv8_rescale8(uint2 u, float ratio) {
+    float a[4], b[4];
+    kv8_decode4<CODE>(u.x, a);
+    kv8_decode4<CODE>(u.y, b);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        a[i] = __fmul_rn(a[i], ratio);
+        b[i] = __fmul_rn(b[i], ratio);
+    }
+    return make_uint2(kv8_pack4<CODE>(a), kv8_pack4<CODE>(b));
+}
+
+// largest of a value over the block's threads; `red` has room for one word per warp.  All threads call it.
+__device__ __forceinline__ uint32_t kv8_block_max(uint32_t v, uint32_t *red) {
+    v = __reduce_max_sync(0xffffffffu, v);
+    const int nw = (blockDim.x + 31) >> 5;
+    if (nw == 1) return v;
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = ((int)(threadIdx.x & 31) < nw) ? red[threadIdx.x & 31] : 0u;
+    v = __reduce_max_sync(0xffffffffu, v);
+    return v;
+}
+
+} // namespace flb

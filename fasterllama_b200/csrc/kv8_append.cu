@@ -1,0 +1,100 @@
+// kv8_append.cu — fresh K/V rows into the 8-bit cache: dequantise, rotate (RoPE), one scale per block of rows and head.
+//
+// HBM-bound streaming pass: a token row and head costs 2 d (e_in + 1) bytes.  One CTA takes one block of rows of one head, K or V:
+// block_len * d values, 32 per thread held in registers between the two halves of the work (largest magnitude, then
+// codes), so every value is read once.  Blocks of the K/V heads of the same tokens are neighbours in the grid: together
+// they read whole rows of the [B,S,Hkv,d] input.
+#include "kv8.cuh"
+
+namespace flb {
+
+namespace {
+
+constexpr int kChunks = 4; // 8-value chunks per thread
+
+template <int D, int CODE, int MODE> __global__ void __launch_bounds__(1024) flb_kv8_append_kernel(const __grid_constant__ Kv8AppendArgs a) {
+    constexpr int CPR = D / 8; // chunks per row
+    __shared__ uint32_t red[32];
+    unsigned id = blockIdx.x;
+    const int kv = (int)(id & 1u);
+    id >>= 1;
+    const int h = (int)(id % (unsigned)a.c.H);
+    id /= (unsigned)a.c.H;
+    const int j = (int)(id % (unsigned)a.nwin), b = (int)(id / (unsigned)a.nwin);
+
+    const int past = a.past_lens ? __ldg(a.past_lens + b) : a.start_pos;
+    const int n = a.new_lens ? __ldg(a.new_lens + b) : a.S;
+    if (past < 0 || n < 0 || n > a.S || past > a.c.T - n) { // nothing of this sequence is touched
+        if (threadIdx.x == 0 && a.status) atomicOr(a.status, kKv8BadLen);
+        return;
+    }
+    const int blk = (past >> a.c.block_shift) + j;
+    const int row0 = blk << a.c.block_shift, row1 = row0 + (1 << a.c.block_shift);
+    const int lo = max(past, row0), hi = min(past + n, row1); // new rows of this block
+    if (lo >= hi) return;
+
+    const size_t unit = (size_t)b * a.c.H + h;
+    uint8_t *codes = a.c.codes[kv] + (unit * a.c.T + row0) * D;
+    float *scale_p = a.c.scale[kv] + unit * a.c.nblk + blk;
+    const int pos0 = (a.token_pos ? __ldg(a.token_pos + b) : past) - past; // position = row + pos0
+
+    float x[kChunks][8];
+    uint32_t amax = 0;
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+        const int ch = threadIdx.x + i * blockDim.x;
+        const int row = row0 + ch / CPR, col = (ch % CPR) * 8;
+        if (row >= lo && row < hi) {
+            kv8_load8<MODE>(a.in[kv], a.act_scale, (size_t)b * a.S + (row - past), h * D + col, x[i]);
+            if (kv == 0 && a.freq_cis) kv8_rotate8(a.freq_cis + (size_t)kv8_table_row(row + pos0, a.freq_rows, a.status) * D + col, x[i]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) amax = max(amax, kv8_abs_bits(x[i][e]));
+        }
+    }
+    amax = kv8_block_max(amax, red);
+    const float old = (row0 >= past) ? 0.f : *scale_p;
+    __syncthreads(); // every thread has read the old scale
+    const float scale = kv8_new_scale<CODE>(amax, old);
+    const bool grown = old > 0.f && scale > old;
+    const float ratio = grown ? __fdiv_rn(old, scale) : 1.f;
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+        const int ch = threadIdx.x + i * blockDim.x;
+        const int row = row0 + ch / CPR;
+        uint2 *dst = reinterpret_cast<uint2 *>(codes) + ch;
+        if (row >= lo && row < hi)
+            *dst = kv8_encode8<CODE>(x[i], scale);
+        else if (row < past && grown)
+            *dst = kv8_rescale8<CODE>(*dst, ratio);
+    }
+    if (threadIdx.x == 0) *scale_p = scale;
+    if (kv == 0 && a.c.row_pos)
+        for (int r = lo + (int)threadIdx.x; r < hi; r += blockDim.x) a.c.row_pos[unit * a.c.T + r] = r + pos0;
+}
+
+template <int D, int CODE> cudaError_t launch_t(const Kv8AppendArgs &a, int input_mode, cudaStream_t stream) {
+    const unsigned threads = (unsigned)((D << a.c.block_shift) / (8 * kChunks));
+    const unsigned grid = 2u * (unsigned)a.c.H * (unsigned)a.nwin * (unsigned)a.c.B;
+    if (input_mode == 0)
+        flb_kv8_append_kernel<D, CODE, 0><<<grid, threads, 0, stream>>>(a);
+    else if (input_mode == 1)
+        flb_kv8_append_kernel<D, CODE, 1><<<grid, threads, 0, stream>>>(a);
+    else
+        flb_kv8_append_kernel<D, CODE, 2><<<grid, threads, 0, stream>>>(a);
+    return cudaGetLastError();
+}
+
+} // namespace
+
+cudaError_t launch_kv8_append(const Kv8AppendArgs &a, int d, int code, int input_mode, cudaStream_t stream) {
+    if (code == kCodeI8) {
+        if (d == 64) return launch_t<64, kCodeI8>(a, input_mode, stream);
+        if (d == 256) return launch_t<256, kCodeI8>(a, input_mode, stream);
+        return launch_t<128, kCodeI8>(a, input_mode, stream);
+    }
+    if (d == 64) return launch_t<64, kCodeE4M3>(a, input_mode, stream);
+    if (d == 256) return launch_t<256, kCodeE4M3>(a, input_mode, stream);
+    return launch_t<128, kCodeE4M3>(a, input_mode, stream);
+}
+
+} // namespace flb

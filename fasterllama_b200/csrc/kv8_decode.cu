@@ -1,0 +1,508 @@
+// kv8_decode.cu — single-token attention over the 8-bit cache, the new token's append included.
+//
+// For one K/V head and its G q heads:  x_r = c q.(code_r scale_r),  out = sum_r p_r code_r scale_r / sum_r p_r.
+// HBM-bound: 2 d bytes per cached row and K/V head, read once for all G heads.
+//   * grid = K/V heads x splits of `split_len` rows; four warps per CTA, warp w takes the 16-row steps w, w + 4, ... of its
+//     split.  Codes go from global memory straight into registers in the order the matrix instructions want them (every
+//     byte is used by one lane only, so shared memory would add nothing), one step ahead of their use.
+//   * both products run on the warp-level matrix instructions with exact operands: a code is a whole number below 2^11 (or
+//     an e4m3 value) and fits fp16 as it is.  The 8-bit -> fp16 conversion (1.25 to 1.5 instructions per code) is
+//     then all the arithmetic per cached byte.  q and the weights p are split into a high and a low fp16 part in
+//     neighbouring columns, which carries 22 bits of them through: the columns are there anyway (N = 8 holds four heads).
+//     S = K q:       A = 16 rows of codes, B = q parts;   lane (g, t) ends with rows g, g + 8 of head t
+//     O^T += V^T p:  A = codes of 16 dims x 16 rows (two rows' bytes interleaved), B = p parts, an 8x8 transpose away from S
+//   * scales of a block are uniform over a step (blocks hold at least 16 rows): K's goes into the score, V's into p.
+//   * each warp keeps its own running maximum per head, raised only when a score passes it by 2^8 (exact: sum and result
+//     share the reference); warps merge in warp order, splits in split order by the CTA that arrives last.  The
+//     result depends on the sequence and on split_len alone.
+//   * the CTA of the last split codes the new token and rescales its block if that has to grow, before it reads it; no
+//     other CTA reads that block (splits are multiples of blocks).  Where several CTAs share a K/V head (more q heads than
+//     fit one), the append kernel runs first instead.
+//   * weights for an eviction need the final maximum and sum: scores are left in scratch (fp32) and a second small kernel turns
+//     them into weights and adds them up over the group.
+#include "kv8.cuh"
+
+#include "flb_ptx.cuh"
+
+namespace flb {
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNoMax = -1e30f;   // running maximum before the first visible key (finite: -inf - -inf is NaN)
+constexpr float kRaise = 8.0f;     // log2: a weight stays below 2^8
+constexpr int kWarps = 4;
+constexpr int kStep = 16;          // rows per warp step
+constexpr int kMaxSplitScales = 8192 / 16;
+
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
+
+// Two codes (bytes i0, i1 of w) as an fp16 pair.  int8: byte + 128 under the exponent of 1024, minus 1152.
+template <int CODE> __device__ __forceinline__ void codes_to_halves(uint32_t w, uint32_t &lo, uint32_t &hi) {
+    if (CODE == kCodeI8) {
+        w ^= 0x80808080u;
+        const uint32_t bias = 0x64806480u;
+        uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
+        lo = h2_bits(__hsub2(*reinterpret_cast<__half2 *>(&a), *reinterpret_cast<const __half2 *>(&bias)));
+        hi = h2_bits(__hsub2(*reinterpret_cast<__half2 *>(&b), *reinterpret_cast<const __half2 *>(&bias)));
+    } else {
+        lo = h2_bits(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3)));
+        hi = h2_bits(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3)));
+    }
+}
+
+template <int BYTES> struct Raw {
+    uint32_t w[BYTES / 4];
+};
+// BYTES (8, 16 or 32) consecutive bytes; streamed once
+template <int BYTES> __device__ __forceinline__ void load_raw(Raw<BYTES> &r, const uint8_t *p) {
+    if (BYTES == 8) {
+        const uint2 u = __ldcs(reinterpret_cast<const uint2 *>(p));
+        r.w[0] = u.x;
+        r.w[1] = u.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < BYTES / 16; ++i) {
+            const uint4 u = __ldcs(reinterpret_cast<const uint4 *>(p) + i);
+            r.w[4 * i] = u.x;
+            r.w[4 * i + 1] = u.y;
+            r.w[4 * i + 2] = u.z;
+            r.w[4 * i + 3] = u.w;
+        }
+    }
+}
+
+// a few rows per CTA: the input form is looked at here and not compiled in
+__device__ __forceinline__ void load8(const Kv8DecodeArgs &a, int which, size_t token, int col, float (&x)[8]) {
+    if (a.input_mode == 0)
+        kv8_load8<0>(a.in[which], a.act_scale, token, col, x);
+    else if (a.input_mode == 1)
+        kv8_load8<1>(a.in[which], a.act_scale, token, col, x);
+    else
+        kv8_load8<2>(a.in[which], a.act_scale, token, col, x);
+}
+
+// The new token's k and v of one K/V head into its block, by the CTA's first D / 8 (k) and next D / 8 (v) threads per row; the
+// block's held codes follow a scale that grew.  All threads call it; ends with a barrier.
+template <int D, int CODE>
+__device__ __forceinline__ void append_token(const Kv8DecodeArgs &a, size_t unit, int b, int h, int past, int pos, int prow, uint32_t *red2) {
+    constexpr int CPR = D / 8;
+    const int blk = past >> a.c.block_shift, row0 = blk << a.c.block_shift;
+    const bool fresh = row0 == past;
+    const int tid = threadIdx.x;
+    const int kv = tid / CPR, ch = tid % CPR;
+    float x[8];
+    uint32_t amax = 0;
+    if (tid < 2) red2[tid] = 0u;
+    __syncthreads();
+    if (kv < 2) {
+        load8(a, 1 + kv, (size_t)b, h * D + ch * 8, x);
+        if (kv == 0 && a.freq_cis) kv8_rotate8(a.freq_cis + (size_t)prow * D + ch * 8, x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) amax = max(amax, kv8_abs_bits(x[e]));
+        atomicMax(red2 + kv, amax);
+    }
+    __syncthreads();
+    const size_t sidx = unit * a.c.nblk + blk;
+    float scale[2], ratio[2];
+    bool grown[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const float old = fresh ? 0.f : a.c.scale[i][sidx];
+        scale[i] = kv8_new_scale<CODE>(red2[i], old);
+        grown[i] = old > 0.f && scale[i] > old;
+        ratio[i] = grown[i] ? __fdiv_rn(old, scale[i]) : 1.f;
+    }
+    __syncthreads(); // every thread has read the old scales
+    if (tid == 0) {
+        a.c.scale[0][sidx] = scale[0];
+        a.c.scale[1][sidx] = scale[1];
+        if (a.c.row_pos) a.c.row_pos[unit * a.c.T + past] = pos;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        uint2 *rows = reinterpret_cast<uint2 *>(a.c.codes[i] + (unit * a.c.T + row0) * D);
+        if (grown[i])
+            for (int c = tid; c < (past - row0) * CPR; c += blockDim.x) rows[c] = kv8_rescale8<CODE>(rows[c], ratio[i]);
+        if (kv == i) rows[(past - row0) * CPR + ch] = kv8_encode8<CODE>(x, scale[i]);
+    }
+    __syncthreads();
+}
+
+// FORM: capped scores, distance bias or key_begin.  NT: column tiles of eight = four q heads each.
+template <int D, int CODE, int NT, bool FORM>
+__global__ void __launch_bounds__(kWarps * 32) flb_kv8_decode_kernel(const __grid_constant__ Kv8DecodeArgs a) {
+    constexpr int HEADS = 4 * NT;
+    constexpr int KCH = D / 64;   // 16-byte chunks of a K row per lane
+    constexpr int VB = D / 8;     // bytes of a V row per lane
+    constexpr int MT = D / 16;    // output tiles of 16 dims
+    constexpr int NTHREADS = kWarps * 32;
+    __shared__ __align__(16) __half q_s[2 * HEADS][D];     // [2 head + part]
+    __shared__ float q_unit[HEADS];                        // what a product with q_s is to be multiplied by
+    __shared__ float sc_s[2][kMaxSplitScales];             // scales of the split's blocks
+    __shared__ float w_m[kWarps][HEADS], w_l[kWarps][HEADS];
+    __shared__ __align__(16) float w_o[kWarps][HEADS][D];
+    __shared__ uint32_t red[32];
+    __shared__ int last_flag;
+
+    const int split = (int)(blockIdx.x % (unsigned)a.nsplit_max);
+    const unsigned uc = blockIdx.x / (unsigned)a.nsplit_max;
+    const int chunk = (int)(uc % (unsigned)a.nchunk);
+    const size_t unit = uc / (unsigned)a.nchunk;
+    const int b = (int)(unit / a.c.H), h = (int)(unit - (size_t)b * a.c.H);
+    const int head0 = h * a.G + chunk * HEADS, nheads = min(HEADS, a.G - chunk * HEADS);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+
+    const int past = a.past_lens ? __ldg(a.past_lens + b) : a.start_pos;
+    if (past < 0 || past >= a.c.T || past >= a.nsplit_max * a.split_len) { // flagged, nothing stored, zeros returned
+        if (split == 0) {
+            if (tid == 0) atomicOr(a.status, kKv8BadLen);
+            for (int i = tid; i < nheads * D; i += NTHREADS) {
+                const size_t o = ((size_t)b * a.Hq + head0) * D + i;
+                if (a.out_f16) ((__half *)a.out)[o] = __float2half_rn(0.f); else ((float *)a.out)[o] = 0.f;
+            }
+        }
+        return;
+    }
+    const int nsplit = past / a.split_len + 1;
+    if (split >= nsplit) return;
+    const int row0 = split * a.split_len, row1 = min(row0 + a.split_len, past + 1);
+    const bool is_last = split == nsplit - 1;
+    const int pos = a.token_pos ? __ldg(a.token_pos + b) : past;
+    const int prow = a.freq_cis ? kv8_table_row(pos, a.freq_rows, a.status) : 0;
+    const int begin = (FORM && a.key_begin) ? __ldg(a.key_begin + b) : INT_MIN;
+
+    if (is_last && a.append) append_token<D, CODE>(a, unit, b, h, past, pos, prow, red);
+
+    // ---- q: rotated, brought to [2^8, 2^9) by a power of two, split into two fp16 parts; one warp per head
+    for (int hh = warp; hh < HEADS; hh += kWarps) {
+        float x[8];
+        uint32_t amax = 0;
+        const bool on = hh < nheads && lane < D / 8;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = 0.f;
+        static_assert(D <= 256, "a warp holds a row, eight dims to a lane");
+        if (on) {
+            load8(a, 0, (size_t)b, (head0 + hh) * D + lane * 8, x);
+            if (a.freq_cis) kv8_rotate8(a.freq_cis + (size_t)prow * D + lane * 8, x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) amax = max(amax, kv8_abs_bits(x[e]));
+        }
+        amax = __reduce_max_sync(0xffffffffu, amax);
+        const int ex = min(max((int)(amax >> 23) - 127, -110), 126);
+        const float up = __uint_as_float((uint32_t)(8 - ex + 127) << 23), down = __uint_as_float((uint32_t)(ex - 8 + 127) << 23);
+        if (lane < D / 8) {
+            __half2 hi[4], lo[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float u = x[2 * e] * up, v = x[2 * e + 1] * up;
+                hi[e] = __floats2half2_rn(u, v);
+                const float2 f = __half22float2(hi[e]);
+                lo[e] = __floats2half2_rn(u - f.x, v - f.y);
+            }
+            *reinterpret_cast<uint4 *>(&q_s[2 * hh][lane * 8]) = *reinterpret_cast<uint4 *>(hi);
+            *reinterpret_cast<uint4 *>(&q_s[2 * hh + 1][lane * 8]) = *reinterpret_cast<uint4 *>(lo);
+        }
+        if (lane == 0) q_unit[hh] = down * a.scale_log2e;
+    }
+    // ---- scales of the split's blocks; the largest of V's decides by which power of two the weights are raised
+    uint32_t vmax = 0;
+    {
+        const int nb = ((row1 - 1) >> a.c.block_shift) - (row0 >> a.c.block_shift) + 1;
+        const size_t s0 = unit * a.c.nblk + (row0 >> a.c.block_shift);
+        for (int i = tid; i < nb; i += NTHREADS) {
+            sc_s[0][i] = __ldcg(a.c.scale[0] + s0 + i);
+            const float v = __ldcg(a.c.scale[1] + s0 + i);
+            sc_s[1][i] = v;
+            vmax = max(vmax, kv8_abs_bits(v));
+        }
+    }
+    vmax = kv8_block_max(vmax, red);
+    __syncthreads();
+    const int vex = min(max((int)(vmax >> 23) - 127, -100), 100);
+    const float v_up = __uint_as_float((uint32_t)(5 - vex + 127) << 23), v_down = __uint_as_float((uint32_t)(vex - 5 + 127) << 23);
+
+    uint32_t qf[NT][4 * KCH][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int s = 0; s < 4 * KCH; ++s) {
+            const uint2 u = *reinterpret_cast<const uint2 *>(&q_s[8 * n + g][(s >> 2) * 64 + 16 * t + 4 * (s & 3)]);
+            qf[n][s][0] = u.x;
+            qf[n][s][1] = u.y;
+        }
+    float qu[NT], m_run[NT], l_run[NT], slope[NT];
+    float o[NT][MT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        qu[n] = q_unit[4 * n + t];
+        m_run[n] = kNoMax;
+        l_run[n] = 0.f;
+        slope[n] = (FORM && a.slopes && 4 * n + t < nheads) ? __ldg(a.slopes + head0 + 4 * n + t) * kLog2e : 0.f;
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[n][i][e] = 0.f;
+    }
+    const float inv_cap = (FORM && a.cap_log2e > 0.f) ? 1.0f / a.cap_log2e : 0.f;
+
+    // ---- the pass over the rows
+    int r = row0 + warp * kStep;
+    // rows in position order: nothing below key_begin is read
+    if (FORM && a.key_begin && !a.c.row_pos && begin > r) {
+        const int skip = (int)(((long long)min(begin, a.c.T) - r) / (kWarps * kStep));
+        r += skip * (kWarps * kStep);
+    }
+    const uint8_t *kp = a.c.codes[0] + (unit * a.c.T + r + g) * (size_t)D + 16 * t;
+    const uint8_t *vp = a.c.codes[1] + (unit * a.c.T + r + 2 * t) * (size_t)D + g * VB;
+    Raw<16> kr[2][KCH];
+    Raw<VB> vr[4];
+    auto load_k = [&]() {
+#pragma unroll
+        for (int c = 0; c < KCH; ++c) {
+            load_raw<16>(kr[0][c], kp + c * 64);
+            load_raw<16>(kr[1][c], kp + 8 * D + c * 64);
+        }
+        kp += (size_t)kWarps * kStep * D;
+    };
+    auto load_v = [&]() {
+        load_raw<VB>(vr[0], vp);
+        load_raw<VB>(vr[1], vp + D);
+        load_raw<VB>(vr[2], vp + 8 * D);
+        load_raw<VB>(vr[3], vp + 9 * D);
+        vp += (size_t)kWarps * kStep * D;
+    };
+    if (r < row1) {
+        load_k();
+        load_v();
+    }
+    for (; r < row1; r += kWarps * kStep) {
+        const bool more = r + kWarps * kStep < row1;
+        float s[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+#pragma unroll
+        for (int c = 0; c < KCH; ++c)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                uint32_t f[4];
+                codes_to_halves<CODE>(kr[0][c].w[w], f[0], f[2]);
+                codes_to_halves<CODE>(kr[1][c].w[w], f[1], f[3]);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) mma16816(s[n], f, qf[n][4 * c + w][0], qf[n][4 * c + w][1]);
+            }
+        if (more) load_k();
+
+        const int sb = (r - row0) >> a.c.block_shift;
+        const float ks = sc_s[0][sb], vs = sc_s[1][sb] * v_up;
+        int kpos[2] = {r + g, r + g + 8};
+        bool vis[2] = {r + g < row1, r + g + 8 < row1};
+        if (FORM) {
+            if (a.c.row_pos && (a.slopes || a.key_begin)) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) kpos[i] = __ldcg(a.c.row_pos + unit * a.c.T + r + g + 8 * i);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) vis[i] = vis[i] && kpos[i] >= begin;
+        }
+        uint32_t pb[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            float x[2] = {(s[n][0] + s[n][1]) * (ks * qu[n]), (s[n][2] + s[n][3]) * (ks * qu[n])};
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (FORM) {
+                    if (a.cap_log2e > 0.f) x[i] = a.cap_log2e * tanhf(x[i] * inv_cap);
+                    x[i] = fmaf(-slope[n], fabsf((float)(pos - kpos[i])), x[i]);
+                }
+                x[i] = vis[i] ? x[i] : -INFINITY;
+            }
+            if (a.scores && 4 * n + t < nheads) {
+                float *sp = a.scores + ((size_t)b * a.Hq + head0 + 4 * n + t) * a.c.T + r + g;
+                if (r + g < row1) sp[0] = x[0];
+                if (r + g + 8 < row1) sp[8] = x[1];
+            }
+            const float top = fmaxf(x[0], x[1]);
+            if (__any_sync(0xffffffffu, top > m_run[n] + kRaise)) {
+                float mx = top;
+#pragma unroll
+                for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+                const float m_new = fmaxf(m_run[n], mx);
+                const float corr = ex2(m_run[n] - m_new);
+                m_run[n] = m_new;
+                l_run[n] *= corr;
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[n][i][e] *= corr;
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float p = ex2(x[i] - m_run[n]);
+                l_run[n] += p;
+                const float pv = vis[i] ? p * vs : 0.f;
+                const __half hi = __float2half_rn(pv);
+                const __half lo = __float2half_rn(pv - __half2float(hi));
+                pb[n][i] = transpose8x8(h2_bits(__halves2half2(hi, lo)));
+            }
+        }
+        if (CODE == kCodeE4M3 && r + kStep > row1) { // codes behind the sequence may be NaN patterns
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (r + 2 * t + (i & 1) + (i >> 1) * 8 >= row1)
+#pragma unroll
+                    for (int w = 0; w < VB / 4; ++w) vr[i].w[w] = 0u;
+        }
+#pragma unroll
+        for (int w = 0; w < VB / 4; ++w) { // four dims: two output tiles
+            uint32_t f0[4], f1[4];
+            const uint32_t e0 = __byte_perm(vr[0].w[w], vr[1].w[w], 0x5140), e1 = __byte_perm(vr[0].w[w], vr[1].w[w], 0x7362);
+            const uint32_t e2 = __byte_perm(vr[2].w[w], vr[3].w[w], 0x5140), e3 = __byte_perm(vr[2].w[w], vr[3].w[w], 0x7362);
+            codes_to_halves<CODE>(e0, f0[0], f0[1]);
+            codes_to_halves<CODE>(e2, f0[2], f0[3]);
+            codes_to_halves<CODE>(e1, f1[0], f1[1]);
+            codes_to_halves<CODE>(e3, f1[2], f1[3]);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                mma16816(o[n][2 * w], f0, pb[n][0], pb[n][1]);
+                mma16816(o[n][2 * w + 1], f1, pb[n][0], pb[n][1]);
+            }
+        }
+        if (more) load_v();
+    }
+
+    // ---- warps to shared memory: sums over the eight row groups, high and low parts together
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) l_run[n] += __shfl_xor_sync(0xffffffffu, l_run[n], off);
+        if (g == 0) {
+            w_m[warp][4 * n + t] = m_run[n];
+            w_l[warp][4 * n + t] = l_run[n];
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+            *reinterpret_cast<float2 *>(&w_o[warp][4 * n + t][g * (D / 8) + 2 * i]) =
+                make_float2((o[n][i][0] + o[n][i][1]) * v_down, (o[n][i][2] + o[n][i][3]) * v_down);
+    }
+    __syncthreads();
+
+    // ---- merge in warp order
+    const size_t pbase = ((unit * a.nchunk + chunk) * a.nsplit_max + split) * HEADS;
+    for (int i = tid; i < nheads * D; i += NTHREADS) {
+        const int hh = i / D, col = i - hh * D;
+        float M = kNoMax, acc = 0.f, l = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) M = fmaxf(M, w_m[w][hh]);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const float e = ex2(w_m[w][hh] - M);
+            acc = fmaf(w_o[w][hh][col], e, acc);
+            l = fmaf(w_l[w][hh], e, l);
+        }
+        if (nsplit == 1) {
+            const size_t oo = ((size_t)b * a.Hq + head0 + hh) * D + col;
+            const float y = (l > 0.f || l != l) ? acc / l : 0.f;
+            if (a.out_f16) ((__half *)a.out)[oo] = __float2half_rn(y); else ((float *)a.out)[oo] = y;
+            if (a.ml && col == 0) {
+                a.ml[((size_t)b * a.Hq + head0 + hh) * 2] = M;
+                a.ml[((size_t)b * a.Hq + head0 + hh) * 2 + 1] = l;
+            }
+        } else {
+            a.part_o[(pbase + hh) * D + col] = acc;
+            if (col == 0) {
+                a.part_ml[(pbase + hh) * 2] = M;
+                a.part_ml[(pbase + hh) * 2 + 1] = l;
+            }
+        }
+    }
+    if (nsplit == 1) return;
+    __syncthreads();
+    if (tid == 0) {
+        __threadfence();
+        const unsigned old = atomicAdd(a.counters + unit * a.nchunk + chunk, 1u);
+        last_flag = old == (unsigned)(nsplit - 1);
+    }
+    __syncthreads();
+    if (!last_flag) return;
+    __threadfence();
+    const size_t mbase = (unit * a.nchunk + chunk) * a.nsplit_max;
+    for (int i = tid; i < nheads * D; i += NTHREADS) {
+        const int hh = i / D, col = i - hh * D;
+        float M = kNoMax, acc = 0.f, l = 0.f;
+        for (int s = 0; s < nsplit; ++s) M = fmaxf(M, __ldcg(a.part_ml + ((mbase + s) * HEADS + hh) * 2));
+        for (int s = 0; s < nsplit; ++s) {
+            const size_t p = (mbase + s) * HEADS + hh;
+            const float e = ex2(__ldcg(a.part_ml + p * 2) - M);
+            acc = fmaf(__ldcg(a.part_o + p * D + col), e, acc);
+            l = fmaf(__ldcg(a.part_ml + p * 2 + 1), e, l);
+        }
+        const size_t oo = ((size_t)b * a.Hq + head0 + hh) * D + col;
+        const float y = (l > 0.f || l != l) ? acc / l : 0.f;
+        if (a.out_f16) ((__half *)a.out)[oo] = __float2half_rn(y); else ((float *)a.out)[oo] = y;
+        if (a.ml && col == 0) {
+            a.ml[((size_t)b * a.Hq + head0 + hh) * 2] = M;
+            a.ml[((size_t)b * a.Hq + head0 + hh) * 2 + 1] = l;
+        }
+    }
+    if (tid == 0) a.counters[unit * a.nchunk + chunk] = 0u; // ready for the next call
+}
+
+// weight_out = weight_in + sum over the group of 2^(score - max) / sum; one thread per row and K/V head.
+__global__ void __launch_bounds__(256) flb_kv8_weights_kernel(const __grid_constant__ Kv8DecodeArgs a, int blocks_per_unit) {
+    const size_t unit = blockIdx.x / (unsigned)blocks_per_unit;
+    const int r = (int)(blockIdx.x % (unsigned)blocks_per_unit) * 256 + threadIdx.x;
+    const int b = (int)(unit / a.c.H), h = (int)(unit - (size_t)b * a.c.H);
+    const int past = a.past_lens ? __ldg(a.past_lens + b) : a.start_pos;
+    if (past < 0 || past >= a.c.T || past >= a.nsplit_max * a.split_len || r > past) return;
+    const size_t i = unit * a.c.T + r;
+    float w = (r == past) ? 0.f : a.weight_in[i];
+    const bool hidden = a.key_begin && !a.c.row_pos && r < __ldg(a.key_begin + b); // no score was left for it
+    for (int j = 0; j < a.G; ++j) {
+        const size_t hq = (size_t)b * a.Hq + h * a.G + j;
+        const float l = __ldg(a.ml + hq * 2 + 1);
+        if (hidden) continue;
+        if (l > 0.f || l != l) w += ex2(__ldcs(a.scores + hq * a.c.T + r) - __ldg(a.ml + hq * 2)) / l;
+    }
+    a.weight_out[i] = w;
+}
+
+template <int D, int CODE, int NT> cudaError_t launch_t(const Kv8DecodeArgs &a, cudaStream_t stream) {
+    const unsigned grid = (unsigned)a.c.B * (unsigned)a.c.H * (unsigned)a.nchunk * (unsigned)a.nsplit_max;
+    const bool form = a.cap_log2e > 0.f || a.slopes || a.key_begin;
+    if (form)
+        flb_kv8_decode_kernel<D, CODE, NT, true><<<grid, kWarps * 32, 0, stream>>>(a);
+    else
+        flb_kv8_decode_kernel<D, CODE, NT, false><<<grid, kWarps * 32, 0, stream>>>(a);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess || !a.weight_out) return e;
+    const int rows = min(a.c.T, a.nsplit_max * a.split_len), bpu = (rows + 255) / 256;
+    flb_kv8_weights_kernel<<<(unsigned)a.c.B * (unsigned)a.c.H * (unsigned)bpu, 256, 0, stream>>>(a, bpu);
+    return cudaGetLastError();
+}
+
+template <int CODE> cudaError_t launch_code(const Kv8DecodeArgs &a, int d, int nt, cudaStream_t stream) {
+    if (d == 256) return launch_t<256, CODE, 1>(a, stream);
+    if (d == 64) return nt == 2 ? launch_t<64, CODE, 2>(a, stream) : launch_t<64, CODE, 1>(a, stream);
+    return nt == 2 ? launch_t<128, CODE, 2>(a, stream) : launch_t<128, CODE, 1>(a, stream);
+}
+
+} // namespace
+
+cudaError_t launch_kv8_decode(const Kv8DecodeArgs &a, int d, int code, int nt, cudaStream_t stream) {
+    return code == kCodeI8 ? launch_code<kCodeI8>(a, d, nt, stream) : launch_code<kCodeE4M3>(a, d, nt, stream);
+}
+
+} // namespace flb

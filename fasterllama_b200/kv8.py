@@ -1,0 +1,349 @@
+"""The 8-bit K/V cache: host-side entry to include/flb_kv8.h.
+
+A `Cache` names the tensors of one layer's cache.  `append` stores tokens (a prompt, a chunk, one), `decode` stores one
+token per sequence and attends over everything cached, `evict` cuts sequences down to a budget of rows by the attention weight
+that `decode` accumulated.  Everything is stream-ordered and works in the caller's tensors; scratch comes from the caller
+as in `attention` (`decode_workspace_bytes`, `evict_workspace_bytes`).  Calls run on the device of the cache, on its
+current stream unless one is given."""
+from __future__ import annotations
+
+import ctypes as C
+import math
+from dataclasses import dataclass
+from typing import Any
+
+import torch
+
+from . import _lib
+from ._lib import FLB_F16, FLB_F32, FLB_IN_F16, FLB_IN_F32, FLB_IN_INT32  # noqa: F401
+
+FLB_KV8_I8, FLB_KV8_E4M3 = 0, 1
+STATUS_BAD_LEN, STATUS_BAD_POS = 4, 32
+
+_IN_MODE = {torch.int32: FLB_IN_INT32, torch.float32: FLB_IN_F32, torch.float16: FLB_IN_F16}
+_OUT = {torch.float32: FLB_F32, torch.float16: FLB_F16}
+_CODE = {torch.int8: FLB_KV8_I8, torch.float8_e4m3fn: FLB_KV8_E4M3}
+
+
+class FlbKv8Cache(C.Structure):
+    """struct flb_kv8_cache, field for field."""
+
+    _fields_ = [(n, C.c_int) for n in ("batch_size", "kv_head_num", "size_per_head", "total_len", "block_len", "code_type")] + [
+        (n, C.c_void_p) for n in ("k_codes", "v_codes", "k_scale", "v_scale", "row_pos")]
+
+
+class FlbKv8Append(C.Structure):
+    """struct flb_kv8_append_params, field for field."""
+
+    _fields_ = [
+        ("cache", FlbKv8Cache), ("seq_len", C.c_int), ("start_pos", C.c_int), ("past_lens", C.c_void_p), ("new_lens", C.c_void_p),
+        ("token_pos", C.c_void_p), ("input_mode", C.c_int), ("k", C.c_void_p), ("v", C.c_void_p), ("kv_row_stride", C.c_int),
+        ("act_scale", C.c_void_p), ("k_w_scale", C.c_void_p), ("v_w_scale", C.c_void_p), ("freq_cis", C.c_void_p), ("freq_rows", C.c_int),
+        ("status", C.c_void_p),
+    ]
+
+
+class FlbKv8Decode(C.Structure):
+    """struct flb_kv8_decode_params, field for field."""
+
+    _fields_ = [
+        ("cache", FlbKv8Cache), ("head_num", C.c_int), ("start_pos", C.c_int), ("past_lens", C.c_void_p), ("max_past_len", C.c_int),
+        ("token_pos", C.c_void_p), ("input_mode", C.c_int), ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("q_row_stride", C.c_int),
+        ("kv_row_stride", C.c_int), ("act_scale", C.c_void_p), ("q_w_scale", C.c_void_p), ("k_w_scale", C.c_void_p), ("v_w_scale", C.c_void_p),
+        ("freq_cis", C.c_void_p), ("freq_rows", C.c_int), ("softmax_scale", C.c_float), ("softcap", C.c_float), ("alibi_slopes", C.c_void_p),
+        ("key_begin", C.c_void_p), ("weight_in", C.c_void_p), ("weight_out", C.c_void_p), ("out", C.c_void_p), ("out_dtype", C.c_int),
+        ("scratch", C.c_void_p), ("scratch_bytes", C.c_size_t), ("scratch_zeroed", C.c_int), ("split_len", C.c_int),
+    ]
+
+
+class FlbKv8Evict(C.Structure):
+    """struct flb_kv8_evict_params, field for field."""
+
+    _fields_ = [
+        ("cache", FlbKv8Cache), ("start_pos", C.c_int), ("past_lens", C.c_void_p), ("len_out", C.c_void_p), ("budget", C.c_int),
+        ("recent", C.c_int), ("sinks", C.c_int), ("next_pos", C.c_void_p), ("weight", C.c_void_p), ("weight_out", C.c_void_p),
+        ("pos_out", C.c_void_p), ("scratch", C.c_void_p), ("scratch_bytes", C.c_size_t),
+    ]
+
+
+# every symbol include/flb_kv8.h declares: name -> (restype, argtypes)
+_SIZE = C.POINTER(C.c_size_t)
+EXPORTS = {
+    "flb_kv8_validate_append": (C.c_int, [C.POINTER(FlbKv8Append)]),
+    "flb_kv8_validate_decode": (C.c_int, [C.POINTER(FlbKv8Decode)]),
+    "flb_kv8_validate_evict": (C.c_int, [C.POINTER(FlbKv8Evict)]),
+    "flb_kv8_decode_workspace_bytes": (C.c_int, [C.POINTER(FlbKv8Decode), _SIZE]),
+    "flb_kv8_counter_bytes": (C.c_int, [C.POINTER(FlbKv8Decode), _SIZE]),
+    "flb_kv8_evict_workspace_bytes": (C.c_int, [C.POINTER(FlbKv8Evict), _SIZE]),
+    "flb_kv8_append": (C.c_int, [C.POINTER(FlbKv8Append), C.c_void_p]),
+    "flb_kv8_decode": (C.c_int, [C.POINTER(FlbKv8Decode), C.c_void_p]),
+    "flb_kv8_evict": (C.c_int, [C.POINTER(FlbKv8Evict), C.c_void_p]),
+}
+
+_typed: C.CDLL | None = None
+
+
+def load_library() -> C.CDLL:
+    """The library with the entry points of flb_kv8.h typed.  Raises if it is absent or lacks one: there is no fallback."""
+    global _typed
+    lib = _lib.load_library()
+    if _typed is not lib:
+        for name, (res, args) in EXPORTS.items():
+            fn = getattr(lib, name)
+            fn.restype, fn.argtypes = res, args
+        _typed = lib
+    return lib
+
+
+@dataclass
+class Cache:
+    """One layer's cache.  k, v: codes [B,Hkv,T,d], int8 or float8_e4m3fn; k_scale, v_scale: float32 [B,Hkv,T/block_len]; row_pos:
+    int32 [B,Hkv,T] or None (row r is at position r)."""
+
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+    row_pos: torch.Tensor | None = None
+
+    @property
+    def block_len(self) -> int:
+        return self.k.shape[2] // self.k_scale.shape[2]
+
+    def tensors(self) -> dict[str, torch.Tensor]:
+        t = {"k": self.k, "v": self.v, "k_scale": self.k_scale, "v_scale": self.v_scale}
+        if self.row_pos is not None:
+            t["row_pos"] = self.row_pos
+        return t
+
+    def dequantize(self) -> tuple[torch.Tensor, torch.Tensor]:
+        """What the codes stand for, float32 [B,Hkv,T,d] twice (a look at the cache, not a step of the path)."""
+        def one(codes, scale):
+            B, H, T, d = codes.shape
+            n = scale.shape[2]
+            return (codes.float().view(B, H, n, T // n, d) * scale[..., None, None]).view(B, H, T, d)
+
+        return one(self.k, self.k_scale), one(self.v, self.v_scale)
+
+
+def empty_cache(batch_size: int, kv_head_num: int, total_len: int, size_per_head: int, *, block_len: int = 64, dtype=torch.int8,
+                row_pos: bool = False, device="cuda") -> Cache:
+    """An empty cache; total_len is rounded up to whole blocks.  `row_pos`: keep positions, which eviction needs."""
+    n = -(-total_len // block_len)
+    shape = (batch_size, kv_head_num, n * block_len, size_per_head)
+    codes = [torch.zeros(shape, dtype=torch.int8, device=device).view(dtype) for _ in range(2)]
+    scales = [torch.zeros(batch_size, kv_head_num, n, device=device) for _ in range(2)]
+    pos = torch.zeros(batch_size, kv_head_num, n * block_len, dtype=torch.int32, device=device) if row_pos else None
+    return Cache(*codes, *scales, row_pos=pos)
+
+
+def _dense(t: torch.Tensor, name: str, shape, dtype, device) -> int:
+    """Address of a dense tensor of this shape, type and device."""
+    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        raise ValueError(f"{name} must be a dense {dtype} tensor of shape {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the cache on {device}")
+    return t.data_ptr()
+
+
+def _opt(t: torch.Tensor | None, name: str, shape, dtype, device) -> int | None:
+    return None if t is None else _dense(t, name, shape, dtype, device)
+
+
+def _cache(c: Cache) -> FlbKv8Cache:
+    k = c.k
+    if k.dim() != 4 or k.dtype not in _CODE:
+        raise ValueError("cache codes must be int8 or float8_e4m3fn tensors [B,Hkv,T,d]")
+    B, H, T, d = k.shape
+    n = c.k_scale.shape[-1]
+    if n <= 0 or T % n:
+        raise ValueError("cache scales must be [B,Hkv,T/block_len]")
+    dev = k.device
+    return FlbKv8Cache(
+        B, H, d, T, T // n, _CODE[k.dtype], _dense(k, "k", (B, H, T, d), k.dtype, dev), _dense(c.v, "v", (B, H, T, d), k.dtype, dev),
+        _dense(c.k_scale, "k_scale", (B, H, n), torch.float32, dev), _dense(c.v_scale, "v_scale", (B, H, n), torch.float32, dev),
+        _opt(c.row_pos, "row_pos", (B, H, T), torch.int32, dev))
+
+
+def _rows(t: torch.Tensor, name: str, shape, dtype, device) -> tuple[int, int]:
+    """Address and token-row stride (elements) of q, k or v [B,S,heads,d]: dense heads, one stride between tokens."""
+    if t.dtype != dtype or tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must be {dtype} of shape {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the cache on {device}")
+    B, S, H, d = shape
+    if t.is_contiguous():
+        return t.data_ptr(), H * d
+    st = t.stride()
+    row = st[1] if S > 1 else (st[0] if B > 1 else H * d)
+    if st[3] != 1 or (H > 1 and st[2] != d) or (S > 1 and st[1] != row) or (B > 1 and st[0] != S * row) or row < H * d:
+        raise ValueError(f"{name} must be [B,S,heads,d] with unit element stride, head stride d and one stride between tokens")
+    return t.data_ptr(), row
+
+
+def _kv_rows(k, v, shape, dtype, device):
+    kp, ks = _rows(k, "k", shape, dtype, device)
+    vp, vs = _rows(v, "v", shape, dtype, device)
+    if ks != vs:
+        raise ValueError("k and v must share one token-row stride")
+    return kp, vp, ks
+
+
+def _scales(mode, act, named, B, S, device):
+    """Addresses of the activation scale and of the weight scales (name -> (tensor, heads * d))."""
+    if mode != FLB_IN_INT32:
+        return [None] * (1 + len(named))
+    if act is None or any(t is None for t, _ in named.values()):
+        raise ValueError("int32 inputs need act_scale and the weight scales")
+    if act.numel() != B * S:
+        raise ValueError("act_scale must hold one value per token")
+    return [_dense(act, "act_scale", act.shape, torch.float32, device)] + [
+        _dense(t, n, (w,), torch.float32, device) for n, (t, w) in named.items()]
+
+
+def _rope(freq_cis, d, device):
+    if freq_cis is None:
+        return None, 0
+    return _dense(freq_cis, "freq_cis", (freq_cis.shape[0], d), torch.float32, device), freq_cis.shape[0]
+
+
+def _scratch(scratch, device):
+    if scratch is None:
+        return None, 0
+    if scratch.device != device or not scratch.is_contiguous():
+        raise ValueError("scratch must be a dense tensor on the cache's device")
+    return scratch.data_ptr(), scratch.numel() * scratch.element_size()
+
+
+def _call(fn, params, device, stream) -> None:
+    if device.type != "cuda":
+        raise ValueError("the 8-bit cache lives on a CUDA device")
+    if torch.cuda.current_device() == device.index:
+        h = stream if stream is not None else torch.cuda.current_stream()
+        _lib.check(fn(C.byref(params), getattr(h, "cuda_stream", h)))
+        return
+    with torch.cuda.device(device):
+        h = stream if stream is not None else torch.cuda.current_stream()
+        _lib.check(fn(C.byref(params), getattr(h, "cuda_stream", h)))
+
+
+def append_params(cache: Cache, k, v, *, start_pos: int = 0, past_lens=None, new_lens=None, token_pos=None, act_scale=None, k_w_scale=None,
+                  v_w_scale=None, freq_cis=None, scratch=None) -> FlbKv8Append:
+    """The parameter block of `append`."""
+    c, dev = _cache(cache), cache.k.device
+    B, H, d = c.batch_size, c.kv_head_num, c.size_per_head
+    S = k.shape[1]
+    mode = _IN_MODE.get(k.dtype)
+    if mode is None:
+        raise ValueError("k and v must be int32, float32 or float16")
+    kp, vp, row = _kv_rows(k, v, (B, S, H, d), k.dtype, dev)
+    act, kw, vw = _scales(mode, act_scale, {"k_w_scale": (k_w_scale, H * d), "v_w_scale": (v_w_scale, H * d)}, B, S, dev)
+    fr, frows = _rope(freq_cis, d, dev)
+    sp, _ = _scratch(scratch, dev)
+    return FlbKv8Append(c, S, start_pos, _opt(past_lens, "past_lens", (B,), torch.int32, dev), _opt(new_lens, "new_lens", (B,), torch.int32, dev),
+                        _opt(token_pos, "token_pos", (B,), torch.int32, dev), mode, kp, vp, row, act, kw, vw, fr, frows, sp)
+
+
+def append(cache: Cache, k, v, *, stream=None, **kw) -> None:
+    """Stores the tokens k, v [B,S,Hkv,d] (int32 sums with their scales, float32 or float16) behind the rows each sequence has:
+    `past_lens` int32 [B], or `start_pos` for all.  `new_lens` int32 [B]: how many of the S tokens of a padded batch count.
+    `token_pos` int32 [B]: position of the first new token, where it is not the cached length.  `freq_cis`: RoPE table, row = position.
+    `scratch`: its first word collects error bits (`attention.scratch_status`); may be None."""
+    _call(load_library().flb_kv8_append, append_params(cache, k, v, **kw), cache.k.device, stream)
+
+
+def decode_params(cache: Cache, q, k, v, out, *, start_pos: int = 0, past_lens=None, max_past_len: int = 0, token_pos=None, act_scale=None,
+                  q_w_scale=None, k_w_scale=None, v_w_scale=None, freq_cis=None, softmax_scale: float | None = None, softcap: float = 0.0,
+                  alibi_slopes=None, key_begin=None, weight_in=None, weight_out=None, scratch=None, scratch_zeroed: bool = False,
+                  split_len: int = 0) -> FlbKv8Decode:
+    """The parameter block of `decode`."""
+    c, dev = _cache(cache), cache.k.device
+    B, Hkv, d, T = c.batch_size, c.kv_head_num, c.size_per_head, c.total_len
+    Hq = q.shape[2]
+    mode = _IN_MODE.get(q.dtype)
+    if mode is None or out.dtype not in _OUT:
+        raise ValueError("q, k and v must be int32, float32 or float16, out float32 or float16")
+    qp, qrow = _rows(q, "q", (B, 1, Hq, d), q.dtype, dev)
+    kp, vp, row = _kv_rows(k, v, (B, 1, Hkv, d), q.dtype, dev)
+    act, qw, kw, vw = _scales(mode, act_scale, {"q_w_scale": (q_w_scale, Hq * d), "k_w_scale": (k_w_scale, Hkv * d), "v_w_scale": (v_w_scale, Hkv * d)},
+                              B, 1, dev)
+    fr, frows = _rope(freq_cis, d, dev)
+    sp, sbytes = _scratch(scratch, dev)
+    i32, f32 = torch.int32, torch.float32
+    return FlbKv8Decode(
+        c, Hq, start_pos, _opt(past_lens, "past_lens", (B,), i32, dev), max_past_len, _opt(token_pos, "token_pos", (B,), i32, dev), mode, qp, kp, vp,
+        qrow, row, act, qw, kw, vw, fr, frows, softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(d), softcap,
+        _opt(alibi_slopes, "alibi_slopes", (Hq,), f32, dev), _opt(key_begin, "key_begin", (B,), i32, dev),
+        _opt(weight_in, "weight_in", (B, Hkv, T), f32, dev), _opt(weight_out, "weight_out", (B, Hkv, T), f32, dev),
+        _dense(out, "out", (B, Hq, 1, d), out.dtype, dev), _OUT[out.dtype], sp, sbytes, 1 if scratch_zeroed else 0, split_len)
+
+
+def decode(cache: Cache, q, k, v, out, *, stream=None, **kw) -> None:
+    """One token per sequence: k, v [B,1,Hkv,d] are stored as by `append`, then q [B,1,H,d] attends over the rows 0..past into out [B,H,1,d].
+    H is a multiple of Hkv.  `max_past_len`: host's bound on past_lens (0 = T - 1).  `softcap`: scores become
+    softcap * tanh(score / softcap); `alibi_slopes` float32 [H]: minus slope times distance; `key_begin` int32 [B]: rows at an earlier
+    position are not seen.  `weight_in`, `weight_out` float32 [B,Hkv,T]: attention weights accumulated over the group (for `evict`), in place
+    when both are the same tensor.  `scratch_zeroed`: the first `counter_bytes` bytes of scratch are zero (each call leaves them so)."""
+    _call(load_library().flb_kv8_decode, decode_params(cache, q, k, v, out, **kw), cache.k.device, stream)
+
+
+def evict_params(cache: Cache, *, len_out, budget: int, weight, start_pos: int = 0, past_lens=None, recent: int = 0, sinks: int = 0, next_pos=None,
+                 weight_out=None, pos_out=None, scratch=None) -> FlbKv8Evict:
+    """The parameter block of `evict`."""
+    c, dev = _cache(cache), cache.k.device
+    B, H, T = c.batch_size, c.kv_head_num, c.total_len
+    if cache.row_pos is None:
+        raise ValueError("eviction needs a cache with row_pos")
+    i32, f32 = torch.int32, torch.float32
+    sp, sbytes = _scratch(scratch, dev)
+    return FlbKv8Evict(
+        c, start_pos, _opt(past_lens, "past_lens", (B,), i32, dev), _dense(len_out, "len_out", (B,), i32, dev), budget, recent, sinks,
+        _opt(next_pos, "next_pos", (B,), i32, dev), _dense(weight, "weight", (B, H, T), f32, dev),
+        _dense(weight if weight_out is None else weight_out, "weight_out", (B, H, T), f32, dev),
+        _dense(cache.row_pos if pos_out is None else pos_out, "pos_out", (B, H, T), i32, dev), sp, sbytes)
+
+
+def evict(cache: Cache, *, stream=None, **kw) -> None:
+    """Keeps `budget` rows per head of every sequence: those at a position below `sinks` or at or behind next_pos - `recent`, then those of the
+    largest accumulated `weight`.  Rows move within the cache, weights and positions along (into weight_out and pos_out, or in place);
+    len_out int32 [B] gets min(cached rows, budget) and may be past_lens.  The order of rows is no longer that of positions afterwards."""
+    _call(load_library().flb_kv8_evict, evict_params(cache, **kw), cache.k.device, stream)
+
+
+def decode_workspace_bytes(batch_size: int, head_num: int, kv_head_num: int, total_len: int, size_per_head: int = 128, *, block_len: int = 64,
+                           weights: bool = False, split_len: int = 0) -> int:
+    """Scratch of a `decode` call on a full cache of these sizes."""
+    p = _sized(batch_size, head_num, kv_head_num, total_len, size_per_head, block_len, weights, split_len)
+    n = C.c_size_t(0)
+    _lib.check(load_library().flb_kv8_decode_workspace_bytes(C.byref(p), C.byref(n)))
+    return n.value
+
+
+def counter_bytes(batch_size: int, head_num: int, kv_head_num: int, size_per_head: int = 128, *, block_len: int = 64) -> int:
+    """Bytes at the start of a `decode` scratch that `scratch_zeroed` speaks of."""
+    p = _sized(batch_size, head_num, kv_head_num, block_len, size_per_head, block_len, False, 0)
+    n = C.c_size_t(0)
+    _lib.check(load_library().flb_kv8_counter_bytes(C.byref(p), C.byref(n)))
+    return n.value
+
+
+def evict_workspace_bytes(batch_size: int, kv_head_num: int, total_len: int, size_per_head: int = 128, *, block_len: int = 64) -> int:
+    p = FlbKv8Evict()
+    p.cache = FlbKv8Cache(batch_size, kv_head_num, size_per_head, -(-total_len // block_len) * block_len, block_len)
+    n = C.c_size_t(0)
+    _lib.check(load_library().flb_kv8_evict_workspace_bytes(C.byref(p), C.byref(n)))
+    return n.value
+
+
+def _sized(B, Hq, Hkv, T, d, block_len, weights, split_len) -> FlbKv8Decode:
+    p = FlbKv8Decode()
+    p.cache = FlbKv8Cache(B, Hkv, d, -(-T // block_len) * block_len, block_len)
+    p.head_num, p.split_len, p.weight_out = Hq, split_len, (16 if weights else None)
+    return p
+
+
+def validate(p: Any) -> int:
+    """Status of the host-side checks of a parameter block (no CUDA call)."""
+    lib = load_library()
+    fn = {FlbKv8Append: lib.flb_kv8_validate_append, FlbKv8Decode: lib.flb_kv8_validate_decode, FlbKv8Evict: lib.flb_kv8_validate_evict}[type(p)]
+    return int(fn(C.byref(p)))
