@@ -98,8 +98,22 @@ class FlbPeerExchange(C.Structure):
     ]
 
 
+class FlbScoreForm(C.Structure):
+    """struct flb_score_form, field for field."""
+
+    _fields_ = [
+        ("kv_head_num", C.c_int),
+        ("kv_row_stride", C.c_int),
+        ("softcap", C.c_float),
+        ("alibi_slopes", C.c_void_p),
+        ("key_begin", C.c_void_p),
+        ("key_end", C.c_void_p),
+    ]
+
+
 # every symbol include/flb_attn.h declares: name -> (restype, argtypes)
 _PP = C.POINTER(FlbAttnParams)
+_PF = C.POINTER(FlbScoreForm)
 EXPORTS = {
     "flb_attn_abi_version": (C.c_int, []),
     "flb_status_string": (C.c_char_p, [C.c_int]),
@@ -109,6 +123,11 @@ EXPORTS = {
     "flb_attn_decode": (C.c_int, [_PP, C.c_void_p]),
     "flb_attn_prefill": (C.c_int, [_PP, C.c_void_p]),
     "flb_attn_forward": (C.c_int, [_PP, C.c_void_p]),
+    "flb_attn_validate_scored": (C.c_int, [_PP, _PF]),
+    "flb_attn_scored_workspace_bytes": (C.c_int, [_PP, _PF, C.POINTER(C.c_size_t)]),
+    "flb_attn_decode_scored": (C.c_int, [_PP, _PF, C.c_void_p]),
+    "flb_attn_prefill_scored": (C.c_int, [_PP, _PF, C.c_void_p]),
+    "flb_attn_forward_scored": (C.c_int, [_PP, _PF, C.c_void_p]),
     "flb_attn_classify_mask": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.POINTER(C.c_int), C.c_void_p]),
     "flb_attn_scratch_status": (C.c_int, [C.c_void_p, C.POINTER(C.c_uint), C.c_void_p]),
     "flb_attn_decode_static_scratch": (C.c_int, [_PP, C.c_void_p]),

@@ -25,6 +25,7 @@ from ._lib import (  # noqa: F401  (re-exported)
     FLB_MASK_NONE,
     FlbAttnParams,
     FlbError,
+    FlbScoreForm,
 )
 
 
@@ -155,6 +156,51 @@ def make_params(
     return p
 
 
+def make_scored_params(*, q, k, v, k_cache, v_cache, out, softcap: float = 0.0, alibi_slopes=None, key_begin=None, key_end=None,
+                       **kw) -> tuple[FlbAttnParams, FlbScoreForm]:
+    """The parameter block of `make_params` and the score form beside it (see flb_score_form): capped scores, distance bias (float32 [H]),
+    per-row key bounds (int32, decode [B], prefill [B,S]), and k, v [B,S,Hkv,d] with caches [B,Hkv,T,d] of fewer heads than q."""
+    B, S, H, d = (int(x) for x in q.shape)
+    Hkv = int(k.shape[2])
+    if tuple(k.shape) != (B, S, Hkv, d) or tuple(v.shape) != (B, S, Hkv, d) or H % Hkv:
+        raise ValueError("k and v must be [B,S,Hkv,d] with a number of heads that divides q's")
+    if tuple(k_cache.shape) != tuple(v_cache.shape) or tuple(k_cache.shape[:2]) != (B, Hkv) or k_cache.shape[3] != d:
+        raise ValueError("caches must be [B, Hkv, T, d]")
+    if not _is_contiguous(k_cache) or not _is_contiguous(v_cache):
+        raise ValueError("the caches must be contiguous")
+    if _dtype_name(k) != _dtype_name(q) or _dtype_name(v) != _dtype_name(q):
+        raise ValueError("q, k and v must share one type")
+    rows = (B,) if S == 1 else (B, S)
+    for name, t, shape, dtype in (("alibi_slopes", alibi_slopes, (H,), "float32"), ("key_begin", key_begin, rows, "int32"), ("key_end", key_end, rows, "int32")):
+        if t is not None and (tuple(t.shape) != shape or _dtype_name(t) != dtype or not _is_contiguous(t)):
+            raise ValueError(f"{name} must be a dense {dtype} tensor of shape {shape}")
+    strides = {_token_row_stride(t, B, S, Hkv, d) for t in (k, v)}
+    if len(strides) != 1:
+        raise ValueError("k and v must share one token-row stride")
+    # make_params looks at one head count: q stands in for k and v there, and their own addresses and sizes follow
+    p = make_params(q=q, k=q, v=q, k_cache=_Heads(k_cache, H), v_cache=_Heads(v_cache, H), out=out, **kw)
+    p.k, p.v = _ptr(k), _ptr(v)
+    f = FlbScoreForm()
+    f.kv_head_num, f.kv_row_stride, f.softcap = Hkv, strides.pop(), float(softcap)
+    f.alibi_slopes, f.key_begin, f.key_end = _ptr(alibi_slopes), _ptr(key_begin), _ptr(key_end)
+    p._keep = (*p._keep, k, v, k_cache, v_cache)
+    f._keep = (alibi_slopes, key_begin, key_end)
+    return p, f
+
+
+class _Heads:
+    """A cache seen with another number of heads, for the shape checks of `make_params`."""
+
+    def __init__(self, t, heads: int):
+        self.t, self.shape, self.dtype = t, (t.shape[0], heads, t.shape[2], t.shape[3]), t.dtype
+
+    def data_ptr(self) -> int:
+        return _ptr(self.t)
+
+    def is_contiguous(self) -> bool:
+        return True
+
+
 def workspace_bytes(batch_size: int, head_num: int, total_len: int, seq_len: int = 1, split_len: int = 0,
                     size_per_head: int = 128) -> int:
     """Scratch bytes for every call these dimensions allow (decode on a full cache, prefill of
@@ -164,6 +210,13 @@ def workspace_bytes(batch_size: int, head_num: int, total_len: int, seq_len: int
     p.total_len, p.seq_len, p.split_len = total_len, seq_len, split_len
     n = C.c_size_t(0)
     _lib.check(_lib.load_library().flb_attn_workspace_bytes(C.byref(p), C.byref(n)))
+    return int(n.value)
+
+
+def scored_workspace_bytes(p: FlbAttnParams, f: FlbScoreForm | None) -> int:
+    """Scratch bytes of a scored call with these sizes (only the sizes of `p` are looked at, and which bounds `f` has)."""
+    n = C.c_size_t(0)
+    _lib.check(_lib.load_library().flb_attn_scored_workspace_bytes(C.byref(p), _form(f), C.byref(n)))
     return int(n.value)
 
 
@@ -187,6 +240,27 @@ def _stream_handle(stream) -> int | None:
 
 def validate(p: FlbAttnParams) -> int:
     return int(_lib.load_library().flb_attn_validate(C.byref(p)))
+
+
+def _form(f: FlbScoreForm | None):
+    return None if f is None else C.byref(f)
+
+
+def validate_scored(p: FlbAttnParams, f: FlbScoreForm | None) -> int:
+    return int(_lib.load_library().flb_attn_validate_scored(C.byref(p), _form(f)))
+
+
+def forward_scored(p: FlbAttnParams, f: FlbScoreForm | None, stream=None) -> None:
+    """`forward` with a score form (both from `make_scored_params`)."""
+    _lib.check(_lib.load_library().flb_attn_forward_scored(C.byref(p), _form(f), _stream_handle(stream)))
+
+
+def decode_scored(p: FlbAttnParams, f: FlbScoreForm | None, stream=None) -> None:
+    _lib.check(_lib.load_library().flb_attn_decode_scored(C.byref(p), _form(f), _stream_handle(stream)))
+
+
+def prefill_scored(p: FlbAttnParams, f: FlbScoreForm | None, stream=None) -> None:
+    _lib.check(_lib.load_library().flb_attn_prefill_scored(C.byref(p), _form(f), _stream_handle(stream)))
 
 
 def forward(p: FlbAttnParams, stream=None) -> None:

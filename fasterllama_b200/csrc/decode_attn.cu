@@ -70,9 +70,9 @@ template <> struct CacheIO<__half> {
 // between sequences (H*d when dense).
 // FLB_IN_INT32: float(acc) * act_scale[b] * w_scale[h*d+i], in this order (decoder_kernels.cu:449).
 template <int D>
-__device__ __forceinline__ float load_input(const DecodeArgs &a, const void *base, const float *w_scale, int unit, int b,
+__device__ __forceinline__ float load_input(const DecodeArgs &a, const void *base, const float *w_scale, int row_stride, int b,
                                             int h, int i) {
-    const size_t off = (size_t)b * a.row_stride + (size_t)h * D + i;
+    const size_t off = (size_t)b * row_stride + (size_t)h * D + i;
     if (a.input_mode == 0) {
         const float acc = (float)__ldg((const int32_t *)base + off);
         return acc * __ldg(a.act_scale + b) * __ldg(w_scale + (size_t)h * D + i);
@@ -152,7 +152,9 @@ __device__ __forceinline__ void quantize_row_if_last(const DecodeArgs &a, int b,
     }
 }
 
-template <typename CacheT, int HD, int TILE_ROWS, int STAGES, int NWARPS>
+// FORM: a score form is in use (capped scores, distance bias, key_begin, K/V heads shared by several q heads); the plain
+// kernel carries none of its code.
+template <typename CacheT, int HD, int TILE_ROWS, int STAGES, int NWARPS, bool FORM>
 __global__ void __launch_bounds__((NWARPS + 1) * 32) flb_decode_attn_kernel(const __grid_constant__ DecodeArgs a) {
     constexpr int D = HD;
     constexpr int ROW_BYTES = D * (int)sizeof(CacheT);
@@ -195,8 +197,17 @@ __global__ void __launch_bounds__((NWARPS + 1) * 32) flb_decode_attn_kernel(cons
     if (a.early_start) grid_launch_dependents();
     if (split >= nsplit) return;
 
-    const int row0 = split * a.split_len;
-    const int rows = max(0, min(a.split_len, past - row0));
+    const int hk = FORM ? h / a.G : h;                                   // K/V head
+    const size_t kv_unit = FORM ? (size_t)b * a.Hkv + hk : (size_t)unit; // its cache slab
+    const int kv_row_stride = FORM ? a.kv_row_stride : a.row_stride;
+    const int begin = (FORM && a.key_begin) ? __ldg(a.key_begin + b) : 0;
+    int row0 = split * a.split_len;
+    int rows = max(0, min(a.split_len, past - row0));
+    if (FORM && begin > row0) { // whole tiles below the first visible key are not read
+        const int skip = min(begin - row0, rows) / TILE_ROWS * TILE_ROWS;
+        row0 += skip;
+        rows -= skip;
+    }
     const int ntiles = (rows + TILE_ROWS - 1) / TILE_ROWS;
     const bool is_last = (split == nsplit - 1);
 
@@ -220,8 +231,8 @@ __global__ void __launch_bounds__((NWARPS + 1) * 32) flb_decode_attn_kernel(cons
     if (warp == NWARPS) {
         // ---------------- producer warp: one lane issues the bulk copies -------------------
         if (lane == 0) {
-            const unsigned char *kb = (const unsigned char *)a.k_cache + ((size_t)unit * a.T + row0) * ROW_BYTES;
-            const unsigned char *vb = (const unsigned char *)a.v_cache + ((size_t)unit * a.T + row0) * ROW_BYTES;
+            const unsigned char *kb = (const unsigned char *)a.k_cache + (kv_unit * a.T + row0) * ROW_BYTES;
+            const unsigned char *vb = (const unsigned char *)a.v_cache + (kv_unit * a.T + row0) * ROW_BYTES;
             for (int t = 0; t < ntiles; ++t) {
                 const int s = t % STAGES;
                 const uint32_t use = (uint32_t)(t / STAGES);
@@ -259,8 +270,8 @@ __global__ void __launch_bounds__((NWARPS + 1) * 32) flb_decode_attn_kernel(cons
                 const int i = tid + e * NC; // head dimension of this thread
                 float qraw = 0.f, kraw = 0.f;
                 if (i < D) {
-                    qraw = load_input<D>(a, a.q, a.q_w_scale, unit, b, h, i);
-                    if (is_last) kraw = load_input<D>(a, a.k, a.k_w_scale, unit, b, h, i);
+                    qraw = load_input<D>(a, a.q, a.q_w_scale, a.row_stride, b, h, i);
+                    if (is_last) kraw = load_input<D>(a, a.k, a.k_w_scale, kv_row_stride, b, hk, i);
                 }
                 float qrot = qraw, krot = kraw;
                 if (a.freq_cis) {
@@ -302,6 +313,7 @@ __global__ void __launch_bounds__((NWARPS + 1) * 32) flb_decode_attn_kernel(cons
 #pragma unroll
                 for (int w = 0; w < NWARPS; ++w) t += red[w];
                 s_new = t;
+                if (FORM && a.cap_log2e > 0.f) s_new = a.cap_log2e * tanhf(s_new / a.cap_log2e); // at distance 0: no bias
                 switch (a.mask_mode) {
                 case 1: // generic additive mask, row = query position, column = key position
                     s_new += __ldg(a.attn_mask + (size_t)past * a.mask_row_stride + past) * kLog2e;
@@ -314,6 +326,7 @@ __global__ void __launch_bounds__((NWARPS + 1) * 32) flb_decode_attn_kernel(cons
                     new_visible = true;
                     break;
                 }
+                if (FORM && begin > past) new_visible = false;
             }
         }
 
@@ -332,6 +345,7 @@ __global__ void __launch_bounds__((NWARPS + 1) * 32) flb_decode_attn_kernel(cons
 #pragma unroll
             for (int j = 0; j < EPL; ++j) o[k][j] = 0.f;
 
+        const float slope = (FORM && a.slopes) ? __ldg(a.slopes + h) * kLog2e : 0.f;
         const float *mask_row = (a.mask_mode == 1) ? a.attn_mask + (size_t)past * a.mask_row_stride + row0 : nullptr;
 
         bool ok = true;
@@ -373,8 +387,14 @@ __global__ void __launch_bounds__((NWARPS + 1) * 32) flb_decode_attn_kernel(cons
                 const int r = (it * NWARPS + warp) * RPI + sub;
                 if (r >= rvalid) {
                     sc[it] = -INFINITY;
-                } else if (mask_row) {
-                    sc[it] += __ldg(mask_row + t * TILE_ROWS + r) * kLog2e;
+                } else {
+                    if (FORM) { // scores are few beside the elements they came from: the accurate tanh costs nothing
+                        const int key = row0 + t * TILE_ROWS + r;
+                        if (a.cap_log2e > 0.f) sc[it] = a.cap_log2e * tanhf(sc[it] / a.cap_log2e);
+                        sc[it] = fmaf(-slope, (float)(past - key), sc[it]);
+                        if (key < begin) sc[it] = -INFINITY;
+                    }
+                    if (mask_row) sc[it] += __ldg(mask_row + t * TILE_ROWS + r) * kLog2e;
                 }
                 mt = fmaxf(mt, sc[it]);
             }
@@ -391,7 +411,7 @@ __global__ void __launch_bounds__((NWARPS + 1) * 32) flb_decode_attn_kernel(cons
 #pragma unroll
             for (int it = 0; it < ITERS; ++it) {
                 const int r = (it * NWARPS + warp) * RPI + sub;
-                if (r < rvalid) {
+                if (r < rvalid && !(FORM && row0 + t * TILE_ROWS + r < begin)) {
                     const float p = ex2(sc[it] - m_new);
                     l_run += p;
 #pragma unroll
@@ -418,11 +438,13 @@ __global__ void __launch_bounds__((NWARPS + 1) * 32) flb_decode_attn_kernel(cons
             for (int e = 0; e < DPT; ++e) {
                 const int i = tid + e * NC;
                 if (i < D) {
-                    const float vraw = load_input<D>(a, a.v, a.v_w_scale, unit, b, h, i);
+                    const float vraw = load_input<D>(a, a.v, a.v_w_scale, kv_row_stride, b, hk, i);
                     vnew[e] = CacheIO<CacheT>::round(vraw);
-                    const size_t cidx = ((size_t)unit * a.T + past) * D + i;
-                    CacheIO<CacheT>::store((CacheT *)a.k_cache + cidx, krot_keep[e]);
-                    CacheIO<CacheT>::store((CacheT *)a.v_cache + cidx, vraw);
+                    const size_t cidx = (kv_unit * a.T + past) * D + i;
+                    if (!FORM || hk * a.G == h) { // the first q head of a K/V head stores for all; none of them reads the row back
+                        CacheIO<CacheT>::store((CacheT *)a.k_cache + cidx, krot_keep[e]);
+                        CacheIO<CacheT>::store((CacheT *)a.v_cache + cidx, vraw);
+                    }
                 }
             }
         }
@@ -528,12 +550,12 @@ __global__ void __launch_bounds__((NWARPS + 1) * 32) flb_decode_attn_kernel(cons
 
 // ---- host-side launcher ------------------------------------------------------------------
 
-template <typename CacheT, int HD, int TILE_ROWS, int STAGES, int NWARPS>
-static cudaError_t launch_decode_t(const DecodeArgs &a, cudaStream_t stream) {
+template <typename CacheT, int HD, int TILE_ROWS, int STAGES, int NWARPS, bool FORM>
+static cudaError_t launch_decode_form(const DecodeArgs &a, cudaStream_t stream) {
     constexpr int TILE_BYTES = TILE_ROWS * HD * (int)sizeof(CacheT);
     constexpr size_t smem = (size_t)STAGES * 2 * TILE_BYTES + 2 * STAGES * sizeof(uint64_t) +
                             sizeof(float) * (HD + 2 * NWARPS + NWARPS * HD + NWARPS) + 16;
-    auto kern = flb_decode_attn_kernel<CacheT, HD, TILE_ROWS, STAGES, NWARPS>;
+    auto kern = flb_decode_attn_kernel<CacheT, HD, TILE_ROWS, STAGES, NWARPS, FORM>;
     // the shared-memory opt-in is a property of (kernel, device): set once per device, not on every call (it costs about
     // a microsecond of host time, which an isolated call sees in full)
     static std::atomic<unsigned long long> opted_in{0};
@@ -562,6 +584,12 @@ static cudaError_t launch_decode_t(const DecodeArgs &a, cudaStream_t stream) {
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, kern, a);
+}
+
+template <typename CacheT, int HD, int TILE_ROWS, int STAGES, int NWARPS>
+static cudaError_t launch_decode_t(const DecodeArgs &a, cudaStream_t stream) {
+    return a.form ? launch_decode_form<CacheT, HD, TILE_ROWS, STAGES, NWARPS, true>(a, stream)
+                  : launch_decode_form<CacheT, HD, TILE_ROWS, STAGES, NWARPS, false>(a, stream);
 }
 
 cudaError_t launch_decode(const DecodeArgs &a, bool cache_f16, int head_dim, cudaStream_t stream) {

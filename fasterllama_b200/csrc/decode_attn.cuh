@@ -58,6 +58,13 @@ struct DecodeArgs {
     int early_start; // launched with programmatic stream serialisation: cache tiles may be fetched before the wait
     float *part_o;      // [B*H, nsplit_max, d]
     float *part_ml;     // [B*H, nsplit_max, 2]  (running max in the log2 domain, sum)
+    // score form; the plain kernels look at none of it
+    int form;              // any of the below is in use
+    int G, Hkv;            // q heads per K/V head, K/V heads
+    int kv_row_stride;
+    float cap_log2e;       // softcap * log2(e), 0 = none
+    const float *slopes;   // [H]
+    const int *key_begin;  // [B]
 };
 
 } // namespace flb

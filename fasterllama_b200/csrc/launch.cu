@@ -94,6 +94,13 @@ int check_common(const flb_attn_params *p) {
     return FLB_OK;
 }
 
+// K/V heads of a call, and the elements between two tokens' rows of its k and v
+inline int kv_heads(const flb_attn_params *p, const flb_score_form *f) { return f && f->kv_head_num > 0 ? f->kv_head_num : p->head_num; }
+inline int kv_row_stride(const flb_attn_params *p, const flb_score_form *f) {
+    if (f && f->kv_row_stride) return f->kv_row_stride;
+    return p->qkv_row_stride ? p->qkv_row_stride : kv_heads(p, f) * p->size_per_head;
+}
+
 int max_past_of(const flb_attn_params *p) {
     if (!p->past_lens) return p->start_pos;
     return (p->max_past_len > 0) ? p->max_past_len : p->total_len - 1;
@@ -167,9 +174,11 @@ int flb_attn_workspace_bytes(const flb_attn_params *p, size_t *bytes_out) {
     return FLB_OK;
 }
 
-int flb_attn_decode(const flb_attn_params *p, void *cuda_stream) {
+int flb_attn_decode(const flb_attn_params *p, void *cuda_stream) { return flb_attn_decode_scored(p, nullptr, cuda_stream); }
+
+int flb_attn_decode_scored(const flb_attn_params *p, const flb_score_form *f, void *cuda_stream) {
     if (p && p->seq_len != 1) return FLB_ERR_BAD_SHAPE;
-    const int st = flb_attn_validate(p);
+    const int st = flb_attn_validate_scored(p, f);
     if (st != FLB_OK) return st;
     cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
 
@@ -223,21 +232,60 @@ int flb_attn_decode(const flb_attn_params *p, void *cuda_stream) {
     a.part_ml = reinterpret_cast<float *>(sc + l.ml_off);
     a.part_o = reinterpret_cast<float *>(sc + l.o_off);
 
+    a.Hkv = kv_heads(p, f);
+    a.G = p->head_num / a.Hkv;
+    a.kv_row_stride = kv_row_stride(p, f);
+    a.cap_log2e = f ? f->softcap * 1.4426950408889634f : 0.f;
+    a.slopes = f ? f->alibi_slopes : nullptr;
+    a.key_begin = f ? f->key_begin : nullptr;
+    a.form = a.Hkv != a.H || a.kv_row_stride != a.row_stride || a.cap_log2e > 0.f || a.slopes || a.key_begin;
+
     if (flb::launch_decode(a, p->cache_dtype == FLB_F16, p->size_per_head, stream) != cudaSuccess) return FLB_ERR_LAUNCH;
     return FLB_OK;
 }
 
-int flb_attn_prefill(const flb_attn_params *p, void *cuda_stream) {
+int flb_attn_prefill(const flb_attn_params *p, void *cuda_stream) { return flb_attn_prefill_scored(p, nullptr, cuda_stream); }
+
+int flb_attn_prefill_scored(const flb_attn_params *p, const flb_score_form *f, void *cuda_stream) {
     if (p && p->seq_len <= 1) return FLB_ERR_BAD_SHAPE;
-    const int st = flb_attn_validate(p);
+    const int st = flb_attn_validate_scored(p, f);
     if (st != FLB_OK) return st;
-    return flb::launch_prefill(p, static_cast<cudaStream_t>(cuda_stream));
+    return flb::launch_prefill(p, f, static_cast<cudaStream_t>(cuda_stream));
 }
 
 int flb_attn_forward(const flb_attn_params *p, void *cuda_stream) {
     if (!p) return FLB_ERR_NULL_POINTER;
     // same switch as open_decoder.cu:179 / :216
     return (p->seq_len > 1) ? flb_attn_prefill(p, cuda_stream) : flb_attn_decode(p, cuda_stream);
+}
+
+int flb_attn_forward_scored(const flb_attn_params *p, const flb_score_form *f, void *cuda_stream) {
+    if (!p) return FLB_ERR_NULL_POINTER;
+    return (p->seq_len > 1) ? flb_attn_prefill_scored(p, f, cuda_stream) : flb_attn_decode_scored(p, f, cuda_stream);
+}
+
+int flb_attn_validate_scored(const flb_attn_params *p, const flb_score_form *f) {
+    const int st = flb_attn_validate(p);
+    if (st != FLB_OK || !f) return st;
+    if (f->kv_head_num < 0 || (f->kv_head_num > 0 && (f->kv_head_num > p->head_num || p->head_num % f->kv_head_num))) return FLB_ERR_BAD_SHAPE;
+    if (f->kv_row_stride != 0) {
+        if (f->kv_row_stride < kv_heads(p, f) * p->size_per_head) return FLB_ERR_BAD_SHAPE;
+        if (((size_t)f->kv_row_stride * (p->input_mode == FLB_IN_F16 ? 2 : 4)) % 16u) return FLB_ERR_MISALIGNED;
+    }
+    if (!(f->softcap >= 0.f) || f->softcap > 3.402823466e38f) return FLB_ERR_BAD_SHAPE;
+    if (p->seq_len == 1) return f->key_end ? FLB_ERR_UNSUPPORTED : FLB_OK; // a decode call sees what is cached
+    if (p->scratch_bytes < flb::prefill_scored_scratch_bytes(p->batch_size, p->head_num, p->seq_len, p->size_per_head, f))
+        return FLB_ERR_SCRATCH_TOO_SMALL;
+    return FLB_OK;
+}
+
+int flb_attn_scored_workspace_bytes(const flb_attn_params *p, const flb_score_form *f, size_t *bytes_out) {
+    const int st = flb_attn_workspace_bytes(p, bytes_out);
+    if (st != FLB_OK || p->seq_len == 1) return st;
+    const int d = p->size_per_head > 0 ? p->size_per_head : flb::kHeadDim;
+    const size_t pre = flb::prefill_scored_scratch_bytes(p->batch_size, p->head_num, p->seq_len, d, f);
+    if (pre > *bytes_out) *bytes_out = pre;
+    return FLB_OK;
 }
 
 int flb_attn_quantize(const float *attn, int8_t *q8, float *scale, int batch_size, int head_num, int seq_len, int size_per_head,

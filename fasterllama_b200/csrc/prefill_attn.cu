@@ -112,6 +112,13 @@ struct PrefillArgs {
     int heads_per_group; // work list: groups of this many (b,h) units, heavy query blocks first inside a group
     int v_direct; // fp16 v into an fp16 cache: nothing to convert, so the attention kernel takes the V tiles straight from the
                   // caller's v and stores them into the cache itself; the streaming pass leaves v alone
+    // score form; the plain kernels look at none of it
+    int Hkv, G;        // K/V heads, q heads per K/V head
+    int kv_row_stride; // of k and v
+    float cap_log2e, cap_in; // softcap * log2(e); what a raw score is multiplied by to become the tanh's argument
+    const float *slopes;
+    const int *key_begin, *key_end; // [B,S]
+    int2 *ranges;      // [B][query tiles]: first key that a row of the 128-row tile sees, one past the last; empty = (INT_MAX, 0)
 };
 
 // ------------------------------------------------------------------------------------------------
@@ -196,16 +203,47 @@ __device__ __forceinline__ void rope8(const float4 &f0, const float4 &f1, float 
     }
 }
 
-template <int MODE, int HD> __global__ void __launch_bounds__(256) flb_prefill_prologue_kernel(const PrefillArgs a) {
+// Keys that query row s of sequence b sees: [lo, hi).
+__device__ __forceinline__ void visible_keys(const PrefillArgs &a, int b, int s, int &lo, int &hi) {
+    lo = a.key_begin ? max(0, __ldg(a.key_begin + (size_t)b * a.S + s)) : 0;
+    hi = a.key_end ? min(a.S, __ldg(a.key_end + (size_t)b * a.S + s)) : a.S;
+    if (a.mask_mode == 2) hi = min(hi, s + 1);
+    if (a.mask_mode == 3) hi = min(hi, s);
+}
+
+// SCORED: a score form is in use: k and v may have fewer heads, and with per-row key bounds the blocks behind the token
+// rows work out the key range of every query tile (a warp per tile).
+template <int MODE, int HD, bool SCORED> __global__ void __launch_bounds__(256) flb_prefill_prologue_kernel(const PrefillArgs a) {
     constexpr int R = kRowsPerThread;
     constexpr int D = HD;
     constexpr int TPR = D / 8;    // threads per token row
     constexpr int RPP = 256 / TPR; // token rows a block covers per pass
     const int sblocks = (a.S + RPP * R - 1) / (RPP * R);
+    if (SCORED && a.ranges && blockIdx.x >= (unsigned)sblocks * a.H * a.B) {
+        grid_launch_dependents();
+        const int tiles = (a.S + 2 * BM - 1) / (2 * BM) * 2, lane = threadIdx.x & 31;
+        const int id = (int)(blockIdx.x - (unsigned)sblocks * a.H * a.B) * 8 + (threadIdx.x >> 5);
+        if (id >= a.B * tiles) return;
+        int first = INT_MAX, end = 0;
+        for (int s = id % tiles * BM + lane; s < min(a.S, id % tiles * BM + BM); s += 32) {
+            int lo, hi;
+            visible_keys(a, id / tiles, s, lo, hi);
+            if (lo < hi) {
+                first = min(first, lo);
+                end = max(end, hi);
+            }
+        }
+        first = __reduce_min_sync(0xffffffffu, first);
+        end = __reduce_max_sync(0xffffffffu, end);
+        if (lane == 0) a.ranges[id] = make_int2(first, end);
+        return;
+    }
     const int c = threadIdx.x % TPR;
     const int s0 = (int)(blockIdx.x % sblocks) * (RPP * R) + (threadIdx.x / TPR);
     const int h = (int)((blockIdx.x / sblocks) % a.H);
     const int b = (int)(blockIdx.x / ((size_t)sblocks * a.H));
+    const int hk = SCORED ? h / a.G : h;
+    const bool kv = !SCORED || hk * a.G == h; // the first q head of a K/V head brings its k and v
     Raw8 rq[R], rk[R], rv[R];
     float4 f0[R], f1[R];
     float as[R];
@@ -219,8 +257,9 @@ template <int MODE, int HD> __global__ void __launch_bounds__(256) flb_prefill_p
         const int s = min(s0 + RPP * r, a.S - 1); // rows past the end load a valid row and are not stored
         const size_t in_off = ((size_t)b * a.S + s) * a.row_stride + (size_t)h * D + c * 8;
         rq[r] = load_raw8<MODE>(a.q, in_off);
-        rk[r] = load_raw8<MODE>(a.k, in_off);
-        if (!(MODE == 2 && a.v_direct)) rv[r] = load_raw8<MODE>(a.v, in_off);
+        const size_t kv_off = SCORED ? ((size_t)b * a.S + s) * a.kv_row_stride + (size_t)hk * D + c * 8 : in_off;
+        if (kv) rk[r] = load_raw8<MODE>(a.k, kv_off);
+        if (kv && !(MODE == 2 && a.v_direct)) rv[r] = load_raw8<MODE>(a.v, kv_off);
         as[r] = (MODE == 0) ? __ldg(a.act_scale + (size_t)b * a.S + s) : 1.0f;
         if (a.freq_cis) {
             const float4 *fr = reinterpret_cast<const float4 *>(a.freq_cis + (size_t)(a.rope_pos0 + s) * D + c * 8);
@@ -234,28 +273,29 @@ template <int MODE, int HD> __global__ void __launch_bounds__(256) flb_prefill_p
         const size_t wo = (size_t)h * D + c * 8;
         wq0 = __ldg(reinterpret_cast<const float4 *>(a.q_w_scale + wo));
         wq1 = __ldg(reinterpret_cast<const float4 *>(a.q_w_scale + wo) + 1);
-        wk0 = __ldg(reinterpret_cast<const float4 *>(a.k_w_scale + wo));
-        wk1 = __ldg(reinterpret_cast<const float4 *>(a.k_w_scale + wo) + 1);
-        wv0 = __ldg(reinterpret_cast<const float4 *>(a.v_w_scale + wo));
-        wv1 = __ldg(reinterpret_cast<const float4 *>(a.v_w_scale + wo) + 1);
+        const size_t wkv = (size_t)hk * D + c * 8;
+        wk0 = __ldg(reinterpret_cast<const float4 *>(a.k_w_scale + wkv));
+        wk1 = __ldg(reinterpret_cast<const float4 *>(a.k_w_scale + wkv) + 1);
+        wv0 = __ldg(reinterpret_cast<const float4 *>(a.v_w_scale + wkv));
+        wv1 = __ldg(reinterpret_cast<const float4 *>(a.v_w_scale + wkv) + 1);
     }
     // ---- then convert, rotate, store
     const size_t bh = (size_t)b * a.H + h;
+    const size_t bk = SCORED ? (size_t)b * a.Hkv + hk : bh;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         const int s = s0 + RPP * r;
         if (s < a.S) {
             float q[8], k[8], v[8];
             convert8<MODE>(rq[r], as[r], wq0, wq1, q);
+            if (a.freq_cis) rope8(f0[r], f1[r], q);
+            *reinterpret_cast<uint4 *>(a.qh + (bh * a.S + s) * D + c * 8) = pack8(q); // [B,H,S,d]
+            if (!kv) continue;
             convert8<MODE>(rk[r], as[r], wk0, wk1, k);
             if (!(MODE == 2 && a.v_direct)) convert8<MODE>(rv[r], as[r], wv0, wv1, v);
-            if (a.freq_cis) {
-                rope8(f0[r], f1[r], q);
-                rope8(f0[r], f1[r], k);
-            }
-            const size_t st_off = (bh * a.S + s) * D + c * 8; // [B,H,S,d]
-            const size_t ca_off = (bh * a.T + s) * D + c * 8; // [B,H,T,d]
-            *reinterpret_cast<uint4 *>(a.qh + st_off) = pack8(q);
+            if (a.freq_cis) rope8(f0[r], f1[r], k);
+            const size_t st_off = (bk * a.S + s) * D + c * 8; // [B,Hkv,S,d]
+            const size_t ca_off = (bk * a.T + s) * D + c * 8; // [B,Hkv,T,d]
             store_cache8(a, a.k_cache, ca_off, k);
             if (!(MODE == 2 && a.v_direct)) store_cache8(a, a.v_cache, ca_off, v);
             if (!a.cache_f16) {
@@ -326,8 +366,9 @@ __device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, Prefill
 // A work item is 256 query rows of one (b,h): two 128-row tiles, each with its own S/P and O columns in TMEM.
 struct ItemGeom {
     int q0[2];   // first query row of tile t
-    int n[2];    // key tiles query tile t attends over (n[0] <= n[1])
+    int n[2];    // key tiles query tile t attends over
     int nmax;
+    int j0;      // first key tile of the item (a score form's key bounds; else 0)
 };
 __device__ __forceinline__ ItemGeom item_geom(int qb, int S, bool causal) {
     ItemGeom g;
@@ -341,6 +382,22 @@ __device__ __forceinline__ ItemGeom item_geom(int qb, int S, bool causal) {
         g.n[t] = causal ? min(n_all, (g.q0[t] + BM - 1) / BN + 1) : n_all;
     }
     g.nmax = max(g.n[0], g.n[1]);
+    g.j0 = 0;
+    return g;
+}
+// The same with per-row key bounds: the tiles from the first key any row of the item sees on.  A query tile that sees none
+// takes one (masked) tile, so that every item has the same steps.
+template <bool SCORED> __device__ __forceinline__ ItemGeom item_geom_of(const PrefillArgs &a, int bh, int qb, bool causal) {
+    ItemGeom g = item_geom(qb, a.S, causal);
+    if (SCORED && a.ranges) {
+        const int2 *r = a.ranges + (size_t)(bh / a.H) * ((a.S + 2 * BM - 1) / (2 * BM) * 2) + 2 * qb;
+        const int2 r0 = __ldcg(r), r1 = __ldcg(r + 1); // written by the kernel in front
+        const int first = min(r0.x, r1.x);
+        g.j0 = first == INT_MAX ? 0 : first / BN;
+        g.n[0] = max(1, (r0.y + BN - 1) / BN - g.j0);
+        g.n[1] = max(1, (r1.y + BN - 1) / BN - g.j0);
+        g.nmax = max(g.n[0], g.n[1]);
+    }
     return g;
 }
 
@@ -369,6 +426,51 @@ template <bool GENERIC> __device__ __forceinline__ void mask_chunk(uint32_t (&r)
         r[i] = __float_as_uint(x);
     }
 }
+// The same with a first visible key: [from, lim).
+template <bool GENERIC> __device__ __forceinline__ void mask_range(uint32_t (&r)[32], int base, int from, int lim, float scale, const float *mrow) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+        float x = -INFINITY;
+        if (base + i >= from && base + i < lim) x = GENERIC ? fmaf(__ldg(mrow + base + i), kLog2e, __uint_as_float(r[i]) * scale) : __uint_as_float(r[i]) * scale;
+        r[i] = __float_as_uint(x);
+    }
+}
+// Raw scores to capped ones in units of log2: cap * tanh(u), u = raw * cap_in.  Up to |u| = 1 tanh(u) / u is a polynomial in u^2 (own
+// minimax fit: 2.8e-6 of tanh, 2e-4 of a score at a cap of 50, below the fp16 rounding of the weight) on packed FMAs; it
+// costs no special-function result, of which the exponentials already take half the pipe.  Beyond, for warps that have such a score:
+// 1 - 2 / (1 + e^2|u|).
+__device__ __forceinline__ void cap_chunk(uint32_t (&r)[32], float cap_in, float cap) {
+    float big = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) big = max3(big, fabsf(__uint_as_float(r[i])), fabsf(__uint_as_float(r[i + 1])));
+    if (__any_sync(0xffffffffu, !(big * cap_in <= 1.0f))) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            const float u = __uint_as_float(r[i]) * cap_in;
+            const float e = ex2(fabsf(u) * (2.0f * kLog2e));
+            r[i] = __float_as_uint(copysignf(cap - __fdividef(2.0f * cap, 1.0f + fminf(e, 1e30f)), u));
+        }
+        return;
+    }
+    const float2 in2 = make_float2(cap_in, cap_in);
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+        const float2 u = __fmul2_rn(make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), in2);
+        const float2 y = __fmul2_rn(u, u);
+        float2 p = __ffma2_rn(y, make_float2(0.0083658826f, 0.0083658826f), make_float2(-0.043299854f, -0.043299854f));
+        p = __ffma2_rn(p, y, make_float2(0.12922066f, 0.12922066f));
+        p = __ffma2_rn(p, y, make_float2(-0.33265823f, -0.33265823f));
+        p = __ffma2_rn(p, y, make_float2(0.99996847f, 0.99996847f));
+        p = __fmul2_rn(p, __fmul2_rn(u, make_float2(cap, cap)));
+        r[i] = __float_as_uint(p.x);
+        r[i + 1] = __float_as_uint(p.y);
+    }
+}
+// minus slope times the distance to the row's own position (`ahead`: query row - first key of the chunk); scale first
+__device__ __forceinline__ void bias_chunk(uint32_t (&r)[32], float scale, float slope, int ahead) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(fmaf(-slope, fabsf((float)(ahead - i)), __uint_as_float(r[i]) * scale));
+}
 __device__ __forceinline__ float chunk_max(const uint32_t (&r)[32], float m) {
 #pragma unroll
     for (int i = 0; i < 32; i += 2) m = max3(m, __uint_as_float(r[i]), __uint_as_float(r[i + 1]));
@@ -394,7 +496,8 @@ __device__ __forceinline__ void chunk_exp(const uint32_t (&r)[32], float scale, 
 
 // GENERIC_MASK: the caller's additive mask is read (mask_mode GENERIC); OUT_F16: the output element type.  Compile-time so
 // that each form carries only its own code: what the sixteen warps execute has to share the instruction cache.
-template <int EMUL, bool GENERIC_MASK, bool OUT_F16, int HD>
+// SCORED: a score form is in use.
+template <int EMUL, bool GENERIC_MASK, bool OUT_F16, int HD, bool SCORED>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
     flb_prefill_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                             const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmVin, const PrefillArgs a,
@@ -552,7 +655,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                         pb->v_store_bh[vs] = late_bh;
                         pb->v_store_j[vs] = late_j;
                     }
-                    const int b = late_bh / a.H, h = late_bh - b * a.H;
+                    const int heads = SCORED ? a.Hkv : a.H, b = late_bh / heads, h = late_bh - b * heads;
                     mbar_arrive_expect_tx(&pb->v_full[vs], KV_TILE_BYTES);
                     tma_load_5d(dv, &tmVin, 0, late_j * BN, 0, h, b, &pb->v_full[vs]);
                 } else {
@@ -582,11 +685,17 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                 const int nxt = fetch(); // in flight while the first tile of `cur` is issued
                 int bh, qb;
                 decode(cur, bh, qb);
-                const ItemGeom g = item_geom(qb, a.S, causal);
-                const bool keeper = (qb == nqb - 1); // its query rows see every key tile of the unit
-                ok = load_k(bh, 0, keeper);
+                const ItemGeom g = item_geom_of<SCORED>(a, bh, qb, causal);
+                bool keeper = (qb == nqb - 1); // its query rows see every key tile of the unit
+                int kvu = bh;
+                if (SCORED) {
+                    const int b = bh / a.H, h = bh - b * a.H;
+                    kvu = b * a.Hkv + h / a.G;
+                    keeper = keeper && h % a.G == 0; // one q head stores for its K/V head
+                }
+                ok = load_k(kvu, g.j0, keeper);
                 if (ok) ok = publish(nxt); // one item of look-ahead for the other roles
-                for (int j = 1; j < g.nmax && ok; ++j) ok = load_k(bh, j, keeper);
+                for (int j = 1; j < g.nmax && ok; ++j) ok = load_k(kvu, g.j0 + j, keeper);
                 cur = nxt;
             }
             if (ok) ok = load_v_late(); // the last V tile
@@ -631,7 +740,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                     sched_release(pb, taken++);
                     valid = bh >= 0;
                     if (!valid) break;
-                    const ItemGeom g = item_geom(qb, a.S, causal);
+                    const ItemGeom g = item_geom_of<SCORED>(a, bh, qb, causal);
                     nmax = g.nmax;
                     n_t = t ? g.n[1] : g.n[0];
                     j = 0;
@@ -691,7 +800,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                     if (!ok) break;
                     sched_release(pb, taken++);
                     if (bh < 0) break;
-                    const ItemGeom g = item_geom(qb, a.S, causal);
+                    const ItemGeom g = item_geom_of<SCORED>(a, bh, qb, causal);
                     nmax = g.nmax;
                     n[0] = g.n[0];
                     n[1] = g.n[1];
@@ -752,16 +861,22 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             if (lane == 0) sched_release(pb, taken);
             ++taken;
             if (bh < 0) break;
-            const ItemGeom g = item_geom(qb, a.S, causal);
+            const ItemGeom g = item_geom_of<SCORED>(a, bh, qb, causal);
             const int n_t = t ? g.n[1] : g.n[0];
             const int q0 = t ? g.q0[1] : g.q0[0], row = q0 + lrow;
             float m_used = -1e30f;
             float2 l2 = make_float2(0.f, 0.f);
+            int row_lo = 0, row_hi = 0; // SCORED: the keys this row sees
+            float slope = 0.f;
+            if (SCORED) {
+                if (row < a.S) visible_keys(a, bh / a.H, row, row_lo, row_hi);
+                if (a.slopes) slope = __ldg(a.slopes + bh % a.H) * kLog2e;
+            }
             uint32_t ra[32], rb[32];
             for (int j = 0; j < n_t; ++j) {
                 // One key tile = one step of the online softmax: load the 64 scores of this row, maximum, (rarely)
                 // rescale, P = 2^(x - m) stored over the scores as fp16 pairs, hand the buffer to the tensor core.
-                const int k0 = j * BN;
+                const int k0 = (SCORED ? g.j0 + j : j) * BN;
                 const uint32_t buf = ct & 1u;
                 ok = wait_bar(s_full + buf, (ct >> 1) & 1u, pb, a.status);
                 ok = __all_sync(0xffffffffu, ok);
@@ -784,7 +899,23 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                 const float *mrow = GENERIC_MASK ? a.attn_mask + (size_t)min(row, a.S - 1) * a.mask_row_stride + k0 : nullptr;
                 tmem_wait_ld(ra, rb);
                 float sc = a.scale_log2e;
-                if (mode != 0) { // rare: the causal diagonal, the end of the prompt, or a caller-supplied mask
+                if (SCORED) {
+                    if (a.cap_log2e > 0.f) {
+                        cap_chunk(ra, a.cap_in, a.cap_log2e);
+                        cap_chunk(rb, a.cap_in, a.cap_log2e);
+                        sc = 1.0f;
+                    }
+                    if (a.slopes) {
+                        bias_chunk(ra, sc, slope, row - k0);
+                        bias_chunk(rb, sc, slope, row - k0 - 32);
+                        sc = 1.0f;
+                    }
+                    if (GENERIC_MASK || !__all_sync(0xffffffffu, row_lo <= k0 && row_hi >= k0 + BN)) {
+                        mask_range<GENERIC_MASK>(ra, 0, row_lo - k0, row_hi - k0, sc, mrow);
+                        mask_range<GENERIC_MASK>(rb, 32, row_lo - k0, row_hi - k0, sc, mrow);
+                        sc = 1.0f;
+                    }
+                } else if (mode != 0) { // rare: the causal diagonal, the end of the prompt, or a caller-supplied mask
                     mask_chunk<GENERIC_MASK>(ra, 0, lim, sc, mrow);
                     mask_chunk<GENERIC_MASK>(rb, 32, lim, sc, mrow);
                     sc = 1.0f;
@@ -858,7 +989,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             if (lane == 0) sched_release(pb, taken);
             ++taken;
             if (bh < 0) break;
-            const ItemGeom g = item_geom(qb, a.S, causal);
+            const ItemGeom g = item_geom_of<SCORED>(a, bh, qb, causal);
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 if (g.n[t] == 0) continue;
@@ -978,7 +1109,13 @@ bool make_map(EncodeTiledFn enc, CUtensorMap *tm, const void *base, int BH, int 
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int D> int launch_prefill_hd(const flb_attn_params *p, cudaStream_t stream) {
+using AttnKernel = void (*)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const CUtensorMap, const PrefillArgs, const int);
+template <int D, bool SCORED> AttnKernel attn_kernel_of(bool generic_mask, bool out_f16) {
+    return generic_mask ? (out_f16 ? flb_prefill_attn_kernel<kExpOnFmaEvery, true, true, D, SCORED> : flb_prefill_attn_kernel<kExpOnFmaEvery, true, false, D, SCORED>)
+                        : (out_f16 ? flb_prefill_attn_kernel<kExpOnFmaEvery, false, true, D, SCORED> : flb_prefill_attn_kernel<kExpOnFmaEvery, false, false, D, SCORED>);
+}
+
+template <int D> int launch_prefill_hd(const flb_attn_params *p, const flb_score_form *f, cudaStream_t stream) {
     if (p->freq_cis && (reinterpret_cast<uintptr_t>(p->freq_cis) & 15u)) return FLB_ERR_MISALIGNED;
     if (p->input_mode == FLB_IN_INT32 &&
         ((reinterpret_cast<uintptr_t>(p->q_w_scale) | reinterpret_cast<uintptr_t>(p->k_w_scale) |
@@ -989,6 +1126,8 @@ template <int D> int launch_prefill_hd(const flb_attn_params *p, cudaStream_t st
 
     const int B = p->batch_size, H = p->head_num, S = p->seq_len, T = p->total_len;
     const size_t one = ((size_t)B * H * S * D * 2 + 255) / 256 * 256;
+    const int Hkv = f && f->kv_head_num > 0 ? f->kv_head_num : H;
+    const bool bounded = f && (f->key_begin || f->key_end);
     unsigned char *sc = static_cast<unsigned char *>(p->scratch);
 
     PrefillArgs a;
@@ -1011,7 +1150,18 @@ template <int D> int launch_prefill_hd(const flb_attn_params *p, cudaStream_t st
     a.out_f16 = (p->out_dtype == FLB_F16);
     a.scale_log2e = p->softmax_scale * kLog2e;
     a.status = reinterpret_cast<unsigned *>(sc);
-    a.v_direct = (a.input_mode == FLB_IN_F16 && a.cache_f16) ? 1 : 0;
+    a.Hkv = Hkv;
+    a.G = H / Hkv;
+    a.kv_row_stride = f && f->kv_row_stride ? f->kv_row_stride : (p->qkv_row_stride ? p->qkv_row_stride : Hkv * D);
+    a.cap_log2e = f ? f->softcap * kLog2e : 0.f;
+    a.cap_in = f && f->softcap > 0.f ? p->softmax_scale / f->softcap : 0.f;
+    a.slopes = f ? f->alibi_slopes : nullptr;
+    a.key_begin = f ? f->key_begin : nullptr;
+    a.key_end = f ? f->key_end : nullptr;
+    a.ranges = bounded ? reinterpret_cast<int2 *>(sc + 256 + 3 * one) : nullptr;
+    const bool scored = Hkv != H || a.kv_row_stride != a.row_stride || a.cap_log2e > 0.f || a.slopes || bounded;
+    // with key bounds no item is sure to load every V tile, so the streaming pass stores V then
+    a.v_direct = (a.input_mode == FLB_IN_F16 && a.cache_f16 && !bounded) ? 1 : 0;
     // The larger the group, the closer the list is to heaviest-first over everything (measured at batch 8 x 32 heads x 1024
     // tokens: 142 us with groups of 32 units, 138 us with 64, 139 us with 128, 141 us with all 256 in one group; at
     // batch 32 x 512 tokens 210 us with 32 or 64, 214 us with 256); the limit is what a group's K and V rows (fp16) take in
@@ -1027,15 +1177,15 @@ template <int D> int launch_prefill_hd(const flb_attn_params *p, cudaStream_t st
     CUtensorMap tmQ, tmK, tmV;
     bool ok = make_map(enc, &tmQ, a.qh, B * H, S, S, BM, D);
     if (a.cache_f16) {
-        ok = ok && make_map(enc, &tmK, p->k_cache, B * H, S, T, BN, D) && make_map(enc, &tmV, p->v_cache, B * H, S, T, BN, D);
+        ok = ok && make_map(enc, &tmK, p->k_cache, B * Hkv, S, T, BN, D) && make_map(enc, &tmV, p->v_cache, B * Hkv, S, T, BN, D);
     } else {
-        ok = ok && make_map(enc, &tmK, a.kh, B * H, S, S, BN, D) && make_map(enc, &tmV, a.vh, B * H, S, S, BN, D);
+        ok = ok && make_map(enc, &tmK, a.kh, B * Hkv, S, S, BN, D) && make_map(enc, &tmV, a.vh, B * Hkv, S, S, BN, D);
     }
     // the caller's v as a [batch][head][token][128] view of its [B,S,H,d] rows, for the V tiles taken from it directly
     CUtensorMap tmVin = tmV;
     if (ok && a.v_direct) {
-        const cuuint64_t dims[5] = {64, (cuuint64_t)S, (cuuint64_t)(D / 64), (cuuint64_t)H, (cuuint64_t)B};
-        const cuuint64_t strides[4] = {(cuuint64_t)a.row_stride * 2, 128, (cuuint64_t)D * 2, (cuuint64_t)S * a.row_stride * 2};
+        const cuuint64_t dims[5] = {64, (cuuint64_t)S, (cuuint64_t)(D / 64), (cuuint64_t)Hkv, (cuuint64_t)B};
+        const cuuint64_t strides[4] = {(cuuint64_t)a.kv_row_stride * 2, 128, (cuuint64_t)D * 2, (cuuint64_t)S * a.kv_row_stride * 2};
         const cuuint32_t box[5] = {64, (cuuint32_t)BN, (cuuint32_t)(D / 64), 1, 1};
         const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
         ok = enc(&tmVin, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, const_cast<void *>(a.v), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -1050,16 +1200,17 @@ template <int D> int launch_prefill_hd(const flb_attn_params *p, cudaStream_t st
     constexpr int pro_rows = (256 / (D / 8)) * kRowsPerThread; // token rows per block of the streaming pass
     const size_t pro_blocks = (size_t)B * H * ((S + pro_rows - 1) / pro_rows);
     cfg.numAttrs = 0; // the prologue is launched the ordinary way (measured: starting it early costs 25 us)
-    cfg.gridDim = dim3((unsigned)pro_blocks);
+    const size_t range_blocks = bounded ? ((size_t)B * ((S + 2 * BM - 1) / (2 * BM) * 2) + 7) / 8 : 0;
+    cfg.gridDim = dim3((unsigned)(pro_blocks + range_blocks));
     cfg.blockDim = dim3(256);
     cfg.dynamicSmemBytes = 0;
     cudaError_t le;
     if (a.input_mode == 0)
-        le = cudaLaunchKernelEx(&cfg, flb_prefill_prologue_kernel<0, D>, a);
+        le = cudaLaunchKernelEx(&cfg, scored ? flb_prefill_prologue_kernel<0, D, true> : flb_prefill_prologue_kernel<0, D, false>, a);
     else if (a.input_mode == 1)
-        le = cudaLaunchKernelEx(&cfg, flb_prefill_prologue_kernel<1, D>, a);
+        le = cudaLaunchKernelEx(&cfg, scored ? flb_prefill_prologue_kernel<1, D, true> : flb_prefill_prologue_kernel<1, D, false>, a);
     else
-        le = cudaLaunchKernelEx(&cfg, flb_prefill_prologue_kernel<2, D>, a);
+        le = cudaLaunchKernelEx(&cfg, scored ? flb_prefill_prologue_kernel<2, D, true> : flb_prefill_prologue_kernel<2, D, false>, a);
     if (le != cudaSuccess) return FLB_ERR_LAUNCH;
 
     // The attention kernel is launched with programmatic stream serialisation: its CTAs set themselves up
@@ -1070,8 +1221,7 @@ template <int D> int launch_prefill_hd(const flb_attn_params *p, cudaStream_t st
     pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     pdl[0].val.programmaticStreamSerializationAllowed = 1;
     const bool generic_mask = (a.mask_mode == FLB_MASK_GENERIC);
-    auto kern = generic_mask ? (a.out_f16 ? flb_prefill_attn_kernel<kExpOnFmaEvery, true, true, D> : flb_prefill_attn_kernel<kExpOnFmaEvery, true, false, D>)
-                             : (a.out_f16 ? flb_prefill_attn_kernel<kExpOnFmaEvery, false, true, D> : flb_prefill_attn_kernel<kExpOnFmaEvery, false, false, D>);
+    auto kern = scored ? attn_kernel_of<D, true>(generic_mask, a.out_f16) : attn_kernel_of<D, false>(generic_mask, a.out_f16);
     constexpr size_t smem_bytes = prefill_smem(D);
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes) != cudaSuccess) return FLB_ERR_LAUNCH;
     const long long num_items = (long long)B * H * ((S + 2 * BM - 1) / (2 * BM));
@@ -1091,9 +1241,9 @@ template <int D> int launch_prefill_hd(const flb_attn_params *p, cudaStream_t st
 
 } // namespace
 
-int launch_prefill(const flb_attn_params *p, cudaStream_t stream) {
-    if (p->size_per_head == 128) return launch_prefill_hd<128>(p, stream);
-    if (p->size_per_head == 64) return launch_prefill_hd<64>(p, stream);
+int launch_prefill(const flb_attn_params *p, const flb_score_form *f, cudaStream_t stream) {
+    if (p->size_per_head == 128) return launch_prefill_hd<128>(p, f, stream);
+    if (p->size_per_head == 64) return launch_prefill_hd<64>(p, f, stream);
     return FLB_ERR_UNSUPPORTED;
 }
 

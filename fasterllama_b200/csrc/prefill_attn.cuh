@@ -14,8 +14,14 @@ inline size_t prefill_scratch_bytes(int B, int H, int S, int d) {
     return 256 + 3 * ((one + 255) / 256 * 256);
 }
 
-// Launches prologue + attention on `stream`; returns a flb_status.
-int launch_prefill(const flb_attn_params *p, cudaStream_t stream);
+// With key_begin or key_end the key range of every 128-row query tile follows, behind the staging copies.
+inline size_t prefill_scored_scratch_bytes(int B, int H, int S, int d, const flb_score_form *f) {
+    const size_t tiles = f && (f->key_begin || f->key_end) ? (size_t)B * ((S + 255) / 256 * 2) : 0;
+    return prefill_scratch_bytes(B, H, S, d) + (tiles * 2 * sizeof(int) + 255) / 256 * 256;
+}
+
+// Launches prologue + attention on `stream`; returns a flb_status.  f: score form, or NULL.
+int launch_prefill(const flb_attn_params *p, const flb_score_form *f, cudaStream_t stream);
 
 // The reference's attention-output quantisation + transpose on a [B,H,S,d] fp32 tensor, d = 64 or 128 (one block per token row).
 int launch_quantize(const float *attn, int8_t *q8, float *scale, int B, int H, int S, int d, cudaStream_t stream);

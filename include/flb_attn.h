@@ -230,6 +230,27 @@ typedef struct flb_peer_exchange {
 
 #define FLB_STATUS_PEER_WAIT 0x100u
 
+/* ---- score forms ------------------------------------------------------------------- */
+/* How a score becomes a weight, beyond the scale and the mask of flb_attn_params, and K/V heads shared by several q
+ * heads; for the _scored calls below.  All zero = the plain call.  No counterpart in the reference.
+ *   x = softmax_scale * q.k;  softcap > 0: x = softcap * tanh(x / softcap);
+ *   slope: x -= alibi_slopes[h] * |query position - key position|  (row numbers of the cache);
+ * then the mask of flb_attn_params is added.  A key is seen only if the mask mode lets it and key_begin <= key < key_end of its
+ * query row: documents packed into one prompt (key_begin = first token of the row's document), windows
+ * (key_begin = row - width + 1), a prefix that every row sees (mask mode NONE and key_end = max(row + 1, prefix)), prompts padded on the
+ * right (key_end = 0 behind the prompt).  Bounds outside 0..S (a decode call: 0..past) act like the nearest one.  A row
+ * that sees no key returns zeros.  Values of k and v have to be finite in all rows of a prefill call, unseen ones included (a
+ * masked key has weight 0, and 0 times infinity is NaN); rows that a decode call does not see are not read into its result. */
+typedef struct flb_score_form {
+    int kv_head_num;           /* Hkv: k, v are [B,S,Hkv,d] and the caches [B,Hkv,T,d]; q head h reads K/V head
+                                  h / (head_num / Hkv).  0 = head_num                              */
+    int kv_row_stride;         /* elements between two tokens' rows of k and v; 0 = qkv_row_stride if that is set, else Hkv * d */
+    float softcap;             /* 0 = none                                                         */
+    const float *alibi_slopes; /* device [head_num] or NULL                                        */
+    const int *key_begin;      /* device int, decode [B], prefill [B,S]; NULL = 0                  */
+    const int *key_end;        /* device int, prefill [B,S]; NULL = S.  A decode call takes none   */
+} flb_score_form;
+
 /* ---- entry points --------------------------------------------------------------- */
 
 /* ABI version of the loaded library (== FLB_ATTN_ABI_VERSION it was built with). */
@@ -310,6 +331,15 @@ int flb_attn_static_scratch_status(unsigned *status_out, void *cuda_stream);
  * for callers that assemble the [B,H,S,d] tensor themselves, e.g. after an all-gather.  d is 64 or 128. */
 int flb_attn_quantize(const float *attn, int8_t *q8, float *scale, int batch_size, int head_num, int seq_len,
                       int size_per_head, void *cuda_stream);
+
+/* flb_attn_validate / _workspace_bytes / _decode / _prefill / _forward with a score form (NULL = none).  A prefill call needs a
+ * little more scratch than the plain one: flb_attn_scored_workspace_bytes().  Everything else of flb_attn_params keeps its meaning,
+ * early_start included (the form's arrays have to be final when the cache rows have to). */
+int flb_attn_validate_scored(const flb_attn_params *p, const flb_score_form *f);
+int flb_attn_scored_workspace_bytes(const flb_attn_params *p, const flb_score_form *f, size_t *bytes_out);
+int flb_attn_decode_scored(const flb_attn_params *p, const flb_score_form *f, void *cuda_stream);
+int flb_attn_prefill_scored(const flb_attn_params *p, const flb_score_form *f, void *cuda_stream);
+int flb_attn_forward_scored(const flb_attn_params *p, const flb_score_form *f, void *cuda_stream);
 
 /* Signal + bounded wait + copy described at flb_peer_exchange.  One small kernel; no host
  * synchronisation.  No counterpart in the reference. */
