@@ -3,8 +3,9 @@
 // For one K/V head and its G q heads:  x_r = c q.(code_r scale_r),  out = sum_r p_r code_r scale_r / sum_r p_r.
 // HBM-bound: 2 d bytes per cached row and K/V head, read once for all G heads.
 //   * grid = K/V heads x splits of `split_len` rows; four warps per CTA, warp w takes the 16-row steps w, w + 4, ... of its
-//     split.  Codes go from global memory straight into registers in the order the matrix instructions want them (every
-//     byte is used by one lane only, so shared memory would add nothing), one step ahead of their use.
+//     split.  Every warp copies its own steps (cp.async, 16 bytes a lane) into a ring of its own in shared memory, three and more
+//     steps ahead: 192 KB per SM under way, no barrier between warps.  The first copies leave before q is looked at.
+//     16-byte chunks are permuted within the rows so that both products' fragment loads are free of bank conflicts.
 //   * both products run on the warp-level matrix instructions with exact operands: a code is a whole number below 2^11 (or
 //     an e4m3 value) and fits fp16 as it is.  The 8-bit -> fp16 conversion (1.25 to 1.5 instructions per code) is
 //     then all the arithmetic per cached byte.  q and the weights p are split into a high and a low fp16 part in
@@ -23,6 +24,8 @@
 #include "kv8.cuh"
 
 #include "flb_ptx.cuh"
+
+#include <atomic>
 
 namespace flb {
 
@@ -61,24 +64,56 @@ template <int CODE> __device__ __forceinline__ void codes_to_halves(uint32_t w, 
     }
 }
 
-template <int BYTES> struct Raw {
-    uint32_t w[BYTES / 4];
+// ---- a warp's ring: one slot holds 16 rows of K codes, then 16 rows of V codes
+template <int D> struct Ring {
+    static constexpr int kRowsBytes = kStep * D;
+    static constexpr int kSlot = 2 * kRowsBytes;
+    static constexpr int kStages = D == 64 ? 4 : 2; // 12 KB per warp (d = 256: 24 KB)
+    static constexpr int kWarpBytes = kStages * kSlot;
+    // Where chunk c (16 bytes) of row r lies.  K is read as rows r, r + 1 x four neighbouring chunks per eight lanes, V as rows r, r + 2, r + 4,
+    // r + 6 x two neighbouring chunks: the permutations send both to eight different chunks of the 128-byte bank line.
+    static __device__ __forceinline__ int at(int r, int c) {
+        if (D == 64) return (r >> 1) * 128 + ((((r >> 1) ^ r) & 1) << 6) + ((c ^ ((r >> 1) & 2)) << 4);
+        return r * D + ((c ^ ((r & 6) ^ ((r & 1) << 2))) << 4);
+    }
 };
-// BYTES (8, 16 or 32) consecutive bytes; streamed once
-template <int BYTES> __device__ __forceinline__ void load_raw(Raw<BYTES> &r, const uint8_t *p) {
-    if (BYTES == 8) {
-        const uint2 u = __ldcs(reinterpret_cast<const uint2 *>(p));
-        r.w[0] = u.x;
-        r.w[1] = u.y;
-    } else {
+__device__ __forceinline__ void copy16(uint32_t dst, const uint8_t *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// 16 rows from `k` and `v` into a slot
+template <int D> __device__ __forceinline__ void copy_step(uint32_t slot, const uint8_t *k, const uint8_t *v, int lane) {
+    constexpr int CPR = D / 16, PER = kStep * CPR / 32;
 #pragma unroll
-        for (int i = 0; i < BYTES / 16; ++i) {
-            const uint4 u = __ldcs(reinterpret_cast<const uint4 *>(p) + i);
-            r.w[4 * i] = u.x;
-            r.w[4 * i + 1] = u.y;
-            r.w[4 * i + 2] = u.z;
-            r.w[4 * i + 3] = u.w;
-        }
+    for (int i = 0; i < PER; ++i) {
+        const int id = lane + 32 * i, r = id / CPR, c = id % CPR;
+        const int to = Ring<D>::at(r, c);
+        copy16(slot + to, k + id * 16);
+        copy16(slot + Ring<D>::kRowsBytes + to, v + id * 16);
+    }
+}
+
+// cap * tanh(x / cap): where no score of the warp passes the cap, a polynomial (own minimax fit of tanh(u) / u in u^2 on |u| <= 1, 2e-8
+// of tanh), else CUDA's tanhf, whose branches cost a warp four times as much.
+__device__ __forceinline__ void cap_scores(float (&x)[2], float cap, float inv_cap) {
+    float u[2] = {x[0] * inv_cap, x[1] * inv_cap};
+    if (__any_sync(0xffffffffu, !(fmaxf(fabsf(u[0]), fabsf(u[1])) <= 1.0f))) {
+        x[0] = cap * tanhf(u[0]);
+        x[1] = cap * tanhf(u[1]);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const float y = u[i] * u[i];
+        float p = fmaf(y, 0.0009637718f, -0.0059512793f);
+        p = fmaf(p, y, 0.019973271f);
+        p = fmaf(p, y, -0.053265836f);
+        p = fmaf(p, y, 0.13319583f);
+        p = fmaf(p, y, -0.3333213f);
+        p = fmaf(p, y, 0.9999997f);
+        x[i] = p * (u[i] * cap);
     }
 }
 
@@ -144,14 +179,15 @@ template <int D, int CODE, int NT, bool FORM>
 __global__ void __launch_bounds__(kWarps * 32) flb_kv8_decode_kernel(const __grid_constant__ Kv8DecodeArgs a) {
     constexpr int HEADS = 4 * NT;
     constexpr int KCH = D / 64;   // 16-byte chunks of a K row per lane
-    constexpr int VB = D / 8;     // bytes of a V row per lane
+    constexpr int VW = D / 32;    // 32-bit words of a V row per lane
     constexpr int MT = D / 16;    // output tiles of 16 dims
     constexpr int NTHREADS = kWarps * 32;
     __shared__ __align__(16) __half q_s[2 * HEADS][D];     // [2 head + part]
     __shared__ float q_unit[HEADS];                        // what a product with q_s is to be multiplied by
     __shared__ float sc_s[2][kMaxSplitScales];             // scales of the split's blocks
     __shared__ float w_m[kWarps][HEADS], w_l[kWarps][HEADS];
-    __shared__ __align__(16) float w_o[kWarps][HEADS][D];
+    extern __shared__ __align__(128) unsigned char ring_smem[];
+    float(*w_o)[HEADS][D] = reinterpret_cast<float(*)[HEADS][D]>(ring_smem); // the rings' room, once they are through
     __shared__ uint32_t red[32];
     __shared__ int last_flag;
 
@@ -182,7 +218,40 @@ __global__ void __launch_bounds__(kWarps * 32) flb_kv8_decode_kernel(const __gri
     const int prow = a.freq_cis ? kv8_table_row(pos, a.freq_rows, a.status) : 0;
     const int begin = (FORM && a.key_begin) ? __ldg(a.key_begin + b) : INT_MIN;
 
-    if (is_last && a.append) append_token<D, CODE>(a, unit, b, h, past, pos, prow, red);
+    // ---- the warp's steps: rows r, r + 64, ...
+    using R = Ring<D>;
+    constexpr int kStride = kWarps * kStep;
+    int r = row0 + warp * kStep;
+    // rows in position order: nothing below key_begin is read
+    if (FORM && a.key_begin && !a.c.row_pos && begin > r) r += (int)(((long long)min(begin, a.c.T) - r) / kStride) * kStride;
+    const uint32_t ring = smem_u32(ring_smem) + (uint32_t)(warp * R::kWarpBytes);
+    const uint8_t *ksrc = a.c.codes[0] + (unit * a.c.T + r) * (size_t)D, *vsrc = a.c.codes[1] + (unit * a.c.T + r) * (size_t)D;
+    int fetch = r, fslot = 0; // next step to copy, and its slot
+    auto copy_next = [&](int end) {
+        if (fetch < end) {
+            copy_step<D>(ring + fslot * R::kSlot, ksrc, vsrc, lane);
+            ksrc += (size_t)kStride * D;
+            vsrc += (size_t)kStride * D;
+            fetch += kStride;
+            fslot = fslot + 1 == R::kStages ? 0 : fslot + 1;
+        }
+    };
+    // Everything but the block that the new token goes into can be on its way at once.
+    const bool storing = is_last && a.append;
+    const int settled = storing ? min(row1, past >> a.c.block_shift << a.c.block_shift) : row1;
+    int groups = 0;
+#pragma unroll
+    for (int i = 0; i < R::kStages; ++i)
+        if (fetch < settled) {
+            copy_next(settled);
+            copy_commit();
+            ++groups;
+        }
+    if (storing) append_token<D, CODE>(a, unit, b, h, past, pos, prow, red);
+    for (; groups < R::kStages; ++groups) { // a group per stage, empty where there is no step
+        copy_next(row1);
+        copy_commit();
+    }
 
     // ---- q: rotated, brought to [2^8, 2^9) by a power of two, split into two fp16 parts; one warp per head
     for (int hh = warp; hh < HEADS; hh += kWarps) {
@@ -257,53 +326,32 @@ __global__ void __launch_bounds__(kWarps * 32) flb_kv8_decode_kernel(const __gri
     const float inv_cap = (FORM && a.cap_log2e > 0.f) ? 1.0f / a.cap_log2e : 0.f;
 
     // ---- the pass over the rows
-    int r = row0 + warp * kStep;
-    // rows in position order: nothing below key_begin is read
-    if (FORM && a.key_begin && !a.c.row_pos && begin > r) {
-        const int skip = (int)(((long long)min(begin, a.c.T) - r) / (kWarps * kStep));
-        r += skip * (kWarps * kStep);
-    }
-    const uint8_t *kp = a.c.codes[0] + (unit * a.c.T + r + g) * (size_t)D + 16 * t;
-    const uint8_t *vp = a.c.codes[1] + (unit * a.c.T + r + 2 * t) * (size_t)D + g * VB;
-    Raw<16> kr[2][KCH];
-    Raw<VB> vr[4];
-    auto load_k = [&]() {
-#pragma unroll
-        for (int c = 0; c < KCH; ++c) {
-            load_raw<16>(kr[0][c], kp + c * 64);
-            load_raw<16>(kr[1][c], kp + 8 * D + c * 64);
-        }
-        kp += (size_t)kWarps * kStep * D;
-    };
-    auto load_v = [&]() {
-        load_raw<VB>(vr[0], vp);
-        load_raw<VB>(vr[1], vp + D);
-        load_raw<VB>(vr[2], vp + 8 * D);
-        load_raw<VB>(vr[3], vp + 9 * D);
-        vp += (size_t)kWarps * kStep * D;
-    };
-    if (r < row1) {
-        load_k();
-        load_v();
-    }
-    for (; r < row1; r += kWarps * kStep) {
-        const bool more = r + kWarps * kStep < row1;
+    // This lane's reads of a slot: K rows g, g + 8 (the rows of a step's tile are dealt out so that eight lanes meet eight chunks), V rows
+    // 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+    int slot = 0;
+    for (; r < row1; r += kStride) {
+        copy_wait<R::kStages - 1>();
+        __syncwarp();
+        const unsigned char *ks_p = ring_smem + warp * R::kWarpBytes + slot * R::kSlot, *vs_p = ks_p + R::kRowsBytes;
         float s[NT][4];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
 #pragma unroll
-        for (int c = 0; c < KCH; ++c)
+        for (int c = 0; c < KCH; ++c) {
+            const uint4 k0 = *reinterpret_cast<const uint4 *>(ks_p + R::at(g, 4 * c + t));
+            const uint4 k1 = *reinterpret_cast<const uint4 *>(ks_p + R::at(g + 8, 4 * c + t));
+            const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
                 uint32_t f[4];
-                codes_to_halves<CODE>(kr[0][c].w[w], f[0], f[2]);
-                codes_to_halves<CODE>(kr[1][c].w[w], f[1], f[3]);
+                codes_to_halves<CODE>(w0[w], f[0], f[2]);
+                codes_to_halves<CODE>(w1[w], f[1], f[3]);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) mma16816(s[n], f, qf[n][4 * c + w][0], qf[n][4 * c + w][1]);
             }
-        if (more) load_k();
+        }
 
         const int sb = (r - row0) >> a.c.block_shift;
         const float ks = sc_s[0][sb], vs = sc_s[1][sb] * v_up;
@@ -321,10 +369,10 @@ __global__ void __launch_bounds__(kWarps * 32) flb_kv8_decode_kernel(const __gri
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             float x[2] = {(s[n][0] + s[n][1]) * (ks * qu[n]), (s[n][2] + s[n][3]) * (ks * qu[n])};
+            if (FORM && a.cap_log2e > 0.f) cap_scores(x, a.cap_log2e, inv_cap);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 if (FORM) {
-                    if (a.cap_log2e > 0.f) x[i] = a.cap_log2e * tanhf(x[i] * inv_cap);
                     x[i] = fmaf(-slope[n], fabsf((float)(pos - kpos[i])), x[i]);
                 }
                 x[i] = vis[i] ? x[i] : -INFINITY;
@@ -358,18 +406,33 @@ __global__ void __launch_bounds__(kWarps * 32) flb_kv8_decode_kernel(const __gri
                 pb[n][i] = transpose8x8(h2_bits(__halves2half2(hi, lo)));
             }
         }
-        if (CODE == kCodeE4M3 && r + kStep > row1) { // codes behind the sequence may be NaN patterns
+        uint32_t v[4][VW];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (r + 2 * t + (i & 1) + (i >> 1) * 8 >= row1)
+        for (int i = 0; i < 4; ++i) {
+            const int vr = 2 * t + (i & 1) + (i >> 1) * 8;
+            if (D == 64) {
+                const uint2 u = *reinterpret_cast<const uint2 *>(vs_p + R::at(vr, g >> 1) + (g & 1) * 8);
+                v[i][0] = u.x;
+                v[i][1] = u.y;
+            } else {
 #pragma unroll
-                    for (int w = 0; w < VB / 4; ++w) vr[i].w[w] = 0u;
+                for (int j = 0; j < VW / 4; ++j) { // dims 16 g .. (d = 256: and 128 + 16 g ..)
+                    const uint4 u = *reinterpret_cast<const uint4 *>(vs_p + R::at(vr, g + 8 * j));
+                    v[i][4 * j] = u.x;
+                    v[i][4 * j + 1] = u.y;
+                    v[i][4 * j + 2] = u.z;
+                    v[i][4 * j + 3] = u.w;
+                }
+            }
+            if (CODE == kCodeE4M3 && r + vr >= row1) // codes behind the sequence may be NaN patterns
+#pragma unroll
+                for (int w = 0; w < VW; ++w) v[i][w] = 0u;
         }
 #pragma unroll
-        for (int w = 0; w < VB / 4; ++w) { // four dims: two output tiles
+        for (int w = 0; w < VW; ++w) { // four dims: two output tiles
             uint32_t f0[4], f1[4];
-            const uint32_t e0 = __byte_perm(vr[0].w[w], vr[1].w[w], 0x5140), e1 = __byte_perm(vr[0].w[w], vr[1].w[w], 0x7362);
-            const uint32_t e2 = __byte_perm(vr[2].w[w], vr[3].w[w], 0x5140), e3 = __byte_perm(vr[2].w[w], vr[3].w[w], 0x7362);
+            const uint32_t e0 = __byte_perm(v[0][w], v[1][w], 0x5140), e1 = __byte_perm(v[0][w], v[1][w], 0x7362);
+            const uint32_t e2 = __byte_perm(v[2][w], v[3][w], 0x5140), e3 = __byte_perm(v[2][w], v[3][w], 0x7362);
             codes_to_halves<CODE>(e0, f0[0], f0[1]);
             codes_to_halves<CODE>(e2, f0[2], f0[3]);
             codes_to_halves<CODE>(e1, f1[0], f1[1]);
@@ -380,8 +443,13 @@ __global__ void __launch_bounds__(kWarps * 32) flb_kv8_decode_kernel(const __gri
                 mma16816(o[n][2 * w + 1], f1, pb[n][0], pb[n][1]);
             }
         }
-        if (more) load_v();
+        __syncwarp(); // the slot has been read
+        copy_next(row1);
+        copy_commit();
+        slot = slot + 1 == R::kStages ? 0 : slot + 1;
     }
+    copy_wait<0>();
+    __syncthreads(); // the rings' room is free
 
     // ---- warps to shared memory: sums over the eight row groups, high and low parts together
 #pragma unroll
@@ -394,7 +462,7 @@ __global__ void __launch_bounds__(kWarps * 32) flb_kv8_decode_kernel(const __gri
         }
 #pragma unroll
         for (int i = 0; i < MT; ++i)
-            *reinterpret_cast<float2 *>(&w_o[warp][4 * n + t][g * (D / 8) + 2 * i]) =
+            *reinterpret_cast<float2 *>(&w_o[warp][4 * n + t][(i >> 3) * 128 + g * (D == 64 ? 8 : 16) + 2 * (i & 7)]) =
                 make_float2((o[n][i][0] + o[n][i][1]) * v_down, (o[n][i][2] + o[n][i][3]) * v_down);
     }
     __syncthreads();
@@ -438,23 +506,81 @@ __global__ void __launch_bounds__(kWarps * 32) flb_kv8_decode_kernel(const __gri
     __syncthreads();
     if (!last_flag) return;
     __threadfence();
+    // The last split joins all: maximum and sum per head by a warp, then every thread four columns of one head over its share of the
+    // splits, eight loads under way, weights of 64 splits at a time in shared memory; the shares are added up in order.
     const size_t mbase = (unit * a.nchunk + chunk) * a.nsplit_max;
-    for (int i = tid; i < nheads * D; i += NTHREADS) {
-        const int hh = i / D, col = i - hh * D;
-        float M = kNoMax, acc = 0.f, l = 0.f;
-        for (int s = 0; s < nsplit; ++s) M = fmaxf(M, __ldcg(a.part_ml + ((mbase + s) * HEADS + hh) * 2));
-        for (int s = 0; s < nsplit; ++s) {
-            const size_t p = (mbase + s) * HEADS + hh;
-            const float e = ex2(__ldcg(a.part_ml + p * 2) - M);
-            acc = fmaf(__ldcg(a.part_o + p * D + col), e, acc);
-            l = fmaf(__ldcg(a.part_ml + p * 2 + 1), e, l);
+    float *const e_s = reinterpret_cast<float *>(ring_smem) + NTHREADS * 4; // [64][HEADS] behind the shares
+    for (int hh = warp; hh < nheads; hh += kWarps) {
+        const float2 *ml = reinterpret_cast<const float2 *>(a.part_ml) + mbase * HEADS + hh;
+        float M = kNoMax, l = 0.f;
+        for (int s = lane; s < nsplit; s += 32) M = fmaxf(M, __ldcg(ml + (size_t)s * HEADS).x);
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+        for (int s = lane; s < nsplit; s += 32) {
+            const float2 v = __ldcg(ml + (size_t)s * HEADS);
+            l = fmaf(v.y, ex2(v.x - M), l);
         }
-        const size_t oo = ((size_t)b * a.Hq + head0 + hh) * D + col;
-        const float y = (l > 0.f || l != l) ? acc / l : 0.f;
-        if (a.out_f16) ((__half *)a.out)[oo] = __float2half_rn(y); else ((float *)a.out)[oo] = y;
-        if (a.ml && col == 0) {
-            a.ml[((size_t)b * a.Hq + head0 + hh) * 2] = M;
-            a.ml[((size_t)b * a.Hq + head0 + hh) * 2 + 1] = l;
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+        if (lane == 0) {
+            w_m[0][hh] = M;
+            w_l[0][hh] = l;
+        }
+    }
+    __syncthreads();
+    const int quads = nheads * (D / 4), shares = max(1, NTHREADS / quads);
+    for (int q0 = 0; q0 < quads; q0 += NTHREADS) {
+        const int quad = shares > 1 ? tid % quads : q0 + tid, share = shares > 1 ? tid / quads : 0;
+        const bool on = quad < quads && share < shares;
+        const int hh = on ? quad / (D / 4) : 0;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        const float4 *po = reinterpret_cast<const float4 *>(a.part_o) + mbase * HEADS * (D / 4) + quad;
+        for (int s0 = 0; s0 < nsplit; s0 += 64) {
+            const int ns = min(64, nsplit - s0);
+            __syncthreads();
+            for (int i = tid; i < ns * nheads; i += NTHREADS) {
+                const int s = i / nheads, hd = i - s * nheads;
+                e_s[s * HEADS + hd] = ex2(__ldcg(a.part_ml + ((mbase + s0 + s) * HEADS + hd) * 2) - w_m[0][hd]);
+            }
+            __syncthreads();
+            if (!on) continue;
+#pragma unroll 8
+            for (int s = share; s < ns; s += shares) {
+                const float4 v = __ldcg(po + (size_t)(s0 + s) * HEADS * (D / 4));
+                const float e = e_s[s * HEADS + hh];
+                acc.x = fmaf(v.x, e, acc.x);
+                acc.y = fmaf(v.y, e, acc.y);
+                acc.z = fmaf(v.z, e, acc.z);
+                acc.w = fmaf(v.w, e, acc.w);
+            }
+        }
+        if (shares > 1) {
+            float4 *sum = reinterpret_cast<float4 *>(ring_smem);
+            sum[tid] = acc;
+            __syncthreads();
+            if (on && share == 0)
+                for (int j = 1; j < shares; ++j) {
+                    const float4 v = sum[j * quads + quad];
+                    acc.x += v.x;
+                    acc.y += v.y;
+                    acc.z += v.z;
+                    acc.w += v.w;
+                }
+        }
+        if (on && share == 0) {
+            const float l = w_l[0][hh];
+            const float y[4] = {acc.x / l, acc.y / l, acc.z / l, acc.w / l};
+            const bool some = l > 0.f || l != l;
+            const size_t oo = ((size_t)b * a.Hq + head0 + hh) * D + (quad - hh * (D / 4)) * 4;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float r4 = some ? y[e] : 0.f;
+                if (a.out_f16) ((__half *)a.out)[oo + e] = __float2half_rn(r4); else ((float *)a.out)[oo + e] = r4;
+            }
+            if (a.ml && quad == hh * (D / 4)) {
+                a.ml[((size_t)b * a.Hq + head0 + hh) * 2] = w_m[0][hh];
+                a.ml[((size_t)b * a.Hq + head0 + hh) * 2 + 1] = l;
+            }
         }
     }
     if (tid == 0) a.counters[unit * a.nchunk + chunk] = 0u; // ready for the next call
@@ -482,11 +608,22 @@ __global__ void __launch_bounds__(256) flb_kv8_weights_kernel(const __grid_const
 template <int D, int CODE, int NT> cudaError_t launch_t(const Kv8DecodeArgs &a, cudaStream_t stream) {
     const unsigned grid = (unsigned)a.c.B * (unsigned)a.c.H * (unsigned)a.nchunk * (unsigned)a.nsplit_max;
     const bool form = a.cap_log2e > 0.f || a.slopes || a.key_begin;
-    if (form)
-        flb_kv8_decode_kernel<D, CODE, NT, true><<<grid, kWarps * 32, 0, stream>>>(a);
-    else
-        flb_kv8_decode_kernel<D, CODE, NT, false><<<grid, kWarps * 32, 0, stream>>>(a);
-    cudaError_t e = cudaGetLastError();
+    constexpr int smem = kWarps * Ring<D>::kWarpBytes;
+    static_assert(smem >= kWarps * 4 * NT * D * (int)sizeof(float), "the warps' results take the rings' room");
+    auto kern = form ? flb_kv8_decode_kernel<D, CODE, NT, true> : flb_kv8_decode_kernel<D, CODE, NT, false>;
+    // the shared-memory opt-in is a property of (kernel, device): set once per device
+    static std::atomic<unsigned long long> opted_in[2] = {{0}, {0}};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const unsigned long long bit = (dev >= 0 && dev < 64) ? (1ull << dev) : 0ull;
+    if (!(opted_in[form].load(std::memory_order_acquire) & bit)) {
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return e;
+        if (bit) opted_in[form].fetch_or(bit, std::memory_order_release);
+    }
+    kern<<<grid, kWarps * 32, smem, stream>>>(a);
+    e = cudaGetLastError();
     if (e != cudaSuccess || !a.weight_out) return e;
     const int rows = min(a.c.T, a.nsplit_max * a.split_len), bpu = (rows + 255) / 256;
     flb_kv8_weights_kernel<<<(unsigned)a.c.B * (unsigned)a.c.H * (unsigned)bpu, 256, 0, stream>>>(a, bpu);
