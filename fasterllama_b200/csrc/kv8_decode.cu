@@ -6,12 +6,13 @@
 //     split.  Every warp copies its own steps (cp.async, 16 bytes a lane) into a ring of its own in shared memory, three and more
 //     steps ahead: 192 KB per SM under way, no barrier between warps.  The first copies leave before q is looked at.
 //     16-byte chunks are permuted within the rows so that both products' fragment loads are free of bank conflicts.
-//   * both products run on the warp-level matrix instructions with exact operands: a code is a whole number below 2^11 (or
-//     an e4m3 value) and fits fp16 as it is.  The 8-bit -> fp16 conversion (1.25 to 1.5 instructions per code) is
-//     then all the arithmetic per cached byte.  q and the weights p are split into a high and a low fp16 part in
-//     neighbouring columns, which carries 22 bits of them through: the columns are there anyway (N = 8 holds four heads).
-//     S = K q:       A = 16 rows of codes, B = q parts;   lane (g, t) ends with rows g, g + 8 of head t
-//     O^T += V^T p:  A = codes of 16 dims x 16 rows (two rows' bytes interleaved), B = p parts, an 8x8 transpose away from S
+//   * both products run on the warp-level matrix instructions with exact operands, the columns being parts of q or p:
+//     S = K q, int8:  A = 16 rows of codes as they are, B = q as a 28-bit whole number in four base-128 digits (two tiles of four
+//                     heads); the int32 sums are exact, no code is converted
+//     S = K q, e4m3:  A = codes as fp16 (exact), B = q in a high and a low fp16 part, 22 bits
+//     O^T += V^T p:   A = codes of 16 dims x 16 rows as fp16 (two rows' bytes interleaved; 1.5 instructions per code), B = p in two
+//                     fp16 parts, an 8x8 transpose away from S.  Floating parts keep small weights exact too, digits would not.
+//     Lane (g, t) ends with rows g, g + 8 of head t, both parts in its own registers.
 //   * scales of a block are uniform over a step (blocks hold at least 16 rows): K's goes into the score, V's into p.
 //   * each warp keeps its own running maximum per head, raised only when a score passes it by 2^8 (exact: sum and result
 //     share the reference); warps merge in warp order, splits in split order by the CTA that arrives last.  The
@@ -36,11 +37,15 @@ constexpr float kNoMax = -1e30f;   // running maximum before the first visible k
 constexpr float kRaise = 8.0f;     // log2: a weight stays below 2^8
 constexpr int kWarps = 4;
 constexpr int kStep = 16;          // rows per warp step
-constexpr int kMaxSplitScales = 8192 / 16;
 
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16832(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
@@ -127,51 +132,36 @@ __device__ __forceinline__ void load8(const Kv8DecodeArgs &a, int which, size_t 
         kv8_load8<2>(a.in[which], a.act_scale, token, col, x);
 }
 
-// The new token's k and v of one K/V head into its block, by the CTA's first D / 8 (k) and next D / 8 (v) threads per row; the
-// block's held codes follow a scale that grew.  All threads call it; ends with a barrier.
+// What the new token does to its block, K and V: the block's scale from now on, and what the codes it held are to be multiplied by.
+struct TokenScales {
+    float scale[2], ratio[2];
+    int grown[2];
+};
+// Stores k (kv = 0) or v of the new token, by one warp; lane i has eight dims.
 template <int D, int CODE>
-__device__ __forceinline__ void append_token(const Kv8DecodeArgs &a, size_t unit, int b, int h, int past, int pos, int prow, uint32_t *red2) {
-    constexpr int CPR = D / 8;
-    const int blk = past >> a.c.block_shift, row0 = blk << a.c.block_shift;
-    const bool fresh = row0 == past;
-    const int tid = threadIdx.x;
-    const int kv = tid / CPR, ch = tid % CPR;
+__device__ __forceinline__ void append_token(const Kv8DecodeArgs &a, int kv, size_t unit, int b, int h, int past, int pos, int prow, TokenScales *ts) {
+    const int lane = threadIdx.x & 31, blk = past >> a.c.block_shift;
+    const size_t sidx = unit * a.c.nblk + blk;
+    const float old = (blk << a.c.block_shift) == past ? 0.f : a.c.scale[kv][sidx];
     float x[8];
     uint32_t amax = 0;
-    if (tid < 2) red2[tid] = 0u;
-    __syncthreads();
-    if (kv < 2) {
-        load8(a, 1 + kv, (size_t)b, h * D + ch * 8, x);
-        if (kv == 0 && a.freq_cis) kv8_rotate8(a.freq_cis + (size_t)prow * D + ch * 8, x);
+    if (lane < D / 8) {
+        load8(a, 1 + kv, (size_t)b, h * D + lane * 8, x);
+        if (kv == 0 && a.freq_cis) kv8_rotate8(a.freq_cis + (size_t)prow * D + lane * 8, x);
 #pragma unroll
         for (int e = 0; e < 8; ++e) amax = max(amax, kv8_abs_bits(x[e]));
-        atomicMax(red2 + kv, amax);
     }
-    __syncthreads();
-    const size_t sidx = unit * a.c.nblk + blk;
-    float scale[2], ratio[2];
-    bool grown[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const float old = fresh ? 0.f : a.c.scale[i][sidx];
-        scale[i] = kv8_new_scale<CODE>(red2[i], old);
-        grown[i] = old > 0.f && scale[i] > old;
-        ratio[i] = grown[i] ? __fdiv_rn(old, scale[i]) : 1.f;
+    amax = __reduce_max_sync(0xffffffffu, amax);
+    const float scale = kv8_new_scale<CODE>(amax, old);
+    if (lane < D / 8) *reinterpret_cast<uint2 *>(a.c.codes[kv] + (unit * a.c.T + past) * D + lane * 8) = kv8_encode8<CODE>(x, scale);
+    if (lane == 0) {
+        a.c.scale[kv][sidx] = scale;
+        if (kv == 0 && a.c.row_pos) a.c.row_pos[unit * a.c.T + past] = pos;
+        const bool grown = old > 0.f && scale > old;
+        ts->scale[kv] = scale;
+        ts->grown[kv] = grown;
+        ts->ratio[kv] = grown ? __fdiv_rn(old, scale) : 1.f;
     }
-    __syncthreads(); // every thread has read the old scales
-    if (tid == 0) {
-        a.c.scale[0][sidx] = scale[0];
-        a.c.scale[1][sidx] = scale[1];
-        if (a.c.row_pos) a.c.row_pos[unit * a.c.T + past] = pos;
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        uint2 *rows = reinterpret_cast<uint2 *>(a.c.codes[i] + (unit * a.c.T + row0) * D);
-        if (grown[i])
-            for (int c = tid; c < (past - row0) * CPR; c += blockDim.x) rows[c] = kv8_rescale8<CODE>(rows[c], ratio[i]);
-        if (kv == i) rows[(past - row0) * CPR + ch] = kv8_encode8<CODE>(x, scale[i]);
-    }
-    __syncthreads();
 }
 
 // FORM: capped scores, distance bias or key_begin.  NT: column tiles of eight = four q heads each.
@@ -182,13 +172,13 @@ __global__ void __launch_bounds__(kWarps * 32) flb_kv8_decode_kernel(const __gri
     constexpr int VW = D / 32;    // 32-bit words of a V row per lane
     constexpr int MT = D / 16;    // output tiles of 16 dims
     constexpr int NTHREADS = kWarps * 32;
-    __shared__ __align__(16) __half q_s[2 * HEADS][D];     // [2 head + part]
+    constexpr int QH = HEADS / kWarps; // q heads that a warp prepares
+    __shared__ __align__(16) unsigned char q_s[HEADS * D * 4]; // e4m3: fp16 [2 head + part][D]; int8: bytes [part][head][D]
     __shared__ float q_unit[HEADS];                        // what a product with q_s is to be multiplied by
-    __shared__ float sc_s[2][kMaxSplitScales];             // scales of the split's blocks
     __shared__ float w_m[kWarps][HEADS], w_l[kWarps][HEADS];
     extern __shared__ __align__(128) unsigned char ring_smem[];
     float(*w_o)[HEADS][D] = reinterpret_cast<float(*)[HEADS][D]>(ring_smem); // the rings' room, once they are through
-    __shared__ uint32_t red[32];
+    __shared__ TokenScales ts;
     __shared__ int last_flag;
 
     const int split = (int)(blockIdx.x % (unsigned)a.nsplit_max);
@@ -200,6 +190,15 @@ __global__ void __launch_bounds__(kWarps * 32) flb_kv8_decode_kernel(const __gri
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
 
     const int past = a.past_lens ? __ldg(a.past_lens + b) : a.start_pos;
+    const int pos = a.token_pos ? __ldg(a.token_pos + b) : past;
+    float qx[QH][8];
+    static_assert(D <= 256, "a warp holds a row, eight dims to a lane");
+#pragma unroll
+    for (int i = 0; i < QH; ++i) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) qx[i][e] = 0.f;
+        if (warp + i * kWarps < nheads && lane < D / 8) load8(a, 0, (size_t)b, (head0 + warp + i * kWarps) * D + lane * 8, qx[i]);
+    }
     if (past < 0 || past >= a.c.T || past >= a.nsplit_max * a.split_len) { // flagged, nothing stored, zeros returned
         if (split == 0) {
             if (tid == 0) atomicOr(a.status, kKv8BadLen);
@@ -214,7 +213,6 @@ __global__ void __launch_bounds__(kWarps * 32) flb_kv8_decode_kernel(const __gri
     if (split >= nsplit) return;
     const int row0 = split * a.split_len, row1 = min(row0 + a.split_len, past + 1);
     const bool is_last = split == nsplit - 1;
-    const int pos = a.token_pos ? __ldg(a.token_pos + b) : past;
     const int prow = a.freq_cis ? kv8_table_row(pos, a.freq_rows, a.status) : 0;
     const int begin = (FORM && a.key_begin) ? __ldg(a.key_begin + b) : INT_MIN;
 
@@ -247,69 +245,100 @@ __global__ void __launch_bounds__(kWarps * 32) flb_kv8_decode_kernel(const __gri
             copy_commit();
             ++groups;
         }
-    if (storing) append_token<D, CODE>(a, unit, b, h, past, pos, prow, red);
+    // scales of the warp's steps: lane i has those of step i
+    float sc_k = 0.f, sc_v = 0.f;
+    const int sblk = (r + lane * kStride) >> a.c.block_shift;
+    if (r + lane * kStride < settled) {
+        sc_k = __ldcg(a.c.scale[0] + unit * a.c.nblk + sblk);
+        sc_v = __ldcg(a.c.scale[1] + unit * a.c.nblk + sblk);
+    }
+    if (storing && warp >= 2) append_token<D, CODE>(a, warp - 2, unit, b, h, past, pos, prow, &ts);
+
+    // ---- q: rotated, brought to a fixed range by a power of two, cut into parts; one warp per head
+#pragma unroll
+    for (int i = 0; i < QH; ++i) {
+        const int hh = warp + i * kWarps;
+        uint32_t amax = 0;
+        if (hh < nheads && lane < D / 8 && a.freq_cis) kv8_rotate8(a.freq_cis + (size_t)prow * D + lane * 8, qx[i]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) amax = max(amax, kv8_abs_bits(qx[i][e]));
+        amax = __reduce_max_sync(0xffffffffu, amax);
+        // int8: |q| < 2^27 as a whole number in four signed base-128 digits; e4m3: |q| < 2^9 in two fp16 parts
+        constexpr int kTop = CODE == kCodeI8 ? 26 : 8;
+        const int ex = min(max((int)(amax >> 23) - 127, -100), 126);
+        const float up = __uint_as_float((uint32_t)(kTop - ex + 127) << 23), down = __uint_as_float((uint32_t)(ex - kTop + 127) << 23);
+        if (lane < D / 8) {
+            if (CODE == kCodeI8) {
+                uint32_t dig[4][2] = {};
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int v = __float2int_rn(qx[i][e] * up);
+                    const int sh = 8 * (e & 3);
+                    dig[0][e >> 2] |= (uint32_t)((v >> 21) & 0xff) << sh; // -64..64
+                    dig[1][e >> 2] |= (uint32_t)((v >> 14) & 0x7f) << sh;
+                    dig[2][e >> 2] |= (uint32_t)((v >> 7) & 0x7f) << sh;
+                    dig[3][e >> 2] |= (uint32_t)(v & 0x7f) << sh;
+                }
+#pragma unroll
+                for (int p = 0; p < 4; ++p) *reinterpret_cast<uint2 *>(q_s + (p * HEADS + hh) * D + lane * 8) = make_uint2(dig[p][0], dig[p][1]);
+            } else {
+                __half2 hi[4], lo[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float u = qx[i][2 * e] * up, v = qx[i][2 * e + 1] * up;
+                    hi[e] = __floats2half2_rn(u, v);
+                    const float2 f = __half22float2(hi[e]);
+                    lo[e] = __floats2half2_rn(u - f.x, v - f.y);
+                }
+                *reinterpret_cast<uint4 *>(q_s + (2 * hh * D + lane * 8) * 2) = *reinterpret_cast<uint4 *>(hi);
+                *reinterpret_cast<uint4 *>(q_s + ((2 * hh + 1) * D + lane * 8) * 2) = *reinterpret_cast<uint4 *>(lo);
+            }
+        }
+        // an infinite or NaN q makes its scores NaN
+        if (lane == 0) q_unit[hh] = amax < 0x7f800000u ? down * a.scale_log2e : __uint_as_float(0x7fffffffu);
+    }
+    __syncthreads();
+    if (storing) {
+        if (ts.grown[0] || ts.grown[1]) { // the codes that the block held follow its scale
+            const int blk0 = past >> a.c.block_shift << a.c.block_shift;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                uint2 *rows = reinterpret_cast<uint2 *>(a.c.codes[i] + (unit * a.c.T + blk0) * D);
+                if (ts.grown[i])
+                    for (int c = tid; c < (past - blk0) * (D / 8); c += NTHREADS) rows[c] = kv8_rescale8<CODE>(rows[c], ts.ratio[i]);
+            }
+            __syncthreads();
+        }
+        if (r + lane * kStride >= settled) { // steps of that block
+            sc_k = ts.scale[0];
+            sc_v = ts.scale[1];
+        }
+    }
     for (; groups < R::kStages; ++groups) { // a group per stage, empty where there is no step
         copy_next(row1);
         copy_commit();
     }
-
-    // ---- q: rotated, brought to [2^8, 2^9) by a power of two, split into two fp16 parts; one warp per head
-    for (int hh = warp; hh < HEADS; hh += kWarps) {
-        float x[8];
-        uint32_t amax = 0;
-        const bool on = hh < nheads && lane < D / 8;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = 0.f;
-        static_assert(D <= 256, "a warp holds a row, eight dims to a lane");
-        if (on) {
-            load8(a, 0, (size_t)b, (head0 + hh) * D + lane * 8, x);
-            if (a.freq_cis) kv8_rotate8(a.freq_cis + (size_t)prow * D + lane * 8, x);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) amax = max(amax, kv8_abs_bits(x[e]));
-        }
-        amax = __reduce_max_sync(0xffffffffu, amax);
-        const int ex = min(max((int)(amax >> 23) - 127, -110), 126);
-        const float up = __uint_as_float((uint32_t)(8 - ex + 127) << 23), down = __uint_as_float((uint32_t)(ex - 8 + 127) << 23);
-        if (lane < D / 8) {
-            __half2 hi[4], lo[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float u = x[2 * e] * up, v = x[2 * e + 1] * up;
-                hi[e] = __floats2half2_rn(u, v);
-                const float2 f = __half22float2(hi[e]);
-                lo[e] = __floats2half2_rn(u - f.x, v - f.y);
-            }
-            *reinterpret_cast<uint4 *>(&q_s[2 * hh][lane * 8]) = *reinterpret_cast<uint4 *>(hi);
-            *reinterpret_cast<uint4 *>(&q_s[2 * hh + 1][lane * 8]) = *reinterpret_cast<uint4 *>(lo);
-        }
-        if (lane == 0) q_unit[hh] = down * a.scale_log2e;
-    }
-    // ---- scales of the split's blocks; the largest of V's decides by which power of two the weights are raised
-    uint32_t vmax = 0;
-    {
-        const int nb = ((row1 - 1) >> a.c.block_shift) - (row0 >> a.c.block_shift) + 1;
-        const size_t s0 = unit * a.c.nblk + (row0 >> a.c.block_shift);
-        for (int i = tid; i < nb; i += NTHREADS) {
-            sc_s[0][i] = __ldcg(a.c.scale[0] + s0 + i);
-            const float v = __ldcg(a.c.scale[1] + s0 + i);
-            sc_s[1][i] = v;
-            vmax = max(vmax, kv8_abs_bits(v));
-        }
-    }
-    vmax = kv8_block_max(vmax, red);
-    __syncthreads();
+    // the largest V scale decides by which power of two the weights are raised before they are cut into fp16 parts
+    const uint32_t vmax = __reduce_max_sync(0xffffffffu, r + lane * kStride < row1 ? kv8_abs_bits(sc_v) : 0u);
     const int vex = min(max((int)(vmax >> 23) - 127, -100), 100);
     const float v_up = __uint_as_float((uint32_t)(5 - vex + 127) << 23), v_down = __uint_as_float((uint32_t)(vex - 5 + 127) << 23);
 
-    uint32_t qf[NT][4 * KCH][2];
+    // q as the matrix instructions take it.  Lane (g, t) meets dims 64 c + 16 t .. + 15 of a row; column 2 t + i of a tile is part i (int8: of the second
+    // tile part 2 + i) of head t
+    constexpr int QT = CODE == kCodeI8 ? 2 : 1, QS = CODE == kCodeI8 ? 2 * KCH : 4 * KCH;
+    uint32_t qf[NT][QT][QS][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int s = 0; s < 4 * KCH; ++s) {
-            const uint2 u = *reinterpret_cast<const uint2 *>(&q_s[8 * n + g][(s >> 2) * 64 + 16 * t + 4 * (s & 3)]);
-            qf[n][s][0] = u.x;
-            qf[n][s][1] = u.y;
-        }
+        for (int p = 0; p < QT; ++p)
+#pragma unroll
+            for (int st = 0; st < QS; ++st) {
+                const unsigned char *src = CODE == kCodeI8 ? q_s + ((2 * p + (g & 1)) * HEADS + 4 * n + (g >> 1)) * D + (st >> 1) * 64 + 16 * t + 8 * (st & 1)
+                                                           : q_s + ((8 * n + g) * D + (st >> 2) * 64 + 16 * t + 4 * (st & 3)) * 2;
+                const uint2 u = *reinterpret_cast<const uint2 *>(src);
+                qf[n][p][st][0] = u.x;
+                qf[n][p][st][1] = u.y;
+            }
     float qu[NT], m_run[NT], l_run[NT], slope[NT];
     float o[NT][MT][4];
 #pragma unroll
@@ -328,35 +357,62 @@ __global__ void __launch_bounds__(kWarps * 32) flb_kv8_decode_kernel(const __gri
     // ---- the pass over the rows
     // This lane's reads of a slot: K rows g, g + 8 (the rows of a step's tile are dealt out so that eight lanes meet eight chunks), V rows
     // 2 t, 2 t + 1, 2 t + 8, 2 t + 9
-    int slot = 0;
+    int slot = 0, step = 0;
     for (; r < row1; r += kStride) {
         copy_wait<R::kStages - 1>();
         __syncwarp();
         const unsigned char *ks_p = ring_smem + warp * R::kWarpBytes + slot * R::kSlot, *vs_p = ks_p + R::kRowsBytes;
-        float s[NT][4];
+        float x[NT][2]; // scores of rows g, g + 8 by head, as products of codes
+        {
+            float sf[NT][4];
+            int si[NT][2][4];
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+                for (int e = 0; e < 4; ++e) {
+                    sf[n][e] = 0.f;
+                    si[n][0][e] = si[n][1][e] = 0;
+                }
 #pragma unroll
-        for (int c = 0; c < KCH; ++c) {
-            const uint4 k0 = *reinterpret_cast<const uint4 *>(ks_p + R::at(g, 4 * c + t));
-            const uint4 k1 = *reinterpret_cast<const uint4 *>(ks_p + R::at(g + 8, 4 * c + t));
-            const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+            for (int c = 0; c < KCH; ++c) {
+                const uint4 k0 = *reinterpret_cast<const uint4 *>(ks_p + R::at(g, 4 * c + t));
+                const uint4 k1 = *reinterpret_cast<const uint4 *>(ks_p + R::at(g + 8, 4 * c + t));
+                const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+                if (CODE == kCodeI8) {
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                uint32_t f[4];
-                codes_to_halves<CODE>(w0[w], f[0], f[2]);
-                codes_to_halves<CODE>(w1[w], f[1], f[3]);
+                    for (int w = 0; w < 2; ++w) {
+                        const uint32_t f[4] = {w0[2 * w], w1[2 * w], w0[2 * w + 1], w1[2 * w + 1]};
 #pragma unroll
-                for (int n = 0; n < NT; ++n) mma16816(s[n], f, qf[n][4 * c + w][0], qf[n][4 * c + w][1]);
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int p = 0; p < 2; ++p) mma16832(si[n][p], f, qf[n][p % QT][2 * c + w][0], qf[n][p % QT][2 * c + w][1]);
+                    }
+                } else {
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        uint32_t f[4];
+                        codes_to_halves<CODE>(w0[w], f[0], f[2]);
+                        codes_to_halves<CODE>(w1[w], f[1], f[3]);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) mma16816(sf[n], f, qf[n][0][(4 * c + w) % QS][0], qf[n][0][(4 * c + w) % QS][1]);
+                    }
+                }
             }
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    x[n][i] = CODE == kCodeI8 ? fmaf((float)(si[n][0][2 * i] * 128 + si[n][0][2 * i + 1]), 16384.0f, (float)(si[n][1][2 * i] * 128 + si[n][1][2 * i + 1]))
+                                              : sf[n][2 * i] + sf[n][2 * i + 1];
         }
-
-        const int sb = (r - row0) >> a.c.block_shift;
-        const float ks = sc_s[0][sb], vs = sc_s[1][sb] * v_up;
+        const float ks = __shfl_sync(0xffffffffu, sc_k, step), vs = __shfl_sync(0xffffffffu, sc_v, step) * v_up;
+        ++step;
         int kpos[2] = {r + g, r + g + 8};
-        bool vis[2] = {r + g < row1, r + g + 8 < row1};
+        bool vis[2] = {true, true};
+        if (r + kStep > row1) {
+            vis[0] = r + g < row1;
+            vis[1] = r + g + 8 < row1;
+        }
         if (FORM) {
             if (a.c.row_pos && (a.slopes || a.key_begin)) {
 #pragma unroll
@@ -368,21 +424,20 @@ __global__ void __launch_bounds__(kWarps * 32) flb_kv8_decode_kernel(const __gri
         uint32_t pb[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            float x[2] = {(s[n][0] + s[n][1]) * (ks * qu[n]), (s[n][2] + s[n][3]) * (ks * qu[n])};
-            if (FORM && a.cap_log2e > 0.f) cap_scores(x, a.cap_log2e, inv_cap);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) x[n][i] *= ks * qu[n];
+            if (FORM && a.cap_log2e > 0.f) cap_scores(x[n], a.cap_log2e, inv_cap);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                if (FORM) {
-                    x[i] = fmaf(-slope[n], fabsf((float)(pos - kpos[i])), x[i]);
-                }
-                x[i] = vis[i] ? x[i] : -INFINITY;
+                if (FORM) x[n][i] = fmaf(-slope[n], fabsf((float)(pos - kpos[i])), x[n][i]);
+                x[n][i] = vis[i] ? x[n][i] : -INFINITY;
             }
             if (a.scores && 4 * n + t < nheads) {
                 float *sp = a.scores + ((size_t)b * a.Hq + head0 + 4 * n + t) * a.c.T + r + g;
-                if (r + g < row1) sp[0] = x[0];
-                if (r + g + 8 < row1) sp[8] = x[1];
+                if (r + g < row1) sp[0] = x[n][0];
+                if (r + g + 8 < row1) sp[8] = x[n][1];
             }
-            const float top = fmaxf(x[0], x[1]);
+            const float top = fmaxf(x[n][0], x[n][1]);
             if (__any_sync(0xffffffffu, top > m_run[n] + kRaise)) {
                 float mx = top;
 #pragma unroll
@@ -398,7 +453,7 @@ __global__ void __launch_bounds__(kWarps * 32) flb_kv8_decode_kernel(const __gri
             }
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const float p = ex2(x[i] - m_run[n]);
+                const float p = ex2(x[n][i] - m_run[n]);
                 l_run[n] += p;
                 const float pv = vis[i] ? p * vs : 0.f;
                 const __half hi = __float2half_rn(pv);
@@ -512,11 +567,13 @@ __global__ void __launch_bounds__(kWarps * 32) flb_kv8_decode_kernel(const __gri
     float *const e_s = reinterpret_cast<float *>(ring_smem) + NTHREADS * 4; // [64][HEADS] behind the shares
     for (int hh = warp; hh < nheads; hh += kWarps) {
         const float2 *ml = reinterpret_cast<const float2 *>(a.part_ml) + mbase * HEADS + hh;
-        float M = kNoMax, l = 0.f;
-        for (int s = lane; s < nsplit; s += 32) M = fmaxf(M, __ldcg(ml + (size_t)s * HEADS).x);
+        const float2 own = lane < nsplit ? __ldcg(ml + (size_t)lane * HEADS) : make_float2(kNoMax, 0.f);
+        float M = own.x;
+        for (int s = lane + 32; s < nsplit; s += 32) M = fmaxf(M, __ldcg(ml + (size_t)s * HEADS).x);
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
-        for (int s = lane; s < nsplit; s += 32) {
+        float l = own.y * ex2(own.x - M);
+        for (int s = lane + 32; s < nsplit; s += 32) {
             const float2 v = __ldcg(ml + (size_t)s * HEADS);
             l = fmaf(v.y, ex2(v.x - M), l);
         }

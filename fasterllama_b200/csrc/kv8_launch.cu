@@ -113,7 +113,7 @@ int check_decode_sizes(const flb_kv8_decode_params *p) {
     const int st = check_sizes(p->cache);
     if (st != FLB_OK) return st;
     if (p->head_num <= 0 || p->head_num % p->cache.kv_head_num) return FLB_ERR_BAD_SHAPE;
-    if (p->split_len < 0 || p->split_len % 128 || p->split_len > 8192) return FLB_ERR_BAD_SHAPE;
+    if (p->split_len < 0 || p->split_len % 128 || p->split_len > 2048) return FLB_ERR_BAD_SHAPE;
     if ((size_t)p->cache.batch_size * p->head_num > (size_t)1 << 24) return FLB_ERR_TOO_LARGE;
     return FLB_OK;
 }

@@ -106,7 +106,7 @@ typedef struct flb_kv8_decode_params {
     void *scratch;           /* flb_kv8_decode_workspace_bytes()                        */
     size_t scratch_bytes;
     int scratch_zeroed;      /* promise: the first flb_kv8_counter_bytes() bytes are zero on entry (they are left zero) */
-    int split_len;           /* rows of one split of a sequence, a multiple of 128 up to 8192; 0 = default.  Results
+    int split_len;           /* rows of one split of a sequence, a multiple of 128 up to 2048; 0 = default.  Results
                                 depend on it and on each sequence alone, never on the batch or the grid */
 } flb_kv8_decode_params;
 
