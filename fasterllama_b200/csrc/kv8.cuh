@@ -6,7 +6,31 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "flb_ptx.cuh"
+
 namespace flb {
+
+// Every kernel of this family is launched with programmatic stream serialisation: its CTAs may become resident while the kernel in front
+// drains.  They touch nothing before that kernel, and with it everything before, has completed, and let the next one go after that
+// only: for a caller a launch is as ordered as any, it merely starts sooner.  All threads call it first.
+__device__ __forceinline__ void kv8_begin() {
+    grid_dependency_wait();
+    grid_launch_dependents();
+}
+template <typename Kernel, typename... Args>
+inline cudaError_t kv8_launch(Kernel kernel, unsigned grid, unsigned threads, size_t smem, cudaStream_t stream, const Args &...args) {
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
 
 enum : unsigned { kKv8BadLen = 4u, kKv8BadPos = 32u };
 

@@ -15,6 +15,7 @@ constexpr int kChunks = 4; // 8-value chunks per thread
 template <int D, int CODE, int MODE> __global__ void __launch_bounds__(1024) flb_kv8_append_kernel(const __grid_constant__ Kv8AppendArgs a) {
     constexpr int CPR = D / 8; // chunks per row
     __shared__ uint32_t red[32];
+    kv8_begin();
     unsigned id = blockIdx.x;
     const int kv = (int)(id & 1u);
     id >>= 1;
@@ -75,13 +76,8 @@ template <int D, int CODE, int MODE> __global__ void __launch_bounds__(1024) flb
 template <int D, int CODE> cudaError_t launch_t(const Kv8AppendArgs &a, int input_mode, cudaStream_t stream) {
     const unsigned threads = (unsigned)((D << a.c.block_shift) / (8 * kChunks));
     const unsigned grid = 2u * (unsigned)a.c.H * (unsigned)a.nwin * (unsigned)a.c.B;
-    if (input_mode == 0)
-        flb_kv8_append_kernel<D, CODE, 0><<<grid, threads, 0, stream>>>(a);
-    else if (input_mode == 1)
-        flb_kv8_append_kernel<D, CODE, 1><<<grid, threads, 0, stream>>>(a);
-    else
-        flb_kv8_append_kernel<D, CODE, 2><<<grid, threads, 0, stream>>>(a);
-    return cudaGetLastError();
+    auto kern = input_mode == 0 ? flb_kv8_append_kernel<D, CODE, 0> : input_mode == 1 ? flb_kv8_append_kernel<D, CODE, 1> : flb_kv8_append_kernel<D, CODE, 2>;
+    return kv8_launch(kern, grid, threads, 0, stream, a);
 }
 
 } // namespace

@@ -24,8 +24,6 @@
 //     them into weights and adds them up over the group.
 #include "kv8.cuh"
 
-#include "flb_ptx.cuh"
-
 #include <atomic>
 
 namespace flb {
@@ -73,7 +71,7 @@ template <int CODE> __device__ __forceinline__ void codes_to_halves(uint32_t w, 
 template <int D> struct Ring {
     static constexpr int kRowsBytes = kStep * D;
     static constexpr int kSlot = 2 * kRowsBytes;
-    static constexpr int kStages = D == 64 ? 4 : 2; // 12 KB per warp (d = 256: 24 KB)
+    static constexpr int kStages = D == 64 ? 6 : D == 128 ? 3 : 2; // 12 KB per warp (d = 256: 16 KB)
     static constexpr int kWarpBytes = kStages * kSlot;
     // Where chunk c (16 bytes) of row r lies.  K is read as rows r, r + 1 x four neighbouring chunks per eight lanes, V as rows r, r + 2, r + 4,
     // r + 6 x two neighbouring chunks: the permutations send both to eight different chunks of the 128-byte bank line.
@@ -166,7 +164,7 @@ __device__ __forceinline__ void append_token(const Kv8DecodeArgs &a, int kv, siz
 
 // FORM: capped scores, distance bias or key_begin.  NT: column tiles of eight = four q heads each.
 template <int D, int CODE, int NT, bool FORM>
-__global__ void __launch_bounds__(kWarps * 32) flb_kv8_decode_kernel(const __grid_constant__ Kv8DecodeArgs a) {
+__global__ void __launch_bounds__(kWarps * 32, D == 128 && NT == 1 ? 4 : 1) flb_kv8_decode_kernel(const __grid_constant__ Kv8DecodeArgs a) {
     constexpr int HEADS = 4 * NT;
     constexpr int KCH = D / 64;   // 16-byte chunks of a K row per lane
     constexpr int VW = D / 32;    // 32-bit words of a V row per lane
@@ -181,6 +179,7 @@ __global__ void __launch_bounds__(kWarps * 32) flb_kv8_decode_kernel(const __gri
     __shared__ TokenScales ts;
     __shared__ int last_flag;
 
+    kv8_begin();
     const int split = (int)(blockIdx.x % (unsigned)a.nsplit_max);
     const unsigned uc = blockIdx.x / (unsigned)a.nsplit_max;
     const int chunk = (int)(uc % (unsigned)a.nchunk);
@@ -643,23 +642,37 @@ __global__ void __launch_bounds__(kWarps * 32) flb_kv8_decode_kernel(const __gri
     if (tid == 0) a.counters[unit * a.nchunk + chunk] = 0u; // ready for the next call
 }
 
-// weight_out = weight_in + sum over the group of 2^(score - max) / sum; one thread per row and K/V head.
+// weight_out = weight_in + sum over the group of 2^(score - max) / sum.  A thread takes four rows of one K/V head; HBM-bound, 4 (G + 2) bytes a
+// row and head (100001 rows, 8 heads of 4 q heads, from L2: 4 us).
 __global__ void __launch_bounds__(256) flb_kv8_weights_kernel(const __grid_constant__ Kv8DecodeArgs a, int blocks_per_unit) {
+    kv8_begin();
     const size_t unit = blockIdx.x / (unsigned)blocks_per_unit;
-    const int r = (int)(blockIdx.x % (unsigned)blocks_per_unit) * 256 + threadIdx.x;
+    const int r = ((int)(blockIdx.x % (unsigned)blocks_per_unit) * 256 + threadIdx.x) * 4;
     const int b = (int)(unit / a.c.H), h = (int)(unit - (size_t)b * a.c.H);
     const int past = a.past_lens ? __ldg(a.past_lens + b) : a.start_pos;
     if (past < 0 || past >= a.c.T || past >= a.nsplit_max * a.split_len || r > past) return;
-    const size_t i = unit * a.c.T + r;
-    float w = (r == past) ? 0.f : a.weight_in[i];
-    const bool hidden = a.key_begin && !a.c.row_pos && r < __ldg(a.key_begin + b); // no score was left for it
+    const size_t i = unit * a.c.T + r; // T is a multiple of 16: four rows never leave the slab
+    const int begin = a.key_begin && !a.c.row_pos ? __ldg(a.key_begin + b) : INT_MIN; // no score was left below it
+    const float4 in = *reinterpret_cast<const float4 *>(a.weight_in + i);
+    float w[4] = {in.x, in.y, in.z, in.w};
+    const size_t hq0 = (size_t)b * a.Hq + h * a.G;
+    if (r <= past && past < r + 4) w[past - r] = 0.f;
+#pragma unroll 4
     for (int j = 0; j < a.G; ++j) {
-        const size_t hq = (size_t)b * a.Hq + h * a.G + j;
-        const float l = __ldg(a.ml + hq * 2 + 1);
-        if (hidden) continue;
-        if (l > 0.f || l != l) w += ex2(__ldcs(a.scores + hq * a.c.T + r) - __ldg(a.ml + hq * 2)) / l;
+        const float4 s4 = __ldcs(reinterpret_cast<const float4 *>(a.scores + (hq0 + j) * a.c.T + r));
+        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(a.ml) + hq0 + j);
+        const float s[4] = {s4.x, s4.y, s4.z, s4.w};
+        const float inv = (ml.y > 0.f || ml.y != ml.y) ? 1.0f / ml.y : 0.f;
+        if (inv != 0.f)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (r + e >= begin) w[e] += ex2(s[e] - ml.x) * inv;
     }
-    a.weight_out[i] = w;
+    if (r + 3 <= past) {
+        *reinterpret_cast<float4 *>(a.weight_out + i) = make_float4(w[0], w[1], w[2], w[3]);
+    } else {
+        for (int e = 0; e < 4 && r + e <= past; ++e) a.weight_out[i + e] = w[e];
+    }
 }
 
 template <int D, int CODE, int NT> cudaError_t launch_t(const Kv8DecodeArgs &a, cudaStream_t stream) {
@@ -679,12 +692,10 @@ template <int D, int CODE, int NT> cudaError_t launch_t(const Kv8DecodeArgs &a, 
         if (e != cudaSuccess) return e;
         if (bit) opted_in[form].fetch_or(bit, std::memory_order_release);
     }
-    kern<<<grid, kWarps * 32, smem, stream>>>(a);
-    e = cudaGetLastError();
+    e = kv8_launch(kern, grid, kWarps * 32, smem, stream, a);
     if (e != cudaSuccess || !a.weight_out) return e;
-    const int rows = min(a.c.T, a.nsplit_max * a.split_len), bpu = (rows + 255) / 256;
-    flb_kv8_weights_kernel<<<(unsigned)a.c.B * (unsigned)a.c.H * (unsigned)bpu, 256, 0, stream>>>(a, bpu);
-    return cudaGetLastError();
+    const int rows = min(a.c.T, a.nsplit_max * a.split_len), bpu = (rows + 1023) / 1024;
+    return kv8_launch(flb_kv8_weights_kernel, (unsigned)a.c.B * (unsigned)a.c.H * (unsigned)bpu, 256, 0, stream, a, bpu);
 }
 
 template <int CODE> cudaError_t launch_code(const Kv8DecodeArgs &a, int d, int nt, cudaStream_t stream) {

@@ -98,7 +98,7 @@ typedef struct flb_kv8_decode_params {
     const int *key_begin;      /* device int[B] or NULL                                 */
     /* Accumulated attention, for flb_kv8_evict(): weight_out[b][h][r] = weight_in[b][h][r] + the sum of the weights that
      * the group's q heads give row r, for r = 0..past (row past starts from 0); further rows are left alone.  Both
-     * [B,Hkv,T]; they may be the same buffer.  NULL, NULL = off. */
+     * [B,Hkv,T], 16-byte aligned; they may be the same buffer.  NULL, NULL = off. */
     const float *weight_in;
     float *weight_out;
     void *out;               /* [B,H,1,d]                                               */
