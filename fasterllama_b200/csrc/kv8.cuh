@@ -99,6 +99,7 @@ struct Kv8EvictArgs {
     unsigned *status;
     int *moves;    // [B*H][T / 2] sources: the i-th kept row at or behind m
     int *holes;    // [B*H][T / 2] holes below m, rising
+    int *seq_len;      // [B][2] m, and what becomes of len_out
     float *edge_scale; // [B*H][2] scales of the block that row m lies in, as they were
     int *hole_off; // [B*H][nblk + 1] holes in front of each block
 };
@@ -171,34 +172,53 @@ template <int CODE> __device__ __forceinline__ float kv8_new_scale(uint32_t amax
     return (old != old || need <= old) ? old : need; // NaN on either side stays NaN
 }
 
-// four values to four codes (values of finite size; a scale of 0, infinity or NaN gives codes 0)
+// Four values to four codes: rne, as a byte each.  int8: the addition of 1.5 * 2^23 rounds to a whole number and leaves it in the low byte.
 template <int CODE> __device__ __forceinline__ uint32_t kv8_pack4(const float (&y)[4]) {
-    uint32_t r = 0;
     if (CODE == kCodeI8) {
+        uint32_t t[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            int q;
-            asm("cvt.rni.sat.s8.f32 %0, %1;" : "=r"(q) : "f"(fmaxf(y[i], -127.0f)));
-            r |= (uint32_t)(q & 0xff) << (8 * i);
-        }
-    } else {
-        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3);
-        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3);
-        r = lo | (hi << 16);
+        for (int i = 0; i < 4; ++i) t[i] = __float_as_uint(__fadd_rn(y[i], 12582912.0f));
+        return __byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410);
     }
-    return r;
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3);
+    return lo | (hi << 16);
 }
-template <int CODE> __device__ __forceinline__ uint2 kv8_encode8(const float (&x)[8], float scale) {
+// Whether a quotient that is off by up to 2^-22 of itself could round to another code than the exact one: it lies that near to the middle
+// between two codes.
+template <int CODE> __device__ __forceinline__ bool kv8_near_tie(float y) {
+    if (CODE == kCodeI8) {
+        const float whole = __fsub_rn(__fadd_rn(y, 12582912.0f), 12582912.0f);
+        return fabsf(y - whole) > 0.5f - 6.1035156e-5f; // 2^-14 > 127 * 2^-22
+    }
+    // e4m3 keeps 3 of the 23 mantissa bits (fewer below 2^-6: always looked at exactly there)
+    const uint32_t u = __float_as_uint(y) & 0x7fffffffu;
+    return u < 0x3c800000u || ((u + 8u) & 0xfffffu) - 0x80000u <= 16u;
+}
+// Eight values over their block's scale, rounded to codes; `inv` = 1 / scale.  The quotient is defined as one IEEE division; multiplying by
+// the reciprocal is off by 2^-22 at most, which shows only next to a tie, and there the division is done.  A scale of 0, infinity or NaN gives
+// codes 0.
+template <int CODE> __device__ __forceinline__ uint2 kv8_encode8(const float (&x)[8], float scale, float inv) {
     const bool ok = scale > 0.f && scale <= 3.402823466e38f;
+    const bool exact = !(inv <= 3.402823466e38f && scale <= 1e37f); // the reciprocal of a subnormal scale overflows, that of a huge one is subnormal
     float y[2][4];
+    bool near = false;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i >> 2][i & 3] = ok ? __fdiv_rn(x[i], scale) : 0.f;
+    for (int i = 0; i < 8; ++i) {
+        y[i >> 2][i & 3] = ok ? __fmul_rn(x[i], inv) : 0.f;
+        near = near || kv8_near_tie<CODE>(y[i >> 2][i & 3]);
+    }
+    if (ok && (near || exact)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i >> 2][i & 3] = __fdiv_rn(x[i], scale);
+    }
     return make_uint2(kv8_pack4<CODE>(y[0]), kv8_pack4<CODE>(y[1]));
 }
 template <int CODE> __device__ __forceinline__ void kv8_decode4(uint32_t w, float (&x)[4]) {
     if (CODE == kCodeI8) {
+        w ^= 0x80808080u; // byte + 128 under the exponent of 2^23
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = (float)(int8_t)(w >> (8 * i));
+        for (int i = 0; i < 4; ++i) x[i] = __fsub_rn(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 + i)), 8388736.0f);
     } else {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {

@@ -57,14 +57,14 @@ template <int D, int CODE, int MODE> __global__ void __launch_bounds__(1024) flb
     __syncthreads(); // every thread has read the old scale
     const float scale = kv8_new_scale<CODE>(amax, old);
     const bool grown = old > 0.f && scale > old;
-    const float ratio = grown ? __fdiv_rn(old, scale) : 1.f;
+    const float ratio = grown ? __fdiv_rn(old, scale) : 1.f, inv = __fdiv_rn(1.f, scale);
 #pragma unroll
     for (int i = 0; i < kChunks; ++i) {
         const int ch = threadIdx.x + i * blockDim.x;
         const int row = row0 + ch / CPR;
         uint2 *dst = reinterpret_cast<uint2 *>(codes) + ch;
         if (row >= lo && row < hi)
-            *dst = kv8_encode8<CODE>(x[i], scale);
+            *dst = kv8_encode8<CODE>(x[i], scale, inv);
         else if (row < past && grown)
             *dst = kv8_rescale8<CODE>(*dst, ratio);
     }

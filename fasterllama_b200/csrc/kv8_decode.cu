@@ -151,7 +151,7 @@ __device__ __forceinline__ void append_token(const Kv8DecodeArgs &a, int kv, siz
     }
     amax = __reduce_max_sync(0xffffffffu, amax);
     const float scale = kv8_new_scale<CODE>(amax, old);
-    if (lane < D / 8) *reinterpret_cast<uint2 *>(a.c.codes[kv] + (unit * a.c.T + past) * D + lane * 8) = kv8_encode8<CODE>(x, scale);
+    if (lane < D / 8) *reinterpret_cast<uint2 *>(a.c.codes[kv] + (unit * a.c.T + past) * D + lane * 8) = kv8_encode8<CODE>(x, scale, __fdiv_rn(1.f, scale));
     if (lane == 0) {
         a.c.scale[kv][sidx] = scale;
         if (kv == 0 && a.c.row_pos) a.c.row_pos[unit * a.c.T + past] = pos;

@@ -1,21 +1,26 @@
 // kv8_evict.cu — the cached rows that drew the least attention leave, the others close up.
 //
-// 1. flb_kv8_select_kernel, one CTA per K/V head: which rows stay.  A radix selection over the weights (as ordered
-//    integers) finds the smallest kept weight and how many rows of exactly that weight stay (the lowest of them); one pass
-//    in row order then lists the holes below m = min(n, budget) and the kept rows behind it.
-// 2. flb_kv8_move_kernel, one CTA per block of rows with a hole, K and V apart: the i-th hole takes the i-th
+// 1. flb_kv8_select_kernel, a CTA or a cluster of eight per K/V head: which rows stay.  A radix selection over the weights (as ordered
+//    integers, in registers; histograms meet in distributed shared memory) finds the smallest kept weight and how many rows of
+//    exactly that weight stay (the lowest of them); prefix sums in row order then list the holes below m = min(n, budget) and
+//    the kept rows behind it, and weights and positions move.
+// 2. flb_kv8_move_kernel, K and V apart, a CTA per four blocks of rows: the i-th hole takes the i-th
 //    kept row from behind m.  Sources lie at or behind m and targets below it, so nothing waits for anything.  The
-//    block's scale grows by the rule of an append (32 values per thread, held in registers in between).
+//    block's scale grows by the rule of an append (the codes are held in registers in between).
 // Filling holes moves at most n - m rows and recodes only those (and a block whose scale grows); closing the gaps in row order
 // would move nearly every row and round nearly every code once more at each eviction.
 #include "kv8.cuh"
 
+#include <cooperative_groups.h>
+
 namespace flb {
+
+namespace cg = cooperative_groups;
 
 namespace {
 
 constexpr int kSelThreads = 1024;
-constexpr int kRowsPerThread = 4; // a thread's rows of a pass are neighbours
+constexpr int kRegRows = 16; // rows whose keys a thread keeps in registers
 
 // weights as integers of the same order; NaN above everything
 __device__ __forceinline__ uint32_t ordered(float w) {
@@ -28,261 +33,342 @@ __device__ __forceinline__ bool is_safe(const Kv8EvictArgs &a, int pos, int next
     return pos < a.sinks || (a.next_pos && (long long)pos >= (long long)next - a.recent);
 }
 
-// sum over the block in thread order: exclusive prefix of this thread and the total.  `ws`: one word per warp + 1.
-__device__ __forceinline__ int block_scan(int v, int *ws, int &total) {
+// Exclusive prefix over the block in thread order, and the total.  `ws`: a word per warp.
+__device__ __forceinline__ long long block_scan(long long v, long long *ws, long long &total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int inc = v;
+    long long inc = v;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
-        const int o = __shfl_up_sync(0xffffffffu, inc, off);
+        const long long o = __shfl_up_sync(0xffffffffu, inc, off);
         if (lane >= off) inc += o;
     }
     if (lane == 31) ws[warp] = inc;
     __syncthreads();
-    if (warp == 0) {
-        int s = ws[lane];
+    long long s = ws[lane]; // every warp adds the warps up for itself
 #pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-            const int o = __shfl_up_sync(0xffffffffu, s, off);
-            if (lane >= off) s += o;
-        }
-        ws[lane] = s;
+    for (int off = 1; off < 32; off <<= 1) {
+        const long long o = __shfl_up_sync(0xffffffffu, s, off);
+        if (lane >= off) s += o;
     }
-    __syncthreads();
-    const int before = warp ? ws[warp - 1] : 0;
-    total = ws[31];
-    __syncthreads();
-    return before + inc - v;
+    total = __shfl_sync(0xffffffffu, s, 31);
+    const long long before = __shfl_sync(0xffffffffu, s, (warp + 31) & 31);
+    return (warp ? before : 0) + inc - v;
 }
 
-__global__ void __launch_bounds__(kSelThreads) flb_kv8_select_kernel(const __grid_constant__ Kv8EvictArgs a) {
-    __shared__ int hist[256];
-    __shared__ int ws[32];
-    __shared__ int sh_digit, sh_above, sh_safe;
-    const size_t unit = blockIdx.x;
+// A barrier over the cluster; a cluster of one needs no more than its own.
+__device__ __forceinline__ void all_sync(cg::cluster_group &cluster, int ranks) {
+    if (ranks == 1)
+        __syncthreads();
+    else
+        cluster.sync();
+}
+
+// A cluster of CTAs (one, for short slabs) per K/V head; every thread has `per` neighbouring rows.  REGS: their keys stay in registers over
+// the passes; else (beyond 16 rows a thread) they are read again.
+template <bool REGS> __global__ void __launch_bounds__(kSelThreads) flb_kv8_select_kernel(const __grid_constant__ Kv8EvictArgs a) {
+    __shared__ int hist[4][256];
+    __shared__ int tot[4][256];
+    __shared__ long long ws[2][32];
+    __shared__ int n_safe;
+    __shared__ int n_equal;
+    __shared__ long long n_lists; // holes, and kept rows behind m in the upper half
+    kv8_begin();
+    cg::cluster_group cluster = cg::this_cluster();
+    const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const size_t unit = blockIdx.x / (unsigned)ranks;
     const int b = (int)(unit / a.c.H);
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, lane = tid & 31;
     int *off = a.hole_off + unit * (a.c.nblk + 1);
-    int n = a.past_lens ? __ldg(a.past_lens + b) : a.start_pos;
-    if (n < 0 || n > a.c.T) { // flagged; the sequence is left alone
-        if (tid == 0) atomicOr(a.status, kKv8BadLen);
-        for (int j = tid; j <= a.c.nblk; j += kSelThreads) off[j] = 0;
-        return;
-    }
-    const int m = min(n, a.budget);
-    if (n <= a.budget) {
-        for (int j = tid; j <= a.c.nblk; j += kSelThreads) off[j] = 0;
-        return;
-    }
     const float *w = a.weight + unit * a.c.T;
     const int *pos = a.c.row_pos + unit * a.c.T;
-    const int next = a.next_pos ? __ldg(a.next_pos + b) : 0;
-
+    float *w_out = a.weight_out + unit * a.c.T;
+    int *p_out = a.pos_out + unit * a.c.T;
+    const int n = a.past_lens ? __ldcg(a.past_lens + b) : a.start_pos;
+    const int next = a.next_pos ? __ldcg(a.next_pos + b) : 0;
+    const bool bad = n < 0 || n > a.c.T; // flagged; the sequence is left alone
+    const int m = bad ? 0 : min(n, a.budget);
+    if (tid == 0 && rank == 0) {
+        a.seq_len[2 * b] = m; // the same from every head
+        a.seq_len[2 * b + 1] = bad ? n : m;
+    }
+    const int span = (m + 3) / 4, v0 = (int)((long long)span * rank / ranks), v1 = (int)((long long)span * (rank + 1) / ranks);
+    if (bad || n <= a.budget) {
+        for (int j = rank * kSelThreads + tid; j <= a.c.nblk; j += ranks * kSelThreads) off[j] = 0;
+        if (w_out != w || p_out != pos)
+            for (int r = 4 * v0 + tid; r < min(m, 4 * v1); r += kSelThreads) {
+                w_out[r] = w[r];
+                p_out[r] = pos[r];
+            }
+        return; // the whole cluster alike
+    }
     // Sources may share a block with targets, the one that row m lies in.  Its rows from m on are left as they are and the scale
     // they were coded with is kept aside, so the order in which the blocks are filled does not matter.
-    if (tid < 2) a.edge_scale[unit * 2 + tid] = a.c.scale[tid][unit * a.c.nblk + (m >> a.c.block_shift)];
+    if (tid < 2 && rank == 0) a.edge_scale[unit * 2 + tid] = a.c.scale[tid][unit * a.c.nblk + (m >> a.c.block_shift)];
 
-    // protected rows
-    if (tid == 0) sh_safe = 0;
+    for (int i = tid; i < 4 * 256; i += kSelThreads) hist[i >> 8][i & 255] = 0;
+    if (tid == 0) n_safe = n_equal = 0;
     __syncthreads();
-    {
-        int c = 0;
-        for (int r = tid; r < n; r += kSelThreads) c += is_safe(a, pos[r], next);
-        c = __reduce_add_sync(0xffffffffu, c);
-        if ((tid & 31) == 0 && c) atomicAdd(&sh_safe, c);
+
+    // this thread's rows [r0, r1)
+    const int per = (((n + ranks - 1) / ranks + kSelThreads - 1) / kSelThreads + 3) & ~3;
+    const int r0 = min(n, (rank * kSelThreads + tid) * per), r1 = min(n, r0 + per);
+    uint32_t key[REGS ? kRegRows : 1];
+    uint32_t safe_bits = 0;
+    int safe = 0;
+    if (REGS) {
+#pragma unroll
+        for (int v = 0; v < kRegRows; v += 4) {
+            float4 wv = make_float4(0.f, 0.f, 0.f, 0.f);
+            int4 pv = make_int4(0, 0, 0, 0);
+            if (r0 + v < r1) { // rows come in fours: the slab's length is a multiple of 16
+                wv = *reinterpret_cast<const float4 *>(w + r0 + v);
+                pv = *reinterpret_cast<const int4 *>(pos + r0 + v);
+            }
+            key[(v + 0) % (REGS ? kRegRows : 1)] = ordered(wv.x);
+            key[(v + 1) % (REGS ? kRegRows : 1)] = ordered(wv.y);
+            key[(v + 2) % (REGS ? kRegRows : 1)] = ordered(wv.z);
+            key[(v + 3) % (REGS ? kRegRows : 1)] = ordered(wv.w);
+            safe_bits |= (uint32_t)(is_safe(a, pv.x, next) | is_safe(a, pv.y, next) << 1 | is_safe(a, pv.z, next) << 2 | is_safe(a, pv.w, next) << 3) << v;
+        }
+        if (r1 - r0 < 32) safe_bits &= (1u << (r1 - r0)) - 1u;
+        safe = __popc(safe_bits);
+    } else {
+        for (int r = r0; r < r1; ++r) safe += is_safe(a, pos[r], next);
     }
-    __syncthreads();
+    safe = __reduce_add_sync(0xffffffffu, safe);
+    if (lane == 0 && safe) atomicAdd(&n_safe, safe);
+    // f(row, key, protected) for each of this thread's rows
+    auto each = [&](auto f) {
+        if (REGS) {
+#pragma unroll
+            for (int i = 0; i < kRegRows; ++i)
+                if (r0 + i < r1) f(r0 + i, key[i % (REGS ? kRegRows : 1)], (safe_bits >> i & 1u) != 0);
+        } else {
+            for (int r = r0; r < r1; ++r) f(r, ordered(w[r]), is_safe(a, pos[r], next));
+        }
+    };
+    all_sync(cluster, ranks);
+    int all_safe = 0;
+    for (int c = 0; c < ranks; ++c) all_safe += *cluster.map_shared_rank(&n_safe, c);
     // More protected rows than room (positions given twice): the selection is among them.  Else they all stay and it is among the others.
-    const bool among_safe = sh_safe > m;
-    int want = among_safe ? m : m - sh_safe; // rows to select
+    const bool among_safe = all_safe > m;
+    const int want = among_safe ? m : m - all_safe; // rows to select
     uint32_t prefix = 0, mask = 0;
     int above = 0; // rows of a larger weight than the prefix allows
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        for (int i = tid; i < 256; i += kSelThreads) hist[i] = 0;
-        __syncthreads();
-        for (int r = tid; r < n; r += kSelThreads) {
-            const uint32_t k = ordered(w[r]);
-            if (is_safe(a, pos[r], next) == among_safe && (k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255u], 1);
+#pragma unroll 1
+    for (int pass = 0; pass < 4; ++pass) {
+        const int shift = 24 - 8 * pass;
+        each([&](int, uint32_t k, bool s) {
+            if (s == among_safe && (k & mask) == prefix) atomicAdd(&hist[pass][(k >> shift) & 255u], 1);
+        });
+        all_sync(cluster, ranks);
+        if (tid < 256) {
+            int t = 0;
+            for (int c = 0; c < ranks; ++c) t += cluster.map_shared_rank(&hist[pass][0], c)[tid];
+            tot[pass][tid] = t;
         }
         __syncthreads();
-        if (tid < 32) { // the digit at which the count from above reaches `want`: lane i holds the bins 255 - 8 i and below
-            int s[8], sum = 0;
+        // the digit at which the count from above reaches `want`, by every warp for itself: lane i holds the bins 255 - 8 i and below
+        int s[8], sum = 0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum += s[i] = hist[255 - 8 * tid - i];
-            int inc = sum;
+        for (int i = 0; i < 8; ++i) sum += s[i] = tot[pass][255 - 8 * lane - i];
+        int inc = sum;
 #pragma unroll
-            for (int off = 1; off < 32; off <<= 1) {
-                const int v = __shfl_up_sync(0xffffffffu, inc, off);
-                if (tid >= off) inc += v;
-            }
-            const unsigned reach = __ballot_sync(0xffffffffu, above + inc >= want);
-            if (tid == __ffs(reach) - 1) {
-                int c = above + inc - sum, d = 255 - 8 * tid;
-                bool found = false;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += v;
+        }
+        const int at = __ffs(__ballot_sync(0xffffffffu, above + inc >= want)) - 1;
+        int c = above + inc - sum, d = 255 - 8 * lane;
+        bool found = false;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    found = found || c + s[i] >= want;
-                    if (!found) {
-                        c += s[i];
-                        --d;
-                    }
-                }
-                sh_digit = d;
-                sh_above = c;
+        for (int i = 0; i < 8; ++i) {
+            found = found || c + s[i] >= want;
+            if (!found) {
+                c += s[i];
+                --d;
             }
         }
-        __syncthreads();
-        prefix |= (uint32_t)sh_digit << shift;
+        prefix |= (uint32_t)__shfl_sync(0xffffffffu, d, at) << shift;
+        above = __shfl_sync(0xffffffffu, c, at);
         mask |= 255u << shift;
-        above = sh_above;
-        __syncthreads();
     }
-    const uint32_t least = prefix;       // smallest kept weight; above it everything stays
-    const int equals = want - above;     // so many rows of that weight stay, the lowest ones (none when want is 0)
+    const uint32_t least = prefix;   // smallest kept weight; above it everything stays
+    const int equals = want - above; // so many rows of that weight stay, the lowest ones (none when nothing is wanted)
 
-    int seen = 0, holes = 0, kept_behind = 0;
-    int *hole_list = a.holes + unit * (a.c.T / 2), *move_list = a.moves + unit * (a.c.T / 2);
-    for (int base = 0; base < n; base += kSelThreads * kRowsPerThread) {
-        const int r0 = base + tid * kRowsPerThread;
-        uint32_t eq = 0, keep = 0; // bit i: row r0 + i
-#pragma unroll
-        for (int i = 0; i < kRowsPerThread; ++i) {
-            const int r = r0 + i;
-            if (r >= n) continue;
-            const bool safe = is_safe(a, pos[r], next);
-            if (safe != among_safe) {
-                if (safe) keep |= 1u << i;
-                continue;
-            }
-            const uint32_t k = ordered(w[r]);
-            if (k > least) keep |= (want > 0) ? 1u << i : 0u;
-            else if (k == least) eq |= 1u << i;
+    // rows of that weight in front of this thread
+    int eq = 0;
+    each([&](int, uint32_t k, bool s) { eq += s == among_safe && k == least; });
+    long long total;
+    int e = (int)block_scan(eq, ws[0], total);
+    if (tid == 0) n_equal = (int)total;
+    all_sync(cluster, ranks);
+    for (int c = 0; c < rank; ++c) e += *cluster.map_shared_rank(&n_equal, c);
+    // holes and sources in front of this thread
+    int holes = 0, behind = 0;
+    const int e0 = e;
+    uint32_t stay_bits = 0; // REGS: what the first look found
+    auto kept = [&](uint32_t k, bool s) { // in row order
+        if (s != among_safe) return s;
+        if (k == least) return e++ < equals;
+        return k > least && want > 0;
+    };
+    each([&](int r, uint32_t k, bool s) {
+        const bool stay = kept(k, s);
+        if (REGS) stay_bits |= (uint32_t)stay << (r - r0);
+        holes += r < m && !stay;
+        behind += r >= m && stay;
+    });
+    const long long before = block_scan((long long)holes | ((long long)behind << 32), ws[1], total);
+    if (tid == 0) n_lists = total;
+    all_sync(cluster, ranks);
+    int hr = (int)(before & 0xffffffff), br = (int)(before >> 32), all_holes = 0;
+    for (int c = 0; c < ranks; ++c) {
+        const long long t = *cluster.map_shared_rank(&n_lists, c);
+        if (c < rank) {
+            hr += (int)(t & 0xffffffff);
+            br += (int)(t >> 32);
         }
-        int total;
-        int e = seen + block_scan(__popc(eq), ws, total);
-        seen += total;
-#pragma unroll
-        for (int i = 0; i < kRowsPerThread; ++i)
-            if (eq >> i & 1u) {
-                if (e < equals) keep |= 1u << i;
-                ++e;
-            }
-        uint32_t hole = 0, from = 0;
-#pragma unroll
-        for (int i = 0; i < kRowsPerThread; ++i) {
-            const int r = r0 + i;
-            if (r < m) hole |= (~keep >> i & 1u) << i;
-            else if (r < n) from |= (keep >> i & 1u) << i;
-        }
-        int hrank = holes + block_scan(__popc(hole), ws, total);
-        holes += total;
-        int frank = kept_behind + block_scan(__popc(from), ws, total);
-        kept_behind += total;
-#pragma unroll
-        for (int i = 0; i < kRowsPerThread; ++i) {
-            const int r = r0 + i;
-            if (r <= m && (r & ((1 << a.c.block_shift) - 1)) == 0) off[r >> a.c.block_shift] = hrank;
-            if (hole >> i & 1u) hole_list[hrank++] = r;
-            if (from >> i & 1u) move_list[frank++] = r;
-        }
+        all_holes += (int)(t & 0xffffffff);
     }
+    e = e0;
+    int *hole_list = a.holes + unit * (a.c.T / 2), *move_list = a.moves + unit * (a.c.T / 2);
+    const int in_block = (1 << a.c.block_shift) - 1;
+    each([&](int r, uint32_t k, bool s) {
+        const bool stay = REGS ? (stay_bits >> (r - r0) & 1u) != 0 : kept(k, s);
+        if (r <= m && (r & in_block) == 0) off[r >> a.c.block_shift] = hr;
+        if (r < m && !stay) hole_list[hr++] = r;
+        if (r >= m && stay) move_list[br++] = r;
+    });
     // blocks from the one behind row m on: no holes
-    const int first = (m + (1 << a.c.block_shift) - 1) >> a.c.block_shift;
-    for (int j = first + tid; j <= a.c.nblk; j += kSelThreads) off[j] = holes;
+    for (int j = ((m + in_block) >> a.c.block_shift) + rank * kSelThreads + tid; j <= a.c.nblk; j += ranks * kSelThreads) off[j] = all_holes;
+    __threadfence();
+    all_sync(cluster, ranks); // the lists are whole; nobody's shared memory is read any more
+    // weights and positions: what stays, where the result is another buffer, then the holes
+    if (w_out != w || p_out != pos) {
+        for (int r = 4 * v0 + tid; r < min(m, 4 * v1); r += kSelThreads) {
+            w_out[r] = w[r];
+            p_out[r] = pos[r];
+        }
+        __threadfence();
+        all_sync(cluster, ranks);
+    }
+    for (int i = rank * kSelThreads + tid; i < all_holes; i += ranks * kSelThreads) {
+        const int to = __ldcg(hole_list + i), from = __ldcg(move_list + i);
+        w_out[to] = w[from];
+        p_out[to] = pos[from];
+    }
 }
 
 constexpr int kChunks = 4; // 8-code chunks per thread
 
-template <int D, int CODE> __global__ void __launch_bounds__(1024) flb_kv8_move_kernel(const __grid_constant__ Kv8EvictArgs a) {
+constexpr int kGroup = 4;  // blocks that a CTA looks after, one after the other
+
+template <int D, int CODE> __global__ void __launch_bounds__(1024) flb_kv8_move_kernel(const __grid_constant__ Kv8EvictArgs a, int groups) {
     constexpr int CPR = D / 8;
     __shared__ uint32_t red[32];
     __shared__ int from_s[128]; // source of every row of the block, -1 = stays
+    kv8_begin();
+    if (blockIdx.x == 0) { // len_out may be past_lens: nobody reads that any more
+        int bad = 0;
+        for (int b = threadIdx.x; b < a.c.B; b += blockDim.x) {
+            const int n = __ldcg(a.seq_len + 2 * b + 1);
+            a.len_out[b] = n;
+            bad |= n < 0 || n > a.c.T;
+        }
+        bad = __syncthreads_or(bad);
+        if (threadIdx.x == 0) *a.status = bad ? kKv8BadLen : 0u;
+    }
     unsigned id = blockIdx.x;
     const int kv = (int)(id & 1u);
     id >>= 1;
-    const int blk = (int)(id % (unsigned)a.c.nblk);
-    const size_t unit = id / (unsigned)a.c.nblk;
-    const int b = (int)(unit / a.c.H);
-    const int n = a.past_lens ? __ldg(a.past_lens + b) : a.start_pos;
-    if (n < 0 || n > a.c.T) return;
-    const int m = min(n, a.budget);
-    const int rows = 1 << a.c.block_shift, row0 = blk << a.c.block_shift;
-    if (row0 >= m) return;
-    const int lo = a.hole_off[unit * (a.c.nblk + 1) + blk], hi = a.hole_off[unit * (a.c.nblk + 1) + blk + 1];
+    const int blk0 = (int)(id % (unsigned)groups) * kGroup;
+    const size_t unit = id / (unsigned)groups;
+    const int *off = a.hole_off + unit * (a.c.nblk + 1);
+    const int blk1 = min(blk0 + kGroup, a.c.nblk);
+    if (__ldcg(off + blk0) == __ldcg(off + blk1)) return; // no hole in any of them
+    const int m = __ldcg(a.seq_len + 2 * (int)(unit / a.c.H));
+    const int rows = 1 << a.c.block_shift, edge = m >> a.c.block_shift;
     const int *hole_list = a.holes + unit * (a.c.T / 2), *move_list = a.moves + unit * (a.c.T / 2);
-    const size_t urow = unit * a.c.T;
-    const bool along = kv == 0 && (lo < hi || a.weight_out != a.weight || a.pos_out != a.c.row_pos);
-    if (lo >= hi && !along) return;
-    for (int i = threadIdx.x; i < rows; i += blockDim.x) from_s[i] = -1;
-    __syncthreads();
-    for (int i = lo + (int)threadIdx.x; i < hi; i += blockDim.x) from_s[hole_list[i] - row0] = move_list[i];
-    __syncthreads();
-    if (along) {
-        for (int i = threadIdx.x; i < rows && row0 + i < m; i += blockDim.x) {
-            const int src = from_s[i] < 0 ? row0 + i : from_s[i];
-            const float w = a.weight[urow + src];
-            const int p = a.c.row_pos[urow + src];
-            a.weight_out[urow + row0 + i] = w;
-            a.pos_out[urow + row0 + i] = p;
+    const uint8_t *all = a.c.codes[kv] + unit * a.c.T * D;
+    float *scales = a.c.scale[kv] + unit * a.c.nblk;
+    for (int blk = blk0; blk < blk1; ++blk) {
+        const int lo = __ldcg(off + blk), hi = __ldcg(off + blk + 1);
+        if (lo >= hi) continue;
+        const int row0 = blk << a.c.block_shift;
+        const float old = scales[blk];
+        __syncthreads(); // the block before is done with the shared arrays
+        for (int i = threadIdx.x; i < rows; i += blockDim.x) from_s[i] = -1;
+        __syncthreads();
+        for (int i = lo + (int)threadIdx.x; i < hi; i += blockDim.x) from_s[__ldcg(hole_list + i) - row0] = __ldcg(move_list + i);
+        __syncthreads();
+        uint2 *mine = reinterpret_cast<uint2 *>(a.c.codes[kv] + (unit * a.c.T + row0) * D);
+        uint2 u[kChunks];
+        float s[kChunks];
+#pragma unroll
+        for (int i = 0; i < kChunks; ++i) {
+            const int ch = threadIdx.x + i * blockDim.x, src = from_s[ch / CPR];
+            if (src < 0) continue;
+            u[i] = *reinterpret_cast<const uint2 *>(all + (size_t)src * D + (ch % CPR) * 8);
+            s[i] = (src >> a.c.block_shift) == edge ? __ldcg(a.edge_scale + unit * 2 + kv) : scales[src >> a.c.block_shift];
         }
-    }
-    if (lo >= hi) return;
-
-    const uint8_t *all = a.c.codes[kv] + urow * D;
-    uint2 *mine = reinterpret_cast<uint2 *>(a.c.codes[kv] + (urow + row0) * D);
-    const float *scales = a.c.scale[kv] + unit * a.c.nblk;
-    float x[kChunks][8];
-    uint32_t amax = 0;
-#pragma unroll
-    for (int i = 0; i < kChunks; ++i) {
-        const int ch = threadIdx.x + i * blockDim.x, src = from_s[ch / CPR];
-        if (src >= 0) {
-            const uint2 u = *reinterpret_cast<const uint2 *>(all + (size_t)src * D + (ch % CPR) * 8);
-            const float s = (src >> a.c.block_shift) == (m >> a.c.block_shift) ? a.edge_scale[unit * 2 + kv] : scales[src >> a.c.block_shift];
+        auto value = [&](int i, float(&x)[8]) {
             float p[4], q[4];
-            kv8_decode4<CODE>(u.x, p);
-            kv8_decode4<CODE>(u.y, q);
+            kv8_decode4<CODE>(u[i].x, p);
+            kv8_decode4<CODE>(u[i].y, q);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                x[i][e] = __fmul_rn(e < 4 ? p[e & 3] : q[e & 3], s);
-                amax = max(amax, kv8_abs_bits(x[i][e]));
+            for (int e = 0; e < 8; ++e) x[e] = __fmul_rn(e < 4 ? p[e & 3] : q[e & 3], s[i]);
+        };
+        uint32_t amax = 0;
+#pragma unroll
+        for (int i = 0; i < kChunks; ++i) {
+            if (from_s[(threadIdx.x + i * blockDim.x) / CPR] < 0) continue;
+            float x[8];
+            value(i, x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) amax = max(amax, kv8_abs_bits(x[e]));
+        }
+        amax = kv8_block_max(amax, red);
+        const float scale = kv8_new_scale<CODE>(amax, old);
+        const bool grown = old > 0.f && scale > old;
+        const float ratio = grown ? __fdiv_rn(old, scale) : 1.f, inv = __fdiv_rn(1.f, scale);
+#pragma unroll
+        for (int i = 0; i < kChunks; ++i) {
+            const int ch = threadIdx.x + i * blockDim.x;
+            if (from_s[ch / CPR] >= 0) {
+                float x[8];
+                value(i, x);
+                mine[ch] = kv8_encode8<CODE>(x, scale, inv);
+            } else if (grown && row0 + ch / CPR < m) {
+                mine[ch] = kv8_rescale8<CODE>(mine[ch], ratio);
             }
         }
-    }
-    amax = kv8_block_max(amax, red);
-    const float old = scales[blk];
-    __syncthreads(); // the old scale has been read
-    const float scale = kv8_new_scale<CODE>(amax, old);
-    const bool grown = old > 0.f && scale > old;
-    const float ratio = grown ? __fdiv_rn(old, scale) : 1.f;
-#pragma unroll
-    for (int i = 0; i < kChunks; ++i) {
-        const int ch = threadIdx.x + i * blockDim.x;
-        if (from_s[ch / CPR] >= 0)
-            mine[ch] = kv8_encode8<CODE>(x[i], scale);
-        else if (grown && row0 + ch / CPR < m)
-            mine[ch] = kv8_rescale8<CODE>(mine[ch], ratio);
-    }
-    if (threadIdx.x == 0) a.c.scale[kv][unit * a.c.nblk + blk] = scale;
-}
-
-__global__ void flb_kv8_lens_kernel(const __grid_constant__ Kv8EvictArgs a) {
-    for (int b = threadIdx.x; b < a.c.B; b += blockDim.x) {
-        const int n = a.past_lens ? a.past_lens[b] : a.start_pos;
-        a.len_out[b] = (n < 0 || n > a.c.T) ? n : min(n, a.budget);
+        if (threadIdx.x == 0) scales[blk] = scale;
     }
 }
 
 template <int D, int CODE> cudaError_t launch_t(const Kv8EvictArgs &a, cudaStream_t stream) {
     const unsigned units = (unsigned)a.c.B * (unsigned)a.c.H;
-    flb_kv8_select_kernel<<<units, kSelThreads, 0, stream>>>(a);
-    cudaError_t e = cudaGetLastError();
+    // One CTA per head up to 8192 rows, eight beyond (a portable cluster); up to 16 rows per thread keys stay in registers.
+    const int ranks = a.c.T <= 8192 ? 1 : 8;
+    const bool regs = (long long)a.c.T <= (long long)ranks * kSelThreads * kRegRows;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)ranks;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(units * (unsigned)ranks);
+    cfg.blockDim = dim3(kSelThreads);
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, regs ? flb_kv8_select_kernel<true> : flb_kv8_select_kernel<false>, a);
     if (e != cudaSuccess) return e;
-    flb_kv8_move_kernel<D, CODE><<<units * (unsigned)a.c.nblk * 2u, (unsigned)((D << a.c.block_shift) / (8 * kChunks)), 0, stream>>>(a);
-    e = cudaGetLastError();
-    if (e != cudaSuccess) return e;
-    flb_kv8_lens_kernel<<<1, 256, 0, stream>>>(a); // last: len_out may be past_lens
-    return cudaGetLastError();
+    const int kept_blocks = (min(a.c.T, a.budget) + (1 << a.c.block_shift) - 1) >> a.c.block_shift;
+    const int groups = (kept_blocks + kGroup - 1) / kGroup;
+    return kv8_launch(flb_kv8_move_kernel<D, CODE>, units * (unsigned)groups * 2u, (unsigned)((D << a.c.block_shift) / (8 * kChunks)), 0, stream, a, groups);
 }
 
 } // namespace

@@ -122,7 +122,7 @@ int check_decode_sizes(const flb_kv8_decode_params *p) {
 
 size_t evict_bytes(const flb_kv8_cache &c) {
     const size_t units = (size_t)c.batch_size * c.kv_head_num;
-    return 256 + round_up(units * 2 * sizeof(float), 256) + round_up(units * (c.total_len / c.block_len + 1) * sizeof(int), 256) +
+    return 256 + round_up((size_t)c.batch_size * 2 * sizeof(int), 256) + round_up(units * 2 * sizeof(float), 256) + round_up(units * (c.total_len / c.block_len + 1) * sizeof(int), 256) +
            2 * round_up(units * (c.total_len / 2) * sizeof(int), 256); // a hole has a source: at most half the rows are either
 }
 
@@ -186,7 +186,8 @@ int flb_kv8_validate_evict(const flb_kv8_evict_params *p) {
     if (p->budget <= 0 || p->recent < 0 || p->sinks < 0 || p->recent > p->budget || p->sinks > p->budget - p->recent) return FLB_ERR_BAD_SHAPE;
     if (!p->past_lens && (p->start_pos < 0 || p->start_pos > p->cache.total_len)) return FLB_ERR_BAD_SHAPE;
     if (!aligned16(p->scratch)) return FLB_ERR_MISALIGNED;
-    if (2ull * p->cache.batch_size * p->cache.kv_head_num * (p->cache.total_len / p->cache.block_len) > 0x7fffffffull) return FLB_ERR_TOO_LARGE;
+    if (!aligned16(p->weight) || !aligned16(p->cache.row_pos) || !aligned4(p->weight_out) || !aligned4(p->pos_out)) return FLB_ERR_MISALIGNED;
+    if (8ull * p->cache.batch_size * p->cache.kv_head_num * (p->cache.total_len / p->cache.block_len + 1) > 0x7fffffffull) return FLB_ERR_TOO_LARGE;
     if (p->scratch_bytes < evict_bytes(p->cache)) return FLB_ERR_SCRATCH_TOO_SMALL;
     return FLB_OK;
 }
@@ -308,7 +309,6 @@ int flb_kv8_evict(const flb_kv8_evict_params *p, void *cuda_stream) {
     cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
     const size_t units = (size_t)p->cache.batch_size * p->cache.kv_head_num, T = p->cache.total_len;
     unsigned char *sc = static_cast<unsigned char *>(p->scratch);
-    if (cudaMemsetAsync(sc, 0, 16, stream) != cudaSuccess) return FLB_ERR_LAUNCH;
     flb::Kv8EvictArgs a;
     a.c = cache_of(p->cache);
     a.start_pos = p->start_pos;
@@ -323,6 +323,8 @@ int flb_kv8_evict(const flb_kv8_evict_params *p, void *cuda_stream) {
     a.pos_out = p->pos_out;
     a.status = reinterpret_cast<unsigned *>(sc);
     size_t o = 256;
+    a.seq_len = reinterpret_cast<int *>(sc + o);
+    o += round_up((size_t)p->cache.batch_size * 2 * sizeof(int), 256);
     a.edge_scale = reinterpret_cast<float *>(sc + o);
     o += round_up(units * 2 * sizeof(float), 256);
     a.hole_off = reinterpret_cast<int *>(sc + o);
