@@ -175,70 +175,97 @@ template <int CODE> __device__ __forceinline__ float kv8_new_scale(uint32_t amax
 // Four values to four codes: rne, as a byte each.  int8: the addition of 1.5 * 2^23 rounds to a whole number and leaves it in the low byte.
 template <int CODE> __device__ __forceinline__ uint32_t kv8_pack4(const float (&y)[4]) {
     if (CODE == kCodeI8) {
-        uint32_t t[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) t[i] = __float_as_uint(__fadd_rn(y[i], 12582912.0f));
-        return __byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410);
+        const float2 magic = make_float2(12582912.0f, 12582912.0f);
+        const float2 a = __fadd2_rn(make_float2(y[0], y[1]), magic), b = __fadd2_rn(make_float2(y[2], y[3]), magic);
+        return __byte_perm(__byte_perm(__float_as_uint(a.x), __float_as_uint(a.y), 0x0040), __byte_perm(__float_as_uint(b.x), __float_as_uint(b.y), 0x0040), 0x5410);
     }
     const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3);
     const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3);
     return lo | (hi << 16);
 }
-// Whether a quotient that is off by up to 2^-22 of itself could round to another code than the exact one: it lies that near to the middle
-// between two codes.
-template <int CODE> __device__ __forceinline__ bool kv8_near_tie(float y) {
+// Whether among quotients that are off by up to 2^-22 of themselves one could round to another code than the exact one: it lies that near
+// to the middle between two codes.
+template <int CODE> __device__ __forceinline__ bool kv8_near_tie(const float (&y)[8]) {
     if (CODE == kCodeI8) {
-        const float whole = __fsub_rn(__fadd_rn(y, 12582912.0f), 12582912.0f);
-        return fabsf(y - whole) > 0.5f - 6.1035156e-5f; // 2^-14 > 127 * 2^-22
+        const float2 magic = make_float2(12582912.0f, 12582912.0f), back = make_float2(-12582912.0f, -12582912.0f);
+        float far = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) { // distance to the whole number
+            const float2 v = make_float2(y[i], y[i + 1]), w = __fadd2_rn(__fadd2_rn(v, magic), back);
+            const float2 d = __fadd2_rn(v, make_float2(-w.x, -w.y));
+            far = max3(far, fabsf(d.x), fabsf(d.y));
+        }
+        return far > 0.5f - 6.1035156e-5f; // 2^-14 > 127 * 2^-22
     }
     // e4m3 keeps 3 of the 23 mantissa bits (fewer below 2^-6: always looked at exactly there)
-    const uint32_t u = __float_as_uint(y) & 0x7fffffffu;
-    return u < 0x3c800000u || ((u + 8u) & 0xfffffu) - 0x80000u <= 16u;
+    bool near = false;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t u = __float_as_uint(y[i]) & 0x7fffffffu;
+        near = near || u < 0x3c800000u || ((u + 8u) & 0xfffffu) - 0x80000u <= 16u;
+    }
+    return near;
 }
 // Eight values over their block's scale, rounded to codes; `inv` = 1 / scale.  The quotient is defined as one IEEE division; multiplying by
 // the reciprocal is off by 2^-22 at most, which shows only next to a tie, and there the division is done.  A scale of 0, infinity or NaN gives
 // codes 0.
 template <int CODE> __device__ __forceinline__ uint2 kv8_encode8(const float (&x)[8], float scale, float inv) {
-    const bool ok = scale > 0.f && scale <= 3.402823466e38f;
+    if (!(scale > 0.f && scale <= 3.402823466e38f)) return make_uint2(0u, 0u);
     const bool exact = !(inv <= 3.402823466e38f && scale <= 1e37f); // the reciprocal of a subnormal scale overflows, that of a huge one is subnormal
-    float y[2][4];
-    bool near = false;
+    float y[8];
+    const float2 inv2 = make_float2(inv, inv);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        y[i >> 2][i & 3] = ok ? __fmul_rn(x[i], inv) : 0.f;
-        near = near || kv8_near_tie<CODE>(y[i >> 2][i & 3]);
+    for (int i = 0; i < 8; i += 2) {
+        const float2 v = __fmul2_rn(make_float2(x[i], x[i + 1]), inv2);
+        y[i] = v.x;
+        y[i + 1] = v.y;
     }
-    if (ok && (near || exact)) {
+    if (exact || kv8_near_tie<CODE>(y)) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i >> 2][i & 3] = __fdiv_rn(x[i], scale);
+        for (int i = 0; i < 8; ++i) y[i] = __fdiv_rn(x[i], scale);
     }
-    return make_uint2(kv8_pack4<CODE>(y[0]), kv8_pack4<CODE>(y[1]));
+    const float a[4] = {y[0], y[1], y[2], y[3]}, b[4] = {y[4], y[5], y[6], y[7]};
+    return make_uint2(kv8_pack4<CODE>(a), kv8_pack4<CODE>(b));
 }
-template <int CODE> __device__ __forceinline__ void kv8_decode4(uint32_t w, float (&x)[4]) {
-    if (CODE == kCodeI8) {
-        w ^= 0x80808080u; // byte + 128 under the exponent of 2^23
+// what eight codes stand for, before the scale
+template <int CODE> __device__ __forceinline__ void kv8_decode8(uint2 u, float (&x)[8]) {
+    const uint32_t w[2] = {u.x, u.y};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = __fsub_rn(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 + i)), 8388736.0f);
-    } else {
+    for (int j = 0; j < 2; ++j) {
+        if (CODE == kCodeI8) { // byte + 128 under the exponent of 2^23
+            const uint32_t v = w[j] ^ 0x80808080u;
+            const float2 back = make_float2(-8388736.0f, -8388736.0f);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> (16 * i)), __NV_E4M3);
-            const float2 f = __half22float2(__half2(h));
-            x[2 * i] = f.x;
-            x[2 * i + 1] = f.y;
+            for (int i = 0; i < 4; i += 2) {
+                const float2 f = __fadd2_rn(make_float2(__uint_as_float(__byte_perm(v, 0x4b000000u, 0x7440 + i)), __uint_as_float(__byte_perm(v, 0x4b000000u, 0x7441 + i))), back);
+                x[4 * j + i] = f.x;
+                x[4 * j + i + 1] = f.y;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[j] >> (16 * i)), __NV_E4M3);
+                const float2 f = __half22float2(__half2(h));
+                x[4 * j + 2 * i] = f.x;
+                x[4 * j + 2 * i + 1] = f.y;
+            }
         }
+    }
+}
+__device__ __forceinline__ void kv8_scale8(float (&x)[8], float s) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        const float2 v = __fmul2_rn(make_float2(x[i], x[i + 1]), make_float2(s, s));
+        x[i] = v.x;
+        x[i + 1] = v.y;
     }
 }
 // codes of a block that a larger scale takes over: ratio = old / new
 template <int CODE> __device__ __forceinline__ uint2 kv8_rescale8(uint2 u, float ratio) {
-    float a[4], b[4];
-    kv8_decode4<CODE>(u.x, a);
-    kv8_decode4<CODE>(u.y, b);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        a[i] = __fmul_rn(a[i], ratio);
-        b[i] = __fmul_rn(b[i], ratio);
-    }
+    float x[8];
+    kv8_decode8<CODE>(u, x);
+    kv8_scale8(x, ratio);
+    const float a[4] = {x[0], x[1], x[2], x[3]}, b[4] = {x[4], x[5], x[6], x[7]};
     return make_uint2(kv8_pack4<CODE>(a), kv8_pack4<CODE>(b));
 }
 
