@@ -109,12 +109,27 @@ cudaError_t launch_kv8_decode(const Kv8DecodeArgs &a, int d, int code, int nt, c
 cudaError_t launch_kv8_evict(const Kv8EvictArgs &a, int d, int code, cudaStream_t stream);
 
 // ---- inputs --------------------------------------------------------------------------------------
-// Eight consecutive values of a row.  MODE 0: float(acc) * act_scale * w_scale, in this order; 1: fp32; 2: fp16.
-template <int MODE> __device__ __forceinline__ void kv8_load8(const Kv8Input &in, const float *act_scale, size_t token, int col, float (&x)[8]) {
+// Eight consecutive elements as they lie in memory, and what they stand for.  MODE 0: float(acc) * act_scale * w_scale, in this order; 1: fp32;
+// 2: fp16.  Apart, so that a thread can have several loads under way.
+struct Kv8Raw {
+    uint4 lo, hi; // fp16: lo only
+};
+template <int MODE> __device__ __forceinline__ Kv8Raw kv8_raw8(const Kv8Input &in, size_t token, int col) {
     const size_t off = token * in.row_stride + col;
+    Kv8Raw r;
     if (MODE == 2) {
-        const uint4 u = __ldg(reinterpret_cast<const uint4 *>((const __half *)in.p + off));
-        const __half2 *h = reinterpret_cast<const __half2 *>(&u);
+        r.lo = __ldg(reinterpret_cast<const uint4 *>((const __half *)in.p + off));
+        r.hi = make_uint4(0u, 0u, 0u, 0u);
+    } else {
+        const uint4 *p = reinterpret_cast<const uint4 *>((const uint32_t *)in.p + off);
+        r.lo = __ldg(p);
+        r.hi = __ldg(p + 1);
+    }
+    return r;
+}
+template <int MODE> __device__ __forceinline__ void kv8_values8(const Kv8Raw &r, const Kv8Input &in, const float *act_scale, size_t token, int col, float (&x)[8]) {
+    if (MODE == 2) {
+        const __half2 *h = reinterpret_cast<const __half2 *>(&r.lo);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float2 f = __half22float2(h[i]);
@@ -122,34 +137,38 @@ template <int MODE> __device__ __forceinline__ void kv8_load8(const Kv8Input &in
             x[2 * i + 1] = f.y;
         }
     } else {
-        const uint4 *p = reinterpret_cast<const uint4 *>((const uint32_t *)in.p + off);
-        const uint4 a = __ldg(p), b = __ldg(p + 1);
-        const uint32_t r[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        const uint32_t u[8] = {r.lo.x, r.lo.y, r.lo.z, r.lo.w, r.hi.x, r.hi.y, r.hi.z, r.hi.w};
         if (MODE == 1) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(r[i]);
+            for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(u[i]);
         } else {
             const float as = __ldg(act_scale + token);
             const float4 *w = reinterpret_cast<const float4 *>(in.w_scale + col);
             const float4 w0 = __ldg(w), w1 = __ldg(w + 1);
             const float ws[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(__fmul_rn((float)(int)r[i], as), ws[i]);
+            for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(__fmul_rn((float)(int)u[i], as), ws[i]);
         }
     }
+}
+template <int MODE> __device__ __forceinline__ void kv8_load8(const Kv8Input &in, const float *act_scale, size_t token, int col, float (&x)[8]) {
+    kv8_values8<MODE>(kv8_raw8<MODE>(in, token, col), in, act_scale, token, col, x);
 }
 
 // Rotation of the pairs (2i, 2i+1) of eight values by a table row (its entries at the same columns).  Every product is
 // rounded before the sum, so that the stored codes do not depend on where a compiler fuses.
-__device__ __forceinline__ void kv8_rotate8(const float *row, float (&x)[8]) {
-    const float4 f0 = __ldg(reinterpret_cast<const float4 *>(row)), f1 = __ldg(reinterpret_cast<const float4 *>(row) + 1);
+__device__ __forceinline__ void kv8_rotate8(const float4 &f0, const float4 &f1, float (&x)[8]) {
     const float cs[8] = {f0.x, f0.y, f0.z, f0.w, f1.x, f1.y, f1.z, f1.w};
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
         const float a = x[i], b = x[i + 1];
+        // (the packed forms of these would be fused)
         x[i] = __fsub_rn(__fmul_rn(a, cs[i]), __fmul_rn(b, cs[i + 1]));
         x[i + 1] = __fadd_rn(__fmul_rn(b, cs[i]), __fmul_rn(a, cs[i + 1]));
     }
+}
+__device__ __forceinline__ void kv8_rotate8(const float *row, float (&x)[8]) {
+    kv8_rotate8(__ldg(reinterpret_cast<const float4 *>(row)), __ldg(reinterpret_cast<const float4 *>(row) + 1), x);
 }
 
 // table row of a position; one outside the table is flagged and the nearest row taken
@@ -163,6 +182,12 @@ __device__ __forceinline__ int kv8_table_row(int pos, int rows, unsigned *status
 constexpr int kCodeI8 = 0, kCodeE4M3 = 1;
 template <int CODE> __device__ __forceinline__ constexpr float kv8_top() { return CODE == kCodeI8 ? 127.0f : 448.0f; }
 
+// largest magnitude of eight values and `m`; a NaN stays
+__device__ __forceinline__ float kv8_abs_max8(float m, const float (&x)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) asm("max.NaN.abs.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(x[i]), "f"(x[i + 1]));
+    return m;
+}
 // magnitude bits: ordered like the magnitude, NaN above infinity
 __device__ __forceinline__ uint32_t kv8_abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
@@ -192,8 +217,8 @@ template <int CODE> __device__ __forceinline__ bool kv8_near_tie(const float (&y
 #pragma unroll
         for (int i = 0; i < 8; i += 2) { // distance to the whole number
             const float2 v = make_float2(y[i], y[i + 1]), w = __fadd2_rn(__fadd2_rn(v, magic), back);
-            const float2 d = __fadd2_rn(v, make_float2(-w.x, -w.y));
-            far = max3(far, fabsf(d.x), fabsf(d.y));
+            const float2 d = __ffma2_rn(w, make_float2(-1.0f, -1.0f), v);
+            asm("max.abs.f32 %0, %0, %1, %2;" : "+f"(far) : "f"(d.x), "f"(d.y));
         }
         return far > 0.5f - 6.1035156e-5f; // 2^-14 > 127 * 2^-22
     }
@@ -264,7 +289,8 @@ __device__ __forceinline__ void kv8_scale8(float (&x)[8], float s) {
 template <int CODE> __device__ __forceinline__ uint2 kv8_rescale8(uint2 u, float ratio) {
     float x[8];
     kv8_decode8<CODE>(u, x);
-    kv8_scale8(x, ratio);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(x[i], ratio); // rounded, then rounded to a code: not to be fused with the packing's addition
     const float a[4] = {x[0], x[1], x[2], x[3]}, b[4] = {x[4], x[5], x[6], x[7]};
     return make_uint2(kv8_pack4<CODE>(a), kv8_pack4<CODE>(b));
 }
