@@ -37,8 +37,14 @@ def _ptr(t: Any) -> int | None:
     return t.ctypes.data  # numpy
 
 
+_DTYPE_NAMES: dict[Any, str] = {}
+
+
 def _dtype_name(t: Any) -> str:
-    return str(t.dtype).replace("torch.", "")
+    n = _DTYPE_NAMES.get(t.dtype)
+    if n is None:
+        n = _DTYPE_NAMES[t.dtype] = str(t.dtype).replace("torch.", "")
+    return n
 
 
 def _is_contiguous(t: Any) -> bool:
@@ -55,6 +61,8 @@ def _token_row_stride(t: Any, B: int, S: int, H: int, d: int) -> int:
     """Elements between the rows of two consecutive tokens of a q/k/v tensor shaped [B,S,H,d]: H*d when it is dense,
     more when it is a column block of a wider [B*S, row] buffer (the output of one merged QKV projection).  Raises
     for any other layout."""
+    if _is_contiguous(t):
+        return H * d
     if hasattr(t, "stride") and callable(t.stride):
         st = tuple(int(x) for x in t.stride())
     else:
@@ -156,49 +164,87 @@ def make_params(
     return p
 
 
-def make_scored_params(*, q, k, v, k_cache, v_cache, out, softcap: float = 0.0, alibi_slopes=None, key_begin=None, key_end=None,
-                       **kw) -> tuple[FlbAttnParams, FlbScoreForm]:
-    """The parameter block of `make_params` and the score form beside it (see flb_score_form): capped scores, distance bias (float32 [H]),
+_PACK_PARAMS, _PACK_FORM = _lib.packer(FlbAttnParams), _lib.packer(FlbScoreForm)
+
+
+def _check(t: Any, name: str, shape: tuple, dtype: str) -> int:
+    """Address of a dense tensor of this shape and type, 0 for None."""
+    if t is None:
+        return 0
+    if tuple(t.shape) != shape or _dtype_name(t) != dtype or not _is_contiguous(t):
+        raise ValueError(f"{name} must be a dense {dtype} tensor of shape {shape}")
+    return _ptr(t)
+
+
+def make_scored_params(
+    *,
+    q,
+    k,
+    v,
+    k_cache,
+    v_cache,
+    out,
+    softcap: float = 0.0,
+    alibi_slopes=None,
+    key_begin=None,
+    key_end=None,
+    scratch=None,
+    start_pos: int = 0,
+    past_lens=None,
+    max_past_len: int = 0,
+    act_scale=None,
+    q_w_scale=None,
+    k_w_scale=None,
+    v_w_scale=None,
+    freq_cis=None,
+    rope_pos0: int = 0,
+    rope_add_past: bool = False,
+    mask_mode: int = FLB_MASK_CAUSAL_INCLUSIVE,
+    attn_mask=None,
+    mask_row_stride: int = 0,
+    softmax_scale: float | None = None,
+    scratch_zeroed: bool = False,
+    split_len: int = 0,
+    out_q8=None,
+    out_q8_scale=None,
+    early_start: int = 0,
+) -> tuple[FlbAttnParams, FlbScoreForm]:
+    """A parameter block as from `make_params` and the score form beside it (see flb_score_form): capped scores, distance bias (float32 [H]),
     per-row key bounds (int32, decode [B], prefill [B,S]), and k, v [B,S,Hkv,d] with caches [B,Hkv,T,d] of fewer heads than q."""
-    B, S, H, d = (int(x) for x in q.shape)
-    Hkv = int(k.shape[2])
+    B, S, H, d = q.shape
+    Hkv, T, dt = k.shape[2], k_cache.shape[2], _dtype_name(q)
     if tuple(k.shape) != (B, S, Hkv, d) or tuple(v.shape) != (B, S, Hkv, d) or H % Hkv:
         raise ValueError("k and v must be [B,S,Hkv,d] with a number of heads that divides q's")
-    if tuple(k_cache.shape) != tuple(v_cache.shape) or tuple(k_cache.shape[:2]) != (B, Hkv) or k_cache.shape[3] != d:
-        raise ValueError("caches must be [B, Hkv, T, d]")
-    if not _is_contiguous(k_cache) or not _is_contiguous(v_cache):
-        raise ValueError("the caches must be contiguous")
-    if _dtype_name(k) != _dtype_name(q) or _dtype_name(v) != _dtype_name(q):
-        raise ValueError("q, k and v must share one type")
-    rows = (B,) if S == 1 else (B, S)
-    for name, t, shape, dtype in (("alibi_slopes", alibi_slopes, (H,), "float32"), ("key_begin", key_begin, rows, "int32"), ("key_end", key_end, rows, "int32")):
-        if t is not None and (tuple(t.shape) != shape or _dtype_name(t) != dtype or not _is_contiguous(t)):
-            raise ValueError(f"{name} must be a dense {dtype} tensor of shape {shape}")
-    strides = {_token_row_stride(t, B, S, Hkv, d) for t in (k, v)}
-    if len(strides) != 1:
+    if _dtype_name(k) != dt or _dtype_name(v) != dt or dt not in _IN_MODE:
+        raise ValueError("q, k and v must share one type: int32, float32 or float16")
+    cdt, odt = _dtype_name(k_cache), _dtype_name(out)
+    if cdt not in _DT or odt not in _DT:
+        raise ValueError("caches and out must be float32 or float16")
+    row, krow, vrow = _token_row_stride(q, B, S, H, d), _token_row_stride(k, B, S, Hkv, d), _token_row_stride(v, B, S, Hkv, d)
+    if krow != vrow:
         raise ValueError("k and v must share one token-row stride")
-    # make_params looks at one head count: q stands in for k and v there, and their own addresses and sizes follow
-    p = make_params(q=q, k=q, v=q, k_cache=_Heads(k_cache, H), v_cache=_Heads(v_cache, H), out=out, **kw)
-    p.k, p.v = _ptr(k), _ptr(v)
-    f = FlbScoreForm()
-    f.kv_head_num, f.kv_row_stride, f.softcap = Hkv, strides.pop(), float(softcap)
-    f.alibi_slopes, f.key_begin, f.key_end = _ptr(alibi_slopes), _ptr(key_begin), _ptr(key_end)
-    p._keep = (*p._keep, k, v, k_cache, v_cache)
+    rows = (B,) if S == 1 else (B, S)
+    if attn_mask is not None and not mask_row_stride:
+        mask_row_stride = attn_mask.shape[-1]
+    if scratch is None:
+        sp = sn = 0
+    else:
+        sp, sn = _ptr(scratch), scratch.numel() * scratch.element_size() if hasattr(scratch, "numel") else scratch.nbytes
+    p = FlbAttnParams.from_buffer_copy(_PACK_PARAMS.pack(
+        B, H, d, S, start_pos, T, _check(past_lens, "past_lens", (B,), "int32"), max_past_len, _IN_MODE[dt], _ptr(q), _ptr(k), _ptr(v), _ptr(act_scale) or 0,
+        _ptr(q_w_scale) or 0, _ptr(k_w_scale) or 0, _ptr(v_w_scale) or 0, _ptr(freq_cis) or 0, rope_pos0, 1 if rope_add_past else 0, mask_mode,
+        _ptr(attn_mask) or 0, mask_row_stride, _check(k_cache, "k_cache", (B, Hkv, T, d), cdt), _check(v_cache, "v_cache", (B, Hkv, T, d), cdt), _DT[cdt],
+        _check(out, "out", (B, H, S, d), odt), _DT[odt], softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(d), sp, sn, 1 if scratch_zeroed else 0,
+        split_len, _ptr(out_q8) or 0, _ptr(out_q8_scale) or 0, *_NO_PEERS, 0, 0, 0, early_start, 0 if row == H * d else row))
+    f = FlbScoreForm.from_buffer_copy(_PACK_FORM.pack(
+        Hkv, krow, softcap, _check(alibi_slopes, "alibi_slopes", (H,), "float32"), _check(key_begin, "key_begin", rows, "int32"), _check(key_end, "key_end", rows, "int32")))
+    # keep the tensors alive as long as the blocks
+    p._keep = (q, k, v, k_cache, v_cache, out, scratch, past_lens, act_scale, q_w_scale, k_w_scale, v_w_scale, freq_cis, attn_mask, out_q8, out_q8_scale)
     f._keep = (alibi_slopes, key_begin, key_end)
     return p, f
 
 
-class _Heads:
-    """A cache seen with another number of heads, for the shape checks of `make_params`."""
-
-    def __init__(self, t, heads: int):
-        self.t, self.shape, self.dtype = t, (t.shape[0], heads, t.shape[2], t.shape[3]), t.dtype
-
-    def data_ptr(self) -> int:
-        return _ptr(self.t)
-
-    def is_contiguous(self) -> bool:
-        return True
+_NO_PEERS = (0,) * _lib.FLB_MAX_PEERS
 
 
 def workspace_bytes(batch_size: int, head_num: int, total_len: int, seq_len: int = 1, split_len: int = 0,

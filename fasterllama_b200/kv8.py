@@ -66,6 +66,8 @@ class FlbKv8Evict(C.Structure):
     ]
 
 
+_PACK_APPEND, _PACK_DECODE, _PACK_EVICT = (_lib.packer(c) for c in (FlbKv8Append, FlbKv8Decode, FlbKv8Evict))
+
 # every symbol include/flb_kv8.h declares: name -> (restype, argtypes)
 _SIZE = C.POINTER(C.c_size_t)
 EXPORTS = {
@@ -75,9 +77,9 @@ EXPORTS = {
     "flb_kv8_decode_workspace_bytes": (C.c_int, [C.POINTER(FlbKv8Decode), _SIZE]),
     "flb_kv8_counter_bytes": (C.c_int, [C.POINTER(FlbKv8Decode), _SIZE]),
     "flb_kv8_evict_workspace_bytes": (C.c_int, [C.POINTER(FlbKv8Evict), _SIZE]),
-    "flb_kv8_append": (C.c_int, [C.POINTER(FlbKv8Append), C.c_void_p]),
-    "flb_kv8_decode": (C.c_int, [C.POINTER(FlbKv8Decode), C.c_void_p]),
-    "flb_kv8_evict": (C.c_int, [C.POINTER(FlbKv8Evict), C.c_void_p]),
+    "flb_kv8_append": (C.c_int, [C.c_void_p, C.c_void_p]),  # a parameter block, by reference or as its bytes
+    "flb_kv8_decode": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "flb_kv8_evict": (C.c_int, [C.c_void_p, C.c_void_p]),
 }
 
 _typed: C.CDLL | None = None
@@ -137,40 +139,44 @@ def empty_cache(batch_size: int, kv_head_num: int, total_len: int, size_per_head
     return Cache(*codes, *scales, row_pos=pos)
 
 
-def _dense(t: torch.Tensor, name: str, shape, dtype, device) -> int:
+def _refuse(t, name, shape, dtype, dev):
+    if t.get_device() != dev:
+        raise ValueError(f"{name} is on {t.device}, the cache on another device")
+    raise ValueError(f"{name} must be a dense {dtype} tensor of shape {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+
+
+def _dense(t: torch.Tensor, name: str, shape, dtype, dev: int) -> int:
     """Address of a dense tensor of this shape, type and device."""
-    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
-        raise ValueError(f"{name} must be a dense {dtype} tensor of shape {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, the cache on {device}")
+    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous() or t.get_device() != dev:
+        _refuse(t, name, shape, dtype, dev)
     return t.data_ptr()
 
 
-def _opt(t: torch.Tensor | None, name: str, shape, dtype, device) -> int | None:
-    return None if t is None else _dense(t, name, shape, dtype, device)
+def _opt(t: torch.Tensor | None, name: str, shape, dtype, dev: int) -> int:
+    return 0 if t is None else _dense(t, name, shape, dtype, dev)
 
 
-def _cache(c: Cache) -> FlbKv8Cache:
+def _cache(c: Cache) -> tuple:
+    """The values of a flb_kv8_cache, and the device's index (-1: host memory, for the checks alone)."""
     k = c.k
-    if k.dim() != 4 or k.dtype not in _CODE:
+    code = _CODE.get(k.dtype)
+    if code is None or k.dim() != 4:
         raise ValueError("cache codes must be int8 or float8_e4m3fn tensors [B,Hkv,T,d]")
-    B, H, T, d = k.shape
+    shape = k.shape
+    B, H, T, d = shape
     n = c.k_scale.shape[-1]
     if n <= 0 or T % n:
         raise ValueError("cache scales must be [B,Hkv,T/block_len]")
-    dev = k.device
-    return FlbKv8Cache(
-        B, H, d, T, T // n, _CODE[k.dtype], _dense(k, "k", (B, H, T, d), k.dtype, dev), _dense(c.v, "v", (B, H, T, d), k.dtype, dev),
-        _dense(c.k_scale, "k_scale", (B, H, n), torch.float32, dev), _dense(c.v_scale, "v_scale", (B, H, n), torch.float32, dev),
-        _opt(c.row_pos, "row_pos", (B, H, T), torch.int32, dev))
+    dev, scales = k.get_device(), (B, H, n)
+    return (B, H, d, T, T // n, code, _dense(k, "k", shape, k.dtype, dev), _dense(c.v, "v", shape, k.dtype, dev),
+            _dense(c.k_scale, "k_scale", scales, torch.float32, dev), _dense(c.v_scale, "v_scale", scales, torch.float32, dev),
+            _opt(c.row_pos, "row_pos", (B, H, T), torch.int32, dev)), dev
 
 
-def _rows(t: torch.Tensor, name: str, shape, dtype, device) -> tuple[int, int]:
+def _rows(t: torch.Tensor, name: str, shape, dtype, dev: int) -> tuple[int, int]:
     """Address and token-row stride (elements) of q, k or v [B,S,heads,d]: dense heads, one stride between tokens."""
-    if t.dtype != dtype or tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{name} must be {dtype} of shape {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, the cache on {device}")
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != dev:
+        _refuse(t, name, shape, dtype, dev)
     B, S, H, d = shape
     if t.is_contiguous():
         return t.data_ptr(), H * d
@@ -181,67 +187,74 @@ def _rows(t: torch.Tensor, name: str, shape, dtype, device) -> tuple[int, int]:
     return t.data_ptr(), row
 
 
-def _kv_rows(k, v, shape, dtype, device):
-    kp, ks = _rows(k, "k", shape, dtype, device)
-    vp, vs = _rows(v, "v", shape, dtype, device)
+def _kv_rows(k, v, shape, dtype, dev):
+    kp, ks = _rows(k, "k", shape, dtype, dev)
+    vp, vs = _rows(v, "v", shape, dtype, dev)
     if ks != vs:
         raise ValueError("k and v must share one token-row stride")
     return kp, vp, ks
 
 
-def _scales(mode, act, named, B, S, device):
-    """Addresses of the activation scale and of the weight scales (name -> (tensor, heads * d))."""
-    if mode != FLB_IN_INT32:
-        return [None] * (1 + len(named))
-    if act is None or any(t is None for t, _ in named.values()):
+def _scales(act, n, named, dev):
+    """Addresses of the activation scale (one per token) and of the weight scales (name, tensor, heads * d) of int32 inputs."""
+    if act is None or any(t is None for _, t, _ in named):
         raise ValueError("int32 inputs need act_scale and the weight scales")
-    if act.numel() != B * S:
+    if act.numel() != n:
         raise ValueError("act_scale must hold one value per token")
-    return [_dense(act, "act_scale", act.shape, torch.float32, device)] + [
-        _dense(t, n, (w,), torch.float32, device) for n, (t, w) in named.items()]
+    return [_dense(act, "act_scale", act.shape, torch.float32, dev)] + [_dense(t, name, (w,), torch.float32, dev) for name, t, w in named]
 
 
-def _rope(freq_cis, d, device):
+def _rope(freq_cis, d, dev):
     if freq_cis is None:
-        return None, 0
-    return _dense(freq_cis, "freq_cis", (freq_cis.shape[0], d), torch.float32, device), freq_cis.shape[0]
+        return 0, 0
+    n = freq_cis.shape[0]
+    return _dense(freq_cis, "freq_cis", (n, d), torch.float32, dev), n
 
 
-def _scratch(scratch, device):
+def _scratch(scratch, dev):
     if scratch is None:
-        return None, 0
-    if scratch.device != device or not scratch.is_contiguous():
+        return 0, 0
+    if scratch.get_device() != dev or not scratch.is_contiguous():
         raise ValueError("scratch must be a dense tensor on the cache's device")
-    return scratch.data_ptr(), scratch.numel() * scratch.element_size()
+    return scratch.data_ptr(), scratch.nbytes
 
 
-def _call(fn, params, device, stream) -> None:
-    if device.type != "cuda":
+def _call(fn, block: bytes, dev: int, stream) -> None:
+    if dev < 0:
         raise ValueError("the 8-bit cache lives on a CUDA device")
-    if torch.cuda.current_device() == device.index:
-        h = stream if stream is not None else torch.cuda.current_stream()
-        _lib.check(fn(C.byref(params), getattr(h, "cuda_stream", h)))
-        return
-    with torch.cuda.device(device):
-        h = stream if stream is not None else torch.cuda.current_stream()
-        _lib.check(fn(C.byref(params), getattr(h, "cuda_stream", h)))
+    if torch.cuda.current_device() != dev:
+        with torch.cuda.device(dev):
+            return _call(fn, block, dev, stream)
+    if stream is None:
+        h = torch._C._cuda_getCurrentRawStream(dev)
+    else:
+        h = getattr(stream, "cuda_stream", stream)
+    st = fn(block, h)
+    if st:
+        _lib.check(st)
 
 
-def append_params(cache: Cache, k, v, *, start_pos: int = 0, past_lens=None, new_lens=None, token_pos=None, act_scale=None, k_w_scale=None,
-                  v_w_scale=None, freq_cis=None, scratch=None) -> FlbKv8Append:
-    """The parameter block of `append`."""
-    c, dev = _cache(cache), cache.k.device
-    B, H, d = c.batch_size, c.kv_head_num, c.size_per_head
-    S = k.shape[1]
-    mode = _IN_MODE.get(k.dtype)
+def _append_block(cache: Cache, k, v, *, start_pos: int = 0, past_lens=None, new_lens=None, token_pos=None, act_scale=None, k_w_scale=None,
+                  v_w_scale=None, freq_cis=None, scratch=None) -> tuple[bytes, int]:
+    c, dev = _cache(cache)
+    B, H, d = c[:3]
+    S, dt, lens = k.shape[1], k.dtype, (B,)
+    mode = _IN_MODE.get(dt)
     if mode is None:
         raise ValueError("k and v must be int32, float32 or float16")
-    kp, vp, row = _kv_rows(k, v, (B, S, H, d), k.dtype, dev)
-    act, kw, vw = _scales(mode, act_scale, {"k_w_scale": (k_w_scale, H * d), "v_w_scale": (v_w_scale, H * d)}, B, S, dev)
-    fr, frows = _rope(freq_cis, d, dev)
-    sp, _ = _scratch(scratch, dev)
-    return FlbKv8Append(c, S, start_pos, _opt(past_lens, "past_lens", (B,), torch.int32, dev), _opt(new_lens, "new_lens", (B,), torch.int32, dev),
-                        _opt(token_pos, "token_pos", (B,), torch.int32, dev), mode, kp, vp, row, act, kw, vw, fr, frows, sp)
+    kp, vp, row = _kv_rows(k, v, (B, S, H, d), dt, dev)
+    act = kw = vw = 0
+    if mode == FLB_IN_INT32:
+        act, kw, vw = _scales(act_scale, B * S, (("k_w_scale", k_w_scale, H * d), ("v_w_scale", v_w_scale, H * d)), dev)
+    i32 = torch.int32
+    return _PACK_APPEND.pack(*c, S, start_pos, _opt(past_lens, "past_lens", lens, i32, dev), _opt(new_lens, "new_lens", lens, i32, dev),
+                             _opt(token_pos, "token_pos", lens, i32, dev), mode, kp, vp, row, act, kw, vw, *_rope(freq_cis, d, dev),
+                             _scratch(scratch, dev)[0]), dev
+
+
+def append_params(cache: Cache, k, v, **kw) -> FlbKv8Append:
+    """The parameter block of `append`."""
+    return FlbKv8Append.from_buffer_copy(_append_block(cache, k, v, **kw)[0])
 
 
 def append(cache: Cache, k, v, *, stream=None, **kw) -> None:
@@ -249,33 +262,38 @@ def append(cache: Cache, k, v, *, stream=None, **kw) -> None:
     `past_lens` int32 [B], or `start_pos` for all.  `new_lens` int32 [B]: how many of the S tokens of a padded batch count.
     `token_pos` int32 [B]: position of the first new token, where it is not the cached length.  `freq_cis`: RoPE table, row = position.
     `scratch`: its first word collects error bits (`attention.scratch_status`); may be None."""
-    _call(load_library().flb_kv8_append, append_params(cache, k, v, **kw), cache.k.device, stream)
+    _call(load_library().flb_kv8_append, *_append_block(cache, k, v, **kw), stream)
 
 
-def decode_params(cache: Cache, q, k, v, out, *, start_pos: int = 0, past_lens=None, max_past_len: int = 0, token_pos=None, act_scale=None,
+def _decode_block(cache: Cache, q, k, v, out, *, start_pos: int = 0, past_lens=None, max_past_len: int = 0, token_pos=None, act_scale=None,
                   q_w_scale=None, k_w_scale=None, v_w_scale=None, freq_cis=None, softmax_scale: float | None = None, softcap: float = 0.0,
                   alibi_slopes=None, key_begin=None, weight_in=None, weight_out=None, scratch=None, scratch_zeroed: bool = False,
-                  split_len: int = 0) -> FlbKv8Decode:
-    """The parameter block of `decode`."""
-    c, dev = _cache(cache), cache.k.device
-    B, Hkv, d, T = c.batch_size, c.kv_head_num, c.size_per_head, c.total_len
-    Hq = q.shape[2]
-    mode = _IN_MODE.get(q.dtype)
-    if mode is None or out.dtype not in _OUT:
+                  split_len: int = 0) -> tuple[bytes, int]:
+    c, dev = _cache(cache)
+    B, Hkv, d, T = c[:4]
+    Hq, dt, lens = q.shape[2], q.dtype, (B,)
+    mode, od = _IN_MODE.get(dt), _OUT.get(out.dtype)
+    if mode is None or od is None:
         raise ValueError("q, k and v must be int32, float32 or float16, out float32 or float16")
-    qp, qrow = _rows(q, "q", (B, 1, Hq, d), q.dtype, dev)
-    kp, vp, row = _kv_rows(k, v, (B, 1, Hkv, d), q.dtype, dev)
-    act, qw, kw, vw = _scales(mode, act_scale, {"q_w_scale": (q_w_scale, Hq * d), "k_w_scale": (k_w_scale, Hkv * d), "v_w_scale": (v_w_scale, Hkv * d)},
-                              B, 1, dev)
-    fr, frows = _rope(freq_cis, d, dev)
-    sp, sbytes = _scratch(scratch, dev)
+    qp, qrow = _rows(q, "q", (B, 1, Hq, d), dt, dev)
+    kp, vp, row = _kv_rows(k, v, (B, 1, Hkv, d), dt, dev)
+    act = qw = kw = vw = 0
+    if mode == FLB_IN_INT32:
+        act, qw, kw, vw = _scales(act_scale, B, (("q_w_scale", q_w_scale, Hq * d), ("k_w_scale", k_w_scale, Hkv * d), ("v_w_scale", v_w_scale, Hkv * d)), dev)
     i32, f32 = torch.int32, torch.float32
-    return FlbKv8Decode(
-        c, Hq, start_pos, _opt(past_lens, "past_lens", (B,), i32, dev), max_past_len, _opt(token_pos, "token_pos", (B,), i32, dev), mode, qp, kp, vp,
-        qrow, row, act, qw, kw, vw, fr, frows, softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(d), softcap,
-        _opt(alibi_slopes, "alibi_slopes", (Hq,), f32, dev), _opt(key_begin, "key_begin", (B,), i32, dev),
-        _opt(weight_in, "weight_in", (B, Hkv, T), f32, dev), _opt(weight_out, "weight_out", (B, Hkv, T), f32, dev),
-        _dense(out, "out", (B, Hq, 1, d), out.dtype, dev), _OUT[out.dtype], sp, sbytes, 1 if scratch_zeroed else 0, split_len)
+    wi = wo = 0
+    if weight_in is not None or weight_out is not None:
+        wi, wo = _opt(weight_in, "weight_in", (B, Hkv, T), f32, dev), _opt(weight_out, "weight_out", (B, Hkv, T), f32, dev)
+    return _PACK_DECODE.pack(
+        *c, Hq, start_pos, _opt(past_lens, "past_lens", lens, i32, dev), max_past_len, _opt(token_pos, "token_pos", lens, i32, dev), mode, qp, kp, vp,
+        qrow, row, act, qw, kw, vw, *_rope(freq_cis, d, dev), softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(d), softcap,
+        _opt(alibi_slopes, "alibi_slopes", (Hq,), f32, dev), _opt(key_begin, "key_begin", lens, i32, dev), wi, wo,
+        _dense(out, "out", (B, Hq, 1, d), out.dtype, dev), od, *_scratch(scratch, dev), 1 if scratch_zeroed else 0, split_len), dev
+
+
+def decode_params(cache: Cache, q, k, v, out, **kw) -> FlbKv8Decode:
+    """The parameter block of `decode`."""
+    return FlbKv8Decode.from_buffer_copy(_decode_block(cache, q, k, v, out, **kw)[0])
 
 
 def decode(cache: Cache, q, k, v, out, *, stream=None, **kw) -> None:
@@ -284,30 +302,33 @@ def decode(cache: Cache, q, k, v, out, *, stream=None, **kw) -> None:
     softcap * tanh(score / softcap); `alibi_slopes` float32 [H]: minus slope times distance; `key_begin` int32 [B]: rows at an earlier
     position are not seen.  `weight_in`, `weight_out` float32 [B,Hkv,T]: attention weights accumulated over the group (for `evict`), in place
     when both are the same tensor.  `scratch_zeroed`: the first `counter_bytes` bytes of scratch are zero (each call leaves them so)."""
-    _call(load_library().flb_kv8_decode, decode_params(cache, q, k, v, out, **kw), cache.k.device, stream)
+    _call(load_library().flb_kv8_decode, *_decode_block(cache, q, k, v, out, **kw), stream)
 
 
-def evict_params(cache: Cache, *, len_out, budget: int, weight, start_pos: int = 0, past_lens=None, recent: int = 0, sinks: int = 0, next_pos=None,
-                 weight_out=None, pos_out=None, scratch=None) -> FlbKv8Evict:
-    """The parameter block of `evict`."""
-    c, dev = _cache(cache), cache.k.device
-    B, H, T = c.batch_size, c.kv_head_num, c.total_len
+def _evict_block(cache: Cache, *, len_out, budget: int, weight, start_pos: int = 0, past_lens=None, recent: int = 0, sinks: int = 0, next_pos=None,
+                 weight_out=None, pos_out=None, scratch=None) -> tuple[bytes, int]:
     if cache.row_pos is None:
         raise ValueError("eviction needs a cache with row_pos")
-    i32, f32 = torch.int32, torch.float32
-    sp, sbytes = _scratch(scratch, dev)
-    return FlbKv8Evict(
-        c, start_pos, _opt(past_lens, "past_lens", (B,), i32, dev), _dense(len_out, "len_out", (B,), i32, dev), budget, recent, sinks,
-        _opt(next_pos, "next_pos", (B,), i32, dev), _dense(weight, "weight", (B, H, T), f32, dev),
-        _dense(weight if weight_out is None else weight_out, "weight_out", (B, H, T), f32, dev),
-        _dense(cache.row_pos if pos_out is None else pos_out, "pos_out", (B, H, T), i32, dev), sp, sbytes)
+    c, dev = _cache(cache)
+    B, H, _, T = c[:4]
+    i32, f32, lens, rows = torch.int32, torch.float32, (B,), (B, H, T)
+    return _PACK_EVICT.pack(
+        *c, start_pos, _opt(past_lens, "past_lens", lens, i32, dev), _dense(len_out, "len_out", lens, i32, dev), budget, recent, sinks,
+        _opt(next_pos, "next_pos", lens, i32, dev), _dense(weight, "weight", rows, f32, dev),
+        _dense(weight if weight_out is None else weight_out, "weight_out", rows, f32, dev),
+        _dense(cache.row_pos if pos_out is None else pos_out, "pos_out", rows, i32, dev), *_scratch(scratch, dev)), dev
+
+
+def evict_params(cache: Cache, **kw) -> FlbKv8Evict:
+    """The parameter block of `evict`."""
+    return FlbKv8Evict.from_buffer_copy(_evict_block(cache, **kw)[0])
 
 
 def evict(cache: Cache, *, stream=None, **kw) -> None:
     """Keeps `budget` rows per head of every sequence: those at a position below `sinks` or at or behind next_pos - `recent`, then those of the
     largest accumulated `weight`.  Rows move within the cache, weights and positions along (into weight_out and pos_out, or in place);
     len_out int32 [B] gets min(cached rows, budget) and may be past_lens.  The order of rows is no longer that of positions afterwards."""
-    _call(load_library().flb_kv8_evict, evict_params(cache, **kw), cache.k.device, stream)
+    _call(load_library().flb_kv8_evict, *_evict_block(cache, **kw), stream)
 
 
 def decode_workspace_bytes(batch_size: int, head_num: int, kv_head_num: int, total_len: int, size_per_head: int = 128, *, block_len: int = 64,
