@@ -274,6 +274,7 @@ int flb_attn_validate_scored(const flb_attn_params *p, const flb_score_form *f) 
     }
     if (!(f->softcap >= 0.f) || f->softcap > 3.402823466e38f) return FLB_ERR_BAD_SHAPE;
     if (p->seq_len == 1) return f->key_end ? FLB_ERR_UNSUPPORTED : FLB_OK; // a decode call sees what is cached
+    if (!(p->softmax_scale > 0.f) || p->softmax_scale > 3.402823466e38f) return FLB_ERR_BAD_SHAPE; // maxima are taken before the scale
     if (p->scratch_bytes < flb::prefill_scored_scratch_bytes(p->batch_size, p->head_num, p->seq_len, p->size_per_head, f))
         return FLB_ERR_SCRATCH_TOO_SMALL;
     return FLB_OK;

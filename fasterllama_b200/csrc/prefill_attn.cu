@@ -116,6 +116,7 @@ struct PrefillArgs {
     int Hkv, G;        // K/V heads, q heads per K/V head
     int kv_row_stride; // of k and v
     float cap_log2e, cap_in; // softcap * log2(e); what a raw score is multiplied by to become the tanh's argument
+    float cap_c[5];          // polynomial of the capped score over the raw one, in the raw one's square, highest power first
     const float *slopes;
     const int *key_begin, *key_end; // [B,S]
     int2 *ranges;      // [B][query tiles]: first key that a row of the 128-row tile sees, one past the last; empty = (INT_MAX, 0)
@@ -392,11 +393,11 @@ template <bool SCORED> __device__ __forceinline__ ItemGeom item_geom_of(const Pr
     if (SCORED && a.ranges) {
         const int2 *r = a.ranges + (size_t)(bh / a.H) * ((a.S + 2 * BM - 1) / (2 * BM) * 2) + 2 * qb;
         const int2 r0 = __ldcg(r), r1 = __ldcg(r + 1); // written by the kernel in front
-        const int first = min(r0.x, r1.x);
-        g.j0 = first == INT_MAX ? 0 : first / BN;
+        // the tiles of the item's own 256 rows are loaded in any case: this item sends their V on into the cache
+        g.j0 = min(min(r0.x, r1.x) / BN, 2 * BM / BN * qb);
         g.n[0] = max(1, (r0.y + BN - 1) / BN - g.j0);
         g.n[1] = max(1, (r1.y + BN - 1) / BN - g.j0);
-        g.nmax = max(g.n[0], g.n[1]);
+        g.nmax = max(max(g.n[0], g.n[1]), (min(a.S, (qb + 1) * 2 * BM) + BN - 1) / BN - g.j0);
     }
     return g;
 }
@@ -426,50 +427,71 @@ template <bool GENERIC> __device__ __forceinline__ void mask_chunk(uint32_t (&r)
         r[i] = __float_as_uint(x);
     }
 }
-// The same with a first visible key: [from, lim).
-template <bool GENERIC> __device__ __forceinline__ void mask_range(uint32_t (&r)[32], int base, int from, int lim, float scale, const float *mrow) {
+// The caller's additive mask on top of visible keys (bits of `seen`).
+__device__ __forceinline__ void add_mask(uint32_t (&r)[32], uint32_t seen, float scale, const float *mrow) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
         float x = -INFINITY;
-        if (base + i >= from && base + i < lim) x = GENERIC ? fmaf(__ldg(mrow + base + i), kLog2e, __uint_as_float(r[i]) * scale) : __uint_as_float(r[i]) * scale;
+        if (seen >> i & 1u) x = fmaf(__ldg(mrow + i), kLog2e, __uint_as_float(r[i]) * scale);
         r[i] = __float_as_uint(x);
     }
 }
+// Scores of keys that are not seen become -inf, scaled or not (the scale is positive).
+__device__ __forceinline__ void hide(uint32_t (&r)[32], uint32_t seen) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) r[i] = (seen >> i & 1u) ? r[i] : 0xff800000u;
+}
+// bits [lo, hi) of a word; lo, hi anywhere
+__device__ __forceinline__ uint32_t bit_range(int lo, int hi) {
+    const uint64_t a = (1ull << min(max(hi, 0), 32)) - 1ull, b = (1ull << min(max(lo, 0), 32)) - 1ull;
+    return (uint32_t)(a & ~b);
+}
 // Raw scores to capped ones in units of log2: cap * tanh(u), u = raw * cap_in.  Up to |u| = 1 tanh(u) / u is a polynomial in u^2 (own
-// minimax fit: 2.8e-6 of tanh, 2e-4 of a score at a cap of 50, below the fp16 rounding of the weight) on packed FMAs; it
-// costs no special-function result, of which the exponentials already take half the pipe.  Beyond, for warps that have such a score:
-// 1 - 2 / (1 + e^2|u|).
-__device__ __forceinline__ void cap_chunk(uint32_t (&r)[32], float cap_in, float cap) {
+// minimax fit: 2.8e-6 of tanh, 2e-4 of a score at a cap of 50, below the fp16 rounding of the weight) on packed FMAs, three per
+// score; it costs no special-function result, of which the exponentials already take half the pipe.  Beyond, for warps that have such a
+// score: 1 - 2 / (1 + e^2|u|).
+constexpr float kTanhPoly[5] = {0.0083658826f, -0.043299854f, 0.12922066f, -0.33265823f, 0.99996847f}; // u^8 .. u^0
+__device__ __forceinline__ void cap_chunk(uint32_t (&r)[32], const PrefillArgs &a) {
     float big = 0.f;
 #pragma unroll
     for (int i = 0; i < 32; i += 2) big = max3(big, fabsf(__uint_as_float(r[i])), fabsf(__uint_as_float(r[i + 1])));
-    if (__any_sync(0xffffffffu, !(big * cap_in <= 1.0f))) {
+    if (__any_sync(0xffffffffu, !(big * a.cap_in <= 1.0f))) {
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
-            const float u = __uint_as_float(r[i]) * cap_in;
+            const float u = __uint_as_float(r[i]) * a.cap_in;
             const float e = ex2(fabsf(u) * (2.0f * kLog2e));
-            r[i] = __float_as_uint(copysignf(cap - __fdividef(2.0f * cap, 1.0f + fminf(e, 1e30f)), u));
+            r[i] = __float_as_uint(copysignf(a.cap_log2e - __fdividef(2.0f * a.cap_log2e, 1.0f + fminf(e, 1e30f)), u));
         }
         return;
     }
-    const float2 in2 = make_float2(cap_in, cap_in);
 #pragma unroll
     for (int i = 0; i < 32; i += 2) {
-        const float2 u = __fmul2_rn(make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), in2);
-        const float2 y = __fmul2_rn(u, u);
-        float2 p = __ffma2_rn(y, make_float2(0.0083658826f, 0.0083658826f), make_float2(-0.043299854f, -0.043299854f));
-        p = __ffma2_rn(p, y, make_float2(0.12922066f, 0.12922066f));
-        p = __ffma2_rn(p, y, make_float2(-0.33265823f, -0.33265823f));
-        p = __ffma2_rn(p, y, make_float2(0.99996847f, 0.99996847f));
-        p = __fmul2_rn(p, __fmul2_rn(u, make_float2(cap, cap)));
+        const float2 x = make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), y = __fmul2_rn(x, x);
+        float2 p = __ffma2_rn(y, make_float2(a.cap_c[0], a.cap_c[0]), make_float2(a.cap_c[1], a.cap_c[1]));
+        p = __ffma2_rn(p, y, make_float2(a.cap_c[2], a.cap_c[2]));
+        p = __ffma2_rn(p, y, make_float2(a.cap_c[3], a.cap_c[3]));
+        p = __ffma2_rn(p, y, make_float2(a.cap_c[4], a.cap_c[4]));
+        p = __fmul2_rn(p, x);
         r[i] = __float_as_uint(p.x);
         r[i + 1] = __float_as_uint(p.y);
     }
 }
-// minus slope times the distance to the row's own position (`ahead`: query row - first key of the chunk); scale first
-__device__ __forceinline__ void bias_chunk(uint32_t (&r)[32], float scale, float slope, int ahead) {
+// Minus slope times the distance to the row's own position (`ahead`: query row - first key of the chunk), scale first.  Where no visible key lies
+// behind the row the distance is ahead - i and the bias one packed FMA per two keys.
+__device__ __forceinline__ void bias_chunk(uint32_t (&r)[32], float scale, float slope, int ahead, bool behind) {
+    const float base = -slope * (float)ahead;
+    if (behind) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(fmaf(-slope, fabsf((float)(ahead - i)), __uint_as_float(r[i]) * scale));
+        for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(fmaf(-slope, fabsf((float)ahead - (float)i), __uint_as_float(r[i]) * scale));
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+        const float2 b = __ffma2_rn(make_float2((float)i, (float)(i + 1)), make_float2(slope, slope), make_float2(base, base));
+        const float2 x = __ffma2_rn(make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), make_float2(scale, scale), b);
+        r[i] = __float_as_uint(x.x);
+        r[i + 1] = __float_as_uint(x.y);
+    }
 }
 __device__ __forceinline__ float chunk_max(const uint32_t (&r)[32], float m) {
 #pragma unroll
@@ -691,11 +713,13 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                 if (SCORED) {
                     const int b = bh / a.H, h = bh - b * a.H;
                     kvu = b * a.Hkv + h / a.G;
-                    keeper = keeper && h % a.G == 0; // one q head stores for its K/V head
+                    keeper = (keeper || a.ranges) && h % a.G == 0; // one q head stores for its K/V head
                 }
-                ok = load_k(kvu, g.j0, keeper);
+                // with key bounds every item keeps the tiles of its own rows instead
+                auto keeps = [&](int j) { return keeper && !(SCORED && a.ranges && j / (2 * BM / BN) != qb); };
+                ok = load_k(kvu, g.j0, keeps(g.j0));
                 if (ok) ok = publish(nxt); // one item of look-ahead for the other roles
-                for (int j = 1; j < g.nmax && ok; ++j) ok = load_k(kvu, g.j0 + j, keeper);
+                for (int j = 1; j < g.nmax && ok; ++j) ok = load_k(kvu, g.j0 + j, keeps(g.j0 + j));
                 cur = nxt;
             }
             if (ok) ok = load_v_late(); // the last V tile
@@ -886,6 +910,19 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                 // it skips itself; the other query tile's share comes from its own softmax warps)
                 if (k_releaser) mbar_arrive(&pb->k_empty[(kbase + (uint32_t)j) % K_STAGES]);
                 const uint32_t ts = tS_t + buf * (uint32_t)BN + lane_addr;
+                if (SCORED && __all_sync(0xffffffffu, row_hi <= k0 || row_lo >= k0 + BN)) {
+                    // none of the warp's 32 rows sees a key of this tile: weights 0, and nothing else changes
+                    uint32_t zero[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) zero[i] = 0u;
+                    tmem_st16(ts, zero);
+                    tmem_st16(ts + 16, zero);
+                    tmem_wait_st();
+                    tc_fence_before();
+                    mbar_arrive(p_full + buf);
+                    ++ct;
+                    continue;
+                }
                 tmem_ld32(ts, ra);
                 tmem_ld32(ts + 32, rb);
                 // a warp whose 32 rows all lie at or below the tile's last key needs no diagonal test (k0 + 63 is never a
@@ -901,19 +938,23 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                 float sc = a.scale_log2e;
                 if (SCORED) {
                     if (a.cap_log2e > 0.f) {
-                        cap_chunk(ra, a.cap_in, a.cap_log2e);
-                        cap_chunk(rb, a.cap_in, a.cap_log2e);
+                        cap_chunk(ra, a);
+                        cap_chunk(rb, a);
                         sc = 1.0f;
                     }
                     if (a.slopes) {
-                        bias_chunk(ra, sc, slope, row - k0);
-                        bias_chunk(rb, sc, slope, row - k0 - 32);
+                        const bool behind = !causal && k0 + BN - 1 > q0 + quarter * 32;
+                        bias_chunk(ra, sc, slope, row - k0, behind);
+                        bias_chunk(rb, sc, slope, row - k0 - 32, behind);
                         sc = 1.0f;
                     }
-                    if (GENERIC_MASK || !__all_sync(0xffffffffu, row_lo <= k0 && row_hi >= k0 + BN)) {
-                        mask_range<GENERIC_MASK>(ra, 0, row_lo - k0, row_hi - k0, sc, mrow);
-                        mask_range<GENERIC_MASK>(rb, 32, row_lo - k0, row_hi - k0, sc, mrow);
+                    if (GENERIC_MASK) {
+                        add_mask(ra, bit_range(row_lo - k0, row_hi - k0), sc, mrow);
+                        add_mask(rb, bit_range(row_lo - k0 - 32, row_hi - k0 - 32), sc, mrow + 32);
                         sc = 1.0f;
+                    } else if (!__all_sync(0xffffffffu, row_lo <= k0 && row_hi >= k0 + BN)) {
+                        hide(ra, bit_range(row_lo - k0, row_hi - k0));
+                        hide(rb, bit_range(row_lo - k0 - 32, row_hi - k0 - 32));
                     }
                 } else if (mode != 0) { // rare: the causal diagonal, the end of the prompt, or a caller-supplied mask
                     mask_chunk<GENERIC_MASK>(ra, 0, lim, sc, mrow);
@@ -922,7 +963,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                 }
                 // two independent chains: the maximum is a latency chain, not a throughput one; scale > 0 commutes with max
                 const float m_tile = fmaxf(chunk_max(ra, -INFINITY), chunk_max(rb, -INFINITY)) * sc;
-                if (j == 0) {
+                if (SCORED ? !__any_sync(0xffffffffu, m_used > -1e29f) : j == 0) { // O_t holds nothing of these rows yet
                     m_used = fmaxf(m_tile, -1e30f);
                 } else {
                     const bool grow = m_tile > m_used + kRescaleThreshold;
@@ -1160,8 +1201,13 @@ template <int D> int launch_prefill_hd(const flb_attn_params *p, const flb_score
     a.key_end = f ? f->key_end : nullptr;
     a.ranges = bounded ? reinterpret_cast<int2 *>(sc + 256 + 3 * one) : nullptr;
     const bool scored = Hkv != H || a.kv_row_stride != a.row_stride || a.cap_log2e > 0.f || a.slopes || bounded;
-    // with key bounds no item is sure to load every V tile, so the streaming pass stores V then
-    a.v_direct = (a.input_mode == FLB_IN_F16 && a.cache_f16 && !bounded) ? 1 : 0;
+    a.v_direct = (a.input_mode == FLB_IN_F16 && a.cache_f16) ? 1 : 0;
+    // cap * tanh(raw * cap_in) = raw * (polynomial in raw^2): the powers of cap_in go into the coefficients
+    for (int i = 0; i < 5; ++i) {
+        double c = (double)kTanhPoly[i] * a.cap_log2e;
+        for (int k = 0; k < 9 - 2 * i; ++k) c *= a.cap_in;
+        a.cap_c[i] = (float)c;
+    }
     // The larger the group, the closer the list is to heaviest-first over everything (measured at batch 8 x 32 heads x 1024
     // tokens: 142 us with groups of 32 units, 138 us with 64, 139 us with 128, 141 us with all 256 in one group; at
     // batch 32 x 512 tokens 210 us with 32 or 64, 214 us with 256); the limit is what a group's K and V rows (fp16) take in
