@@ -116,7 +116,8 @@ struct PrefillArgs {
     int Hkv, G;        // K/V heads, q heads per K/V head
     int kv_row_stride; // of k and v
     float cap_log2e, cap_in; // softcap * log2(e); what a raw score is multiplied by to become the tanh's argument
-    float cap_c[5];          // polynomial of the capped score over the raw one, in the raw one's square, highest power first
+    float cap_c[3];           // polynomial of the capped score over the raw one, in the raw one's square, highest power first
+    int backwards;            // key tiles from the last to the first
     const float *slopes;
     const int *key_begin, *key_end; // [B,S]
     int2 *ranges;      // [B][query tiles]: first key that a row of the 128-row tile sees, one past the last; empty = (INT_MAX, 0)
@@ -370,6 +371,9 @@ struct ItemGeom {
     int n[2];    // key tiles query tile t attends over
     int nmax;
     int j0;      // first key tile of the item (a score form's key bounds; else 0)
+    // Step i of the item's nmax works on key tile j0 + i, or backwards on j0 + nmax - 1 - i; query tile t takes part in n[t] neighbouring steps.
+    template <bool SCORED> __device__ __forceinline__ int first_step(int t, bool backwards) const { return SCORED && backwards ? nmax - n[t] : 0; }
+    template <bool SCORED> __device__ __forceinline__ int tile(int i, bool backwards) const { return SCORED ? (backwards ? j0 + nmax - 1 - i : j0 + i) : i; }
 };
 __device__ __forceinline__ ItemGeom item_geom(int qb, int S, bool causal) {
     ItemGeom g;
@@ -446,34 +450,43 @@ __device__ __forceinline__ uint32_t bit_range(int lo, int hi) {
     const uint64_t a = (1ull << min(max(hi, 0), 32)) - 1ull, b = (1ull << min(max(lo, 0), 32)) - 1ull;
     return (uint32_t)(a & ~b);
 }
-// Raw scores to capped ones in units of log2: cap * tanh(u), u = raw * cap_in.  Up to |u| = 1 tanh(u) / u is a polynomial in u^2 (own
-// minimax fit: 2.8e-6 of tanh, 2e-4 of a score at a cap of 50, below the fp16 rounding of the weight) on packed FMAs, three per
-// score; it costs no special-function result, of which the exponentials already take half the pipe.  Beyond, for warps that have such a
-// score: 1 - 2 / (1 + e^2|u|).
-constexpr float kTanhPoly[5] = {0.0083658826f, -0.043299854f, 0.12922066f, -0.33265823f, 0.99996847f}; // u^8 .. u^0
-__device__ __forceinline__ void cap_chunk(uint32_t (&r)[32], const PrefillArgs &a) {
+// Raw scores to capped ones in units of log2: cap * tanh(u), u = raw * cap_in.  Up to |u| = 0.4, where the scores of nearly all tiles lie,
+// tanh(u) / u is a polynomial in u^2 (own minimax fit: 1.2e-6 of tanh, 9e-5 of a score at a cap of 50, far below the fp16 rounding of
+// the weight) on packed FMAs; it costs no special-function result, of which the exponentials already take half the pipe.
+constexpr float kTanhPoly[3] = {0.11942387f, -0.33225426f, 0.99997884f}; // u^4, u^2, 1
+constexpr float kTanhReach = 0.4f;
+__device__ __forceinline__ float chunk_abs_max(const uint32_t (&r)[32]) {
     float big = 0.f;
 #pragma unroll
     for (int i = 0; i < 32; i += 2) big = max3(big, fabsf(__uint_as_float(r[i])), fabsf(__uint_as_float(r[i + 1])));
-    if (__any_sync(0xffffffffu, !(big * a.cap_in <= 1.0f))) {
+    return big;
+}
+__device__ __forceinline__ void cap_chunk(uint32_t (&r)[32], const PrefillArgs &a) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+        const float2 x = make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), y = __fmul2_rn(x, x);
+        float2 p = __ffma2_rn(y, make_float2(a.cap_c[0], a.cap_c[0]), make_float2(a.cap_c[1], a.cap_c[1]));
+        p = __ffma2_rn(p, y, make_float2(a.cap_c[2], a.cap_c[2]));
+        p = __fmul2_rn(p, x);
+        r[i] = __float_as_uint(p.x);
+        r[i + 1] = __float_as_uint(p.y);
+    }
+}
+// Any score: 1 - 2 / (1 + e^2|u|).  Warps that have one beyond the polynomial's reach send the tile through this once in TMEM, 32 columns at a
+// time (one copy of the code: what the warps execute shares the instruction cache).
+__device__ __forceinline__ void cap_in_tmem(uint32_t ts, uint32_t (&r)[32], const PrefillArgs &a) {
+#pragma unroll 1
+    for (int ch = 0; ch < 2; ++ch) {
+        tmem_ld32(ts + ch * 32, r);
+        tmem_wait_ld(r);
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
             const float u = __uint_as_float(r[i]) * a.cap_in;
             const float e = ex2(fabsf(u) * (2.0f * kLog2e));
             r[i] = __float_as_uint(copysignf(a.cap_log2e - __fdividef(2.0f * a.cap_log2e, 1.0f + fminf(e, 1e30f)), u));
         }
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 32; i += 2) {
-        const float2 x = make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), y = __fmul2_rn(x, x);
-        float2 p = __ffma2_rn(y, make_float2(a.cap_c[0], a.cap_c[0]), make_float2(a.cap_c[1], a.cap_c[1]));
-        p = __ffma2_rn(p, y, make_float2(a.cap_c[2], a.cap_c[2]));
-        p = __ffma2_rn(p, y, make_float2(a.cap_c[3], a.cap_c[3]));
-        p = __ffma2_rn(p, y, make_float2(a.cap_c[4], a.cap_c[4]));
-        p = __fmul2_rn(p, x);
-        r[i] = __float_as_uint(p.x);
-        r[i + 1] = __float_as_uint(p.y);
+        tmem_st32(ts + ch * 32, r);
+        tmem_wait_st();
     }
 }
 // Minus slope times the distance to the row's own position (`ahead`: query row - first key of the chunk), scale first.  Where no visible key lies
@@ -516,16 +529,35 @@ __device__ __forceinline__ void chunk_exp(const uint32_t (&r)[32], float scale, 
     }
 }
 
+// The same on raw scores whose cap goes into the exponent's argument (within the polynomial's reach, every key seen): the polynomial's last
+// multiplication and the subtraction of the maximum are one operation.
+__device__ __forceinline__ void chunk_exp_cap(const uint32_t (&r)[32], const PrefillArgs &a, float neg_m, float2 &l2, uint32_t (&packed)[16]) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+        const float2 x = make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), y = __fmul2_rn(x, x);
+        float2 c = __ffma2_rn(y, make_float2(a.cap_c[0], a.cap_c[0]), make_float2(a.cap_c[1], a.cap_c[1]));
+        c = __ffma2_rn(c, y, make_float2(a.cap_c[2], a.cap_c[2]));
+        c = __ffma2_rn(c, x, make_float2(neg_m, neg_m));
+        const float2 p = make_float2(ex2(c.x), ex2(c.y));
+        l2 = __fadd2_rn(l2, p);
+        const __half2 h2 = __floats2half2_rn(p.x, p.y);
+        packed[i >> 1] = *reinterpret_cast<const uint32_t *>(&h2);
+    }
+}
+
 // GENERIC_MASK: the caller's additive mask is read (mask_mode GENERIC); OUT_F16: the output element type.  Compile-time so
 // that each form carries only its own code: what the sixteen warps execute has to share the instruction cache.
-// SCORED: a score form is in use.
-template <int EMUL, bool GENERIC_MASK, bool OUT_F16, int HD, bool SCORED>
+// FORM: 0 = no score form; kFormBounds = key bounds or shared K/V heads; and capped scores, distance bias.
+constexpr int kFormBounds = 1, kFormCap = 2, kFormBias = 4;
+template <int EMUL, bool GENERIC_MASK, bool OUT_F16, int HD, int FORM>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
     flb_prefill_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                             const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmVin, const PrefillArgs a,
                             const int num_items) {
     // The 128-byte swizzle pattern is a function of address bits [4,10): tiles must start on 1 KB.
     constexpr int D = HD;
+    constexpr bool SCORED = FORM != 0;
+    const bool backwards = (FORM & kFormBias) && a.backwards;
     constexpr int TILE_BYTES = BM * D * 2;
     constexpr int KV_TILE_BYTES = BN * D * 2;
     static_assert(D == 64 || D == 128, "O_t takes D TMEM columns per query tile beside the 256 columns of scores");
@@ -717,9 +749,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                 }
                 // with key bounds every item keeps the tiles of its own rows instead
                 auto keeps = [&](int j) { return keeper && !(SCORED && a.ranges && j / (2 * BM / BN) != qb); };
-                ok = load_k(kvu, g.j0, keeps(g.j0));
+                auto load_step = [&](int i) { const int j = g.tile<SCORED>(i, backwards); return load_k(kvu, j, keeps(j)); };
+                ok = load_step(0);
                 if (ok) ok = publish(nxt); // one item of look-ahead for the other roles
-                for (int j = 1; j < g.nmax && ok; ++j) ok = load_k(kvu, g.j0 + j, keeps(g.j0 + j));
+                for (int j = 1; j < g.nmax && ok; ++j) ok = load_step(j);
                 cur = nxt;
             }
             if (ok) ok = load_v_late(); // the last V tile
@@ -752,7 +785,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                             *const pv_done = &pb->pv_done[t][0];
             unsigned char *const sQ_t = sQ + t * TILE_BYTES;
             uint32_t taken = 0, kt = 0, gs = 0, nq = 0; // items read, ring tiles passed, S issued, query tiles loaded
-            int nmax = 0, n_t = 0, j = 0;
+            int nmax = 0, first_t = 0, end_t = 0, j = 0; // steps of the item, and those that this query tile takes part in
             bool ok = true, valid = true;
             while (ok && valid) {
                 if (j == nmax) {
@@ -766,7 +799,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                     if (!valid) break;
                     const ItemGeom g = item_geom_of<SCORED>(a, bh, qb, causal);
                     nmax = g.nmax;
-                    n_t = t ? g.n[1] : g.n[0];
+                    first_t = t ? g.first_step<SCORED>(1, backwards) : g.first_step<SCORED>(0, backwards);
+                    end_t = first_t + (t ? g.n[1] : g.n[0]);
                     j = 0;
                     if (nq > 0) {
                         ok = wait_bar(q_empty, (nq - 1u) & 1u, pb, a.status);
@@ -781,12 +815,12 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                 ok = wait_bar(&pb->k_full[ks], (kt / K_STAGES) & 1u, pb, a.status);
                 if (!ok) break;
                 ++kt;
-                if (j >= n_t) { // above this query tile's diagonal: nothing of this tile is read on its behalf
+                if (j < first_t || j >= end_t) { // above this query tile's diagonal: nothing of this tile is read on its behalf
                     mbar_arrive(&pb->k_empty[ks]);
                     ++j;
                     continue;
                 }
-                if (j == 0) ok = wait_bar(q_full, (nq - 1u) & 1u, pb, a.status);
+                if (j == first_t) ok = wait_bar(q_full, (nq - 1u) & 1u, pb, a.status);
                 const uint32_t buf = gs & 1u;
                 if (ok && gs >= 2) ok = wait_bar(pv_done + buf, ((gs - 2u) >> 1) & 1u, pb, a.status); // P_{j-2}.V_{j-2} has read this buffer
                 if (!ok) break;
@@ -800,7 +834,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                     umma_f16_ss(ts, dq0 + oq, dk + okk, idesc_qk, kk > 0 ? 1u : 0u);
                 }
                 umma_commit(s_full + buf);
-                if (j == n_t - 1) umma_commit(q_empty); // the query tile's buffer may take the next item's rows
+                if (j == end_t - 1) umma_commit(q_empty); // the query tile's buffer may take the next item's rows
                 ++gs;
                 ++j;
             }
@@ -815,7 +849,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             constexpr uint32_t idesc_pv = umma_idesc_f16(BM, D, false, true);
             const uint64_t dv0 = umma_desc_sw128(smem_u32(sV), KV_HALF_BYTES, 1024);
             uint32_t taken = 0, vt = 0, gp[2] = {0, 0}, ci[2] = {0, 0};
-            int nmax = 0, n[2] = {0, 0}, j = 0;
+            int nmax = 0, first[2] = {0, 0}, end[2] = {0, 0}, j = 0;
             bool ok = true;
             for (;;) {
                 if (j == nmax) {
@@ -826,8 +860,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                     if (bh < 0) break;
                     const ItemGeom g = item_geom_of<SCORED>(a, bh, qb, causal);
                     nmax = g.nmax;
-                    n[0] = g.n[0];
-                    n[1] = g.n[1];
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        first[t] = g.first_step<SCORED>(t, backwards);
+                        end[t] = first[t] + g.n[t];
+                    }
                     j = 0;
                     continue;
                 }
@@ -838,8 +875,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                 ++vt;
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
-                    if (j >= n[t] || !ok) continue; // above this query tile's diagonal
-                    if (j == 0) { // the epilogue has read the previous item's O_t
+                    if (j < first[t] || j >= end[t] || !ok) continue; // above this query tile's diagonal
+                    if (j == first[t]) { // the epilogue has read the previous item's O_t
                         ok = wait_bar(&pb->o_empty[t], (ci[t] & 1u) ^ 1u, pb, a.status);
                         if (!ok) continue;
                     }
@@ -850,9 +887,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                     const uint32_t tp = tmem + (uint32_t)(t * 128) + buf * (uint32_t)BN;
 #pragma unroll
                     for (int kk = 0; kk < BN / 16; ++kk) // 16 keys = 2048 bytes of the tile per step
-                        umma_f16_ts(tO[t], tp + kk * 8, dv + (uint32_t)(kk * (2048 >> 4)), idesc_pv, (j > 0 || kk > 0) ? 1u : 0u);
+                        umma_f16_ts(tO[t], tp + kk * 8, dv + (uint32_t)(kk * (2048 >> 4)), idesc_pv, (j > first[t] || kk > 0) ? 1u : 0u);
                     umma_commit(&pb->pv_done[t][buf]);
-                    if (j == n[t] - 1) {
+                    if (j == end[t] - 1) {
                         umma_commit(&pb->o_full[t]);
                         ++ci[t];
                     }
@@ -886,7 +923,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             ++taken;
             if (bh < 0) break;
             const ItemGeom g = item_geom_of<SCORED>(a, bh, qb, causal);
-            const int n_t = t ? g.n[1] : g.n[0];
+            const int n_t = t ? g.n[1] : g.n[0], first_t = t ? g.first_step<SCORED>(1, backwards) : g.first_step<SCORED>(0, backwards);
             const int q0 = t ? g.q0[1] : g.q0[0], row = q0 + lrow;
             float m_used = -1e30f;
             float2 l2 = make_float2(0.f, 0.f);
@@ -894,13 +931,13 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             float slope = 0.f;
             if (SCORED) {
                 if (row < a.S) visible_keys(a, bh / a.H, row, row_lo, row_hi);
-                if (a.slopes) slope = __ldg(a.slopes + bh % a.H) * kLog2e;
+                if ((FORM & kFormBias) && a.slopes) slope = __ldg(a.slopes + bh % a.H) * kLog2e;
             }
             uint32_t ra[32], rb[32];
             for (int j = 0; j < n_t; ++j) {
                 // One key tile = one step of the online softmax: load the 64 scores of this row, maximum, (rarely)
                 // rescale, P = 2^(x - m) stored over the scores as fp16 pairs, hand the buffer to the tensor core.
-                const int k0 = (SCORED ? g.j0 + j : j) * BN;
+                const int k0 = g.tile<SCORED>(first_t + j, backwards) * BN;
                 const uint32_t buf = ct & 1u;
                 ok = wait_bar(s_full + buf, (ct >> 1) & 1u, pb, a.status);
                 ok = __all_sync(0xffffffffu, ok);
@@ -908,7 +945,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                 tc_fence_after();
                 // S_j has landed, so this query tile's product has finished reading K_j (the issuer hands back the tiles
                 // it skips itself; the other query tile's share comes from its own softmax warps)
-                if (k_releaser) mbar_arrive(&pb->k_empty[(kbase + (uint32_t)j) % K_STAGES]);
+                if (k_releaser) mbar_arrive(&pb->k_empty[(kbase + (uint32_t)(first_t + j)) % K_STAGES]);
                 const uint32_t ts = tS_t + buf * (uint32_t)BN + lane_addr;
                 if (SCORED && __all_sync(0xffffffffu, row_hi <= k0 || row_lo >= k0 + BN)) {
                     // none of the warp's 32 rows sees a key of this tile: weights 0, and nothing else changes
@@ -936,13 +973,25 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                 const float *mrow = GENERIC_MASK ? a.attn_mask + (size_t)min(row, a.S - 1) * a.mask_row_stride + k0 : nullptr;
                 tmem_wait_ld(ra, rb);
                 float sc = a.scale_log2e;
+                bool fused = false; // the cap is taken in the exponent's argument
                 if (SCORED) {
-                    if (a.cap_log2e > 0.f) {
-                        cap_chunk(ra, a);
-                        cap_chunk(rb, a);
+                    if ((FORM & kFormCap) && a.cap_log2e > 0.f) {
+                        const bool near = __all_sync(0xffffffffu, fmaxf(chunk_abs_max(ra), chunk_abs_max(rb)) * a.cap_in <= kTanhReach);
+                        if (!near) {
+                            cap_in_tmem(ts, ra, a);
+                            tmem_ld32(ts, ra);
+                            tmem_ld32(ts + 32, rb);
+                            tmem_wait_ld(ra, rb);
+                        } else {
+                            fused = !GENERIC_MASK && !(FORM & kFormBias) && __all_sync(0xffffffffu, row_lo <= k0 && row_hi >= k0 + BN);
+                            if (!fused) {
+                                cap_chunk(ra, a);
+                                cap_chunk(rb, a);
+                            }
+                        }
                         sc = 1.0f;
                     }
-                    if (a.slopes) {
+                    if ((FORM & kFormBias) && a.slopes) {
                         const bool behind = !causal && k0 + BN - 1 > q0 + quarter * 32;
                         bias_chunk(ra, sc, slope, row - k0, behind);
                         bias_chunk(rb, sc, slope, row - k0 - 32, behind);
@@ -962,7 +1011,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                     sc = 1.0f;
                 }
                 // two independent chains: the maximum is a latency chain, not a throughput one; scale > 0 commutes with max
-                const float m_tile = fmaxf(chunk_max(ra, -INFINITY), chunk_max(rb, -INFINITY)) * sc;
+                float m_tile = fmaxf(chunk_max(ra, -INFINITY), chunk_max(rb, -INFINITY)) * sc;
+                if ((FORM & kFormCap) && fused) { // capping keeps the order
+                    const float y = m_tile * m_tile;
+                    m_tile *= fmaf(fmaf(y, a.cap_c[0], a.cap_c[1]), y, a.cap_c[2]);
+                }
                 if (SCORED ? !__any_sync(0xffffffffu, m_used > -1e29f) : j == 0) { // O_t holds nothing of these rows yet
                     m_used = fmaxf(m_tile, -1e30f);
                 } else {
@@ -992,10 +1045,17 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                 }
                 const float neg_m = -m_used;
                 uint32_t packed[16];
-                chunk_exp<EMUL>(ra, sc, neg_m, l2, packed);
-                tmem_st16(ts, packed);
-                chunk_exp<EMUL>(rb, sc, neg_m, l2, packed);
-                tmem_st16(ts + 16, packed);
+                if ((FORM & kFormCap) && fused) {
+                    chunk_exp_cap(ra, a, neg_m, l2, packed);
+                    tmem_st16(ts, packed);
+                    chunk_exp_cap(rb, a, neg_m, l2, packed);
+                    tmem_st16(ts + 16, packed);
+                } else {
+                    chunk_exp<EMUL>(ra, sc, neg_m, l2, packed);
+                    tmem_st16(ts, packed);
+                    chunk_exp<EMUL>(rb, sc, neg_m, l2, packed);
+                    tmem_st16(ts + 16, packed);
+                }
                 tmem_wait_st();
                 tc_fence_before();
                 mbar_arrive(p_full + buf);
@@ -1151,9 +1211,21 @@ bool make_map(EncodeTiledFn enc, CUtensorMap *tm, const void *base, int BH, int 
 }
 
 using AttnKernel = void (*)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const CUtensorMap, const PrefillArgs, const int);
-template <int D, bool SCORED> AttnKernel attn_kernel_of(bool generic_mask, bool out_f16) {
-    return generic_mask ? (out_f16 ? flb_prefill_attn_kernel<kExpOnFmaEvery, true, true, D, SCORED> : flb_prefill_attn_kernel<kExpOnFmaEvery, true, false, D, SCORED>)
-                        : (out_f16 ? flb_prefill_attn_kernel<kExpOnFmaEvery, false, true, D, SCORED> : flb_prefill_attn_kernel<kExpOnFmaEvery, false, false, D, SCORED>);
+template <int D, bool GENERIC, int FORM> AttnKernel attn_kernel_of(bool out_f16) {
+    return out_f16 ? flb_prefill_attn_kernel<kExpOnFmaEvery, GENERIC, true, D, FORM> : flb_prefill_attn_kernel<kExpOnFmaEvery, GENERIC, false, D, FORM>;
+}
+// Each form has a kernel with its own code only (one for all forms ran 155 -> 193 us at 4001 tokens without cap and bias: what sixteen warps execute has to
+// fit the instruction cache); with a caller's mask on top, which is read from global memory anyway, one does for all.
+template <int D> AttnKernel attn_kernel_of(bool generic_mask, bool out_f16, int form) {
+    constexpr int kAll = kFormBounds | kFormCap | kFormBias;
+    if (generic_mask) return form ? attn_kernel_of<D, true, kAll>(out_f16) : attn_kernel_of<D, true, 0>(out_f16);
+    switch (form) {
+    case 0: return attn_kernel_of<D, false, 0>(out_f16);
+    case kFormBounds: return attn_kernel_of<D, false, kFormBounds>(out_f16);
+    case kFormBounds | kFormCap: return attn_kernel_of<D, false, kFormBounds | kFormCap>(out_f16);
+    case kFormBounds | kFormBias: return attn_kernel_of<D, false, kFormBounds | kFormBias>(out_f16);
+    default: return attn_kernel_of<D, false, kAll>(out_f16);
+    }
 }
 
 template <int D> int launch_prefill_hd(const flb_attn_params *p, const flb_score_form *f, cudaStream_t stream) {
@@ -1203,11 +1275,14 @@ template <int D> int launch_prefill_hd(const flb_attn_params *p, const flb_score
     const bool scored = Hkv != H || a.kv_row_stride != a.row_stride || a.cap_log2e > 0.f || a.slopes || bounded;
     a.v_direct = (a.input_mode == FLB_IN_F16 && a.cache_f16) ? 1 : 0;
     // cap * tanh(raw * cap_in) = raw * (polynomial in raw^2): the powers of cap_in go into the coefficients
-    for (int i = 0; i < 5; ++i) {
+    for (int i = 0; i < 3; ++i) {
         double c = (double)kTanhPoly[i] * a.cap_log2e;
-        for (int k = 0; k < 9 - 2 * i; ++k) c *= a.cap_in;
+        for (int k = 0; k < 5 - 2 * i; ++k) c *= a.cap_in;
         a.cap_c[i] = (float)c;
     }
+    // A distance bias grows towards the diagonal: from the last tile to the first a row's maximum is found at once, the other way round it
+    // passes the rescaling threshold at nearly every tile (4001 tokens, 32 heads: 225 us forwards, BACK us backwards).
+    a.backwards = a.slopes != nullptr;
     // The larger the group, the closer the list is to heaviest-first over everything (measured at batch 8 x 32 heads x 1024
     // tokens: 142 us with groups of 32 units, 138 us with 64, 139 us with 128, 141 us with all 256 in one group; at
     // batch 32 x 512 tokens 210 us with 32 or 64, 214 us with 256); the limit is what a group's K and V rows (fp16) take in
@@ -1267,7 +1342,7 @@ template <int D> int launch_prefill_hd(const flb_attn_params *p, const flb_score
     pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     pdl[0].val.programmaticStreamSerializationAllowed = 1;
     const bool generic_mask = (a.mask_mode == FLB_MASK_GENERIC);
-    auto kern = scored ? attn_kernel_of<D, true>(generic_mask, a.out_f16) : attn_kernel_of<D, false>(generic_mask, a.out_f16);
+    auto kern = attn_kernel_of<D>(generic_mask, a.out_f16, scored ? kFormBounds | (a.cap_log2e > 0.f ? kFormCap : 0) | (a.slopes ? kFormBias : 0) : 0);
     constexpr size_t smem_bytes = prefill_smem(D);
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes) != cudaSuccess) return FLB_ERR_LAUNCH;
     const long long num_items = (long long)B * H * ((S + 2 * BM - 1) / (2 * BM));
