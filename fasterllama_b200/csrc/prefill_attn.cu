@@ -455,6 +455,7 @@ __device__ __forceinline__ uint32_t bit_range(int lo, int hi) {
 // the weight) on packed FMAs; it costs no special-function result, of which the exponentials already take half the pipe.
 constexpr float kTanhPoly[3] = {0.11942387f, -0.33225426f, 0.99997884f}; // u^4, u^2, 1
 constexpr float kTanhReach = 0.4f;
+constexpr float kTiny = 1.1754944e-38f; // smallest normal number: the leading coefficient stays positive however large the cap
 __device__ __forceinline__ float chunk_abs_max(const uint32_t (&r)[32]) {
     float big = 0.f;
 #pragma unroll
@@ -529,14 +530,14 @@ __device__ __forceinline__ void chunk_exp(const uint32_t (&r)[32], float scale, 
     }
 }
 
-// The same on raw scores whose cap goes into the exponent's argument (within the polynomial's reach, every key seen): the polynomial's last
-// multiplication and the subtraction of the maximum are one operation.
-__device__ __forceinline__ void chunk_exp_cap(const uint32_t (&r)[32], const PrefillArgs &a, float neg_m, float2 &l2, uint32_t (&packed)[16]) {
+// The same on raw scores whose cap goes into the exponent's argument: the polynomial's last multiplication and the subtraction of the maximum
+// are one operation.  c[0] > 0, so that a hidden key's -inf comes out as -inf.
+__device__ __forceinline__ void chunk_exp_cap(const uint32_t (&r)[32], const float (&k)[3], float neg_m, float2 &l2, uint32_t (&packed)[16]) {
 #pragma unroll
     for (int i = 0; i < 32; i += 2) {
         const float2 x = make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), y = __fmul2_rn(x, x);
-        float2 c = __ffma2_rn(y, make_float2(a.cap_c[0], a.cap_c[0]), make_float2(a.cap_c[1], a.cap_c[1]));
-        c = __ffma2_rn(c, y, make_float2(a.cap_c[2], a.cap_c[2]));
+        float2 c = __ffma2_rn(y, make_float2(k[0], k[0]), make_float2(k[1], k[1]));
+        c = __ffma2_rn(c, y, make_float2(k[2], k[2]));
         c = __ffma2_rn(c, x, make_float2(neg_m, neg_m));
         const float2 p = make_float2(ex2(c.x), ex2(c.y));
         l2 = __fadd2_rn(l2, p);
@@ -545,8 +546,6 @@ __device__ __forceinline__ void chunk_exp_cap(const uint32_t (&r)[32], const Pre
     }
 }
 
-// GENERIC_MASK: the caller's additive mask is read (mask_mode GENERIC); OUT_F16: the output element type.  Compile-time so
-// that each form carries only its own code: what the sixteen warps execute has to share the instruction cache.
 // FORM: 0 = no score form; kFormBounds = key bounds or shared K/V heads; and capped scores, distance bias.
 constexpr int kFormBounds = 1, kFormCap = 2, kFormBias = 4;
 template <int EMUL, bool GENERIC_MASK, bool OUT_F16, int HD, int FORM>
@@ -557,6 +556,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     // The 128-byte swizzle pattern is a function of address bits [4,10): tiles must start on 1 KB.
     constexpr int D = HD;
     constexpr bool SCORED = FORM != 0;
+    constexpr bool CAP_IN_EXP = (FORM & kFormCap) && !(FORM & kFormBias) && !GENERIC_MASK; // nothing comes between the cap and the exponential
     const bool backwards = (FORM & kFormBias) && a.backwards;
     constexpr int TILE_BYTES = BM * D * 2;
     constexpr int KV_TILE_BYTES = BN * D * 2;
@@ -973,21 +973,20 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                 const float *mrow = GENERIC_MASK ? a.attn_mask + (size_t)min(row, a.S - 1) * a.mask_row_stride + k0 : nullptr;
                 tmem_wait_ld(ra, rb);
                 float sc = a.scale_log2e;
-                bool fused = false; // the cap is taken in the exponent's argument
+                float kc[3] = {a.cap_c[0], a.cap_c[1], a.cap_c[2]};
                 if (SCORED) {
                     if ((FORM & kFormCap) && a.cap_log2e > 0.f) {
-                        const bool near = __all_sync(0xffffffffu, fmaxf(chunk_abs_max(ra), chunk_abs_max(rb)) * a.cap_in <= kTanhReach);
-                        if (!near) {
+                        if (!__all_sync(0xffffffffu, fmaxf(chunk_abs_max(ra), chunk_abs_max(rb)) * a.cap_in <= kTanhReach)) {
                             cap_in_tmem(ts, ra, a);
                             tmem_ld32(ts, ra);
                             tmem_ld32(ts + 32, rb);
                             tmem_wait_ld(ra, rb);
-                        } else {
-                            fused = !GENERIC_MASK && !(FORM & kFormBias) && __all_sync(0xffffffffu, row_lo <= k0 && row_hi >= k0 + BN);
-                            if (!fused) {
-                                cap_chunk(ra, a);
-                                cap_chunk(rb, a);
-                            }
+                            kc[0] = kTiny; // x = x for every finite score
+                            kc[1] = 0.f;
+                            kc[2] = 1.f;
+                        } else if (!CAP_IN_EXP) {
+                            cap_chunk(ra, a);
+                            cap_chunk(rb, a);
                         }
                         sc = 1.0f;
                     }
@@ -1012,9 +1011,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                 }
                 // two independent chains: the maximum is a latency chain, not a throughput one; scale > 0 commutes with max
                 float m_tile = fmaxf(chunk_max(ra, -INFINITY), chunk_max(rb, -INFINITY)) * sc;
-                if ((FORM & kFormCap) && fused) { // capping keeps the order
+                if (CAP_IN_EXP) { // capping keeps the order
                     const float y = m_tile * m_tile;
-                    m_tile *= fmaf(fmaf(y, a.cap_c[0], a.cap_c[1]), y, a.cap_c[2]);
+                    m_tile *= fmaf(fmaf(y, kc[0], kc[1]), y, kc[2]);
                 }
                 if (SCORED ? !__any_sync(0xffffffffu, m_used > -1e29f) : j == 0) { // O_t holds nothing of these rows yet
                     m_used = fmaxf(m_tile, -1e30f);
@@ -1045,10 +1044,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                 }
                 const float neg_m = -m_used;
                 uint32_t packed[16];
-                if ((FORM & kFormCap) && fused) {
-                    chunk_exp_cap(ra, a, neg_m, l2, packed);
+                if (CAP_IN_EXP) {
+                    chunk_exp_cap(ra, kc, neg_m, l2, packed);
                     tmem_st16(ts, packed);
-                    chunk_exp_cap(rb, a, neg_m, l2, packed);
+                    chunk_exp_cap(rb, kc, neg_m, l2, packed);
                     tmem_st16(ts + 16, packed);
                 } else {
                     chunk_exp<EMUL>(ra, sc, neg_m, l2, packed);
@@ -1280,8 +1279,9 @@ template <int D> int launch_prefill_hd(const flb_attn_params *p, const flb_score
         for (int k = 0; k < 5 - 2 * i; ++k) c *= a.cap_in;
         a.cap_c[i] = (float)c;
     }
+    if (a.cap_c[0] < kTiny) a.cap_c[0] = kTiny;
     // A distance bias grows towards the diagonal: from the last tile to the first a row's maximum is found at once, the other way round it
-    // passes the rescaling threshold at nearly every tile (4001 tokens, 32 heads: 225 us forwards, BACK us backwards).
+    // passes the rescaling threshold at nearly every tile (4001 tokens, 32 heads: 225 us forwards, 186 us backwards).
     a.backwards = a.slopes != nullptr;
     // The larger the group, the closer the list is to heaviest-first over everything (measured at batch 8 x 32 heads x 1024
     // tokens: 142 us with groups of 32 units, 138 us with 64, 139 us with 128, 141 us with all 256 in one group; at
