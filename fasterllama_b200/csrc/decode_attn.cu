@@ -313,7 +313,7 @@ __global__ void __launch_bounds__((NWARPS + 1) * 32) flb_decode_attn_kernel(cons
 #pragma unroll
                 for (int w = 0; w < NWARPS; ++w) t += red[w];
                 s_new = t;
-                if (FORM && a.cap_log2e > 0.f) s_new = a.cap_log2e * tanhf(s_new / a.cap_log2e); // at distance 0: no bias
+                if (FORM && a.cap_log2e > 0.f) s_new = cap_score(s_new, a.cap_log2e, a.inv_cap); // at distance 0: no bias
                 switch (a.mask_mode) {
                 case 1: // generic additive mask, row = query position, column = key position
                     s_new += __ldg(a.attn_mask + (size_t)past * a.mask_row_stride + past) * kLog2e;
@@ -388,9 +388,9 @@ __global__ void __launch_bounds__((NWARPS + 1) * 32) flb_decode_attn_kernel(cons
                 if (r >= rvalid) {
                     sc[it] = -INFINITY;
                 } else {
-                    if (FORM) { // scores are few beside the elements they came from: the accurate tanh costs nothing
+                    if (FORM) { // scores are few beside the elements they came from
                         const int key = row0 + t * TILE_ROWS + r;
-                        if (a.cap_log2e > 0.f) sc[it] = a.cap_log2e * tanhf(sc[it] / a.cap_log2e);
+                        if (a.cap_log2e > 0.f) sc[it] = cap_score(sc[it], a.cap_log2e, a.inv_cap);
                         sc[it] = fmaf(-slope, (float)(past - key), sc[it]);
                         if (key < begin) sc[it] = -INFINITY;
                     }

@@ -62,7 +62,7 @@ struct DecodeArgs {
     int form;              // any of the below is in use
     int G, Hkv;            // q heads per K/V head, K/V heads
     int kv_row_stride;
-    float cap_log2e;       // softcap * log2(e), 0 = none
+    float cap_log2e, inv_cap; // softcap * log2(e), 0 = none; its reciprocal
     const float *slopes;   // [H]
     const int *key_begin;  // [B]
 };

@@ -84,6 +84,24 @@ __device__ __forceinline__ float ex2_fma(float x) {
     p = fmaf(p, f, 1.0f);
     return __int_as_float(__float_as_int(p) + (__float_as_int(t) << 23));
 }
+// cap * tanh(x / cap), in any unit; inv_cap = 1 / cap.  Up to |u| = 1 tanh(u) / u is a polynomial in u^2 (own minimax fit, 2e-8 of tanh), beyond
+// tanh |u| = 1 - 2 / (1 + e^2|u|), where the difference cancels nothing: within 2^-22 of the cap everywhere.
+__device__ __forceinline__ float cap_score(float x, float cap, float inv_cap) {
+    const float u = x * inv_cap;
+    if (fabsf(u) <= 1.0f) {
+        const float y = u * u;
+        float p = fmaf(y, 0.0009637718f, -0.0059512793f);
+        p = fmaf(p, y, 0.019973271f);
+        p = fmaf(p, y, -0.053265836f);
+        p = fmaf(p, y, 0.13319583f);
+        p = fmaf(p, y, -0.3333213f);
+        p = fmaf(p, y, 0.9999997f);
+        return p * (u * cap);
+    }
+    const float e = ex2(fminf(fabsf(u), 64.0f) * 2.8853900817779268f); // 2 log2(e)
+    const float r = cap - __fdividef(2.0f * cap, 1.0f + e);
+    return u != u ? u : copysignf(r, u);
+}
 // max of three (one instruction on sm_100)
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;

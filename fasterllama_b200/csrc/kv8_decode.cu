@@ -98,28 +98,6 @@ template <int D> __device__ __forceinline__ void copy_step(uint32_t slot, const 
     }
 }
 
-// cap * tanh(x / cap): where no score of the warp passes the cap, a polynomial (own minimax fit of tanh(u) / u in u^2 on |u| <= 1, 2e-8
-// of tanh), else CUDA's tanhf, whose branches cost a warp four times as much.
-__device__ __forceinline__ void cap_scores(float (&x)[2], float cap, float inv_cap) {
-    float u[2] = {x[0] * inv_cap, x[1] * inv_cap};
-    if (__any_sync(0xffffffffu, !(fmaxf(fabsf(u[0]), fabsf(u[1])) <= 1.0f))) {
-        x[0] = cap * tanhf(u[0]);
-        x[1] = cap * tanhf(u[1]);
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const float y = u[i] * u[i];
-        float p = fmaf(y, 0.0009637718f, -0.0059512793f);
-        p = fmaf(p, y, 0.019973271f);
-        p = fmaf(p, y, -0.053265836f);
-        p = fmaf(p, y, 0.13319583f);
-        p = fmaf(p, y, -0.3333213f);
-        p = fmaf(p, y, 0.9999997f);
-        x[i] = p * (u[i] * cap);
-    }
-}
-
 // a few rows per CTA: the input form is looked at here and not compiled in
 __device__ __forceinline__ void load8(const Kv8DecodeArgs &a, int which, size_t token, int col, float (&x)[8]) {
     if (a.input_mode == 0)
@@ -425,9 +403,9 @@ __global__ void __launch_bounds__(kWarps * 32, D == 128 && NT == 1 ? 4 : 1) flb_
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) x[n][i] *= ks * qu[n];
-            if (FORM && a.cap_log2e > 0.f) cap_scores(x[n], a.cap_log2e, inv_cap);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
+                if (FORM && a.cap_log2e > 0.f) x[n][i] = cap_score(x[n][i], a.cap_log2e, inv_cap);
                 if (FORM) x[n][i] = fmaf(-slope[n], fabsf((float)(pos - kpos[i])), x[n][i]);
                 x[n][i] = vis[i] ? x[n][i] : -INFINITY;
             }

@@ -236,6 +236,7 @@ int flb_attn_decode_scored(const flb_attn_params *p, const flb_score_form *f, vo
     a.G = p->head_num / a.Hkv;
     a.kv_row_stride = kv_row_stride(p, f);
     a.cap_log2e = f ? f->softcap * 1.4426950408889634f : 0.f;
+    a.inv_cap = a.cap_log2e > 0.f ? 1.0f / a.cap_log2e : 0.f;
     a.slopes = f ? f->alibi_slopes : nullptr;
     a.key_begin = f ? f->key_begin : nullptr;
     a.form = a.Hkv != a.H || a.kv_row_stride != a.row_stride || a.cap_log2e > 0.f || a.slopes || a.key_begin;
