@@ -32,9 +32,10 @@ from ._lib import (  # noqa: F401  (re-exported)
 def _ptr(t: Any) -> int | None:
     if t is None:
         return None
-    if hasattr(t, "data_ptr"):
+    try:
         return t.data_ptr()
-    return t.ctypes.data  # numpy
+    except AttributeError:
+        return t.ctypes.data  # numpy
 
 
 _DTYPE_NAMES: dict[Any, str] = {}
@@ -48,9 +49,10 @@ def _dtype_name(t: Any) -> str:
 
 
 def _is_contiguous(t: Any) -> bool:
-    if hasattr(t, "is_contiguous"):
+    try:
         return t.is_contiguous()
-    return bool(t.flags["C_CONTIGUOUS"])
+    except AttributeError:
+        return bool(t.flags["C_CONTIGUOUS"])
 
 
 _IN_MODE = {"int32": FLB_IN_INT32, "float32": FLB_IN_F32, "float16": FLB_IN_F16}
@@ -171,7 +173,7 @@ def _check(t: Any, name: str, shape: tuple, dtype: str) -> int:
     """Address of a dense tensor of this shape and type, 0 for None."""
     if t is None:
         return 0
-    if tuple(t.shape) != shape or _dtype_name(t) != dtype or not _is_contiguous(t):
+    if t.shape != shape or _dtype_name(t) != dtype or not _is_contiguous(t):
         raise ValueError(f"{name} must be a dense {dtype} tensor of shape {shape}")
     return _ptr(t)
 
@@ -213,7 +215,8 @@ def make_scored_params(
     per-row key bounds (int32, decode [B], prefill [B,S]), and k, v [B,S,Hkv,d] with caches [B,Hkv,T,d] of fewer heads than q."""
     B, S, H, d = q.shape
     Hkv, T, dt = k.shape[2], k_cache.shape[2], _dtype_name(q)
-    if tuple(k.shape) != (B, S, Hkv, d) or tuple(v.shape) != (B, S, Hkv, d) or H % Hkv:
+    kv_shape = (B, S, Hkv, d)
+    if k.shape != kv_shape or v.shape != kv_shape or H % Hkv:
         raise ValueError("k and v must be [B,S,Hkv,d] with a number of heads that divides q's")
     if _dtype_name(k) != dt or _dtype_name(v) != dt or dt not in _IN_MODE:
         raise ValueError("q, k and v must share one type: int32, float32 or float16")

@@ -539,18 +539,23 @@ __global__ void __launch_bounds__(kWarps * 32, D == 128 && NT == 1 ? 4 : 1) flb_
     if (!last_flag) return;
     __threadfence();
     // The last split joins all: maximum and sum per head by a warp, then every thread four columns of one head over its share of the
-    // splits, eight loads under way, weights of 64 splits at a time in shared memory; the shares are added up in order.
+    // splits, sixteen loads under way, weights of 64 splits at a time in shared memory; the shares are added up in order.
     const size_t mbase = (unit * a.nchunk + chunk) * a.nsplit_max;
     float *const e_s = reinterpret_cast<float *>(ring_smem) + NTHREADS * 4; // [64][HEADS] behind the shares
     for (int hh = warp; hh < nheads; hh += kWarps) {
         const float2 *ml = reinterpret_cast<const float2 *>(a.part_ml) + mbase * HEADS + hh;
+        // the first 64 splits stay in registers: their weights need no second look
         const float2 own = lane < nsplit ? __ldcg(ml + (size_t)lane * HEADS) : make_float2(kNoMax, 0.f);
-        float M = own.x;
-        for (int s = lane + 32; s < nsplit; s += 32) M = fmaxf(M, __ldcg(ml + (size_t)s * HEADS).x);
+        const float2 own2 = lane + 32 < nsplit ? __ldcg(ml + (size_t)(lane + 32) * HEADS) : make_float2(kNoMax, 0.f);
+        float M = fmaxf(own.x, own2.x);
+        for (int s = lane + 64; s < nsplit; s += 32) M = fmaxf(M, __ldcg(ml + (size_t)s * HEADS).x);
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
-        float l = own.y * ex2(own.x - M);
-        for (int s = lane + 32; s < nsplit; s += 32) {
+        const float e0 = ex2(own.x - M), e1 = ex2(own2.x - M);
+        e_s[lane * HEADS + hh] = e0;
+        e_s[(lane + 32) * HEADS + hh] = e1;
+        float l = fmaf(own2.y, e1, own.y * e0);
+        for (int s = lane + 64; s < nsplit; s += 32) {
             const float2 v = __ldcg(ml + (size_t)s * HEADS);
             l = fmaf(v.y, ex2(v.x - M), l);
         }
@@ -571,14 +576,16 @@ __global__ void __launch_bounds__(kWarps * 32, D == 128 && NT == 1 ? 4 : 1) flb_
         const float4 *po = reinterpret_cast<const float4 *>(a.part_o) + mbase * HEADS * (D / 4) + quad;
         for (int s0 = 0; s0 < nsplit; s0 += 64) {
             const int ns = min(64, nsplit - s0);
-            __syncthreads();
-            for (int i = tid; i < ns * nheads; i += NTHREADS) {
-                const int s = i / nheads, hd = i - s * nheads;
-                e_s[s * HEADS + hd] = ex2(__ldcg(a.part_ml + ((mbase + s0 + s) * HEADS + hd) * 2) - w_m[0][hd]);
+            if (nsplit > 64 && (q0 > 0 || s0 > 0)) { // (the first 64 are there)
+                __syncthreads();
+                for (int i = tid; i < ns * nheads; i += NTHREADS) {
+                    const int s = i / nheads, hd = i - s * nheads;
+                    e_s[s * HEADS + hd] = ex2(__ldcg(a.part_ml + ((mbase + s0 + s) * HEADS + hd) * 2) - w_m[0][hd]);
+                }
+                __syncthreads();
             }
-            __syncthreads();
             if (!on) continue;
-#pragma unroll 8
+#pragma unroll 16
             for (int s = share; s < ns; s += shares) {
                 const float4 v = __ldcg(po + (size_t)(s0 + s) * HEADS * (D / 4));
                 const float e = e_s[s * HEADS + hh];

@@ -1342,9 +1342,19 @@ template <int D> int launch_prefill_hd(const flb_attn_params *p, const flb_score
     pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     pdl[0].val.programmaticStreamSerializationAllowed = 1;
     const bool generic_mask = (a.mask_mode == FLB_MASK_GENERIC);
-    auto kern = attn_kernel_of<D>(generic_mask, a.out_f16, scored ? kFormBounds | (a.cap_log2e > 0.f ? kFormCap : 0) | (a.slopes ? kFormBias : 0) : 0);
+    const int form = scored ? kFormBounds | (a.cap_log2e > 0.f ? kFormCap : 0) | (a.slopes ? kFormBias : 0) : 0;
+    auto kern = attn_kernel_of<D>(generic_mask, a.out_f16, form);
     constexpr size_t smem_bytes = prefill_smem(D);
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes) != cudaSuccess) return FLB_ERR_LAUNCH;
+    // the shared-memory opt-in is a property of (kernel, device): set once per device, not on every call
+    static std::atomic<unsigned long long> opted_in[2][2][8];
+    std::atomic<unsigned long long> &done = opted_in[generic_mask][a.out_f16 ? 1 : 0][form];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return FLB_ERR_DEVICE;
+    const unsigned long long bit = (dev >= 0 && dev < 64) ? (1ull << dev) : 0ull;
+    if (!(done.load(std::memory_order_acquire) & bit)) {
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes) != cudaSuccess) return FLB_ERR_LAUNCH;
+        if (bit) done.fetch_or(bit, std::memory_order_release);
+    }
     const long long num_items = (long long)B * H * ((S + 2 * BM - 1) / (2 * BM));
     cfg.attrs = pdl;
     cfg.numAttrs = 1;
