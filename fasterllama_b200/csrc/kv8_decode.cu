@@ -140,9 +140,15 @@ __device__ __forceinline__ void append_token(const Kv8DecodeArgs &a, int kv, siz
     }
 }
 
+// head dimension of column p of an accumulator row (see the output products: tile i, lane group g, half e)
+template <int D> __device__ __forceinline__ int dim_of(int p) {
+    const int i = p >> 4, g = (p & 15) >> 1;
+    return (i >> 3) * 128 + g * (D == 64 ? 8 : 16) + 2 * (i & 7) + (p & 1);
+}
+
 // FORM: capped scores, distance bias or key_begin.  NT: column tiles of eight = four q heads each.
 template <int D, int CODE, int NT, bool FORM>
-__global__ void __launch_bounds__(kWarps * 32, D == 128 && NT == 1 ? 4 : 1) flb_kv8_decode_kernel(const __grid_constant__ Kv8DecodeArgs a) {
+__global__ void __launch_bounds__(kWarps * 32, D == 128 ? (NT == 1 ? 4 : 3) : 1) flb_kv8_decode_kernel(const __grid_constant__ Kv8DecodeArgs a) {
     constexpr int HEADS = 4 * NT;
     constexpr int KCH = D / 64;   // 16-byte chunks of a K row per lane
     constexpr int VW = D / 32;    // 32-bit words of a V row per lane
@@ -153,7 +159,9 @@ __global__ void __launch_bounds__(kWarps * 32, D == 128 && NT == 1 ? 4 : 1) flb_
     __shared__ float q_unit[HEADS];                        // what a product with q_s is to be multiplied by
     __shared__ float w_m[kWarps][HEADS], w_l[kWarps][HEADS];
     extern __shared__ __align__(128) unsigned char ring_smem[];
-    float(*w_o)[HEADS][D] = reinterpret_cast<float(*)[HEADS][D]>(ring_smem); // the rings' room, once they are through
+    // The warps' results, in the rings' room once they are through.  Dims in the order in which the accumulators hold them (column 16 i + 2 g + e is
+    // dim_of() that) and 16 words between heads: the stores of a warp then meet no bank twice more than they have to.
+    float(*w_o)[HEADS][D + 16] = reinterpret_cast<float(*)[HEADS][D + 16]>(ring_smem);
     __shared__ TokenScales ts;
     __shared__ int last_flag;
 
@@ -494,38 +502,49 @@ __global__ void __launch_bounds__(kWarps * 32, D == 128 && NT == 1 ? 4 : 1) flb_
         }
 #pragma unroll
         for (int i = 0; i < MT; ++i)
-            *reinterpret_cast<float2 *>(&w_o[warp][4 * n + t][(i >> 3) * 128 + g * (D == 64 ? 8 : 16) + 2 * (i & 7)]) =
+            *reinterpret_cast<float2 *>(&w_o[warp][4 * n + t][16 * i + 2 * g]) =
                 make_float2((o[n][i][0] + o[n][i][1]) * v_down, (o[n][i][2] + o[n][i][3]) * v_down);
     }
     __syncthreads();
 
-    // ---- merge in warp order
+    // two finished values of a head, at dims d, d + 1
+    auto put = [&](int hh, int dim, float y0, float y1) {
+        const size_t oo = ((size_t)b * a.Hq + head0 + hh) * D + dim;
+        if (a.out_f16)
+            *reinterpret_cast<__half2 *>((__half *)a.out + oo) = __floats2half2_rn(y0, y1);
+        else
+            *reinterpret_cast<float2 *>((float *)a.out + oo) = make_float2(y0, y1);
+    };
+    auto finish = [&](int hh, int quad, const float4 &acc, float M, float l) { // columns 4 quad ..: two pairs of dims
+        const float inv = (l > 0.f || l != l) ? 1.0f / l : 0.f;
+        put(hh, dim_of<D>(4 * quad), acc.x * inv, acc.y * inv);
+        put(hh, dim_of<D>(4 * quad + 2), acc.z * inv, acc.w * inv);
+        if (a.ml && quad == 0) *reinterpret_cast<float2 *>(a.ml + ((size_t)b * a.Hq + head0 + hh) * 2) = make_float2(M, l);
+    };
+
+    // ---- merge in warp order, four columns to a thread
     const size_t pbase = ((unit * a.nchunk + chunk) * a.nsplit_max + split) * HEADS;
-    for (int i = tid; i < nheads * D; i += NTHREADS) {
-        const int hh = i / D, col = i - hh * D;
-        float M = kNoMax, acc = 0.f, l = 0.f;
+    for (int i = tid; i < nheads * (D / 4); i += NTHREADS) {
+        const int hh = i / (D / 4), quad = i % (D / 4);
+        float M = kNoMax, l = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) M = fmaxf(M, w_m[w][hh]);
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
             const float e = ex2(w_m[w][hh] - M);
-            acc = fmaf(w_o[w][hh][col], e, acc);
+            const float4 v = *reinterpret_cast<const float4 *>(&w_o[w][hh][4 * quad]);
+            acc.x = fmaf(v.x, e, acc.x);
+            acc.y = fmaf(v.y, e, acc.y);
+            acc.z = fmaf(v.z, e, acc.z);
+            acc.w = fmaf(v.w, e, acc.w);
             l = fmaf(w_l[w][hh], e, l);
         }
         if (nsplit == 1) {
-            const size_t oo = ((size_t)b * a.Hq + head0 + hh) * D + col;
-            const float y = (l > 0.f || l != l) ? acc / l : 0.f;
-            if (a.out_f16) ((__half *)a.out)[oo] = __float2half_rn(y); else ((float *)a.out)[oo] = y;
-            if (a.ml && col == 0) {
-                a.ml[((size_t)b * a.Hq + head0 + hh) * 2] = M;
-                a.ml[((size_t)b * a.Hq + head0 + hh) * 2 + 1] = l;
-            }
+            finish(hh, quad, acc, M, l);
         } else {
-            a.part_o[(pbase + hh) * D + col] = acc;
-            if (col == 0) {
-                a.part_ml[(pbase + hh) * 2] = M;
-                a.part_ml[(pbase + hh) * 2 + 1] = l;
-            }
+            reinterpret_cast<float4 *>(a.part_o)[(pbase + hh) * (D / 4) + quad] = acc;
+            if (quad == 0) reinterpret_cast<float2 *>(a.part_ml)[pbase + hh] = make_float2(M, l);
         }
     }
     if (nsplit == 1) return;
@@ -608,21 +627,7 @@ __global__ void __launch_bounds__(kWarps * 32, D == 128 && NT == 1 ? 4 : 1) flb_
                     acc.w += v.w;
                 }
         }
-        if (on && share == 0) {
-            const float l = w_l[0][hh];
-            const float y[4] = {acc.x / l, acc.y / l, acc.z / l, acc.w / l};
-            const bool some = l > 0.f || l != l;
-            const size_t oo = ((size_t)b * a.Hq + head0 + hh) * D + (quad - hh * (D / 4)) * 4;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float r4 = some ? y[e] : 0.f;
-                if (a.out_f16) ((__half *)a.out)[oo + e] = __float2half_rn(r4); else ((float *)a.out)[oo + e] = r4;
-            }
-            if (a.ml && quad == hh * (D / 4)) {
-                a.ml[((size_t)b * a.Hq + head0 + hh) * 2] = w_m[0][hh];
-                a.ml[((size_t)b * a.Hq + head0 + hh) * 2 + 1] = l;
-            }
-        }
+        if (on && share == 0) finish(hh, quad - hh * (D / 4), acc, w_m[0][hh], w_l[0][hh]);
     }
     if (tid == 0) a.counters[unit * a.nchunk + chunk] = 0u; // ready for the next call
 }
@@ -664,7 +669,7 @@ template <int D, int CODE, int NT> cudaError_t launch_t(const Kv8DecodeArgs &a, 
     const unsigned grid = (unsigned)a.c.B * (unsigned)a.c.H * (unsigned)a.nchunk * (unsigned)a.nsplit_max;
     const bool form = a.cap_log2e > 0.f || a.slopes || a.key_begin;
     constexpr int smem = kWarps * Ring<D>::kWarpBytes;
-    static_assert(smem >= kWarps * 4 * NT * D * (int)sizeof(float), "the warps' results take the rings' room");
+    static_assert(smem >= kWarps * 4 * NT * (D + 16) * (int)sizeof(float), "the warps' results take the rings' room");
     auto kern = form ? flb_kv8_decode_kernel<D, CODE, NT, true> : flb_kv8_decode_kernel<D, CODE, NT, false>;
     // the shared-memory opt-in is a property of (kernel, device): set once per device
     static std::atomic<unsigned long long> opted_in[2] = {{0}, {0}};

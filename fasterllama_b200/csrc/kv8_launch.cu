@@ -163,7 +163,7 @@ int flb_kv8_validate_decode(const flb_kv8_decode_params *p) {
     if ((st = check_rope(p->freq_cis, p->freq_rows)) != FLB_OK) return st;
     if (!(p->softcap >= 0.f) || p->softcap > 3.402823466e38f) return FLB_ERR_BAD_SHAPE;
     if (!p->out) return FLB_ERR_NULL_POINTER;
-    if (!aligned4(p->out)) return FLB_ERR_MISALIGNED;
+    if (!aligned16(p->out)) return FLB_ERR_MISALIGNED;
     if ((p->weight_in != nullptr) != (p->weight_out != nullptr)) return FLB_ERR_NULL_POINTER;
     if (!aligned16(p->weight_in) || !aligned16(p->weight_out)) return FLB_ERR_MISALIGNED;
     const int mp = max_past_of(p);
