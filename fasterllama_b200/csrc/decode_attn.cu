@@ -197,17 +197,13 @@ __global__ void __launch_bounds__((NWARPS + 1) * 32) flb_decode_attn_kernel(cons
     if (a.early_start) grid_launch_dependents();
     if (split >= nsplit) return;
 
-    const int hk = FORM ? h / a.G : h;                                   // K/V head
-    const size_t kv_unit = FORM ? (size_t)b * a.Hkv + hk : (size_t)unit; // its cache slab
-    const int kv_row_stride = FORM ? a.kv_row_stride : a.row_stride;
-    const int begin = (FORM && a.key_begin) ? __ldg(a.key_begin + b) : 0;
-    int row0 = split * a.split_len;
-    int rows = max(0, min(a.split_len, past - row0));
-    if (FORM && begin > row0) { // whole tiles below the first visible key are not read
-        const int skip = min(begin - row0, rows) / TILE_ROWS * TILE_ROWS;
-        row0 += skip;
-        rows -= skip;
-    }
+    const int hk = FORM ? h / a.G : h;                   // K/V head
+    const int kv_unit = FORM ? b * a.Hkv + hk : unit;    // its cache slab
+    const int begin = (FORM && a.key_begin) ? max(0, __ldg(a.key_begin + b)) : 0;
+    // whole tiles below the first visible key are not read
+    const int skip = FORM ? min(max(begin - split * a.split_len, 0), max(0, min(a.split_len, past - split * a.split_len))) / TILE_ROWS * TILE_ROWS : 0;
+    const int row0 = split * a.split_len + skip;
+    const int rows = max(0, min(a.split_len - skip, past - row0));
     const int ntiles = (rows + TILE_ROWS - 1) / TILE_ROWS;
     const bool is_last = (split == nsplit - 1);
 
@@ -231,8 +227,8 @@ __global__ void __launch_bounds__((NWARPS + 1) * 32) flb_decode_attn_kernel(cons
     if (warp == NWARPS) {
         // ---------------- producer warp: one lane issues the bulk copies -------------------
         if (lane == 0) {
-            const unsigned char *kb = (const unsigned char *)a.k_cache + (kv_unit * a.T + row0) * ROW_BYTES;
-            const unsigned char *vb = (const unsigned char *)a.v_cache + (kv_unit * a.T + row0) * ROW_BYTES;
+            const unsigned char *kb = (const unsigned char *)a.k_cache + ((size_t)kv_unit * a.T + row0) * ROW_BYTES;
+            const unsigned char *vb = (const unsigned char *)a.v_cache + ((size_t)kv_unit * a.T + row0) * ROW_BYTES;
             for (int t = 0; t < ntiles; ++t) {
                 const int s = t % STAGES;
                 const uint32_t use = (uint32_t)(t / STAGES);
@@ -271,7 +267,7 @@ __global__ void __launch_bounds__((NWARPS + 1) * 32) flb_decode_attn_kernel(cons
                 float qraw = 0.f, kraw = 0.f;
                 if (i < D) {
                     qraw = load_input<D>(a, a.q, a.q_w_scale, a.row_stride, b, h, i);
-                    if (is_last) kraw = load_input<D>(a, a.k, a.k_w_scale, kv_row_stride, b, hk, i);
+                    if (is_last) kraw = load_input<D>(a, a.k, a.k_w_scale, FORM ? a.kv_row_stride : a.row_stride, b, hk, i);
                 }
                 float qrot = qraw, krot = kraw;
                 if (a.freq_cis) {
@@ -382,6 +378,7 @@ __global__ void __launch_bounds__((NWARPS + 1) * 32) flb_decode_attn_kernel(cons
                 for (int off = LPR / 2; off > 0; off >>= 1) sc[it] += __shfl_xor_sync(0xffffffffu, sc[it], off);
             }
             float mt = kMaxInit;
+            const float dist0 = FORM ? (float)(past - row0 - t * TILE_ROWS - warp * RPI - sub) : 0.f; // of this lane's first row
 #pragma unroll
             for (int it = 0; it < ITERS; ++it) {
                 const int r = (it * NWARPS + warp) * RPI + sub;
@@ -389,10 +386,9 @@ __global__ void __launch_bounds__((NWARPS + 1) * 32) flb_decode_attn_kernel(cons
                     sc[it] = -INFINITY;
                 } else {
                     if (FORM) { // scores are few beside the elements they came from
-                        const int key = row0 + t * TILE_ROWS + r;
                         if (a.cap_log2e > 0.f) sc[it] = cap_score(sc[it], a.cap_log2e, a.inv_cap);
-                        sc[it] = fmaf(-slope, (float)(past - key), sc[it]);
-                        if (key < begin) sc[it] = -INFINITY;
+                        sc[it] = fmaf(-slope, dist0 - (float)(it * NWARPS * RPI), sc[it]);
+                        if (row0 + t * TILE_ROWS + r < begin) sc[it] = -INFINITY;
                     }
                     if (mask_row) sc[it] += __ldg(mask_row + t * TILE_ROWS + r) * kLog2e;
                 }
@@ -438,9 +434,9 @@ __global__ void __launch_bounds__((NWARPS + 1) * 32) flb_decode_attn_kernel(cons
             for (int e = 0; e < DPT; ++e) {
                 const int i = tid + e * NC;
                 if (i < D) {
-                    const float vraw = load_input<D>(a, a.v, a.v_w_scale, kv_row_stride, b, hk, i);
+                    const float vraw = load_input<D>(a, a.v, a.v_w_scale, FORM ? a.kv_row_stride : a.row_stride, b, hk, i);
                     vnew[e] = CacheIO<CacheT>::round(vraw);
-                    const size_t cidx = (kv_unit * a.T + past) * D + i;
+                    const size_t cidx = ((size_t)kv_unit * a.T + past) * D + i;
                     if (!FORM || hk * a.G == h) { // the first q head of a K/V head stores for all; none of them reads the row back
                         CacheIO<CacheT>::store((CacheT *)a.k_cache + cidx, krot_keep[e]);
                         CacheIO<CacheT>::store((CacheT *)a.v_cache + cidx, vraw);
