@@ -52,6 +52,7 @@ struct Kv8Input { // q, k or v rows as the projections leave them
 struct Kv8AppendArgs {
     Kv8Cache c;
     int S, nwin; // tokens; blocks that a sequence's tokens can touch
+    int max_past; // sequences with more cached rows are left alone
     int start_pos;
     const int *past_lens, *new_lens, *token_pos;
     Kv8Input in[2]; // k, v
@@ -234,6 +235,12 @@ template <int CODE> __device__ __forceinline__ bool kv8_near_tie(const float (&y
 // Eight values over their block's scale, rounded to codes; `inv` = 1 / scale.  The quotient is defined as one IEEE division; multiplying by
 // the reciprocal is off by 2^-22 at most, which shows only next to a tie, and there the division is done.  A scale of 0, infinity or NaN gives
 // codes 0.
+// (out of line: inlined, its eight divisions are issued under a predicate for every value)
+template <int CODE> __device__ __noinline__ uint2 kv8_encode8_exact(float4 u, float4 v, float scale) {
+    const float a[4] = {__fdiv_rn(u.x, scale), __fdiv_rn(u.y, scale), __fdiv_rn(u.z, scale), __fdiv_rn(u.w, scale)};
+    const float b[4] = {__fdiv_rn(v.x, scale), __fdiv_rn(v.y, scale), __fdiv_rn(v.z, scale), __fdiv_rn(v.w, scale)};
+    return make_uint2(kv8_pack4<CODE>(a), kv8_pack4<CODE>(b));
+}
 template <int CODE> __device__ __forceinline__ uint2 kv8_encode8(const float (&x)[8], float scale, float inv) {
     if (!(scale > 0.f && scale <= 3.402823466e38f)) return make_uint2(0u, 0u);
     const bool exact = !(inv <= 3.402823466e38f && scale <= 1e37f); // the reciprocal of a subnormal scale overflows, that of a huge one is subnormal
@@ -245,10 +252,7 @@ template <int CODE> __device__ __forceinline__ uint2 kv8_encode8(const float (&x
         y[i] = v.x;
         y[i + 1] = v.y;
     }
-    if (exact || kv8_near_tie<CODE>(y)) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = __fdiv_rn(x[i], scale);
-    }
+    if (exact || kv8_near_tie<CODE>(y)) return kv8_encode8_exact<CODE>(make_float4(x[0], x[1], x[2], x[3]), make_float4(x[4], x[5], x[6], x[7]), scale);
     const float a[4] = {y[0], y[1], y[2], y[3]}, b[4] = {y[4], y[5], y[6], y[7]};
     return make_uint2(kv8_pack4<CODE>(a), kv8_pack4<CODE>(b));
 }

@@ -25,7 +25,7 @@ template <int D, int CODE, int MODE> __global__ void __launch_bounds__(1024) flb
 
     const int past = a.past_lens ? __ldg(a.past_lens + b) : a.start_pos;
     const int n = a.new_lens ? __ldg(a.new_lens + b) : a.S;
-    if (past < 0 || n < 0 || n > a.S || past > a.c.T - n) { // nothing of this sequence is touched
+    if (past < 0 || n < 0 || n > a.S || past > min(a.c.T - n, a.max_past)) { // nothing of this sequence is touched
         if (threadIdx.x == 0 && a.status) atomicOr(a.status, kKv8BadLen);
         return;
     }

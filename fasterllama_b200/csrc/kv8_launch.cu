@@ -223,6 +223,7 @@ int flb_kv8_append(const flb_kv8_append_params *p, void *cuda_stream) {
     a.c = cache_of(p->cache);
     a.S = p->seq_len;
     a.nwin = window_blocks(p->cache, p->seq_len, p->past_lens != nullptr, p->start_pos);
+    a.max_past = p->cache.total_len;
     a.start_pos = p->start_pos;
     a.past_lens = p->past_lens;
     a.new_lens = p->new_lens;
@@ -288,6 +289,7 @@ int flb_kv8_decode(const flb_kv8_decode_params *p, void *cuda_stream) {
         t.c = a.c;
         t.S = 1;
         t.nwin = 1;
+        t.max_past = a.nsplit_max * a.split_len - 1; // what the attention kernel will not look at is not stored either
         t.start_pos = a.start_pos;
         t.past_lens = a.past_lens;
         t.new_lens = nullptr;

@@ -105,7 +105,8 @@ typedef struct flb_kv8_decode_params {
     int out_dtype;           /* flb_dtype                                               */
     void *scratch;           /* flb_kv8_decode_workspace_bytes()                        */
     size_t scratch_bytes;
-    int scratch_zeroed;      /* promise: the first flb_kv8_counter_bytes() bytes are zero on entry (they are left zero) */
+    int scratch_zeroed;      /* promise: the first flb_kv8_counter_bytes() bytes are zero on entry.  They are left zero; a call of
+                                other sizes in between may write there */
     int split_len;           /* rows of one split of a sequence, a multiple of 128 up to 2048; 0 = default.  Results
                                 depend on it and on each sequence alone, never on the batch or the grid */
 } flb_kv8_decode_params;
@@ -133,7 +134,8 @@ typedef struct flb_kv8_evict_params {
 } flb_kv8_evict_params;
 
 /* Error bits in the status word (the head of the decode and evict scratch, *status of an append). */
-#define FLB_KV8_STATUS_BAD_LEN 4u   /* a cached length, or length + tokens, outside the slab: that sequence was left alone */
+#define FLB_KV8_STATUS_BAD_LEN 4u   /* a cached length, or length + tokens, outside the slab or above max_past_len: that sequence
+                                       was left alone, and its output rows are zero */
 #define FLB_KV8_STATUS_BAD_POS 32u  /* a position outside the RoPE table: the nearest row was used */
 
 /* Host-side argument checks only (no CUDA call); the launch entry points run them first. */

@@ -355,6 +355,39 @@ def test_decode_bad_length_is_flagged_and_gives_zeros(cuda_device):
     same(c, before)
 
 
+@pytest.mark.parametrize("Hq", [2, 20])  # the attention kernel stores the token itself, or a launch in front does
+def test_decode_length_above_the_promised_bound(cuda_device, Hq):
+    g = gen(15)
+    c = used_cache(g, 2, 2, 512, 64, 16, I8)
+    before = clone(c)
+    q, _ = tokens(g, "float16", 2, 1, Hq, 64)
+    k, _ = tokens(g, "float16", 2, 1, 2, 64)
+    o = torch.full((2, Hq, 1, 64), math.nan, device=DEV)
+    s = torch.zeros(kv8.decode_workspace_bytes(2, Hq, 2, 512, 64, block_len=16), dtype=torch.uint8, device=DEV)
+    kv8.decode(c, q, k, k, o, past_lens=i32([400, 100]), max_past_len=120, scratch=s)
+    torch.cuda.synchronize()
+    assert A.scratch_status(s) == kv8.STATUS_BAD_LEN
+    assert float(o[0].abs().max()) == 0 and bool(o[1].isfinite().all())
+    assert torch.equal(c.k[0], before.k[0]) and torch.equal(c.v_scale[0], before.v_scale[0]) and not torch.equal(c.k[1], before.k[1])
+
+
+def test_decode_q_that_is_not_finite_reaches_its_own_rows_only(cuda_device):
+    for dtype in (I8, E4):
+        g = gen(16)
+        c = used_cache(g, 1, 2, 256, 128, 32, dtype)
+        q, _ = tokens(g, "float32", 1, 1, 8, 128)
+        k, _ = tokens(g, "float32", 1, 1, 2, 128)
+        s = torch.zeros(kv8.decode_workspace_bytes(1, 8, 2, 256, 128, block_len=32), dtype=torch.uint8, device=DEV)
+        a, b = torch.empty(1, 8, 1, 128, device=DEV), torch.empty(1, 8, 1, 128, device=DEV)
+        kv8.decode(c, q, k, k, a, past_lens=i32([200]), scratch=s)
+        q[0, 0, 2, 7], q[0, 0, 5, 100] = math.nan, math.inf
+        kv8.decode(c, q, k, k, b, past_lens=i32([200]), scratch=s)
+        bad = [2, 5]
+        assert bool(b[0, bad].isnan().all())
+        rest = [h for h in range(8) if h not in bad]
+        assert torch.equal(a[0, rest], b[0, rest])
+
+
 def test_decode_on_another_stream_and_in_a_replayed_graph(cuda_device):
     g = gen(13)
     B, H, T, d = 2, 4, 512, 128
@@ -498,6 +531,13 @@ def test_evict_long_slabs(cuda_device):
     """Several passes of the selecting block over the rows, more blocks than a block has threads."""
     run_evict(28, lens=[20000], T=20000 // 16 * 16 + 16, budget=7001, recent=100, sinks=4, d=64, block=16)
     run_evict(29, lens=[40001], T=40064, budget=40000, recent=100, sinks=4, d=64, block=32, H=1)
+
+
+def test_evict_slabs_beyond_the_registers(cuda_device):
+    """More rows than a cluster's threads keep in registers: the keys are read again at every pass."""
+    run_evict(31, lens=[150001], T=150016, budget=3000, recent=100, sinks=4, d=64, block=16, H=1)
+    w = torch.randint(0, 5, (2, 1, 140000), generator=gen(32), device=DEV).float()
+    run_evict(33, lens=[140000, 2500], T=140000, budget=2000, recent=10, sinks=0, d=64, block=32, H=1, weight=w, in_place=True)
 
 
 def test_evict_bad_length_is_flagged_and_left_alone(cuda_device):
