@@ -186,7 +186,7 @@ int flb_kv8_validate_evict(const flb_kv8_evict_params *p) {
     if (p->budget <= 0 || p->recent < 0 || p->sinks < 0 || p->recent > p->budget || p->sinks > p->budget - p->recent) return FLB_ERR_BAD_SHAPE;
     if (!p->past_lens && (p->start_pos < 0 || p->start_pos > p->cache.total_len)) return FLB_ERR_BAD_SHAPE;
     if (!aligned16(p->scratch)) return FLB_ERR_MISALIGNED;
-    if (!aligned16(p->weight) || !aligned16(p->cache.row_pos) || !aligned4(p->weight_out) || !aligned4(p->pos_out)) return FLB_ERR_MISALIGNED;
+    if (!aligned16(p->weight) || !aligned16(p->cache.row_pos) || !aligned16(p->weight_out) || !aligned16(p->pos_out)) return FLB_ERR_MISALIGNED;
     if (8ull * p->cache.batch_size * p->cache.kv_head_num * (p->cache.total_len / p->cache.block_len + 1) > 0x7fffffffull) return FLB_ERR_TOO_LARGE;
     if (p->scratch_bytes < evict_bytes(p->cache)) return FLB_ERR_SCRATCH_TOO_SMALL;
     return FLB_OK;

@@ -126,7 +126,7 @@ typedef struct flb_kv8_evict_params {
     int recent;              /* sinks + recent <= budget                                */
     int sinks;
     const int *next_pos;     /* device int[B]: position of the next token; needed when recent > 0 */
-    const float *weight;     /* [B,Hkv,T]; 16-byte aligned, as row_pos                  */
+    const float *weight;     /* [B,Hkv,T]; this, the two results and row_pos 16-byte aligned */
     float *weight_out;       /* [B,Hkv,T], rows 0..m-1 are written                      */
     int *pos_out;
     void *scratch;           /* flb_kv8_evict_workspace_bytes(); need not be zeroed     */
