@@ -169,13 +169,39 @@ def make_params(
 _PACK_PARAMS, _PACK_FORM = _lib.packer(FlbAttnParams), _lib.packer(FlbScoreForm)
 
 
-def _check(t: Any, name: str, shape: tuple, dtype: str) -> int:
-    """Address of a dense tensor of this shape and type, 0 for None."""
-    if t is None:
-        return 0
-    if t.shape != shape or _dtype_name(t) != dtype or not _is_contiguous(t):
-        raise ValueError(f"{name} must be a dense {dtype} tensor of shape {shape}")
+def _np_dense(t, name, shape, dtype, dev):
+    if t.shape != shape or (dtype is not None and t.dtype != dtype) or not _is_contiguous(t):
+        raise ValueError(f"{name} must be a dense {dtype} array of shape {shape}")
     return _ptr(t)
+
+
+def _np_opt(t, name, shape, dtype, dev):
+    return 0 if t is None else _np_dense(t, name, shape, dtype, dev)
+
+
+def _np_rows(t, name, shape, dtype, dev):
+    if t.shape != shape or (dtype is not None and t.dtype != dtype):
+        raise ValueError(f"{name} must be {dtype} of shape {shape}")
+    return _ptr(t), _token_row_stride(t, *shape)
+
+
+def _checks(t):
+    """Checks for tensors of this kind (see tensor_args.cpp for torch's) and the types float32 and int32."""
+    if not hasattr(t, "data_ptr"):
+        import numpy as np
+
+        return _np_dense, _np_opt, _np_rows, np.float32, np.int32
+    global _torch_checks
+    if _torch_checks is None:
+        import torch
+
+        from . import _tensor_args as n
+
+        _torch_checks = n.dense, n.opt, n.rows, torch.float32, torch.int32
+    return _torch_checks
+
+
+_torch_checks: tuple | None = None
 
 
 def make_scored_params(
@@ -213,34 +239,31 @@ def make_scored_params(
 ) -> tuple[FlbAttnParams, FlbScoreForm]:
     """A parameter block as from `make_params` and the score form beside it (see flb_score_form): capped scores, distance bias (float32 [H]),
     per-row key bounds (int32, decode [B], prefill [B,S]), and k, v [B,S,Hkv,d] with caches [B,Hkv,T,d] of fewer heads than q."""
+    dense, opt, rows, f32, i32 = _checks(q)
     B, S, H, d = q.shape
-    Hkv, T, dt = k.shape[2], k_cache.shape[2], _dtype_name(q)
-    kv_shape = (B, S, Hkv, d)
-    if k.shape != kv_shape or v.shape != kv_shape or H % Hkv:
-        raise ValueError("k and v must be [B,S,Hkv,d] with a number of heads that divides q's")
-    if _dtype_name(k) != dt or _dtype_name(v) != dt or dt not in _IN_MODE:
-        raise ValueError("q, k and v must share one type: int32, float32 or float16")
-    cdt, odt = _dtype_name(k_cache), _dtype_name(out)
-    if cdt not in _DT or odt not in _DT:
-        raise ValueError("caches and out must be float32 or float16")
-    row, krow, vrow = _token_row_stride(q, B, S, H, d), _token_row_stride(k, B, S, Hkv, d), _token_row_stride(v, B, S, Hkv, d)
+    Hkv, T, dt = k.shape[2], k_cache.shape[2], q.dtype
+    mode, cdt, odt = _IN_MODE.get(_dtype_name(q)), _DT.get(_dtype_name(k_cache)), _DT.get(_dtype_name(out))
+    if mode is None or cdt is None or odt is None:
+        raise ValueError("q, k and v must be int32, float32 or float16, caches and out float32 or float16")
+    if H % Hkv:
+        raise ValueError("the number of K/V heads must divide that of the q heads")
+    kv_shape, cache_shape = (B, S, Hkv, d), (B, Hkv, T, d)
+    (qp, row), (kp, krow), (vp, vrow) = rows(q, "q", (B, S, H, d), dt, None), rows(k, "k", kv_shape, dt, None), rows(v, "v", kv_shape, dt, None)
     if krow != vrow:
         raise ValueError("k and v must share one token-row stride")
-    rows = (B,) if S == 1 else (B, S)
+    bounds = (B,) if S == 1 else (B, S)
     if attn_mask is not None and not mask_row_stride:
         mask_row_stride = attn_mask.shape[-1]
-    if scratch is None:
-        sp = sn = 0
-    else:
-        sp, sn = _ptr(scratch), scratch.numel() * scratch.element_size() if hasattr(scratch, "numel") else scratch.nbytes
     p = FlbAttnParams.from_buffer_copy(_PACK_PARAMS.pack(
-        B, H, d, S, start_pos, T, _check(past_lens, "past_lens", (B,), "int32"), max_past_len, _IN_MODE[dt], _ptr(q), _ptr(k), _ptr(v), _ptr(act_scale) or 0,
+        B, H, d, S, start_pos, T, opt(past_lens, "past_lens", (B,), i32, None), max_past_len, mode, qp, kp, vp, _ptr(act_scale) or 0,
         _ptr(q_w_scale) or 0, _ptr(k_w_scale) or 0, _ptr(v_w_scale) or 0, _ptr(freq_cis) or 0, rope_pos0, 1 if rope_add_past else 0, mask_mode,
-        _ptr(attn_mask) or 0, mask_row_stride, _check(k_cache, "k_cache", (B, Hkv, T, d), cdt), _check(v_cache, "v_cache", (B, Hkv, T, d), cdt), _DT[cdt],
-        _check(out, "out", (B, H, S, d), odt), _DT[odt], softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(d), sp, sn, 1 if scratch_zeroed else 0,
+        _ptr(attn_mask) or 0, mask_row_stride, dense(k_cache, "k_cache", cache_shape, k_cache.dtype, None),
+        dense(v_cache, "v_cache", cache_shape, k_cache.dtype, None), cdt, dense(out, "out", (B, H, S, d), out.dtype, None), odt,
+        softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(d), _ptr(scratch) or 0, 0 if scratch is None else scratch.nbytes, 1 if scratch_zeroed else 0,
         split_len, _ptr(out_q8) or 0, _ptr(out_q8_scale) or 0, *_NO_PEERS, 0, 0, 0, early_start, 0 if row == H * d else row))
     f = FlbScoreForm.from_buffer_copy(_PACK_FORM.pack(
-        Hkv, krow, softcap, _check(alibi_slopes, "alibi_slopes", (H,), "float32"), _check(key_begin, "key_begin", rows, "int32"), _check(key_end, "key_end", rows, "int32")))
+        Hkv, krow, softcap, opt(alibi_slopes, "alibi_slopes", (H,), f32, None), opt(key_begin, "key_begin", bounds, i32, None),
+        opt(key_end, "key_end", bounds, i32, None)))
     # keep the tensors alive as long as the blocks
     p._keep = (q, k, v, k_cache, v_cache, out, scratch, past_lens, act_scale, q_w_scale, k_w_scale, v_w_scale, freq_cis, attn_mask, out_q8, out_q8_scale)
     f._keep = (alibi_slopes, key_begin, key_end)
@@ -281,7 +304,7 @@ def _stream_handle(stream) -> int | None:
     if stream is None:
         import torch
 
-        return torch.cuda.current_stream().cuda_stream
+        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
     if hasattr(stream, "cuda_stream"):
         return stream.cuda_stream
     return int(stream)

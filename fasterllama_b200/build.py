@@ -12,6 +12,7 @@ PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG_DIR)
 CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_PATH = os.path.join(PKG_DIR, "libflb_attn.so")
+ARGS_PATH = os.path.join(PKG_DIR, "_tensor_args.so")
 ORACLE_DIR = os.path.join(ROOT, "oracle")
 ORACLE_LIB = os.path.join(ORACLE_DIR, "libflb_oracle.so")
 
@@ -47,6 +48,24 @@ def build_cuda(force: bool = False, verbose: bool = False) -> str:
     cmd = [_nvcc(), *NVCC_FLAGS, *(["-Xptxas", "-v"] if verbose else []), "-o", LIB_PATH, *srcs]
     subprocess.run(cmd, check=True)
     return LIB_PATH
+
+
+def build_tensor_args(force: bool = False) -> str:
+    """The binding's tensor checks (csrc/tensor_args.cpp), a Python extension module against this interpreter and torch."""
+    src = os.path.join(CSRC, "tensor_args.cpp")
+    if not force and _newer(ARGS_PATH, [src]):
+        return ARGS_PATH
+    import sysconfig
+
+    import torch
+
+    root = os.path.dirname(torch.__file__)
+    inc = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include")]
+    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(a for p in inc for a in ("-isystem", p)), "-I" + sysconfig.get_paths()["include"], src, "-o", ARGS_PATH,
+           "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    subprocess.run(cmd, check=True)
+    return ARGS_PATH
 
 
 def build_oracle(force: bool = False) -> str:
@@ -104,6 +123,7 @@ def build_e2e_variants(force: bool = False) -> list[str]:
 
 def build_all(force: bool = False, verbose: bool = False) -> None:
     build_cuda(force, verbose)
+    build_tensor_args(force)
     build_oracle(force)
     build_reference(force)
     build_e2e_variants(force)

@@ -14,7 +14,7 @@ from typing import Any
 
 import torch
 
-from . import _lib
+from . import _lib, _tensor_args
 from ._lib import FLB_F16, FLB_F32, FLB_IN_F16, FLB_IN_F32, FLB_IN_INT32  # noqa: F401
 
 FLB_KV8_I8, FLB_KV8_E4M3 = 0, 1
@@ -139,21 +139,8 @@ def empty_cache(batch_size: int, kv_head_num: int, total_len: int, size_per_head
     return Cache(*codes, *scales, row_pos=pos)
 
 
-def _refuse(t, name, shape, dtype, dev):
-    if t.get_device() != dev:
-        raise ValueError(f"{name} is on {t.device}, the cache on another device")
-    raise ValueError(f"{name} must be a dense {dtype} tensor of shape {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
-
-
-def _dense(t: torch.Tensor, name: str, shape, dtype, dev: int) -> int:
-    """Address of a dense tensor of this shape, type and device."""
-    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous() or t.get_device() != dev:
-        _refuse(t, name, shape, dtype, dev)
-    return t.data_ptr()
-
-
-def _opt(t: torch.Tensor | None, name: str, shape, dtype, dev: int) -> int:
-    return 0 if t is None else _dense(t, name, shape, dtype, dev)
+# (tensor, name, shape, dtype, device index) -> address of a dense tensor, 0 for None, (address, token-row stride) of q, k or v
+_dense, _opt, _rows = _tensor_args.dense, _tensor_args.opt, _tensor_args.rows
 
 
 def _cache(c: Cache) -> tuple:
@@ -171,20 +158,6 @@ def _cache(c: Cache) -> tuple:
     return (B, H, d, T, T // n, code, _dense(k, "k", shape, k.dtype, dev), _dense(c.v, "v", shape, k.dtype, dev),
             _dense(c.k_scale, "k_scale", scales, torch.float32, dev), _dense(c.v_scale, "v_scale", scales, torch.float32, dev),
             _opt(c.row_pos, "row_pos", (B, H, T), torch.int32, dev)), dev
-
-
-def _rows(t: torch.Tensor, name: str, shape, dtype, dev: int) -> tuple[int, int]:
-    """Address and token-row stride (elements) of q, k or v [B,S,heads,d]: dense heads, one stride between tokens."""
-    if t.dtype is not dtype or t.shape != shape or t.get_device() != dev:
-        _refuse(t, name, shape, dtype, dev)
-    B, S, H, d = shape
-    if t.is_contiguous():
-        return t.data_ptr(), H * d
-    st = t.stride()
-    row = st[1] if S > 1 else (st[0] if B > 1 else H * d)
-    if st[3] != 1 or (H > 1 and st[2] != d) or (S > 1 and st[1] != row) or (B > 1 and st[0] != S * row) or row < H * d:
-        raise ValueError(f"{name} must be [B,S,heads,d] with unit element stride, head stride d and one stride between tokens")
-    return t.data_ptr(), row
 
 
 def _kv_rows(k, v, shape, dtype, dev):
