@@ -18,12 +18,12 @@ __device__ __forceinline__ void kv8_begin() {
     grid_launch_dependents();
 }
 template <typename Kernel, typename... Args>
-inline cudaError_t kv8_launch(Kernel kernel, unsigned grid, unsigned threads, size_t smem, cudaStream_t stream, const Args &...args) {
+inline cudaError_t kv8_launch(Kernel kernel, dim3 grid, unsigned threads, size_t smem, cudaStream_t stream, const Args &...args) {
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
+    cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;

@@ -16,12 +16,7 @@ template <int D, int CODE, int MODE> __global__ void __launch_bounds__(1024) flb
     constexpr int CPR = D / 8; // chunks per row
     __shared__ uint32_t red[32];
     kv8_begin();
-    unsigned id = blockIdx.x;
-    const int kv = (int)(id & 1u);
-    id >>= 1;
-    const int h = (int)(id % (unsigned)a.c.H);
-    id /= (unsigned)a.c.H;
-    const int j = (int)(id % (unsigned)a.nwin), b = (int)(id / (unsigned)a.nwin);
+    const int kv = (int)(blockIdx.x & 1u), h = (int)(blockIdx.x >> 1), j = (int)blockIdx.y, b = (int)blockIdx.z;
 
     const int past = a.past_lens ? __ldg(a.past_lens + b) : a.start_pos;
     const int n = a.new_lens ? __ldg(a.new_lens + b) : a.S;
@@ -73,9 +68,8 @@ template <int D, int CODE, int MODE> __global__ void __launch_bounds__(1024) flb
     const float ratio = grown ? __fdiv_rn(old, scale) : 1.f, inv = __fdiv_rn(1.f, scale);
 #pragma unroll
     for (int i = 0; i < kChunks; ++i) {
-        const int ch = threadIdx.x + i * blockDim.x;
         const int row = r0 + i * step;
-        uint2 *dst = reinterpret_cast<uint2 *>(codes) + ch;
+        uint2 *dst = reinterpret_cast<uint2 *>(codes) + threadIdx.x + i * blockDim.x;
         if (row >= lo && row < hi)
             *dst = kv8_encode8<CODE>(x[i], scale, inv);
         else if (row < past && grown)
@@ -88,7 +82,7 @@ template <int D, int CODE, int MODE> __global__ void __launch_bounds__(1024) flb
 
 template <int D, int CODE> cudaError_t launch_t(const Kv8AppendArgs &a, int input_mode, cudaStream_t stream) {
     const unsigned threads = (unsigned)((D << a.c.block_shift) / (8 * kChunks));
-    const unsigned grid = 2u * (unsigned)a.c.H * (unsigned)a.nwin * (unsigned)a.c.B;
+    const dim3 grid(2u * (unsigned)a.c.H, (unsigned)a.nwin, (unsigned)a.c.B);
     auto kern = input_mode == 0 ? flb_kv8_append_kernel<D, CODE, 0> : input_mode == 1 ? flb_kv8_append_kernel<D, CODE, 1> : flb_kv8_append_kernel<D, CODE, 2>;
     return kv8_launch(kern, grid, threads, 0, stream, a);
 }

@@ -142,9 +142,8 @@ int flb_kv8_validate_append(const flb_kv8_append_params *p) {
     if ((st = check_input(p->input_mode, p->v, p->v_w_scale, p->kv_row_stride, dense)) != FLB_OK) return st;
     if ((st = check_rope(p->freq_cis, p->freq_rows)) != FLB_OK) return st;
     if (!p->past_lens && (p->start_pos < 0 || p->start_pos > p->cache.total_len - p->seq_len)) return FLB_ERR_BAD_SHAPE;
-    const unsigned long long grid = 2ull * p->cache.batch_size * p->cache.kv_head_num *
-                                    window_blocks(p->cache, p->seq_len, p->past_lens != nullptr, p->start_pos);
-    if (grid > 0x7fffffffull) return FLB_ERR_TOO_LARGE;
+    // one CTA per block that a call can touch: the grid's second and third extents hold 65535
+    if (p->cache.batch_size > 65535 || window_blocks(p->cache, p->seq_len, p->past_lens != nullptr, p->start_pos) > 65535) return FLB_ERR_TOO_LARGE;
     return FLB_OK;
 }
 
@@ -173,6 +172,7 @@ int flb_kv8_validate_decode(const flb_kv8_decode_params *p) {
     const HeadSplit hs = heads_for(p->head_num / p->cache.kv_head_num, d);
     const unsigned long long units = (unsigned long long)p->cache.batch_size * p->cache.kv_head_num;
     if (units * hs.nchunk * (mp / split_len_of(p) + 1) > 0x7fffffffull || units * (mp / 1024 + 2) > 0x7fffffffull) return FLB_ERR_TOO_LARGE;
+    if (hs.nchunk > 1 && p->cache.batch_size > 65535) return FLB_ERR_TOO_LARGE; // the append in front has a grid extent of that many
     if (p->scratch_bytes < decode_scratch(p, mp, p->weight_out != nullptr).total) return FLB_ERR_SCRATCH_TOO_SMALL;
     return FLB_OK;
 }
