@@ -6,6 +6,8 @@
 // they read whole rows of the [B,S,Hkv,d] input.
 #include "kv8.cuh"
 
+#include <type_traits>
+
 namespace flb {
 
 namespace {
@@ -34,48 +36,57 @@ template <int D, int CODE, int MODE> __global__ void __launch_bounds__(1024) flb
     float *scale_p = a.c.scale[kv] + unit * a.c.nblk + blk;
     const int pos0 = (a.token_pos ? __ldg(a.token_pos + b) : past) - past; // position = row + pos0
 
-    // All loads first: the rows, then the table's.  What is not a new row of this block is read as the nearest that is, and not used.
-    Kv8Raw raw[kChunks];
-    float4 f0[kChunks], f1[kChunks];
-    const bool turn = kv == 0 && a.freq_cis;
     const int col = (int)(threadIdx.x % CPR) * 8, step = (int)(blockDim.x / CPR), r0 = row0 + (int)(threadIdx.x / CPR); // rows r0, r0 + step, ...
-    const int tab0 = pos0, tab1 = a.freq_rows - 1;
-    if (turn && threadIdx.x == 0 && (lo + tab0 < 0 || hi - 1 + tab0 > tab1) && a.status) atomicOr(a.status, kKv8BadPos);
-    const size_t tok0 = (size_t)b * a.S + (lo - past);
+    // All loads first: the rows, then the table's.  What is not a new row of this block is read as the nearest that is, and not used.  FULL: every
+    // row of the block is new, as in most of a prompt.
+    auto work = [&](auto full) {
+        constexpr bool FULL = decltype(full)::value;
+        auto row_of = [&](int i) { return FULL ? r0 + i * step : min(max(r0 + i * step, lo), hi - 1); };
+        Kv8Raw raw[kChunks];
+        float4 f0[kChunks], f1[kChunks];
+        const bool turn = kv == 0 && a.freq_cis;
+        const int tab0 = pos0, tab1 = a.freq_rows - 1;
+        if (turn && threadIdx.x == 0 && (lo + tab0 < 0 || hi - 1 + tab0 > tab1) && a.status) atomicOr(a.status, kKv8BadPos);
+        const size_t tok0 = (size_t)b * a.S + (lo - past);
 #pragma unroll
-    for (int i = 0; i < kChunks; ++i) {
-        const int row = min(max(r0 + i * step, lo), hi - 1);
-        raw[i] = kv8_raw8<MODE>(a.in[kv], tok0 + (row - lo), h * D + col);
-        if (turn) {
-            const float4 *f = reinterpret_cast<const float4 *>(a.freq_cis + (size_t)min(max(row + tab0, 0), tab1) * D + col);
-            f0[i] = __ldg(f);
-            f1[i] = __ldg(f + 1);
+        for (int i = 0; i < kChunks; ++i) {
+            const int row = row_of(i);
+            raw[i] = kv8_raw8<MODE>(a.in[kv], tok0 + (row - lo), h * D + col);
+            if (turn) {
+                const float4 *f = reinterpret_cast<const float4 *>(a.freq_cis + (size_t)min(max(row + tab0, 0), tab1) * D + col);
+                f0[i] = __ldg(f);
+                f1[i] = __ldg(f + 1);
+            }
         }
-    }
-    const float old = (row0 >= past) ? 0.f : *scale_p;
-    float x[kChunks][8];
-    float big = 0.f;
+        const float old = (FULL || row0 >= past) ? 0.f : *scale_p;
+        float x[kChunks][8];
+        float big = 0.f;
 #pragma unroll
-    for (int i = 0; i < kChunks; ++i) {
-        kv8_values8<MODE>(raw[i], a.in[kv], a.act_scale, tok0 + (min(max(r0 + i * step, lo), hi - 1) - lo), h * D + col, x[i]);
-        if (turn) kv8_rotate8(f0[i], f1[i], x[i]);
-        big = kv8_abs_max8(big, x[i]); // rows read in place of others are rows of this block: the maximum is the same
-    }
-    const uint32_t amax = kv8_block_max(kv8_abs_bits(big), red);
-    __syncthreads(); // every thread has read the old scale
-    const float scale = kv8_new_scale<CODE>(amax, old);
-    const bool grown = old > 0.f && scale > old;
-    const float ratio = grown ? __fdiv_rn(old, scale) : 1.f, inv = __fdiv_rn(1.f, scale);
+        for (int i = 0; i < kChunks; ++i) {
+            kv8_values8<MODE>(raw[i], a.in[kv], a.act_scale, tok0 + (row_of(i) - lo), h * D + col, x[i]);
+            if (turn) kv8_rotate8(f0[i], f1[i], x[i]);
+            big = kv8_abs_max8(big, x[i]); // rows read in place of others are rows of this block: the maximum is the same
+        }
+        const uint32_t amax = kv8_block_max(kv8_abs_bits(big), red);
+        __syncthreads(); // every thread has read the old scale
+        const float scale = kv8_new_scale<CODE>(amax, old);
+        const bool grown = old > 0.f && scale > old;
+        const float ratio = grown ? __fdiv_rn(old, scale) : 1.f, inv = __fdiv_rn(1.f, scale);
 #pragma unroll
-    for (int i = 0; i < kChunks; ++i) {
-        const int row = r0 + i * step;
-        uint2 *dst = reinterpret_cast<uint2 *>(codes) + threadIdx.x + i * blockDim.x;
-        if (row >= lo && row < hi)
-            *dst = kv8_encode8<CODE>(x[i], scale, inv);
-        else if (row < past && grown)
-            *dst = kv8_rescale8<CODE>(*dst, ratio);
-    }
-    if (threadIdx.x == 0) *scale_p = scale;
+        for (int i = 0; i < kChunks; ++i) {
+            const int row = r0 + i * step;
+            uint2 *dst = reinterpret_cast<uint2 *>(codes) + threadIdx.x + i * blockDim.x;
+            if (FULL || (row >= lo && row < hi))
+                *dst = kv8_encode8<CODE>(x[i], scale, inv);
+            else if (!FULL && row < past && grown)
+                *dst = kv8_rescale8<CODE>(*dst, ratio);
+        }
+        if (threadIdx.x == 0) *scale_p = scale;
+    };
+    if (lo == row0 && hi == row1)
+        work(std::true_type());
+    else
+        work(std::false_type());
     if (kv == 0 && a.c.row_pos)
         for (int r = lo + (int)threadIdx.x; r < hi; r += blockDim.x) a.c.row_pos[unit * a.c.T + r] = r + pos0;
 }
