@@ -635,33 +635,55 @@ __global__ void __launch_bounds__(kWarps * 32, D == 128 ? (NT == 1 ? 4 : 3) : 1)
 // weight_out = weight_in + sum over the group of 2^(score - max) / sum.  A thread takes four rows of one K/V head; HBM-bound, 4 (G + 2) bytes a
 // row and head (100001 rows, 8 heads of 4 q heads, from L2: 4 us).
 __global__ void __launch_bounds__(256) flb_kv8_weights_kernel(const __grid_constant__ Kv8DecodeArgs a, int blocks_per_unit) {
-    kv8_begin();
     const size_t unit = blockIdx.x / (unsigned)blocks_per_unit;
     const int r = ((int)(blockIdx.x % (unsigned)blocks_per_unit) * 256 + threadIdx.x) * 4;
     const int b = (int)(unit / a.c.H), h = (int)(unit - (size_t)b * a.c.H);
+    // The kernel in front is the attention kernel, which lets this one start only after everything before it has completed, and writes neither
+    // lengths nor weights: they are read while it runs.
     const int past = a.past_lens ? __ldg(a.past_lens + b) : a.start_pos;
-    if (past < 0 || past >= a.c.T || past >= a.nsplit_max * a.split_len || r > past) return;
+    const bool on = past >= 0 && past < a.c.T && past < a.nsplit_max * a.split_len && r <= past;
     const size_t i = unit * a.c.T + r; // T is a multiple of 16: four rows never leave the slab
     const int begin = a.key_begin && !a.c.row_pos ? __ldg(a.key_begin + b) : INT_MIN; // no score was left below it
-    const float4 in = *reinterpret_cast<const float4 *>(a.weight_in + i);
-    float w[4] = {in.x, in.y, in.z, in.w};
-    const size_t hq0 = (size_t)b * a.Hq + h * a.G;
-    if (r <= past && past < r + 4) w[past - r] = 0.f;
-#pragma unroll 4
-    for (int j = 0; j < a.G; ++j) {
-        const float4 s4 = __ldcs(reinterpret_cast<const float4 *>(a.scores + (hq0 + j) * a.c.T + r));
-        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(a.ml) + hq0 + j);
-        const float s[4] = {s4.x, s4.y, s4.z, s4.w};
-        const float inv = (ml.y > 0.f || ml.y != ml.y) ? 1.0f / ml.y : 0.f;
-        if (inv != 0.f)
+    float w[4] = {0.f, 0.f, 0.f, 0.f};
+    if (on) {
+        const float4 in = *reinterpret_cast<const float4 *>(a.weight_in + i);
+        w[0] = in.x;
+        w[1] = in.y;
+        w[2] = in.z;
+        w[3] = in.w;
+    }
+    kv8_begin();
+    if (!on) return;
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (r + e >= begin) w[e] += ex2(s[e] - ml.x) * inv;
+    for (int e = 0; e < 4; ++e)
+        if (r + e == past) w[e] = 0.f;
+    const size_t hq0 = (size_t)b * a.Hq + h * a.G;
+    const float *scores = a.scores + hq0 * a.c.T + r;
+    const float2 *ml = reinterpret_cast<const float2 *>(a.ml) + hq0;
+    for (int j0 = 0; j0 < a.G; j0 += 4) { // four heads' loads at a time
+        float4 s4[4];
+        float2 m4[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int jj = min(j0 + j, a.G - 1);
+            s4[j] = __ldcs(reinterpret_cast<const float4 *>(scores + (size_t)jj * a.c.T));
+            m4[j] = __ldcg(ml + jj);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float s[4] = {s4[j].x, s4[j].y, s4[j].z, s4[j].w};
+            const bool seen = j0 + j < a.G && (m4[j].y > 0.f || m4[j].y != m4[j].y);
+            const float inv = 1.0f / m4[j].y;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] += seen && r + e >= begin ? ex2(s[e] - m4[j].x) * inv : 0.f;
+        }
     }
     if (r + 3 <= past) {
         *reinterpret_cast<float4 *>(a.weight_out + i) = make_float4(w[0], w[1], w[2], w[3]);
     } else {
-        for (int e = 0; e < 4 && r + e <= past; ++e) a.weight_out[i + e] = w[e];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (r + e <= past) a.weight_out[i + e] = w[e];
     }
 }
 
