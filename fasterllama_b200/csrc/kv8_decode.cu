@@ -86,6 +86,16 @@ __device__ __forceinline__ void copy16(uint32_t dst, const uint8_t *src) {
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
+// A store whose line is to outlive the streamed codes in L2: the weights kernel reads it back.
+__device__ __forceinline__ uint64_t keep_policy() {
+    uint64_t p;
+    asm("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(p));
+    return p;
+}
+__device__ __forceinline__ void store_kept(float *p, float x, uint64_t policy) {
+    asm volatile("st.global.L2::cache_hint.f32 [%0], %1, %2;" ::"l"(p), "f"(x), "l"(policy) : "memory");
+}
+
 // 16 rows from `k` and `v` into a slot
 template <int D> __device__ __forceinline__ void copy_step(uint32_t slot, const uint8_t *k, const uint8_t *v, int lane) {
     constexpr int CPR = D / 16, PER = kStep * CPR / 32;
@@ -342,6 +352,7 @@ __global__ void __launch_bounds__(kWarps * 32, D == 128 ? (NT == 1 ? 4 : 3) : 1)
     // ---- the pass over the rows
     // This lane's reads of a slot: K rows g, g + 8 (the rows of a step's tile are dealt out so that eight lanes meet eight chunks), V rows
     // 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+    const uint64_t keep = a.scores ? keep_policy() : 0ull;
     int slot = 0, step = 0;
     for (; r < row1; r += kStride) {
         copy_wait<R::kStages - 1>();
@@ -419,8 +430,8 @@ __global__ void __launch_bounds__(kWarps * 32, D == 128 ? (NT == 1 ? 4 : 3) : 1)
             }
             if (a.scores && 4 * n + t < nheads) {
                 float *sp = a.scores + ((size_t)b * a.Hq + head0 + 4 * n + t) * a.c.T + r + g;
-                if (r + g < row1) sp[0] = x[n][0];
-                if (r + g + 8 < row1) sp[8] = x[n][1];
+                if (r + g < row1) store_kept(sp, x[n][0], keep);
+                if (r + g + 8 < row1) store_kept(sp + 8, x[n][1], keep);
             }
             const float top = fmaxf(x[n][0], x[n][1]);
             if (__any_sync(0xffffffffu, top > m_run[n] + kRaise)) {
@@ -632,6 +643,8 @@ __global__ void __launch_bounds__(kWarps * 32, D == 128 ? (NT == 1 ? 4 : 3) : 1)
     if (tid == 0) a.counters[unit * a.nchunk + chunk] = 0u; // ready for the next call
 }
 
+constexpr int kHeadsAtOnce = 8;
+
 // weight_out = weight_in + sum over the group of 2^(score - max) / sum.  A thread takes four rows of one K/V head; HBM-bound, 4 (G + 2) bytes a
 // row and head (100001 rows, 8 heads of 4 q heads, from L2: 4 us).
 __global__ void __launch_bounds__(256) flb_kv8_weights_kernel(const __grid_constant__ Kv8DecodeArgs a, int blocks_per_unit) {
@@ -652,32 +665,37 @@ __global__ void __launch_bounds__(256) flb_kv8_weights_kernel(const __grid_const
         w[2] = in.z;
         w[3] = in.w;
     }
+    __shared__ float2 ml_s[kHeadsAtOnce];
     kv8_begin();
-    if (!on) return;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
         if (r + e == past) w[e] = 0.f;
     const size_t hq0 = (size_t)b * a.Hq + h * a.G;
     const float *scores = a.scores + hq0 * a.c.T + r;
     const float2 *ml = reinterpret_cast<const float2 *>(a.ml) + hq0;
-    for (int j0 = 0; j0 < a.G; j0 += 4) { // four heads' loads at a time
-        float4 s4[4];
-        float2 m4[4];
+    for (int j0 = 0; j0 < a.G; j0 += kHeadsAtOnce) {
+        const int nj = min(kHeadsAtOnce, a.G - j0);
+        // Maximum and reciprocal sum, read once per block: read by every thread, the few words they are in held the kernel up for 5 us.
+        float4 s4[kHeadsAtOnce];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int jj = min(j0 + j, a.G - 1);
-            s4[j] = __ldcs(reinterpret_cast<const float4 *>(scores + (size_t)jj * a.c.T));
-            m4[j] = __ldcg(ml + jj);
+        for (int j = 0; j < kHeadsAtOnce; ++j)
+            if (on && j < nj) s4[j] = __ldcs(reinterpret_cast<const float4 *>(scores + (size_t)(j0 + j) * a.c.T));
+        __syncthreads();
+        if ((int)threadIdx.x < nj) {
+            const float2 m = __ldcg(ml + j0 + threadIdx.x);
+            ml_s[threadIdx.x] = make_float2(m.x, (m.y > 0.f || m.y != m.y) ? 1.0f / m.y : 0.f);
         }
+        __syncthreads();
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < kHeadsAtOnce; ++j) {
+            if (!on || j >= nj) continue;
             const float s[4] = {s4[j].x, s4[j].y, s4[j].z, s4[j].w};
-            const bool seen = j0 + j < a.G && (m4[j].y > 0.f || m4[j].y != m4[j].y);
-            const float inv = 1.0f / m4[j].y;
+            const float2 m = ml_s[j];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) w[e] += seen && r + e >= begin ? ex2(s[e] - m4[j].x) * inv : 0.f;
+            for (int e = 0; e < 4; ++e) w[e] += m.y != 0.f && r + e >= begin ? ex2(s[e] - m.x) * m.y : 0.f;
         }
     }
+    if (!on) return;
     if (r + 3 <= past) {
         *reinterpret_cast<float4 *>(a.weight_out + i) = make_float4(w[0], w[1], w[2], w[3]);
     } else {
