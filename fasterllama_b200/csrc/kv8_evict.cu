@@ -106,8 +106,9 @@ template <bool REGS> __global__ void __launch_bounds__(kSelThreads) flb_kv8_sele
             }
         }
     }
-    const int n = a.past_lens ? __ldcg(a.past_lens + b) : a.start_pos;
-    const long long first_recent = a.next_pos ? (long long)__ldcg(a.next_pos + b) - a.recent : INT_MAX + 1ll;
+    // (through L1: every warp of every CTA reads these few words)
+    const int n = a.past_lens ? a.past_lens[b] : a.start_pos;
+    const long long first_recent = a.next_pos ? (long long)a.next_pos[b] - a.recent : INT_MAX + 1ll;
     const int recent_from = (int)min((long long)INT_MAX, max((long long)INT_MIN, first_recent));
     const bool any_recent = first_recent <= INT_MAX;
     auto is_safe = [&](int p) { return p < a.sinks || (any_recent && p >= recent_from); };

@@ -326,11 +326,12 @@ struct __align__(8) PrefillBarriers {
     uint64_t l_full[2], l_empty[2];   // row sums of an item in shared memory / read by the epilogue
     uint64_t sched_full[SCHED_DEPTH], sched_empty[SCHED_DEPTH];
     int sched_bh[SCHED_DEPTH], sched_qb[SCHED_DEPTH]; // the published items; bh < 0 = no more work
+    int sched_geom[SCHED_DEPTH][4]; // with key bounds: first key tile, steps of the two query tiles, of the item
     int v_store_bh[V_STAGES], v_store_j[V_STAGES];    // loader's notes: the V tile in stage s still has to go into the cache (bh < 0: not)
     uint32_t tmem_base;
     int abort_flag;
 };
-constexpr int kBarrierSlot = 512;
+constexpr int kBarrierSlot = 640;
 constexpr size_t prefill_smem(int d) {
     return 2 * (size_t)tile_bytes(d) + (size_t)(K_STAGES + V_STAGES) * kv_tile_bytes(d) + 2 * BM * sizeof(float) + kBarrierSlot;
 }
@@ -390,29 +391,39 @@ __device__ __forceinline__ ItemGeom item_geom(int qb, int S, bool causal) {
     g.j0 = 0;
     return g;
 }
-// The same with per-row key bounds: the tiles from the first key any row of the item sees on.  A query tile that sees none
-// takes one (masked) tile, so that every item has the same steps.
-template <bool SCORED> __device__ __forceinline__ ItemGeom item_geom_of(const PrefillArgs &a, int bh, int qb, bool causal) {
+// The same with per-row key bounds: (first key tile, n[0], n[1], nmax) from the tiles' ranges.  A query tile that sees no key takes one (masked)
+// tile, so that every item has the same steps.  Worked out once per item, by the scheduler, which publishes it: read by every warp of every
+// CTA, and by all heads of a sequence at the same time, the few words of the ranges held the items up (documents 150 us against 141 us).
+__device__ __forceinline__ int4 bounded_geom(const PrefillArgs &a, int bh, int qb) {
+    const int2 *r = a.ranges + (size_t)(bh / a.H) * ((a.S + 2 * BM - 1) / (2 * BM) * 2) + 2 * qb;
+    const int2 r0 = __ldcg(r), r1 = __ldcg(r + 1); // written by the kernel in front
+    // the tiles of the item's own 256 rows are loaded in any case: this item sends their V on into the cache
+    const int j0 = min(min(r0.x, r1.x) / BN, 2 * BM / BN * qb);
+    const int n0 = max(1, (r0.y + BN - 1) / BN - j0), n1 = max(1, (r1.y + BN - 1) / BN - j0);
+    return make_int4(j0, n0, n1, max(max(n0, n1), (min(a.S, (qb + 1) * 2 * BM) + BN - 1) / BN - j0));
+}
+template <bool SCORED> __device__ __forceinline__ ItemGeom item_geom_of(const PrefillArgs &a, int qb, bool causal, const int4 &bounded) {
     ItemGeom g = item_geom(qb, a.S, causal);
     if (SCORED && a.ranges) {
-        const int2 *r = a.ranges + (size_t)(bh / a.H) * ((a.S + 2 * BM - 1) / (2 * BM) * 2) + 2 * qb;
-        const int2 r0 = __ldcg(r), r1 = __ldcg(r + 1); // written by the kernel in front
-        // the tiles of the item's own 256 rows are loaded in any case: this item sends their V on into the cache
-        g.j0 = min(min(r0.x, r1.x) / BN, 2 * BM / BN * qb);
-        g.n[0] = max(1, (r0.y + BN - 1) / BN - g.j0);
-        g.n[1] = max(1, (r1.y + BN - 1) / BN - g.j0);
-        g.nmax = max(max(g.n[0], g.n[1]), (min(a.S, (qb + 1) * 2 * BM) + BN - 1) / BN - g.j0);
+        g.j0 = bounded.x;
+        g.n[0] = bounded.y;
+        g.n[1] = bounded.z;
+        g.nmax = bounded.w;
     }
     return g;
 }
 
 // Next published item for a consumer role (`count` = items this role has taken so far).  Single-thread roles
 // release the slot themselves; warp roles read on every lane and let lane 0 release after a __syncwarp().
-__device__ __forceinline__ bool sched_read(PrefillBarriers *pb, unsigned *status, uint32_t count, int &bh, int &qb) {
+template <bool SCORED> __device__ __forceinline__ bool sched_read(PrefillBarriers *pb, unsigned *status, uint32_t count, int &bh, int &qb, int4 &geom) {
     const uint32_t slot = count % SCHED_DEPTH;
     if (!wait_bar(&pb->sched_full[slot], (count / SCHED_DEPTH) & 1u, pb, status)) return false;
     bh = *reinterpret_cast<volatile int *>(&pb->sched_bh[slot]);
     qb = *reinterpret_cast<volatile int *>(&pb->sched_qb[slot]);
+    if (SCORED) {
+        const volatile int *g = pb->sched_geom[slot];
+        geom = make_int4(g[0], g[1], g[2], g[3]);
+    }
     return true;
 }
 __device__ __forceinline__ void sched_release(PrefillBarriers *pb, uint32_t count) { mbar_arrive(&pb->sched_empty[count % SCHED_DEPTH]); }
@@ -637,6 +648,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             const int hpg = a.heads_per_group;
             const int per_group = hpg * nqb, full_groups = BH / hpg;
             uint32_t published = 0, kt = 0;
+            int4 geom_ahead = make_int4(0, 0, 0, 0); // of the item published last
             bool ok = true;
             // item k of the list -> (b,h) unit and query block: groups of 32 units (their K/V stay in L2 while the
             // group is worked on), late = heavy query blocks first inside a group
@@ -660,6 +672,13 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                 decode(k, bh, qb);
                 pb->sched_bh[slot] = bh;
                 pb->sched_qb[slot] = qb;
+                if (SCORED && a.ranges && bh >= 0) {
+                    geom_ahead = bounded_geom(a, bh, qb);
+                    pb->sched_geom[slot][0] = geom_ahead.x;
+                    pb->sched_geom[slot][1] = geom_ahead.y;
+                    pb->sched_geom[slot][2] = geom_ahead.z;
+                    pb->sched_geom[slot][3] = geom_ahead.w;
+                }
                 mbar_arrive(&pb->sched_full[slot]); // release: the two words above are visible to whoever sees the phase
                 ++published;
                 return true;
@@ -736,10 +755,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             int cur = (int)blockIdx.x; // < num_items: the grid never exceeds the item count
             ok = publish(cur);
             while (cur >= 0 && ok) {
+                const int4 bg = geom_ahead; // of `cur`: the next one is published below
                 const int nxt = fetch(); // in flight while the first tile of `cur` is issued
                 int bh, qb;
                 decode(cur, bh, qb);
-                const ItemGeom g = item_geom_of<SCORED>(a, bh, qb, causal);
+                const ItemGeom g = item_geom_of<SCORED>(a, qb, causal, bg);
                 bool keeper = (qb == nqb - 1); // its query rows see every key tile of the unit
                 int kvu = bh;
                 if (SCORED) {
@@ -792,12 +812,13 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                     // ---- next work item: its query rows go into the tile's buffer as soon as the previous item's
                     // last S has retired.  The two key tiles of lead hide the load's latency from the softmax warps.
                     int bh, qb;
-                    ok = sched_read(pb, a.status, taken, bh, qb);
+                    int4 bg;
+                    ok = sched_read<SCORED>(pb, a.status, taken, bh, qb, bg);
                     if (!ok) break;
                     sched_release(pb, taken++);
                     valid = bh >= 0;
                     if (!valid) break;
-                    const ItemGeom g = item_geom_of<SCORED>(a, bh, qb, causal);
+                    const ItemGeom g = item_geom_of<SCORED>(a, qb, causal, bg);
                     nmax = g.nmax;
                     first_t = t ? g.first_step<SCORED>(1, backwards) : g.first_step<SCORED>(0, backwards);
                     end_t = first_t + (t ? g.n[1] : g.n[0]);
@@ -854,11 +875,12 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             for (;;) {
                 if (j == nmax) {
                     int bh, qb;
-                    ok = sched_read(pb, a.status, taken, bh, qb);
+                    int4 bg;
+                    ok = sched_read<SCORED>(pb, a.status, taken, bh, qb, bg);
                     if (!ok) break;
                     sched_release(pb, taken++);
                     if (bh < 0) break;
-                    const ItemGeom g = item_geom_of<SCORED>(a, bh, qb, causal);
+                    const ItemGeom g = item_geom_of<SCORED>(a, qb, causal, bg);
                     nmax = g.nmax;
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {
@@ -915,14 +937,15 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         bool ok = true;
         for (;;) {
             int bh, qb;
-            ok = sched_read(pb, a.status, taken, bh, qb);
+            int4 bg;
+            ok = sched_read<SCORED>(pb, a.status, taken, bh, qb, bg);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             __syncwarp();
             if (lane == 0) sched_release(pb, taken);
             ++taken;
             if (bh < 0) break;
-            const ItemGeom g = item_geom_of<SCORED>(a, bh, qb, causal);
+            const ItemGeom g = item_geom_of<SCORED>(a, qb, causal, bg);
             const int n_t = t ? g.n[1] : g.n[0], first_t = t ? g.first_step<SCORED>(1, backwards) : g.first_step<SCORED>(0, backwards);
             const int q0 = t ? g.q0[1] : g.q0[0], row = q0 + lrow;
             float m_used = -1e30f;
@@ -1082,14 +1105,15 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         bool ok = true;
         for (;;) {
             int bh, qb;
-            ok = sched_read(pb, a.status, taken, bh, qb);
+            int4 bg;
+            ok = sched_read<SCORED>(pb, a.status, taken, bh, qb, bg);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             __syncwarp();
             if (lane == 0) sched_release(pb, taken);
             ++taken;
             if (bh < 0) break;
-            const ItemGeom g = item_geom_of<SCORED>(a, bh, qb, causal);
+            const ItemGeom g = item_geom_of<SCORED>(a, qb, causal, bg);
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 if (g.n[t] == 0) continue;
