@@ -235,10 +235,14 @@ template <int CODE> __device__ __forceinline__ bool kv8_near_tie(const float (&y
 // Eight values over their block's scale, rounded to codes; `inv` = 1 / scale.  The quotient is defined as one IEEE division; multiplying by
 // the reciprocal is off by 2^-22 at most, which shows only next to a tie, and there the division is done.  A scale of 0, infinity or NaN gives
 // codes 0.
-// (out of line: inlined, its eight divisions are issued under a predicate for every value)
+// A subnormal scale may be rounded down by up to a third, so the quotients are held to the largest code; a normal one is off by 2^-24 and needs no
+// such care.  (out of line: inlined, its eight divisions are issued under a predicate for every value)
+template <int CODE> __device__ __forceinline__ float kv8_quotient(float x, float scale) {
+    return fminf(fmaxf(__fdiv_rn(x, scale), -kv8_top<CODE>()), kv8_top<CODE>());
+}
 template <int CODE> __device__ __noinline__ uint2 kv8_encode8_exact(float4 u, float4 v, float scale) {
-    const float a[4] = {__fdiv_rn(u.x, scale), __fdiv_rn(u.y, scale), __fdiv_rn(u.z, scale), __fdiv_rn(u.w, scale)};
-    const float b[4] = {__fdiv_rn(v.x, scale), __fdiv_rn(v.y, scale), __fdiv_rn(v.z, scale), __fdiv_rn(v.w, scale)};
+    const float a[4] = {kv8_quotient<CODE>(u.x, scale), kv8_quotient<CODE>(u.y, scale), kv8_quotient<CODE>(u.z, scale), kv8_quotient<CODE>(u.w, scale)};
+    const float b[4] = {kv8_quotient<CODE>(v.x, scale), kv8_quotient<CODE>(v.y, scale), kv8_quotient<CODE>(v.z, scale), kv8_quotient<CODE>(v.w, scale)};
     return make_uint2(kv8_pack4<CODE>(a), kv8_pack4<CODE>(b));
 }
 template <int CODE> __device__ __forceinline__ uint2 kv8_encode8(const float (&x)[8], float scale, float inv) {

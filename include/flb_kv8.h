@@ -29,7 +29,7 @@ typedef enum flb_kv8_code {
  *     scale' = need               for a block whose first row is new,
  *     scale' = max(scale, need)   for a block that holds rows already; if it grew, the codes it held become
  *                                 rne(code * (scale / scale')),
- *     new code = rne(x / scale')  (0 where scale' is 0 or not finite),
+ *     new code = rne(x / scale')  (0 where scale' is 0 or not finite; held to -top..top, which matters for subnormal scales),
  * each operation one IEEE fp32 operation, so two calls that store the same rows store the same bits.  A block
  * into which an infinity or NaN was stored has an infinite or NaN scale from then on: its rows read as NaN. */
 typedef struct flb_kv8_cache {

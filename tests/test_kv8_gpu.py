@@ -167,6 +167,23 @@ def test_append_zero_rows_denormals_and_values_that_are_not_finite(cuda_device):
     assert math.isnan(float(c.v_scale[0, 2, 0])) and float(c.v_scale[0, 2, 1]) == pytest.approx(1 / 127, rel=1e-6)
 
 
+@pytest.mark.parametrize("dtype", [I8, E4])
+def test_subnormal_rows_keep_their_signs(cuda_device, dtype):
+    """A scale of a few units of the smallest subnormal number is rounded coarsely: quotients pass the largest code and are held to it."""
+    d, tiny = 64, 2.0 ** -149
+    for top in (1, 63, 64, 127, 128, 190, 191, 500, 671, 672, 5000):
+        x = torch.linspace(-1, 1, d, dtype=torch.float64, device=DEV).mul(top).round().mul(tiny).float().expand(1, 3, 1, d).contiguous()
+        c = kv8.empty_cache(1, 1, 32, d, block_len=16, dtype=dtype, device=DEV)
+        want = ref_append(c, x, x, [0], [3], [0], None)
+        kv8.append(c, x, x)
+        same(c, want)
+        one = kv8.empty_cache(1, 1, 32, d, block_len=16, dtype=dtype, device=DEV)
+        s = torch.zeros(kv8.decode_workspace_bytes(1, 1, 1, 32, d, block_len=16), dtype=torch.uint8, device=DEV)
+        for r in range(3):
+            kv8.decode(one, x[:, :1], x[:, :1], x[:, :1], torch.empty(1, 1, 1, d, device=DEV), start_pos=r, scratch=s)
+        same(one, want)
+
+
 def test_append_bad_lengths_are_flagged_and_touch_nothing(cuda_device):
     g = gen(4)
     c = used_cache(g, 5, 1, 64, 64, 32, I8, row_pos=True)
