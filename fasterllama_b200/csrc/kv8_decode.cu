@@ -25,6 +25,7 @@
 #include "kv8.cuh"
 
 #include <atomic>
+#include <climits>
 
 namespace flb {
 
@@ -313,9 +314,22 @@ __global__ void __launch_bounds__(kWarps * 32, D == 128 ? (NT == 1 ? 4 : 3) : 1)
         copy_next(row1);
         copy_commit();
     }
-    // the largest V scale decides by which power of two the weights are raised before they are cut into fp16 parts
-    const uint32_t vmax = __reduce_max_sync(0xffffffffu, r + lane * kStride < row1 ? kv8_abs_bits(sc_v) : 0u);
-    const int vex = min(max((int)(vmax >> 23) - 127, -100), 100);
+    // The largest V scale decides by which power of two the weights are raised before they are cut into fp16 parts.  Steps that hold no visible row
+    // have no say: a scale there may be anything, an infinity or NaN included.
+    bool seen = r + lane * kStride < row1;
+    if (FORM && a.key_begin && seen) {
+        const int s0 = r + lane * kStride, s1 = min(s0 + kStep, row1);
+        if (a.c.row_pos) {
+            int newest = INT_MIN;
+#pragma unroll 4
+            for (int s = s0; s < s1; ++s) newest = max(newest, __ldcg(a.c.row_pos + unit * a.c.T + s));
+            seen = newest >= begin;
+        } else {
+            seen = s1 > begin;
+        }
+    }
+    const uint32_t vmax = __reduce_max_sync(0xffffffffu, seen ? kv8_abs_bits(sc_v) : 0u);
+    const int vex = min(max((int)(vmax >> 23) - 127, -121), 126); // both powers of two below stay normal numbers
     const float v_up = __uint_as_float((uint32_t)(5 - vex + 127) << 23), v_down = __uint_as_float((uint32_t)(vex - 5 + 127) << 23);
 
     // q as the matrix instructions take it.  Lane (g, t) meets dims 64 c + 16 t .. + 15 of a row; column 2 t + i of a tile is part i (int8: of the second

@@ -329,7 +329,7 @@ def test_decode_default_splits_of_long_slabs(cuda_device):
 
 def test_decode_very_large_and_very_small_values(cuda_device):
     """Powers of two are moved out of q and the scales before fp16 sees them: results are relative to the values."""
-    for up in (2.0 ** -60, 2.0 ** 40):
+    for up in (2.0 ** -60, 2.0 ** 40, 2.0 ** 112):
         g = gen(9)
         B, H, T, d, block, past = 1, 2, 128, 128, 32, [100]
         c = used_cache(g, B, H, T, d, block, I8)
@@ -345,6 +345,31 @@ def test_decode_very_large_and_very_small_values(cuda_device):
             kv8.decode(cache, qq, k, vv, o, past_lens=i32(past), softmax_scale=sc, scratch=s)
             outs.append(o)
         assert torch.equal(outs[0] * up, outs[1])
+
+
+@pytest.mark.parametrize("dtype,d,G", [(I8, 128, 1), (E4, 64, 4), (I8, 256, 2), (E4, 128, 8), (I8, 128, 9)])
+@pytest.mark.parametrize("what", [math.nan, math.inf, 1e37])
+@pytest.mark.parametrize("positions", [False, True])
+def test_decode_rows_before_key_begin_may_hold_anything(cuda_device, dtype, d, G, what, positions):
+    """The block in front of key_begin reads as infinity, NaN or a huge number: results are those of a clean cache."""
+    g = gen(17)
+    T, block, n = 512, 16, 300
+    c = used_cache(g, 1, 2, T, d, block, dtype, row_pos=positions)
+    bad = clone(c)
+    for t in (bad.k_scale, bad.v_scale):
+        t[:, :, 0] = what
+        t[:, :, 2] = what
+    q, _ = tokens(g, "float16", 1, 1, 2 * G, d)
+    k, _ = tokens(g, "float16", 1, 1, 2, d)
+    w = torch.zeros(1, 2, T, device=DEV)
+    outs = []
+    for cache in (c, bad):
+        o, wo = torch.empty(1, 2 * G, 1, d, device=DEV), torch.zeros_like(w)
+        s = torch.zeros(kv8.decode_workspace_bytes(1, 2 * G, 2, T, d, block_len=block, weights=True, split_len=128), dtype=torch.uint8, device=DEV)
+        kv8.decode(cache, q, k, k, o, past_lens=i32([n]), key_begin=i32([51]), weight_in=w, weight_out=wo, scratch=s, split_len=128)
+        outs.append((o, wo))
+    assert bool(outs[0][0].isfinite().all())
+    assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])
 
 
 def test_decode_is_deterministic_and_independent_of_the_batch(cuda_device):
