@@ -82,6 +82,7 @@ struct Kv8DecodeArgs {
     void *out;
     int out_f16;
     int append; // the attention kernel stores the new token itself (one CTA per K/V head and split)
+    int max_past; // sequences with more cached rows are left alone
     int nsplit_max, split_len;
     unsigned *status, *counters;
     float *part_o, *part_ml;

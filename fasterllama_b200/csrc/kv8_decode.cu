@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(kWarps * 32, D == 128 ? (NT == 1 ? 4 : 3) : 1)
         for (int e = 0; e < 8; ++e) qx[i][e] = 0.f;
         if (warp + i * kWarps < nheads && lane < D / 8) load8(a, 0, (size_t)b, (head0 + warp + i * kWarps) * D + lane * 8, qx[i]);
     }
-    if (past < 0 || past >= a.c.T || past >= a.nsplit_max * a.split_len) { // flagged, nothing stored, zeros returned
+    if (past < 0 || past > a.max_past) { // flagged, nothing stored, zeros returned
         if (split == 0) {
             if (tid == 0) atomicOr(a.status, kKv8BadLen);
             for (int i = tid; i < nheads * D; i += NTHREADS) {
@@ -668,7 +668,7 @@ __global__ void __launch_bounds__(256) flb_kv8_weights_kernel(const __grid_const
     // The kernel in front is the attention kernel, which lets this one start only after everything before it has completed, and writes neither
     // lengths nor weights: they are read while it runs.
     const int past = a.past_lens ? __ldg(a.past_lens + b) : a.start_pos;
-    const bool on = past >= 0 && past < a.c.T && past < a.nsplit_max * a.split_len && r <= past;
+    const bool on = past >= 0 && past <= a.max_past && r <= past;
     const size_t i = unit * a.c.T + r; // T is a multiple of 16: four rows never leave the slab
     const int begin = a.key_begin && !a.c.row_pos ? __ldg(a.key_begin + b) : INT_MIN; // no score was left below it
     float w[4] = {0.f, 0.f, 0.f, 0.f};

@@ -279,6 +279,7 @@ int flb_kv8_decode(const flb_kv8_decode_params *p, void *cuda_stream) {
     a.out_f16 = p->out_dtype == FLB_F16;
     a.append = hs.nchunk == 1;
     a.split_len = split_len_of(p);
+    a.max_past = mp; // below the slab's capacity
     a.nsplit_max = mp / a.split_len + 1;
     a.status = reinterpret_cast<unsigned *>(sc);
     a.counters = reinterpret_cast<unsigned *>(sc) + 4;
@@ -289,7 +290,7 @@ int flb_kv8_decode(const flb_kv8_decode_params *p, void *cuda_stream) {
         t.c = a.c;
         t.S = 1;
         t.nwin = 1;
-        t.max_past = a.nsplit_max * a.split_len - 1; // what the attention kernel will not look at is not stored either
+        t.max_past = mp; // what the attention kernel will not look at is not stored either
         t.start_pos = a.start_pos;
         t.past_lens = a.past_lens;
         t.new_lens = nullptr;

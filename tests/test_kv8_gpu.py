@@ -397,6 +397,25 @@ def test_decode_bad_length_is_flagged_and_gives_zeros(cuda_device):
     same(c, before)
 
 
+@pytest.mark.parametrize("Hq", [2, 20])
+def test_decode_length_one_above_the_promised_bound(cuda_device, Hq):
+    """Flagged too where the bound is no whole number of splits."""
+    g = gen(18)
+    c = used_cache(g, 2, 2, 512, 64, 16, I8)
+    before = clone(c)
+    q, _ = tokens(g, "float16", 2, 1, Hq, 64)
+    k, _ = tokens(g, "float16", 2, 1, 2, 64)
+    o = torch.full((2, Hq, 1, 64), math.nan, device=DEV)
+    w, wo = torch.ones(2, 2, 512, device=DEV), torch.full((2, 2, 512), 7.0, device=DEV)
+    s = torch.zeros(kv8.decode_workspace_bytes(2, Hq, 2, 512, 64, block_len=16, weights=True), dtype=torch.uint8, device=DEV)
+    kv8.decode(c, q, k, k, o, past_lens=i32([121, 120]), max_past_len=120, weight_in=w, weight_out=wo, scratch=s)
+    torch.cuda.synchronize()
+    assert A.scratch_status(s) == kv8.STATUS_BAD_LEN
+    assert float(o[0].abs().max()) == 0 and bool(o[1].isfinite().all())
+    assert torch.equal(c.k[0], before.k[0]) and not torch.equal(c.k[1], before.k[1])
+    assert bool((wo[0] == 7).all()) and bool((wo[1, :, 121:] == 7).all()) and not bool((wo[1, :, :121] == 7).any())
+
+
 @pytest.mark.parametrize("Hq", [2, 20])  # the attention kernel stores the token itself, or a launch in front does
 def test_decode_length_above_the_promised_bound(cuda_device, Hq):
     g = gen(15)
