@@ -208,7 +208,7 @@ __device__ __forceinline__ void rope8(const float4 &f0, const float4 &f1, float 
 // Keys that query row s of sequence b sees: [lo, hi).
 __device__ __forceinline__ void visible_keys(const PrefillArgs &a, int b, int s, int &lo, int &hi) {
     lo = a.key_begin ? max(0, __ldg(a.key_begin + (size_t)b * a.S + s)) : 0;
-    hi = a.key_end ? min(a.S, __ldg(a.key_end + (size_t)b * a.S + s)) : a.S;
+    hi = a.key_end ? max(0, min(a.S, __ldg(a.key_end + (size_t)b * a.S + s))) : a.S;
     if (a.mask_mode == 2) hi = min(hi, s + 1);
     if (a.mask_mode == 3) hi = min(hi, s);
 }

@@ -54,6 +54,13 @@ def bounds(kind, B, S, g):
         b[:, ::3] = 2147483647
         a[:, 1::5] = -2147483648
         return a, b, A.FLB_MASK_NONE
+    if kind == "ends":
+        low, high = (torch.full((B, S), x, dtype=torch.int32, device=DEV) for x in (-2147483648, 2147483647))
+        a, b = low.clone(), high.clone()
+        b[:, 1::4] = -2147483648
+        a[:, 2::4] = 2147483647
+        b[:, 3::4] = -1
+        return a, b, A.FLB_MASK_NONE
     raise AssertionError(kind)
 
 
@@ -118,6 +125,12 @@ def run_prefill(seed, *, B, H, Hkv, S, d, kind="causal", cap=0.0, alibi=False, c
 @pytest.mark.parametrize("kind", ["documents", "prefix", "padded", "holes", "window"])
 def test_prefill_bounds(cuda_device, S, kind):
     run_prefill(S, B=2, H=2, Hkv=2, S=S, d=128 if S % 2 else 64, kind=kind)
+
+
+@pytest.mark.parametrize("S", [130, 300])
+def test_prefill_bounds_at_the_ends_of_their_type(cuda_device, S):
+    """Rows whose bounds are the type's lowest and highest values, among rows that see every key."""
+    run_prefill(28, B=2, H=2, Hkv=2, S=S, d=64, kind="ends")
 
 
 @pytest.mark.parametrize("kind", ["causal", "strict", "none", "documents", "prefix", "holes"])
