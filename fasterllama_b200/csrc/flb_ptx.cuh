@@ -102,6 +102,8 @@ __device__ __forceinline__ float cap_score(float x, float cap, float inv_cap) {
     const float r = cap - __fdividef(2.0f * cap, 1.0f + e);
     return u != u ? u : copysignf(r, u);
 }
+// A cap that the calls take: 0 = none, else within bounds that keep its reciprocal and its multiples normal numbers.
+inline bool cap_ok(float cap) { return cap == 0.f || (cap >= 0x1p-10f && cap <= 0x1p40f); }
 // max of three (one instruction on sm_100)
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;

@@ -16,6 +16,7 @@ int check_sizes(const flb_kv8_cache &c) {
     if (c.total_len % c.block_len) return FLB_ERR_BAD_SHAPE;
     if ((size_t)c.batch_size * c.kv_head_num > (size_t)1 << 24) return FLB_ERR_TOO_LARGE;
     if (c.total_len > 1 << 30) return FLB_ERR_TOO_LARGE; // row arithmetic in int
+    if ((size_t)c.kv_head_num * c.size_per_head > 0x7fffffffu) return FLB_ERR_TOO_LARGE; // so are row strides
     return FLB_OK;
 }
 int check_cache(const flb_kv8_cache &c) {
@@ -116,7 +117,7 @@ int check_decode_sizes(const flb_kv8_decode_params *p) {
     if (st != FLB_OK) return st;
     if (p->head_num <= 0 || p->head_num % p->cache.kv_head_num) return FLB_ERR_BAD_SHAPE;
     if (p->split_len < 0 || p->split_len % 128 || p->split_len > 2048) return FLB_ERR_BAD_SHAPE;
-    if ((size_t)p->cache.batch_size * p->head_num > (size_t)1 << 24) return FLB_ERR_TOO_LARGE;
+    if ((size_t)p->cache.batch_size * p->head_num > (size_t)1 << 24 || (size_t)p->head_num * p->cache.size_per_head > 0x7fffffffu) return FLB_ERR_TOO_LARGE;
     return FLB_OK;
 }
 
@@ -160,7 +161,7 @@ int flb_kv8_validate_decode(const flb_kv8_decode_params *p) {
     if ((st = check_input(p->input_mode, p->k, p->k_w_scale, p->kv_row_stride, p->cache.kv_head_num * d)) != FLB_OK) return st;
     if ((st = check_input(p->input_mode, p->v, p->v_w_scale, p->kv_row_stride, p->cache.kv_head_num * d)) != FLB_OK) return st;
     if ((st = check_rope(p->freq_cis, p->freq_rows)) != FLB_OK) return st;
-    if (!(p->softcap >= 0.f) || p->softcap > 3.402823466e38f) return FLB_ERR_BAD_SHAPE;
+    if (!flb::cap_ok(p->softcap)) return FLB_ERR_BAD_SHAPE;
     if (!p->out) return FLB_ERR_NULL_POINTER;
     if (!aligned16(p->out)) return FLB_ERR_MISALIGNED;
     if ((p->weight_in != nullptr) != (p->weight_out != nullptr)) return FLB_ERR_NULL_POINTER;

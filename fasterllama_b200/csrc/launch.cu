@@ -3,6 +3,7 @@
 // (except the two set-up/diagnostic calls that say so), no exit(), no exceptions.
 #include "../../include/flb_attn.h"
 #include "decode_attn.cuh"
+#include "flb_ptx.cuh"
 #include "prefill_attn.cuh"
 
 #include <cuda_runtime.h>
@@ -273,9 +274,10 @@ int flb_attn_validate_scored(const flb_attn_params *p, const flb_score_form *f) 
         if (f->kv_row_stride < kv_heads(p, f) * p->size_per_head) return FLB_ERR_BAD_SHAPE;
         if (((size_t)f->kv_row_stride * (p->input_mode == FLB_IN_F16 ? 2 : 4)) % 16u) return FLB_ERR_MISALIGNED;
     }
-    if (!(f->softcap >= 0.f) || f->softcap > 3.402823466e38f) return FLB_ERR_BAD_SHAPE;
+    if (!flb::cap_ok(f->softcap)) return FLB_ERR_BAD_SHAPE;
     if (p->seq_len == 1) return f->key_end ? FLB_ERR_UNSUPPORTED : FLB_OK; // a decode call sees what is cached
     if (!(p->softmax_scale > 0.f) || p->softmax_scale > 3.402823466e38f) return FLB_ERR_BAD_SHAPE; // maxima are taken before the scale
+    if (f->softcap > 0.f && p->softmax_scale > 65536.f * f->softcap) return FLB_ERR_BAD_SHAPE; // its fifth power is a coefficient
     if (p->scratch_bytes < flb::prefill_scored_scratch_bytes(p->batch_size, p->head_num, p->seq_len, p->size_per_head, f))
         return FLB_ERR_SCRATCH_TOO_SMALL;
     return FLB_OK;

@@ -181,10 +181,13 @@ def _rope(freq_cis, d, dev):
     if freq_cis is None:
         return 0, 0
     n = freq_cis.shape[0]
+    if not n:
+        raise ValueError("freq_cis must have a row for every position")
     return _dense(freq_cis, "freq_cis", (n, d), torch.float32, dev), n
 
 
 def _scratch(scratch, dev):
+    """Address and bytes."""
     if scratch is None:
         return 0, 0
     if scratch.get_device() != dev or not scratch.is_contiguous():
@@ -220,9 +223,12 @@ def _append_block(cache: Cache, k, v, *, start_pos: int = 0, past_lens=None, new
     if mode == FLB_IN_INT32:
         act, kw, vw = _scales(act_scale, B * S, (("k_w_scale", k_w_scale, H * d), ("v_w_scale", v_w_scale, H * d)), dev)
     i32 = torch.int32
+    word, size = _scratch(scratch, dev)
+    if scratch is not None and size < 4:
+        raise ValueError("scratch must hold the status word")
     return _PACK_APPEND.pack(*c, S, start_pos, _opt(past_lens, "past_lens", lens, i32, dev), _opt(new_lens, "new_lens", lens, i32, dev),
                              _opt(token_pos, "token_pos", lens, i32, dev), mode, kp, vp, row, act, kw, vw, *_rope(freq_cis, d, dev),
-                             _scratch(scratch, dev)[0]), dev
+                             word), dev
 
 
 def append_params(cache: Cache, k, v, **kw) -> FlbKv8Append:

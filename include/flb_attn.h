@@ -245,7 +245,7 @@ typedef struct flb_score_form {
     int kv_head_num;           /* Hkv: k, v are [B,S,Hkv,d] and the caches [B,Hkv,T,d]; q head h reads K/V head
                                   h / (head_num / Hkv).  0 = head_num                              */
     int kv_row_stride;         /* elements between two tokens' rows of k and v; 0 = qkv_row_stride if that is set, else Hkv * d */
-    float softcap;             /* 0 = none                                                         */
+    float softcap;             /* 0 = none, else 2^-10 .. 2^40 (prefill: and softmax_scale / 2^16 or more) */
     const float *alibi_slopes; /* device [head_num] or NULL                                        */
     const int *key_begin;      /* device int, decode [B], prefill [B,S]; NULL = 0                  */
     const int *key_end;        /* device int, prefill [B,S]; NULL = S.  A decode call takes none   */

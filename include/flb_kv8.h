@@ -93,7 +93,7 @@ typedef struct flb_kv8_decode_params {
     const float *freq_cis;
     int freq_rows;
     float softmax_scale;
-    float softcap;             /* 0 = none                                              */
+    float softcap;             /* 0 = none, else 2^-10 .. 2^40                          */
     const float *alibi_slopes; /* [H] or NULL                                           */
     const int *key_begin;      /* device int[B] or NULL                                 */
     /* Accumulated attention, for flb_kv8_evict(): weight_out[b][h][r] = weight_in[b][h][r] + the sum of the weights that
@@ -138,7 +138,9 @@ typedef struct flb_kv8_evict_params {
                                        was left alone, and its output rows are zero */
 #define FLB_KV8_STATUS_BAD_POS 32u  /* a position outside the RoPE table: the nearest row was used */
 
-/* Host-side argument checks only (no CUDA call); the launch entry points run them first. */
+/* Host-side argument checks only (no CUDA call); the launch entry points run them first.  Beside what the fields say, a call is refused with
+ * FLB_ERR_TOO_LARGE where batch_size * head_num passes 2^24, a row of heads 2^31 elements, or a grid its limits (an append, or a decode of more than 8
+ * (d = 256: 4) q heads per K/V head: more than 65535 sequences, or blocks that one call can touch). */
 int flb_kv8_validate_append(const flb_kv8_append_params *p);
 int flb_kv8_validate_decode(const flb_kv8_decode_params *p);
 int flb_kv8_validate_evict(const flb_kv8_evict_params *p);

@@ -127,6 +127,33 @@ def test_evict_refusals(field, value, status):
     _refused(p, field, value, status)
 
 
+@pytest.mark.parametrize("cap", [1e-30, 2.0 ** -11, 2.0 ** 41, 3.4e38, -0.5])
+def test_caps_that_arithmetic_cannot_hold_are_refused(cap):
+    p, keep = _decode()
+    _refused(p, "softcap", cap, _lib.FLB_ERR_BAD_SHAPE)
+    for good in (0.0, 2.0 ** -10, 30.0, 2.0 ** 40):
+        p.softcap = good
+        assert kv8.validate(p) == _lib.FLB_OK
+
+
+def test_rows_of_more_than_2_31_elements_are_refused():
+    p, keep = _append()
+    p.cache.batch_size, p.cache.kv_head_num = 1, 1 << 24  # times 128
+    assert kv8.validate(p) == _lib.FLB_ERR_TOO_LARGE
+    p, keep = _decode()
+    p.cache.batch_size, p.head_num = 1, 1 << 24
+    assert kv8.validate(p) == _lib.FLB_ERR_TOO_LARGE
+
+
+def test_binding_refuses_a_table_without_rows_and_a_scratch_without_a_word():
+    c = _cache()
+    k = torch.zeros(2, 1, 4, 128, dtype=torch.float16)
+    with pytest.raises(ValueError, match="freq_cis"):
+        kv8.append_params(c, k, k.clone(), freq_cis=torch.zeros(0, 128))
+    with pytest.raises(ValueError, match="scratch"):
+        kv8.append_params(c, k, k.clone(), scratch=torch.zeros(3, dtype=torch.uint8))
+
+
 def test_null_blocks_and_launches_without_a_launch():
     lib = kv8.load_library()
     for name in ("append", "decode", "evict"):

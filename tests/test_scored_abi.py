@@ -38,6 +38,19 @@ def test_refusals(S, field, value, status):
     assert lib.flb_attn_forward_scored(C.byref(p), C.byref(f), None) == status  # refused before any CUDA call
 
 
+@pytest.mark.parametrize("S", [1, 5])
+@pytest.mark.parametrize("cap", [1e-30, 2.0 ** -11, 2.0 ** 41, 3.4e38])
+def test_caps_that_arithmetic_cannot_hold_are_refused(S, cap):
+    p, f, keep = _call(S=S)
+    f.softcap = cap
+    assert A.validate_scored(p, f) == _lib.FLB_ERR_BAD_SHAPE
+    for good in (2.0 ** -10, 30.0, 2.0 ** 40):
+        f.softcap = good
+        assert A.validate_scored(p, f) == _lib.FLB_OK
+    f.softcap, p.softmax_scale = 2.0 ** -10, 65.0
+    assert A.validate_scored(p, f) == (_lib.FLB_OK if S == 1 else _lib.FLB_ERR_BAD_SHAPE)
+
+
 def test_the_wrong_entry_point_and_null_blocks_are_refused():
     lib = _lib.load_library()
     p, f, keep = _call(S=5)

@@ -140,6 +140,26 @@ def test_prefill_forms(cuda_device, kind, H, Hkv, d, cap, alibi, std):
     run_prefill(H + d, B=2, H=H, Hkv=Hkv, S=201, d=d, kind=kind, cap=cap, alibi=alibi, std=std)
 
 
+@pytest.mark.parametrize("cap", [2.0 ** -10, 2.0 ** 40])
+def test_prefill_caps_at_the_ends_of_their_range(cuda_device, cap):
+    """The smallest leaves nearly even weights, the largest leaves the scores (its fit is off by 2.1e-5 of a score there, scores are below 8)."""
+    S, d = 200, 64
+    g = gen(29)
+    q, k, v = rnd(g, 1, S, 2, d), rnd(g, 1, S, 2, d), rnd(g, 1, S, 2, d)
+    outs = []
+    for c in (cap, 0.0):
+        kc, vc = (torch.zeros(1, 2, S, d, dtype=torch.float16, device=DEV) for _ in range(2))
+        o = torch.empty(1, 2, S, d, device=DEV)
+        scratch = torch.zeros(A.workspace_bytes(1, 2, S, S, size_per_head=d) + 65536, dtype=torch.uint8, device=DEV)
+        p, f = A.make_scored_params(q=q, k=k, v=v, k_cache=kc, v_cache=vc, out=o, scratch=scratch, softcap=c, mask_mode=A.FLB_MASK_NONE,
+                                    softmax_scale=0.125 if c else 0.125 if cap > 1 else 1e-30)
+        A.forward_scored(p, f)
+        outs.append(o)
+    # weights: both sides in fp16 (2^-11 each), log-domain difference 2 * cap or 2 * 8 * 2.1e-5
+    tol = float(v.float().abs().max()) * (2 * 2.0 ** -11 + (2 * cap if cap < 1 else 4e-4))
+    assert float((outs[0] - outs[1]).abs().max()) <= tol
+
+
 @pytest.mark.parametrize("cache", ["float16", "float32"])
 @pytest.mark.parametrize("out", ["float16", "float32"])
 @pytest.mark.parametrize("io", ["float16", "float32"])
