@@ -667,6 +667,84 @@ def test_prompt_decode_evict_decode(cuda_device):
             assert set(range(int(pos[0]) - 16, int(pos[0]))) <= set(c.row_pos[0, 0, :90].tolist())
 
 
+def _server(seed, B=2, Hq=8, Hkv=2, T=512, d=128, block=32, long=False):
+    """State of a sequence of calls, and the calls: a chunk appended, three tokens, an eviction, a token; lengths and positions stay on the device."""
+    g = gen(seed)
+    T = 16384 if long else T
+    c = kv8.empty_cache(B, Hkv, T, d, block_len=block, row_pos=True, device=DEV)
+    big = T - 200
+    first = big - 40
+    ins = [tokens(g, "float16", B, S, h, d)[0] for S, h in ((first, Hkv), (first, Hkv), (40, Hkv), (40, Hkv))]
+    steps = [[tokens(g, "float16", B, 1, h, d)[0] for h in (Hq, Hkv, Hkv)] for _ in range(4)]
+    st = dict(c=c, w=torch.zeros(B, Hkv, T, device=DEV), past=i32([0] * B), pos=i32([0] * B), outs=[torch.empty(B, Hq, 1, d, device=DEV) for _ in steps],
+              tab=table(T, d), ds=torch.zeros(kv8.decode_workspace_bytes(B, Hq, Hkv, T, d, block_len=block, weights=True), dtype=torch.uint8, device=DEV),
+              es=torch.zeros(kv8.evict_workspace_bytes(B, Hkv, T, d, block_len=block), dtype=torch.uint8, device=DEV))
+
+    def reset():
+        for t in (*c.tensors().values(), st["w"]):
+            t.zero_() if t.dtype != E4 else t.view(I8).zero_()
+        st["past"].zero_()
+        st["pos"].zero_()
+
+    def run():
+        past, pos, w = st["past"], st["pos"], st["w"]
+        for k, v in (ins[:2], ins[2:]):
+            kv8.append(c, k, v, past_lens=past, token_pos=pos, freq_cis=st["tab"])
+            past.add_(k.shape[1])
+            pos.add_(k.shape[1])
+        for i, (q, k, v) in enumerate(steps):
+            kv8.decode(c, q, k, v, st["outs"][i], past_lens=past, token_pos=pos, freq_cis=st["tab"], softcap=20.0, weight_in=w, weight_out=w,
+                       scratch=st["ds"], scratch_zeroed=i % 2 == 0)  # both with and without a memset in front
+            past.add_(1)
+            pos.add_(1)
+            if i == 2:
+                kv8.evict(c, past_lens=past, len_out=past, budget=big // 2, recent=16, sinks=4, next_pos=pos, weight=w, scratch=st["es"])
+
+    def result():
+        return [t.clone() for t in (*st["outs"], st["w"], st["past"], st["pos"])], clone(c)
+
+    return reset, run, result
+
+
+@pytest.mark.parametrize("long", [False, True])  # an eviction by one CTA per head, and by clusters
+def test_captured_calls_replay_as_they_run(cuda_device, long):
+    reset, run, result = _server(42, long=long)
+    reset()
+    run()
+    want, cache = result()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for _ in range(3):
+        reset()
+        graph.replay()
+        got, now = result()
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+        same(now, cache)
+
+
+def test_two_streams_at_once(cuda_device):
+    """Two servers with caches and scratch of their own, their calls interleaved on two streams."""
+    servers = [_server(43), _server(44, long=True)]
+    want = []
+    for reset, run, result in servers:
+        reset()
+        run()
+        want.append(result())
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in servers]
+    for _ in range(5):
+        for (reset, run, _r), s in zip(servers, streams):
+            with torch.cuda.stream(s):
+                reset()
+                run()
+    torch.cuda.synchronize()
+    for (_a, _b, result), (outs, cache) in zip(servers, want):
+        got, now = result()
+        assert all(torch.equal(a, b) for a, b in zip(outs, got))
+        same(now, cache)
+
+
 def test_empty_cache_and_dequantize(cuda_device):
     c = kv8.empty_cache(1, 2, 100, 64, block_len=64, device=DEV)
     assert tuple(c.k.shape) == (1, 2, 128, 64) and c.block_len == 64 and c.row_pos is None
