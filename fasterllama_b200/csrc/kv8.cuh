@@ -99,7 +99,7 @@ struct Kv8EvictArgs {
     float *weight_out;
     int *pos_out;
     unsigned *status;
-    int *moves;    // [B*H][T / 2] sources: the i-th kept row at or behind m
+    int *moves;    // [B*H][T / 2] sources, rising: the kept rows at or behind m, the last of them at the end of its room
     int *holes;    // [B*H][T / 2] holes below m, rising
     int *seq_len;      // [B][2] m, and what becomes of len_out
     float *edge_scale; // [B*H][2] scales of the block that row m lies in, as they were

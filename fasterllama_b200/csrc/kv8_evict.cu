@@ -24,10 +24,13 @@ namespace {
 
 constexpr int kSelThreads = 1024;
 constexpr int kRanks = 8;    // CTAs of a cluster, where there is more than one
-constexpr int kRegRows = 16; // rows whose keys a thread keeps in registers
 // Digits of 12, 10 and 10 bits: sign, exponent and the first mantissa bits first, which leaves a percent of the rows for the other passes and spreads
 // the additions of the first one over more words than a byte would.
 constexpr int kBins = 4096, kBins2 = 1024;
+constexpr int kCandidates = 256; // rows of one leading digit that one CTA compares with each other rather than sorting them by the other digits
+
+// rows of a slab that a thread looks after, in fours
+__host__ __device__ inline int rows_per_thread(int T, int ranks) { return (((T + ranks - 1) / ranks + kSelThreads - 1) / kSelThreads + 3) & ~3; }
 
 // weights as integers of the same order; NaN above everything
 __device__ __forceinline__ uint32_t ordered(float w) {
@@ -68,17 +71,19 @@ __device__ __forceinline__ void all_sync(cg::cluster_group &cluster, int ranks) 
         cluster.sync();
 }
 
-// A cluster of CTAs (one, for short slabs) per K/V head; every thread has `per` neighbouring rows.  REGS: their keys stay in registers over
-// the passes; else (beyond 16 rows a thread) they are read again.
-template <bool REGS> __global__ void __launch_bounds__(kSelThreads) flb_kv8_select_kernel(const __grid_constant__ Kv8EvictArgs a) {
-    __shared__ __align__(16) int hist[kBins];                  // leading digit, then the two others
-    __shared__ int hist2[2][kBins2];
+// A cluster of CTAs (one, for short slabs) per K/V head; every thread has `per` neighbouring rows.  ROWS: so many of them at most, whose keys stay in
+// registers over the passes; 0: any number, read again.  What bounds it is the chain of dependent steps and, with 32 warps on an SM, every instruction
+// per row (16 rows where 8 do: 17.5 us instead of 14 at 4352 rows).
+template <int ROWS> __global__ void __launch_bounds__(kSelThreads) flb_kv8_select_kernel(const __grid_constant__ Kv8EvictArgs a) {
+    constexpr bool REGS = ROWS > 0;
+    constexpr int K = REGS ? ROWS : 4, V = K / 4;
+    __shared__ __align__(16) int hist[kBins];                  // leading digit
+    __shared__ __align__(16) int hist2[2][kBins2];             // the two others; or the candidates, all of the cluster's and this CTA's
     __shared__ long long ws[32];
     __shared__ int wi[32];
-    __shared__ int n_safe;
-    __shared__ int n_equal;
-    __shared__ int found[3];                     // digit, rows above it, rows in it
-    __shared__ long long n_lists; // holes, and kept rows behind m in the upper half
+    __shared__ int n_safe, n_cand, slice_total, kept_below; // kept_below: kept rows in front of row m
+    __shared__ uint32_t found[3];                 // digit or key, rows above it, rows of it
+    __shared__ long long n_kept;                  // of this CTA: rows that stay for certain; rows of the smallest kept weight in the upper half
     kv8_begin();
     cg::cluster_group cluster = cg::this_cluster();
     const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
@@ -91,18 +96,18 @@ template <bool REGS> __global__ void __launch_bounds__(kSelThreads) flb_kv8_sele
     float *w_out = a.weight_out + unit * a.c.T;
     int *p_out = a.pos_out + unit * a.c.T;
     // This thread's rows are r0 .. r0 + per - 1 of the slab; its weights and positions are on their way before the length is known.
-    const int per = (((a.c.T + ranks - 1) / ranks + kSelThreads - 1) / kSelThreads + 3) & ~3;
+    const int per = rows_per_thread(a.c.T, ranks);
     const int r0 = min(a.c.T, (rank * kSelThreads + tid) * per);
-    float4 wv[REGS ? kRegRows / 4 : 1];
-    int4 pv[REGS ? kRegRows / 4 : 1];
+    float4 wv[V];
+    int4 pv[V];
     if (REGS) {
 #pragma unroll
-        for (int v = 0; v < kRegRows / 4; ++v) {
-            wv[v % (REGS ? kRegRows / 4 : 1)] = make_float4(0.f, 0.f, 0.f, 0.f);
-            pv[v % (REGS ? kRegRows / 4 : 1)] = make_int4(0, 0, 0, 0);
+        for (int v = 0; v < V; ++v) {
+            wv[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+            pv[v] = make_int4(0, 0, 0, 0);
             if (4 * v < per && r0 + 4 * v < a.c.T) { // rows come in fours: the slab's length is a multiple of 16
-                wv[v % (REGS ? kRegRows / 4 : 1)] = *reinterpret_cast<const float4 *>(w + r0 + 4 * v);
-                pv[v % (REGS ? kRegRows / 4 : 1)] = *reinterpret_cast<const int4 *>(pos + r0 + 4 * v);
+                wv[v] = *reinterpret_cast<const float4 *>(w + r0 + 4 * v);
+                pv[v] = *reinterpret_cast<const int4 *>(pos + r0 + 4 * v);
             }
         }
     }
@@ -118,20 +123,22 @@ template <bool REGS> __global__ void __launch_bounds__(kSelThreads) flb_kv8_sele
         a.seq_len[2 * b] = m; // the same from every head
         a.seq_len[2 * b + 1] = bad ? n : m;
     }
+    for (int i = tid; i < kBins / 4; i += kSelThreads) reinterpret_cast<int4 *>(hist)[i] = make_int4(0, 0, 0, 0);
+    for (int i = tid; i < kBins2 / 2; i += kSelThreads) reinterpret_cast<int4 *>(hist2)[i] = make_int4(0, 0, 0, 0);
+    if (tid == 0) n_safe = n_cand = 0;
     // Rows below m into the results, where those are other buffers; the holes are written over at the end.
     if (w_out != w || p_out != pos) {
         if (REGS) {
 #pragma unroll
-            for (int v = 0; v < kRegRows / 4; ++v) {
-                constexpr int V = REGS ? kRegRows / 4 : 1;
+            for (int v = 0; v < V; ++v) {
                 const int r = r0 + 4 * v;
                 if (4 * v >= per || r >= m) continue;
                 if (r + 4 <= m) {
-                    *reinterpret_cast<float4 *>(w_out + r) = wv[v % V];
-                    *reinterpret_cast<int4 *>(p_out + r) = pv[v % V];
+                    *reinterpret_cast<float4 *>(w_out + r) = wv[v];
+                    *reinterpret_cast<int4 *>(p_out + r) = pv[v];
                 } else {
-                    const float x[4] = {wv[v % V].x, wv[v % V].y, wv[v % V].z, wv[v % V].w};
-                    const int y[4] = {pv[v % V].x, pv[v % V].y, pv[v % V].z, pv[v % V].w};
+                    const float x[4] = {wv[v].x, wv[v].y, wv[v].z, wv[v].w};
+                    const int y[4] = {pv[v].x, pv[v].y, pv[v].z, pv[v].w};
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
                         if (r + i < m) {
@@ -154,74 +161,56 @@ template <bool REGS> __global__ void __launch_bounds__(kSelThreads) flb_kv8_sele
     // Sources may share a block with targets, the one that row m lies in.  Its rows from m on are left as they are and the scale
     // they were coded with is kept aside, so the order in which the blocks are filled does not matter.
     if (tid < 2 && rank == 0) a.edge_scale[unit * 2 + tid] = a.c.scale[tid][unit * a.c.nblk + (m >> a.c.block_shift)];
-
-    for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
-    for (int i = tid; i < 2 * kBins2; i += kSelThreads) hist2[0][i] = 0;
-    if (tid == 0) n_safe = n_equal = 0;
     __syncthreads();
 
     const int r1 = max(r0, min(n, r0 + per));
-    uint32_t key[REGS ? kRegRows : 1];
+    const uint32_t all_bits = r1 - r0 < 32 ? (1u << (r1 - r0)) - 1u : ~0u; // (REGS) this thread's cached rows
+    uint32_t key[K];
     uint32_t safe_bits = 0;
     int safe = 0;
     if (REGS) {
 #pragma unroll
-        for (int v = 0; v < kRegRows / 4; ++v) {
-            constexpr int K = REGS ? kRegRows : 1, V = REGS ? kRegRows / 4 : 1;
-            key[(4 * v) % K] = ordered(wv[v % V].x);
-            key[(4 * v + 1) % K] = ordered(wv[v % V].y);
-            key[(4 * v + 2) % K] = ordered(wv[v % V].z);
-            key[(4 * v + 3) % K] = ordered(wv[v % V].w);
-            const int4 p = pv[v % V];
+        for (int v = 0; v < V; ++v) {
+            key[4 * v] = ordered(wv[v].x);
+            key[4 * v + 1] = ordered(wv[v].y);
+            key[4 * v + 2] = ordered(wv[v].z);
+            key[4 * v + 3] = ordered(wv[v].w);
+            const int4 p = pv[v];
             safe_bits |= (uint32_t)(is_safe(p.x) | is_safe(p.y) << 1 | is_safe(p.z) << 2 | is_safe(p.w) << 3) << (4 * v);
         }
-        if (r1 - r0 < 32) safe_bits &= (1u << (r1 - r0)) - 1u;
+        safe_bits &= all_bits;
         safe = __popc(safe_bits);
     } else {
         for (int r = r0; r < r1; ++r) safe += is_safe(pos[r]);
     }
     safe = __reduce_add_sync(0xffffffffu, safe);
     if (lane == 0 && safe) atomicAdd(&n_safe, safe);
-    // f(row, key, protected) for each of this thread's rows
-    auto each = [&](auto f) {
+    // f(key) for each of this thread's rows that are protected, or that are not
+    auto each = [&](bool protected_, auto f) {
         if (REGS) {
+            const uint32_t bits = (protected_ ? safe_bits : ~safe_bits) & all_bits;
 #pragma unroll
-            for (int i = 0; i < kRegRows; ++i)
-                if (i < per && r0 + i < r1) f(r0 + i, key[i % (REGS ? kRegRows : 1)], (safe_bits >> i & 1u) != 0);
+            for (int i = 0; i < K; ++i)
+                if (bits >> i & 1u) f(key[i]);
         } else {
-            for (int r = r0; r < r1; ++r) f(r, ordered(w[r]), is_safe(pos[r]));
+            for (int r = r0; r < r1; ++r)
+                if (is_safe(pos[r]) == protected_) f(ordered(w[r]));
         }
     };
-    // The digit at which the count from above reaches `want`: bins are summed over the cluster, BPT of them per thread from the largest down.
-    auto find = [&](int *bins, auto per_thread, int want, int above) {
-        constexpr int BPT = decltype(per_thread)::value;
-        int c[BPT] = {}, sum = 0;
-        const int top = (tid + 1) * -BPT + kSelThreads * BPT; // bins top .. top + BPT - 1
-        auto add = [&](const int *p) {
-            if (BPT == 4) {
-                const int4 v = *reinterpret_cast<const int4 *>(p + top);
-                c[0] += v.x;
-                c[1 % BPT] += v.y;
-                c[2 % BPT] += v.z;
-                c[3 % BPT] += v.w;
-            } else {
-                c[0] += p[top];
-            }
-        };
-        static_assert(BPT == 4 || BPT == 1, "one load per CTA of the cluster");
+    auto to_all = [&](auto *p, auto value) { // into the same word of every CTA
+        for (int c = 0; c < ranks; ++c) *(ranks == 1 ? p : cluster.map_shared_rank(p, c)) = value;
+    };
+    // The leading digit at which the count from above reaches `want`.  Bins are summed over the cluster, by each CTA an eighth of them (every CTA all of them:
+    // 12000 clocks instead of 4000); four bins per thread in a CTA alone.
+    auto find = [&](int want) {
         if (ranks == 1) {
-            add(bins);
-        } else {
+            const int top = kBins - 4 * (tid + 1);
+            static_assert(kBins == 4 * kSelThreads, "four bins per thread");
+            const int4 v = *reinterpret_cast<const int4 *>(hist + top);
+            const int c[4] = {v.x, v.y, v.z, v.w};
+            int total, at = block_scan(v.x + v.y + v.z + v.w, wi, total);
 #pragma unroll
-            for (int r = 0; r < kRanks; ++r) add(cluster.map_shared_rank(bins, r)); // independent loads: one latency
-        }
-#pragma unroll
-        for (int i = 0; i < BPT; ++i) sum += c[i];
-        int total;
-        int at = above + block_scan(sum, wi, total);
-        if (at < want && at + sum >= want) {
-#pragma unroll
-            for (int i = BPT - 1; i >= 0; --i) {
+            for (int i = 3; i >= 0; --i) {
                 if (at < want && at + c[i] >= want) {
                     found[0] = top + i;
                     found[1] = at;
@@ -229,14 +218,45 @@ template <bool REGS> __global__ void __launch_bounds__(kSelThreads) flb_kv8_sele
                 }
                 at += c[i];
             }
+        } else {
+            constexpr int kSlice = kBins / kRanks;
+            static_assert(kSlice <= kSelThreads, "one bin per thread");
+            const int bin = kBins - rank * kSlice - 1 - tid;
+            int sum = 0;
+            if (tid < kSlice) {
+#pragma unroll
+                for (int c = 0; c < kRanks; ++c) sum += *cluster.map_shared_rank(hist + bin, c); // independent loads: one latency
+            }
+            int total, at = block_scan(sum, wi, total);
+            if (tid == 0) slice_total = total;
+            cluster.sync();
+#pragma unroll
+            for (int c = 0; c < kRanks; ++c) at += c < rank ? *cluster.map_shared_rank(&slice_total, c) : 0;
+            if (tid < kSlice && at < want && at + sum >= want) {
+                to_all(found, (uint32_t)bin);
+                to_all(found + 1, (uint32_t)at);
+                to_all(found + 2, (uint32_t)sum);
+            }
+        }
+        all_sync(cluster, ranks);
+    };
+    // The same for one of the digits of 10 bits, a bin per thread, where there are too many rows of one leading digit to compare them.
+    auto find2 = [&](int *bins, int want, int above) {
+        static_assert(kBins2 == kSelThreads, "one bin per thread");
+        const int bin = kBins2 - 1 - tid;
+        int sum = 0, total;
+        for (int c = 0; c < ranks; ++c) sum += *(ranks == 1 ? bins + bin : cluster.map_shared_rank(bins + bin, c));
+        const int at = above + block_scan(sum, wi, total);
+        if (at < want && at + sum >= want) {
+            found[0] = bin;
+            found[1] = at;
+            found[2] = sum;
         }
         __syncthreads();
     };
     // Protected rows all stay, and the selection is among the others; with more of them than room (positions given twice) it is among them.
     bool among_safe = false;
-    each([&](int, uint32_t k, bool s) {
-        if (!s) atomicAdd(&hist[k >> 20], 1);
-    });
+    each(false, [&](uint32_t k) { atomicAdd(&hist[k >> 20], 1); });
     all_sync(cluster, ranks);
     int all_safe = 0;
     for (int c = 0; c < ranks; ++c) all_safe += ranks == 1 ? n_safe : *cluster.map_shared_rank(&n_safe, c);
@@ -244,90 +264,143 @@ template <bool REGS> __global__ void __launch_bounds__(kSelThreads) flb_kv8_sele
     if (want < 0) {
         among_safe = true;
         want = m;
-        all_sync(cluster, ranks); // nobody reads the histogram of the others any more
+        all_sync(cluster, ranks);
         for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
         __syncthreads();
-        each([&](int, uint32_t k, bool s) {
-            if (s) atomicAdd(&hist[k >> 20], 1);
-        });
+        each(true, [&](uint32_t k) { atomicAdd(&hist[k >> 20], 1); });
         all_sync(cluster, ranks);
     }
     uint32_t least = 0xffffffffu; // smallest kept weight; above it everything stays,
-    int equals = 0, level = 0;    // and of it so many rows, of so many
+    int equals = 0;               // and of it so many rows, the lowest
     if (want > 0) {
-        find(hist, std::integral_constant<int, kBins / kSelThreads>(), want, 0);
-        uint32_t prefix = (uint32_t)found[0] << 20;
-        int above = found[1];
-#pragma unroll 1
-        for (int pass = 0; pass < 2; ++pass) {
-            const int shift = 10 - 10 * pass;
-            each([&](int, uint32_t k, bool s) {
-                if (s == among_safe && ((k ^ prefix) >> (shift + 10)) == 0) atomicAdd(&hist2[pass][(k >> shift) & (kBins2 - 1)], 1);
+        find(want);
+        const uint32_t lead = found[0];
+        const int above = (int)found[1], count = (int)found[2];
+        static_assert(4 * kCandidates <= kBins2, "the lists take the other digits' room");
+        if (count <= kCandidates * (ranks == 1 ? 1 : 4)) {
+            // Few rows share the leading digit with the one looked for (a percent of them, unless weights are equal): they are compared with each other.
+            int *const all = hist2[0], *const mine = hist2[1];
+            each(among_safe, [&](uint32_t k) {
+                if (k >> 20 == lead) (ranks == 1 ? all : mine)[atomicAdd(&n_cand, 1)] = (int)k;
             });
             all_sync(cluster, ranks);
-            find(hist2[pass], std::integral_constant<int, kBins2 / kSelThreads>(), want, above);
-            prefix |= (uint32_t)found[0] << shift;
-            above = found[1];
+            if (ranks > 1) {
+                int nc[kRanks], i = tid, from = kRanks;
+#pragma unroll
+                for (int c = 0; c < kRanks; ++c) nc[c] = *cluster.map_shared_rank(&n_cand, c);
+#pragma unroll
+                for (int c = 0; c < kRanks; ++c) {
+                    if (from == kRanks && i < nc[c]) from = c;
+                    if (from == kRanks) i -= nc[c];
+                }
+                if (from < kRanks) all[tid] = *cluster.map_shared_rank(mine + i, from);
+                __syncthreads();
+            }
+            const int need = want - above, sub = tid & 7; // eight lanes compare one candidate with all, four at a time (behind the last: 0, which no weight is)
+            for (int i0 = (rank * kSelThreads + (tid & ~31)) >> 3; i0 < count; i0 += ranks * kSelThreads / 8) {
+                const int i = i0 + (lane >> 3);
+                const uint32_t k = i < count ? (uint32_t)all[i] : 0u;
+                int gt = 0, eq = 0;
+                for (int j = 4 * sub; j < count; j += 32) {
+                    const uint4 o = *reinterpret_cast<const uint4 *>(all + j);
+                    gt += (o.x > k) + (o.y > k) + (o.z > k) + (o.w > k);
+                    eq += (o.x == k) + (o.y == k) + (o.z == k) + (o.w == k);
+                }
+                int both = gt << 16 | eq;
+#pragma unroll
+                for (int d = 1; d < 8; d <<= 1) both += __shfl_xor_sync(0xffffffffu, both, d);
+                gt = both >> 16;
+                eq = both & 0xffff;
+                if (sub == 0 && i < count && gt < need && gt + eq >= need) { // equal candidates all write the same
+                    to_all(found, k);
+                    to_all(found + 1, (uint32_t)(above + gt));
+                }
+            }
+            all_sync(cluster, ranks);
+            least = found[0];
+            equals = want - (int)found[1];
+        } else {
+            uint32_t prefix = lead << 20;
+            int before = above;
+#pragma unroll 1
+            for (int pass = 0; pass < 2; ++pass) {
+                const int shift = 10 - 10 * pass;
+                each(among_safe, [&](uint32_t k) {
+                    if (((k ^ prefix) >> (shift + 10)) == 0) atomicAdd(&hist2[pass][(k >> shift) & (kBins2 - 1)], 1);
+                });
+                all_sync(cluster, ranks);
+                find2(hist2[pass], want, before);
+                prefix |= found[0] << shift;
+                before = (int)found[1];
+            }
+            least = prefix;
+            equals = want - before;
         }
-        least = prefix;
-        equals = want - above;
-        level = found[2];
     }
 
-    // rows of that weight in front of this thread, where not all of them stay: the lowest do
-    int e = 0;
-    if (equals < level) {
-        int eq = 0;
-        each([&](int, uint32_t k, bool s) { eq += s == among_safe && k == least; });
-        int total;
-        e = block_scan(eq, wi, total);
-        if (tid == 0) n_equal = total;
-        all_sync(cluster, ranks);
-        for (int c = 0; c < rank; ++c) e += *cluster.map_shared_rank(&n_equal, c);
-    }
-    // holes and sources in front of this thread
-    int holes = 0, behind = 0;
-    const int e0 = e;
-    uint32_t stay_bits = 0; // REGS: what the first look found
-    auto kept = [&](uint32_t k, bool s) { // in row order
-        if (s != among_safe) return s;
-        if (k == least) return e++ < equals;
-        return k > least && want > 0;
-    };
-    each([&](int r, uint32_t k, bool s) {
-        const bool stay = kept(k, s);
-        if (REGS) stay_bits |= (uint32_t)stay << (r - r0);
-        holes += r < m && !stay;
-        behind += r >= m && stay;
-    });
-    long long total;
-    const long long before = block_scan((long long)holes | ((long long)behind << 32), ws, total);
-    if (tid == 0) n_lists = total;
-    all_sync(cluster, ranks);
-    int hr = (int)(before & 0xffffffff), br = (int)(before >> 32), all_holes = 0;
-    for (int c = 0; c < ranks; ++c) {
-        const long long t = ranks == 1 ? n_lists : *cluster.map_shared_rank(&n_lists, c);
-        if (c < rank) {
-            hr += (int)(t & 0xffffffff);
-            br += (int)(t >> 32);
+    // Kept rows in front of this thread: those that stay for certain (protected or heavier; or, among the protected, heavier), and the first `equals` of the
+    // smallest kept weight.  Rows below m in front of r less those are the holes in front of r; kept rows behind m are counted from the last, the m-th, back.
+    uint32_t sure_bits = 0, equal_bits = 0;
+    int sure = 0, equal = 0;
+    auto is_sure = [&](uint32_t k, bool s) { return s == among_safe ? k > least : s; };
+    if (REGS) {
+#pragma unroll
+        for (int i = 0; i < K; ++i) {
+            const bool s = (safe_bits >> i & 1u) != 0;
+            sure_bits |= (uint32_t)is_sure(key[i], s) << i;
+            equal_bits |= (uint32_t)(s == among_safe && key[i] == least) << i;
         }
-        all_holes += (int)(t & 0xffffffff);
+        sure_bits &= all_bits;
+        equal_bits &= all_bits;
+        sure = __popc(sure_bits);
+        equal = __popc(equal_bits);
+    } else {
+        for (int r = r0; r < r1; ++r) {
+            const uint32_t k = ordered(w[r]);
+            const bool s = is_safe(pos[r]);
+            sure += is_sure(k, s);
+            equal += s == among_safe && k == least;
+        }
     }
-    e = e0;
-    int *hole_list = a.holes + unit * (a.c.T / 2), *move_list = a.moves + unit * (a.c.T / 2);
+    long long total;
+    long long before = block_scan((long long)sure | ((long long)equal << 32), ws, total);
+    if (ranks > 1) {
+        if (tid == 0) n_kept = total;
+        cluster.sync();
+#pragma unroll
+        for (int c = 0; c < kRanks; ++c) before += c < rank ? *cluster.map_shared_rank(&n_kept, c) : 0ll;
+    }
+    const int room = a.c.T / 2;
+    int *hole_list = a.holes + unit * room, *move_list = a.moves + unit * room;
     const int in_block = (1 << a.c.block_shift) - 1;
-    each([&](int r, uint32_t k, bool s) {
-        const bool stay = REGS ? (stay_bits >> (r - r0) & 1u) != 0 : kept(k, s);
-        if (r <= m && (r & in_block) == 0) off[r >> a.c.block_shift] = hr;
-        if (r < m && !stay) hole_list[hr++] = r;
-        if (r >= m && stay) move_list[br++] = r;
-    });
+    int e = (int)(before >> 32), kept = (int)(before & 0xffffffff) + min(e, equals); // in front of the row
+    auto row = [&](int r, bool sure_, bool equal_) {
+        if (r <= m && (r & in_block) == 0) off[r >> a.c.block_shift] = r - kept;
+        if (r == m) to_all(&kept_below, kept);
+        const bool stay = sure_ || (equal_ && e < equals);
+        e += equal_;
+        if (r < m && !stay) hole_list[r - kept] = r;
+        if (r >= m && stay) move_list[room - m + kept] = r;
+        kept += stay;
+    };
+    if (REGS) {
+#pragma unroll
+        for (int i = 0; i < K; ++i)
+            if (all_bits >> i & 1u) row(r0 + i, (sure_bits >> i & 1u) != 0, (equal_bits >> i & 1u) != 0);
+    } else {
+        for (int r = r0; r < r1; ++r) {
+            const uint32_t k = ordered(w[r]);
+            const bool s = is_safe(pos[r]);
+            row(r, is_sure(k, s), s == among_safe && k == least);
+        }
+    }
+    all_sync(cluster, ranks); // the lists are whole; nobody's shared memory is read or written by others any more
+    const int all_holes = m - kept_below;
     // blocks from the one behind row m on: no holes
     for (int j = ((m + in_block) >> a.c.block_shift) + rank * kSelThreads + tid; j <= a.c.nblk; j += ranks * kSelThreads) off[j] = all_holes;
-    all_sync(cluster, ranks); // the lists are whole; nobody's shared memory is read any more
     // weights and positions of the holes
     for (int i = rank * kSelThreads + tid; i < all_holes; i += ranks * kSelThreads) {
-        const int to = __ldcg(hole_list + i), from = __ldcg(move_list + i);
+        const int to = __ldcg(hole_list + i), from = __ldcg(move_list + room - all_holes + i);
         w_out[to] = w[from];
         p_out[to] = pos[from];
     }
@@ -365,7 +438,7 @@ template <int D, int CODE> __global__ void __launch_bounds__(1024) flb_kv8_move_
     if (lo >= hi) return; // no hole in any of them
     const int m = __ldcg(a.seq_len + 2 * (int)(unit / a.c.H));
     const int rows = 1 << a.c.block_shift, edge = m >> a.c.block_shift, row0 = blk0 << a.c.block_shift;
-    const int *hole_list = a.holes + unit * (a.c.T / 2), *move_list = a.moves + unit * (a.c.T / 2);
+    const int *hole_list = a.holes + unit * (a.c.T / 2), *move_list = a.moves + (unit + 1) * (a.c.T / 2) - __ldcg(off + a.c.nblk); // sources end with their room
     const uint8_t *all = a.c.codes[kv] + unit * a.c.T * D;
     float *scales = a.c.scale[kv] + unit * a.c.nblk;
     for (int i = threadIdx.x; i < nb * rows; i += blockDim.x) from_s[i] = -1;
@@ -438,8 +511,7 @@ template <int D, int CODE> __global__ void __launch_bounds__(1024) flb_kv8_move_
 template <int D, int CODE> cudaError_t launch_t(const Kv8EvictArgs &a, cudaStream_t stream) {
     const unsigned units = (unsigned)a.c.B * (unsigned)a.c.H;
     // One CTA per head up to 8192 rows, eight beyond (a portable cluster); up to 16 rows per thread keys stay in registers.
-    const int ranks = a.c.T <= 8192 ? 1 : kRanks;
-    const bool regs = (long long)a.c.T <= (long long)ranks * kSelThreads * kRegRows;
+    const int ranks = a.c.T <= 8192 ? 1 : kRanks, per = rows_per_thread(a.c.T, ranks);
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -452,7 +524,7 @@ template <int D, int CODE> cudaError_t launch_t(const Kv8EvictArgs &a, cudaStrea
     cfg.stream = stream;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, regs ? flb_kv8_select_kernel<true> : flb_kv8_select_kernel<false>, a);
+    cudaError_t e = cudaLaunchKernelEx(&cfg, per <= 8 ? flb_kv8_select_kernel<8> : per <= 16 ? flb_kv8_select_kernel<16> : flb_kv8_select_kernel<0>, a);
     if (e != cudaSuccess) return e;
     const int kept_blocks = (min(a.c.T, a.budget) + (1 << a.c.block_shift) - 1) >> a.c.block_shift;
     const int groups = (kept_blocks + kGroup - 1) / kGroup;

@@ -594,6 +594,30 @@ def test_evict_long_slabs(cuda_device):
     run_evict(29, lens=[40001], T=40064, budget=40000, recent=100, sinks=4, d=64, block=32, H=1)
 
 
+@pytest.mark.parametrize("T", [4096, 16384, 81920])  # a CTA, a cluster with 8 and one with 16 rows per thread
+@pytest.mark.parametrize("kind", ["random", "few values", "near", "zeros", "special", "protected"])
+def test_evict_selections(cuda_device, T, kind):
+    """Few and many weights that share their leading digit with the one looked for, all equal, all protected."""
+    g = gen(T + len(kind))
+    n, B = T - 7, 1
+    w = torch.rand(B, 1, T, generator=g, device=DEV)
+    more = dict(recent=50, sinks=4)
+    if kind == "few values":
+        w = torch.randint(0, 3, (B, 1, T), generator=g, device=DEV).float()
+    elif kind == "near":  # one leading digit, all different and some not
+        w = 1 + torch.randint(0, T // 2, (B, 1, T), generator=g, device=DEV).float() * 2.0 ** -20
+    elif kind == "zeros":
+        w.zero_()
+    elif kind == "special":
+        w[:, :, ::3], w[:, :, 1::3] = math.nan, math.inf
+    pos = None
+    if kind == "protected":
+        pos = torch.arange(T, dtype=torch.int32, device=DEV).flip(0).expand(B, 1, T) // 4
+        more = dict(recent=100, sinks=40)
+    for budget in (150, T // 3, n - 1):
+        run_evict(45, lens=[n], T=T, budget=budget, H=1, weight=w.clone(), pos=pos, nxt=[T // 4] if kind == "protected" else [n], **more)
+
+
 def test_evict_slabs_beyond_the_registers(cuda_device):
     """More rows than a cluster's threads keep in registers: the keys are read again at every pass."""
     run_evict(31, lens=[150001], T=150016, budget=3000, recent=100, sinks=4, d=64, block=16, H=1)
