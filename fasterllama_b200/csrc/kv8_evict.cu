@@ -27,7 +27,6 @@ constexpr int kRanks = 8;    // CTAs of a cluster, where there is more than one
 // Digits of 12, 10 and 10 bits: sign, exponent and the first mantissa bits first, which leaves a percent of the rows for the other passes and spreads
 // the additions of the first one over more words than a byte would.
 constexpr int kBins = 4096, kBins2 = 1024;
-constexpr int kCandidates = 256; // rows of one leading digit that one CTA compares with each other rather than sorting them by the other digits
 
 // rows of a slab that a thread looks after, in fours
 __host__ __device__ inline int rows_per_thread(int T, int ranks) { return (((T + ranks - 1) / ranks + kSelThreads - 1) / kSelThreads + 3) & ~3; }
@@ -77,8 +76,10 @@ __device__ __forceinline__ void all_sync(cg::cluster_group &cluster, int ranks) 
 template <int ROWS> __global__ void __launch_bounds__(kSelThreads) flb_kv8_select_kernel(const __grid_constant__ Kv8EvictArgs a) {
     constexpr bool REGS = ROWS > 0;
     constexpr int K = REGS ? ROWS : 4, V = K / 4;
-    __shared__ __align__(16) int hist[kBins];                  // leading digit
-    __shared__ __align__(16) int hist2[2][kBins2];             // the two others; or the candidates, all of the cluster's and this CTA's
+    // Counts of the leading digit, then the candidates (the cluster's, this CTA's); counts of the two other digits; at the end both are the lists' room.
+    constexpr int kPool = kBins + 2 * kBins2, kListWords = ROWS * kSelThreads / 2;
+    __shared__ __align__(16) int pool[kPool > kListWords ? kPool : kListWords];
+    int *const hist = pool, *const hist2 = pool + kBins;
     __shared__ long long ws[32];
     __shared__ int wi[32];
     __shared__ int n_safe, n_cand, slice_total, kept_below; // kept_below: kept rows in front of row m
@@ -123,8 +124,7 @@ template <int ROWS> __global__ void __launch_bounds__(kSelThreads) flb_kv8_selec
         a.seq_len[2 * b] = m; // the same from every head
         a.seq_len[2 * b + 1] = bad ? n : m;
     }
-    for (int i = tid; i < kBins / 4; i += kSelThreads) reinterpret_cast<int4 *>(hist)[i] = make_int4(0, 0, 0, 0);
-    for (int i = tid; i < kBins2 / 2; i += kSelThreads) reinterpret_cast<int4 *>(hist2)[i] = make_int4(0, 0, 0, 0);
+    for (int i = tid; i < kPool / 4; i += kSelThreads) reinterpret_cast<int4 *>(pool)[i] = make_int4(0, 0, 0, 0);
     if (tid == 0) n_safe = n_cand = 0;
     // Rows below m into the results, where those are other buffers; the holes are written over at the end.
     if (w_out != w || p_out != pos) {
@@ -240,17 +240,21 @@ template <int ROWS> __global__ void __launch_bounds__(kSelThreads) flb_kv8_selec
         }
         all_sync(cluster, ranks);
     };
-    // The same for one of the digits of 10 bits, a bin per thread, where there are too many rows of one leading digit to compare them.
-    auto find2 = [&](int *bins, int want, int above) {
+    // The same for one of the digits of 10 bits, a bin per thread; `across`: the bins of all CTAs are summed, else these are counts of everything.
+    auto find2 = [&](const int *bins, bool across, int want, int above) {
         static_assert(kBins2 == kSelThreads, "one bin per thread");
         const int bin = kBins2 - 1 - tid;
         int sum = 0, total;
-        for (int c = 0; c < ranks; ++c) sum += *(ranks == 1 ? bins + bin : cluster.map_shared_rank(bins + bin, c));
+        if (across && ranks > 1) {
+#pragma unroll
+            for (int c = 0; c < kRanks; ++c) sum += *cluster.map_shared_rank(bins + bin, c);
+        } else {
+            sum = bins[bin];
+        }
         const int at = above + block_scan(sum, wi, total);
         if (at < want && at + sum >= want) {
             found[0] = bin;
             found[1] = at;
-            found[2] = sum;
         }
         __syncthreads();
     };
@@ -274,14 +278,18 @@ template <int ROWS> __global__ void __launch_bounds__(kSelThreads) flb_kv8_selec
     int equals = 0;               // and of it so many rows, the lowest
     if (want > 0) {
         find(want);
-        const uint32_t lead = found[0];
-        const int above = (int)found[1], count = (int)found[2];
-        static_assert(4 * kCandidates <= kBins2, "the lists take the other digits' room");
-        if (count <= kCandidates * (ranks == 1 ? 1 : 4)) {
-            // Few rows share the leading digit with the one looked for (a percent of them, unless weights are equal): they are compared with each other.
-            int *const all = hist2[0], *const mine = hist2[1];
+        uint32_t prefix = found[0] << 20;
+        int above = (int)found[1];
+        const int count = (int)found[2];
+        static_assert(2 * kSelThreads <= kBins, "the candidates take the leading digit's room");
+        const bool few = count <= kSelThreads;
+        uint32_t cand = 0;
+        if (few) {
+            // So few rows share the leading digit with the one looked for (some percent of a slab, unless weights are equal) that each becomes a
+            // thread's, in every CTA, and the other digits need no look at the rows.
+            int *const all = hist, *const mine = ranks == 1 ? hist : hist + kSelThreads;
             each(among_safe, [&](uint32_t k) {
-                if (k >> 20 == lead) (ranks == 1 ? all : mine)[atomicAdd(&n_cand, 1)] = (int)k;
+                if (((k ^ prefix) >> 20) == 0) mine[atomicAdd(&n_cand, 1)] = (int)k;
             });
             all_sync(cluster, ranks);
             if (ranks > 1) {
@@ -293,49 +301,31 @@ template <int ROWS> __global__ void __launch_bounds__(kSelThreads) flb_kv8_selec
                     if (from == kRanks && i < nc[c]) from = c;
                     if (from == kRanks) i -= nc[c];
                 }
-                if (from < kRanks) all[tid] = *cluster.map_shared_rank(mine + i, from);
-                __syncthreads();
+                if (from < kRanks) cand = (uint32_t)*cluster.map_shared_rank(mine + i, from);
+            } else if (tid < count) {
+                cand = (uint32_t)all[tid];
             }
-            const int need = want - above, sub = tid & 7; // eight lanes compare one candidate with all, four at a time (behind the last: 0, which no weight is)
-            for (int i0 = (rank * kSelThreads + (tid & ~31)) >> 3; i0 < count; i0 += ranks * kSelThreads / 8) {
-                const int i = i0 + (lane >> 3);
-                const uint32_t k = i < count ? (uint32_t)all[i] : 0u;
-                int gt = 0, eq = 0;
-                for (int j = 4 * sub; j < count; j += 32) {
-                    const uint4 o = *reinterpret_cast<const uint4 *>(all + j);
-                    gt += (o.x > k) + (o.y > k) + (o.z > k) + (o.w > k);
-                    eq += (o.x == k) + (o.y == k) + (o.z == k) + (o.w == k);
-                }
-                int both = gt << 16 | eq;
-#pragma unroll
-                for (int d = 1; d < 8; d <<= 1) both += __shfl_xor_sync(0xffffffffu, both, d);
-                gt = both >> 16;
-                eq = both & 0xffff;
-                if (sub == 0 && i < count && gt < need && gt + eq >= need) { // equal candidates all write the same
-                    to_all(found, k);
-                    to_all(found + 1, (uint32_t)(above + gt));
-                }
-            }
-            all_sync(cluster, ranks);
-            least = found[0];
-            equals = want - (int)found[1];
-        } else {
-            uint32_t prefix = lead << 20;
-            int before = above;
-#pragma unroll 1
-            for (int pass = 0; pass < 2; ++pass) {
-                const int shift = 10 - 10 * pass;
-                each(among_safe, [&](uint32_t k) {
-                    if (((k ^ prefix) >> (shift + 10)) == 0) atomicAdd(&hist2[pass][(k >> shift) & (kBins2 - 1)], 1);
-                });
-                all_sync(cluster, ranks);
-                find2(hist2[pass], want, before);
-                prefix |= found[0] << shift;
-                before = (int)found[1];
-            }
-            least = prefix;
-            equals = want - before;
         }
+#pragma unroll 1
+        for (int pass = 0; pass < 2; ++pass) {
+            const int shift = 10 - 10 * pass;
+            int *const bins = hist2 + pass * kBins2;
+            auto add = [&](uint32_t k) {
+                if (((k ^ prefix) >> (shift + 10)) == 0) atomicAdd(bins + ((k >> shift) & (kBins2 - 1)), 1);
+            };
+            if (few) {
+                if (tid < count) add(cand);
+                __syncthreads();
+            } else {
+                each(among_safe, add);
+                all_sync(cluster, ranks);
+            }
+            find2(bins, !few, want, above);
+            prefix |= found[0] << shift;
+            above = (int)found[1];
+        }
+        least = prefix;
+        equals = want - above;
     }
 
     // Kept rows in front of this thread: those that stay for certain (protected or heavier; or, among the protected, heavier), and the first `equals` of the
@@ -362,36 +352,65 @@ template <int ROWS> __global__ void __launch_bounds__(kSelThreads) flb_kv8_selec
             equal += s == among_safe && k == least;
         }
     }
-    long long total;
+    long long total, first = 0; // in this CTA, and in front of it
     long long before = block_scan((long long)sure | ((long long)equal << 32), ws, total);
     if (ranks > 1) {
         if (tid == 0) n_kept = total;
         cluster.sync();
 #pragma unroll
-        for (int c = 0; c < kRanks; ++c) before += c < rank ? *cluster.map_shared_rank(&n_kept, c) : 0ll;
+        for (int c = 0; c < kRanks; ++c) first += c < rank ? *cluster.map_shared_rank(&n_kept, c) : 0ll;
+        before += first;
     }
+    auto kept_of = [&](long long x) { return (int)(x & 0xffffffff) + min((int)(x >> 32), equals); };
     const int room = a.c.T / 2;
     int *hole_list = a.holes + unit * room, *move_list = a.moves + unit * room;
     const int in_block = (1 << a.c.block_shift) - 1;
-    int e = (int)(before >> 32), kept = (int)(before & 0xffffffff) + min(e, equals); // in front of the row
-    auto row = [&](int r, bool sure_, bool equal_) {
-        if (r <= m && (r & in_block) == 0) off[r >> a.c.block_shift] = r - kept;
-        if (r == m) to_all(&kept_below, kept);
-        const bool stay = sure_ || (equal_ && e < equals);
-        e += equal_;
-        if (r < m && !stay) hole_list[r - kept] = r;
-        if (r >= m && stay) move_list[room - m + kept] = r;
-        kept += stay;
-    };
+    int e = (int)(before >> 32), kept = kept_of(before); // in front of the row
+    // The lists are gathered in shared memory, from where they leave in order (straight from the threads, 4 bytes here and there, they took 10000 clocks instead
+    // of 5000): rows of this CTA's stretch, holes from the front, sources up to the end.
+    uint16_t *const list = reinterpret_cast<uint16_t *>(pool);
+    constexpr int kList = ROWS * kSelThreads;
+    const int c0 = rank * kSelThreads * per, c1 = min(n, c0 + kSelThreads * per); // the stretch
+    const int kept0 = kept_of(first), kept1 = kept_of(first + total);             // in front of it, and up to its end
     if (REGS) {
+        uint32_t stay = sure_bits; // and the lowest of the equal ones, as many as still have room
+        if (e + equal <= equals) {
+            stay |= equal_bits;
+        } else {
+            for (uint32_t eb = equal_bits; eb && e < equals; eb &= eb - 1, ++e) stay |= eb & (0u - eb);
+        }
+        auto in_front = [&](int r) { return kept + __popc(stay & ((1u << (r - r0)) - 1u)); };
+        const int rb = (r0 + in_block) & ~in_block; // a block that starts among these rows, of which there is one at most
+        static_assert(ROWS <= 16, "blocks have 16 rows or more");
+        if (rb < r1 && rb <= m) off[rb >> a.c.block_shift] = rb - in_front(rb);
+        if (r0 <= m && m < r1) to_all(&kept_below, in_front(m));
+        const uint32_t low = m <= r0 ? 0u : m - r0 < 32 ? (1u << (m - r0)) - 1u : ~0u; // rows below m
+        const uint32_t hole_bits = ~stay & all_bits & low, source_bits = stay & ~low;
+        uint16_t *h = list + ((r0 - kept) - (c0 - kept0)), *f = list + kList - (kept1 - kept - __popc(stay & low));
 #pragma unroll
-        for (int i = 0; i < K; ++i)
-            if (all_bits >> i & 1u) row(r0 + i, (sure_bits >> i & 1u) != 0, (equal_bits >> i & 1u) != 0);
+        for (int i = 0; i < K; ++i) {
+            if (hole_bits >> i & 1u) *h++ = (uint16_t)(r0 + i - c0);
+            if (source_bits >> i & 1u) *f++ = (uint16_t)(r0 + i - c0);
+        }
+        __syncthreads();
+        if (c0 < c1) {
+            const bool holds_m = c0 <= m && m < c1;
+            const int below = max(0, min(m, c1) - c0); // rows of the stretch below m, and how many of those are kept
+            const int kept_there = c0 >= m ? 0 : (holds_m ? kept_below : kept1) - kept0;
+            const int nh = below - kept_there, ns = kept1 - kept0 - kept_there;
+            for (int i = tid; i < nh; i += kSelThreads) hole_list[c0 - kept0 + i] = c0 + list[i];
+            for (int i = tid; i < ns; i += kSelThreads) move_list[room - m + kept1 - ns + i] = c0 + list[kList - ns + i];
+        }
     } else {
         for (int r = r0; r < r1; ++r) {
             const uint32_t k = ordered(w[r]);
-            const bool s = is_safe(pos[r]);
-            row(r, is_sure(k, s), s == among_safe && k == least);
+            const bool s = is_safe(pos[r]), level = s == among_safe && k == least, stay = is_sure(k, s) || (level && e < equals);
+            if (r <= m && (r & in_block) == 0) off[r >> a.c.block_shift] = r - kept;
+            if (r == m) to_all(&kept_below, kept);
+            if (r < m && !stay) hole_list[r - kept] = r;
+            if (r >= m && stay) move_list[room - m + kept] = r;
+            e += level;
+            kept += stay;
         }
     }
     all_sync(cluster, ranks); // the lists are whole; nobody's shared memory is read or written by others any more
@@ -400,7 +419,8 @@ template <int ROWS> __global__ void __launch_bounds__(kSelThreads) flb_kv8_selec
     for (int j = ((m + in_block) >> a.c.block_shift) + rank * kSelThreads + tid; j <= a.c.nblk; j += ranks * kSelThreads) off[j] = all_holes;
     // weights and positions of the holes
     for (int i = rank * kSelThreads + tid; i < all_holes; i += ranks * kSelThreads) {
-        const int to = __ldcg(hole_list + i), from = __ldcg(move_list + room - all_holes + i);
+        const bool own = REGS && ranks == 1;
+        const int to = own ? list[i] : __ldcg(hole_list + i), from = own ? list[kList - all_holes + i] : __ldcg(move_list + room - all_holes + i);
         w_out[to] = w[from];
         p_out[to] = pos[from];
     }
