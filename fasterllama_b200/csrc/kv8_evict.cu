@@ -461,6 +461,67 @@ template <int D, int CODE> __global__ void __launch_bounds__(1024) flb_kv8_move_
     const int *hole_list = a.holes + unit * (a.c.T / 2), *move_list = a.moves + (unit + 1) * (a.c.T / 2) - __ldcg(off + a.c.nblk); // sources end with their room
     const uint8_t *all = a.c.codes[kv] + unit * a.c.T * D;
     float *scales = a.c.scale[kv] + unit * a.c.nblk;
+    auto scale_of = [&](int src) { return (src >> a.c.block_shift) == edge ? __ldcg(a.edge_scale + unit * 2 + kv) : scales[src >> a.c.block_shift]; };
+    if ((hi - lo) * CPR <= kChunks * (int)blockDim.x) {
+        // Few holes: a thread per chunk that comes in, all blocks at once.  (Block after block the threads mostly find that a row stays.)
+        __shared__ uint32_t top_s[kGroup];
+        __shared__ float old_s[kGroup];
+        if ((int)threadIdx.x < kGroup) {
+            top_s[threadIdx.x] = 0u;
+            old_s[threadIdx.x] = (int)threadIdx.x < nb ? scales[blk0 + threadIdx.x] : 0.f;
+        }
+        uint2 u[kChunks];
+        float s[kChunks];
+        int to[kChunks];
+#pragma unroll
+        for (int i = 0; i < kChunks; ++i) {
+            const int id = (int)threadIdx.x + i * (int)blockDim.x, h = lo + id / CPR;
+            to[i] = -1;
+            if (h < hi) {
+                const int src = __ldcg(move_list + h);
+                to[i] = __ldcg(hole_list + h);
+                u[i] = *reinterpret_cast<const uint2 *>(all + (size_t)src * D + (id % CPR) * 8);
+                s[i] = scale_of(src);
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kChunks; ++i) {
+            if (lo + (int)(threadIdx.x + i * blockDim.x) / CPR >= hi) break; // for whole rows of chunks alike
+            float x[8];
+            uint32_t amax = 0;
+            kv8_decode8<CODE>(u[i], x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) amax = max(amax, kv8_abs_bits(__fmul_rn(x[e], s[i])));
+            atomicMax(top_s + ((to[i] - row0) >> a.c.block_shift), amax);
+        }
+        __syncthreads();
+        bool any = false;
+        for (int j = 0; j < nb; ++j) {
+            const float old = old_s[j], scale = kv8_new_scale<CODE>(top_s[j], old);
+            if (!(old > 0.f && scale > old)) continue;
+            any = true; // the codes that the block held follow; those of the holes are written over below
+            uint2 *mine = reinterpret_cast<uint2 *>(a.c.codes[kv] + (unit * a.c.T + row0 + j * rows) * D);
+            const float ratio = __fdiv_rn(old, scale);
+            for (int ch = threadIdx.x; ch < min(rows, m - row0 - j * rows) * CPR; ch += blockDim.x) mine[ch] = kv8_rescale8<CODE>(mine[ch], ratio);
+        }
+        if (any) __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kChunks; ++i) {
+            if (to[i] < 0) break;
+            const int j = (to[i] - row0) >> a.c.block_shift;
+            const float scale = kv8_new_scale<CODE>(top_s[j], old_s[j]);
+            float x[8];
+            kv8_decode8<CODE>(u[i], x);
+            kv8_scale8(x, s[i]);
+            reinterpret_cast<uint2 *>(a.c.codes[kv] + (unit * a.c.T + to[i]) * D)[(threadIdx.x + i * blockDim.x) % CPR] = kv8_encode8<CODE>(x, scale, __fdiv_rn(1.f, scale));
+        }
+        if ((int)threadIdx.x < nb) {
+            const float old = old_s[threadIdx.x], scale = kv8_new_scale<CODE>(top_s[threadIdx.x], old);
+            if (__float_as_uint(scale) != __float_as_uint(old)) scales[blk0 + threadIdx.x] = scale;
+        }
+        return;
+    }
     for (int i = threadIdx.x; i < nb * rows; i += blockDim.x) from_s[i] = -1;
     __syncthreads();
     for (int i = lo + (int)threadIdx.x; i < hi; i += blockDim.x) from_s[__ldcg(hole_list + i) - row0] = __ldcg(move_list + i);
@@ -474,7 +535,7 @@ template <int D, int CODE> __global__ void __launch_bounds__(1024) flb_kv8_move_
             const int ch = threadIdx.x + i * blockDim.x, src = from_s[j * rows + ch / CPR];
             if (src < 0) continue;
             next_u[i] = *reinterpret_cast<const uint2 *>(all + (size_t)src * D + (ch % CPR) * 8);
-            next_s[i] = (src >> a.c.block_shift) == edge ? __ldcg(a.edge_scale + unit * 2 + kv) : scales[src >> a.c.block_shift];
+            next_s[i] = scale_of(src);
         }
     };
     fetch(0);
