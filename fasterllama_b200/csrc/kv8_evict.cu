@@ -2,11 +2,14 @@
 //
 // 1. flb_kv8_select_kernel, a CTA or a cluster of eight per K/V head: which rows stay.  A radix selection over the weights (as ordered
 //    integers, in registers; histograms meet in distributed shared memory) finds the smallest kept weight and how many rows of
-//    exactly that weight stay (the lowest of them); prefix sums in row order then list the holes below m = min(n, budget) and
-//    the kept rows behind it, and weights and positions move.
+//    exactly that weight stay (the lowest of them); one prefix sum in row order then lists the holes below m = min(n, budget) and
+//    the kept rows behind it, and weights and positions move.  Bound by the chain of its steps: 10 us for slabs of 4352 rows on one CTA
+//    each, 18 us for 65536 rows on eight.
 // 2. flb_kv8_move_kernel, K and V apart, a CTA per four blocks of rows: the i-th hole takes the i-th
 //    kept row from behind m.  Sources lie at or behind m and targets below it, so nothing waits for anything.  The
-//    block's scale grows by the rule of an append (the codes are held in registers in between).
+//    block's scale grows by the rule of an append (the codes are held in registers in between).  Bound by instruction issue where
+//    most rows of a block are filled (about 120 per eight codes): 28 us for 98304 rows of 128
+//    codes coming in, K and V.
 // Filling holes moves at most n - m rows and recodes only those (and a block whose scale grows); closing the gaps in row order
 // would move nearly every row and round nearly every code once more at each eviction.
 #include "kv8.cuh"
@@ -24,8 +27,8 @@ namespace {
 
 constexpr int kSelThreads = 1024;
 constexpr int kRanks = 8;    // CTAs of a cluster, where there is more than one
-// Digits of 12, 10 and 10 bits: sign, exponent and the first mantissa bits first, which leaves a percent of the rows for the other passes and spreads
-// the additions of the first one over more words than a byte would.
+// Digits of 12, 10 and 10 bits: sign, exponent and the first mantissa bits first, which leaves some percent of the rows for the other passes and
+// spreads the additions of the first one over more words than a byte would.
 constexpr int kBins = 4096, kBins2 = 1024;
 
 // rows of a slab that a thread looks after, in fours
@@ -37,7 +40,6 @@ __device__ __forceinline__ uint32_t ordered(float w) {
     const uint32_t u = __float_as_uint(w == 0.f ? 0.f : w); // -0 equals 0
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
-
 
 // Exclusive prefix over the block in thread order, and the total.  `ws`: a word per warp.
 template <typename T> __device__ __forceinline__ T block_scan(T v, T *ws, T &total) {
@@ -71,8 +73,8 @@ __device__ __forceinline__ void all_sync(cg::cluster_group &cluster, int ranks) 
 }
 
 // A cluster of CTAs (one, for short slabs) per K/V head; every thread has `per` neighbouring rows.  ROWS: so many of them at most, whose keys stay in
-// registers over the passes; 0: any number, read again.  What bounds it is the chain of dependent steps and, with 32 warps on an SM, every instruction
-// per row (16 rows where 8 do: 17.5 us instead of 14 at 4352 rows).
+// registers over the passes; 0: any number, read again.  With 32 warps on an SM every instruction per row is eight clocks: code for 16 rows where 8 do
+// took 5000 clocks instead of 2100 to bring the keys into registers.
 template <int ROWS> __global__ void __launch_bounds__(kSelThreads) flb_kv8_select_kernel(const __grid_constant__ Kv8EvictArgs a) {
     constexpr bool REGS = ROWS > 0;
     constexpr int K = REGS ? ROWS : 4, V = K / 4;
@@ -428,14 +430,16 @@ template <int ROWS> __global__ void __launch_bounds__(kSelThreads) flb_kv8_selec
 
 constexpr int kChunks = 4; // 8-code chunks per thread
 
-// Blocks that a CTA looks after, one after the other.  Measured (us, whole eviction): 16 x 8 heads of 2000-4350 rows, where most blocks have no hole and a CTA only
-// looks and leaves, 1: 47.0, 2: 35.0, 3: 32.8, 4: 32.1, 11: 41.3; 8 heads of 65536 rows cut to a quarter 65.1, 61.7, 61.7, 60.4, -.
+// Blocks that a CTA looks after.  Measured (us, whole eviction): 16 x 8 heads of 2000-4350 rows, where most blocks have few holes or none,
+// 2: 26.5, 3: 22.9, 4: 21.1, 6: 20.3, 8: 21.7; 8 heads of 65536 rows cut to a quarter 50.8, 50.1, 48.7, 52.8, 50.8.
 constexpr int kGroup = 4;
 
 template <int D, int CODE> __global__ void __launch_bounds__(1024) flb_kv8_move_kernel(const __grid_constant__ Kv8EvictArgs a, int groups) {
     constexpr int CPR = D / 8;
-    __shared__ uint32_t red[32];
-    __shared__ int from_s[kGroup * 128]; // source of every row of the blocks, -1 = stays
+    __shared__ uint32_t red[2][32];
+    __shared__ int from_s[kGroup * 128], off_s[kGroup + 1]; // the entries of the lists that are these blocks'
+    __shared__ uint16_t to_s[kGroup * 128], held_s[kGroup * 128]; // rows of the group: that are filled, that stay
+    __shared__ uint32_t hole_mask[kGroup * 4];
     kv8_begin();
     if (blockIdx.x == 0) { // len_out may be past_lens: nobody reads that any more
         int bad = 0;
@@ -522,18 +526,37 @@ template <int D, int CODE> __global__ void __launch_bounds__(1024) flb_kv8_move_
         }
         return;
     }
-    for (int i = threadIdx.x; i < nb * rows; i += blockDim.x) from_s[i] = -1;
+    // Block after block, what comes in from consecutive entries of the lists and what stays from a list of its own: a warp that held rows of both kinds
+    // went both ways at every chunk (whole eviction of 8 heads of 65536 rows to a quarter 51.0 us instead of 48.7).
+    for (int i = threadIdx.x; i < kGroup * 4; i += blockDim.x) hole_mask[i] = 0u;
+    if ((int)threadIdx.x <= nb) off_s[threadIdx.x] = __ldcg(off + blk0 + threadIdx.x) - lo;
     __syncthreads();
-    for (int i = lo + (int)threadIdx.x; i < hi; i += blockDim.x) from_s[__ldcg(hole_list + i) - row0] = __ldcg(move_list + i);
+    for (int i = threadIdx.x; i < hi - lo; i += blockDim.x) {
+        const int to = __ldcg(hole_list + lo + i) - row0, r = to & (rows - 1);
+        from_s[i] = __ldcg(move_list + lo + i);
+        to_s[i] = (uint16_t)to;
+        atomicOr(hole_mask + (to >> a.c.block_shift) * 4 + (r >> 5), 1u << (r & 31));
+    }
     __syncthreads();
+    for (int i = threadIdx.x; i < nb * rows; i += blockDim.x) { // rows that stay, in order
+        const int j = i >> a.c.block_shift, r = i & (rows - 1), word = r >> 5;
+        const uint32_t *mask = hole_mask + j * 4;
+        if (row0 + i >= m || (mask[word] >> (r & 31) & 1u)) continue;
+        int before = __popc(~mask[word] & ((1u << (r & 31)) - 1u));
+        for (int q = 0; q < word; ++q) before += __popc(~mask[q]);
+        held_s[(j << a.c.block_shift) + before] = (uint16_t)i;
+    }
+    __syncthreads();
+    int turn = 0;
     uint2 next_u[kChunks];
     float next_s[kChunks], next_old = 0.f;
     auto fetch = [&](int j) { // the rows that come into block j of the group, and the scales they bring
         next_old = scales[blk0 + j];
 #pragma unroll
         for (int i = 0; i < kChunks; ++i) {
-            const int ch = threadIdx.x + i * blockDim.x, src = from_s[j * rows + ch / CPR];
-            if (src < 0) continue;
+            const int ch = threadIdx.x + i * blockDim.x, h = off_s[j] + ch / CPR;
+            if (h >= off_s[j + 1]) break;
+            const int src = from_s[h];
             next_u[i] = *reinterpret_cast<const uint2 *>(all + (size_t)src * D + (ch % CPR) * 8);
             next_s[i] = scale_of(src);
         }
@@ -549,13 +572,13 @@ template <int D, int CODE> __global__ void __launch_bounds__(1024) flb_kv8_move_
             s[i] = next_s[i];
         }
         if (j + 1 < nb) fetch(j + 1); // its scale is read before anybody can get to writing it, its sources are written by nobody
-        const int *from = from_s + j * rows;
-        const int first = row0 + j * rows;
-        uint2 *mine = reinterpret_cast<uint2 *>(a.c.codes[kv] + (unit * a.c.T + first) * D);
+        const int coming = (off_s[j + 1] - off_s[j]) * CPR;
+        if (coming == 0) continue; // for the whole block alike
+        uint2 *const codes = reinterpret_cast<uint2 *>(a.c.codes[kv] + (unit * a.c.T + row0) * D);
         uint32_t amax = 0;
 #pragma unroll
         for (int i = 0; i < kChunks; ++i) {
-            if (from[(threadIdx.x + i * blockDim.x) / CPR] < 0) continue;
+            if ((int)(threadIdx.x + i * blockDim.x) >= coming) break;
             float x[8], big = 0.f;
             kv8_decode8<CODE>(u[i], x);
             if (fabsf(s[i]) <= 3.402823466e38f) { // rounding keeps the order: the largest product is that of the largest code
@@ -567,21 +590,25 @@ template <int D, int CODE> __global__ void __launch_bounds__(1024) flb_kv8_move_
                 for (int e = 0; e < 8; ++e) amax = max(amax, kv8_abs_bits(__fmul_rn(x[e], s[i])));
             }
         }
-        if (j) __syncthreads(); // `red` has been read
-        amax = kv8_block_max(amax, red);
+        amax = kv8_block_max(amax, red[turn++ & 1]); // (the other one may still be read)
         const float scale = kv8_new_scale<CODE>(amax, old);
         const bool grown = old > 0.f && scale > old;
-        const float ratio = grown ? __fdiv_rn(old, scale) : 1.f, inv = __fdiv_rn(1.f, scale);
+        const float inv = __fdiv_rn(1.f, scale);
 #pragma unroll
         for (int i = 0; i < kChunks; ++i) {
             const int ch = threadIdx.x + i * blockDim.x;
-            if (from[ch / CPR] >= 0) {
-                float x[8];
-                kv8_decode8<CODE>(u[i], x);
-                kv8_scale8(x, s[i]);
-                mine[ch] = kv8_encode8<CODE>(x, scale, inv);
-            } else if (grown && first + ch / CPR < m) {
-                mine[ch] = kv8_rescale8<CODE>(mine[ch], ratio);
+            if (ch >= coming) break;
+            float x[8];
+            kv8_decode8<CODE>(u[i], x);
+            kv8_scale8(x, s[i]);
+            codes[to_s[off_s[j] + ch / CPR] * CPR + ch % CPR] = kv8_encode8<CODE>(x, scale, inv);
+        }
+        if (grown) { // the codes that the block holds follow its scale
+            const float ratio = __fdiv_rn(old, scale);
+            const int staying = (min(rows, m - row0 - j * rows) - (off_s[j + 1] - off_s[j])) * CPR;
+            for (int ch = threadIdx.x; ch < staying; ch += blockDim.x) {
+                uint2 *mine = codes + held_s[j * rows + ch / CPR] * CPR + ch % CPR;
+                *mine = kv8_rescale8<CODE>(*mine, ratio);
             }
         }
         // a block behind m, whose scale others read, never gets here with a new one
