@@ -51,9 +51,9 @@ def build_cuda(force: bool = False, verbose: bool = False) -> str:
 
 
 def build_tensor_args(force: bool = False) -> str:
-    """The binding's tensor checks (csrc/tensor_args.cpp), a Python extension module against this interpreter and torch."""
+    """The binding's tensor checks and parameter blocks (csrc/tensor_args.cpp), a Python extension module against this interpreter and torch."""
     src = os.path.join(CSRC, "tensor_args.cpp")
-    if not force and _newer(ARGS_PATH, [src]):
+    if not force and _newer(ARGS_PATH, [src, *(os.path.join(ROOT, "include", f) for f in ("flb_attn.h", "flb_kv8.h"))]):
         return ARGS_PATH
     import sysconfig
 

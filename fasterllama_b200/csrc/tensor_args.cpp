@@ -1,81 +1,294 @@
-// tensor_args.cpp — the argument checks of the Python binding for torch tensors, in C++: shape, type, device and layout of a tensor and its
-// address in about a tenth of a microsecond.  From Python every attribute of a tensor costs that much, and a decode call names a
-// dozen tensors: its host time would be that of three kernel launches.  Python module `_tensor_args`.
+// tensor_args.cpp — the Python binding's view of torch tensors, in C++: shape, type, device and layout of a tensor and its address in about a tenth of
+// a microsecond, and the parameter blocks of flb_kv8.h filled from them.  From Python every attribute of a tensor costs that much, and a decode call
+// names a dozen tensors: its host time would be that of three kernel launches (8-bit decode: 4.2 us from Python, 1.2 us from here).  Python
+// module `_tensor_args`.
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <climits>
+#include <cmath>
+#include <cstring>
+#include <string>
+
+#include "../../include/flb_kv8.h"
+
 namespace {
 
-// t, name, shape (tuple), dtype or None, device index or None -> tensor, or nullptr with the exception set
-const at::Tensor *checked(PyObject *const *a, Py_ssize_t n, const char *what) {
-    if (n != 5) {
-        PyErr_SetString(PyExc_TypeError, "expected (tensor, name, shape, dtype, device)");
-        return nullptr;
-    }
-    if (!THPVariable_Check(a[0])) {
-        PyErr_Format(PyExc_ValueError, "%U must be a torch tensor", a[1]);
-        return nullptr;
-    }
-    const at::Tensor &t = THPVariable_Unpack(a[0]);
-    if (a[4] != Py_None) {
-        const long dev = PyLong_AsLong(a[4]);
-        if (dev == -1 && PyErr_Occurred()) return nullptr;
-        if (t.get_device() != dev) {
-            PyErr_Format(PyExc_ValueError, "%U is on another device (%d) than the cache (%ld)", a[1], (int)t.get_device(), dev);
-            return nullptr;
-        }
-    }
-    bool ok = t.layout() == at::kStrided && (a[3] == Py_None || (THPDtype_Check(a[3]) && t.scalar_type() == reinterpret_cast<THPDtype *>(a[3])->scalar_type));
-    if (ok && PyTuple_Check(a[2])) {
-        ok = t.dim() == PyTuple_GET_SIZE(a[2]);
-        for (int64_t i = 0; ok && i < t.dim(); ++i) {
-            const long long want = PyLong_AsLongLong(PyTuple_GET_ITEM(a[2], i));
-            if (want == -1 && PyErr_Occurred()) return nullptr;
-            ok = t.size(i) == want;
-        }
-    } else {
-        ok = false;
-    }
-    if (!ok) {
-        PyErr_Format(PyExc_ValueError, "%U must be a %s %S tensor of shape %S", a[1], what, a[3], a[2]);
-        return nullptr;
-    }
-    return &t;
+struct Refused {}; // thrown with a Python exception set, caught where Python calls
+
+constexpr at::ScalarType kAnyType = at::ScalarType::Undefined;
+constexpr int kAnyDevice = INT_MIN;
+
+template <typename... A> [[noreturn]] void refuse(const char *format, A... a) {
+    PyErr_Format(PyExc_ValueError, format, a...);
+    throw Refused();
 }
 
-// Address of a dense tensor.
-PyObject *dense(PyObject *, PyObject *const *a, Py_ssize_t n) {
-    const at::Tensor *t = checked(a, n, "dense");
-    if (!t) return nullptr;
-    if (!t->is_contiguous()) return PyErr_Format(PyExc_ValueError, "%U must be a dense tensor", a[1]);
-    return PyLong_FromVoidPtr(t->data_ptr());
+const at::Tensor &tensor(PyObject *o, const char *name, int dev) {
+    if (!THPVariable_Check(o)) refuse("%s must be a torch tensor", name);
+    const at::Tensor &t = THPVariable_Unpack(o);
+    if (dev != kAnyDevice && t.get_device() != dev) refuse("%s is on another device (%d) than the cache (%d)", name, (int)t.get_device(), dev);
+    if (t.layout() != at::kStrided) refuse("%s must be a strided tensor", name);
+    return t;
 }
 
-// The same, 0 for None.
-PyObject *opt(PyObject *self, PyObject *const *a, Py_ssize_t n) {
+const at::Tensor &shaped(PyObject *o, const char *name, at::IntArrayRef shape, at::ScalarType type, int dev) {
+    const at::Tensor &t = tensor(o, name, dev);
+    if (t.sizes() != shape || (type != kAnyType && t.scalar_type() != type)) {
+        std::string want;
+        for (int64_t n : shape) want += (want.empty() ? "" : ",") + std::to_string(n);
+        refuse("%s must be a %s tensor of shape [%s]", name, type == kAnyType ? "dense" : c10::toString(type), want.c_str());
+    }
+    return t;
+}
+
+// address of a dense tensor
+void *dense(PyObject *o, const char *name, at::IntArrayRef shape, at::ScalarType type, int dev) {
+    const at::Tensor &t = shaped(o, name, shape, type, dev);
+    if (!t.is_contiguous()) refuse("%s must be a dense tensor", name);
+    return t.data_ptr();
+}
+template <typename P> P *opt(PyObject *o, const char *name, at::IntArrayRef shape, at::ScalarType type, int dev) {
+    return o == Py_None ? nullptr : static_cast<P *>(dense(o, name, shape, type, dev));
+}
+
+int as_int(int64_t n, const char *name) {
+    if (n < INT_MIN || n > INT_MAX) refuse("%s is out of range", name);
+    return (int)n;
+}
+int integer(PyObject *o, const char *name) {
+    const long long n = PyLong_AsLongLong(o);
+    if (n == -1 && PyErr_Occurred()) throw Refused();
+    return as_int(n, name);
+}
+float number(PyObject *o) {
+    const double x = PyFloat_AsDouble(o);
+    if (x == -1.0 && PyErr_Occurred()) throw Refused();
+    return (float)x;
+}
+
+// q, k or v [B,S,heads,d]: dense heads, one stride between tokens
+void *rows(PyObject *o, const char *name, at::IntArrayRef shape, at::ScalarType type, int dev, int64_t &row) {
+    const at::Tensor &t = shaped(o, name, shape, type, dev);
+    if (t.dim() != 4) refuse("%s must be [B,S,heads,d]", name);
+    const int64_t B = t.size(0), S = t.size(1), H = t.size(2), d = t.size(3);
+    row = H * d;
+    if (!t.is_contiguous()) {
+        row = S > 1 ? t.stride(1) : (B > 1 ? t.stride(0) : H * d);
+        if (t.stride(3) != 1 || (H > 1 && t.stride(2) != d) || (S > 1 && t.stride(1) != row) || (B > 1 && t.stride(0) != S * row) || row < H * d)
+            refuse("%s must be [B,S,heads,d] with unit element stride, head stride d and one stride between tokens", name);
+    }
+    return t.data_ptr();
+}
+// k and v of the tokens; their stride
+int kv_rows(PyObject *ko, PyObject *vo, at::IntArrayRef shape, at::ScalarType type, int dev, const void *&k, const void *&v) {
+    int64_t rk, rv;
+    k = rows(ko, "k", shape, type, dev, rk);
+    v = rows(vo, "v", shape, type, dev, rv);
+    if (rk != rv) refuse("k and v must share one token-row stride");
+    return as_int(rk, "the stride of k");
+}
+
+int input_mode(const at::Tensor &t) {
+    switch (t.scalar_type()) {
+    case at::kInt: return FLB_IN_INT32;
+    case at::kFloat: return FLB_IN_F32;
+    case at::kHalf: return FLB_IN_F16;
+    default: refuse("q, k and v must be int32, float32 or float16");
+    }
+}
+// activation scale of int32 inputs, one per token
+const float *act_scale(PyObject *o, int64_t tokens, int dev) {
+    if (o == Py_None) refuse("int32 inputs need act_scale and the weight scales");
+    const at::Tensor &t = tensor(o, "act_scale", dev);
+    if (t.numel() != tokens) refuse("act_scale must hold one value per token");
+    return static_cast<const float *>(dense(o, "act_scale", t.sizes(), at::kFloat, dev));
+}
+const float *w_scale(PyObject *o, const char *name, int64_t n, int dev) {
+    if (o == Py_None) refuse("int32 inputs need act_scale and the weight scales");
+    return static_cast<const float *>(dense(o, name, {n}, at::kFloat, dev));
+}
+const float *rope(PyObject *o, int64_t d, int dev, int &n) {
+    n = 0;
+    if (o == Py_None) return nullptr;
+    const at::Tensor &t = tensor(o, "freq_cis", dev);
+    if (t.dim() != 2 || t.size(0) == 0) refuse("freq_cis must have a row for every position");
+    n = as_int(t.size(0), "the length of freq_cis");
+    return static_cast<const float *>(dense(o, "freq_cis", {t.size(0), d}, at::kFloat, dev));
+}
+void *scratch(PyObject *o, int dev, size_t &bytes) {
+    bytes = 0;
+    if (o == Py_None) return nullptr;
+    const at::Tensor &t = tensor(o, "scratch", dev);
+    if (!t.is_contiguous()) refuse("scratch must be a dense tensor on the cache's device");
+    bytes = t.nbytes();
+    return t.data_ptr();
+}
+
+// k, v, k_scale, v_scale, row_pos -> the cache block; the index of its device (-1: host memory, for the checks alone)
+int cache_of(PyObject *const *a, flb_kv8_cache &c) {
+    const at::Tensor &k = tensor(a[0], "k", kAnyDevice), &ks = tensor(a[2], "k_scale", kAnyDevice);
+    const at::ScalarType type = k.scalar_type();
+    if (k.dim() != 4 || (type != at::kChar && type != at::kFloat8_e4m3fn)) refuse("cache codes must be int8 or float8_e4m3fn tensors [B,Hkv,T,d]");
+    const int dev = (int)k.get_device();
+    const int64_t B = k.size(0), H = k.size(1), T = k.size(2), n = ks.dim() ? ks.size(-1) : 0;
+    if (n <= 0 || T % n) refuse("cache scales must be [B,Hkv,T/block_len]");
+    c.batch_size = as_int(B, "the batch");
+    c.kv_head_num = as_int(H, "the number of heads");
+    c.size_per_head = as_int(k.size(3), "the head size");
+    c.total_len = as_int(T, "the cache's length");
+    c.block_len = as_int(T / n, "the block");
+    c.code_type = type == at::kChar ? FLB_KV8_I8 : FLB_KV8_E4M3;
+    c.k_codes = dense(a[0], "k", k.sizes(), type, dev);
+    c.v_codes = dense(a[1], "v", k.sizes(), type, dev);
+    c.k_scale = static_cast<float *>(dense(a[2], "k_scale", {B, H, n}, at::kFloat, dev));
+    c.v_scale = static_cast<float *>(dense(a[3], "v_scale", {B, H, n}, at::kFloat, dev));
+    c.row_pos = opt<int>(a[4], "row_pos", {B, H, T}, at::kInt, dev);
+    return dev;
+}
+
+// f(block) fills a parameter block and gives its device -> (bytes of the block, device)
+template <typename Block, int ARGS, typename F> PyObject *block(Py_ssize_t n, F fill) {
+    if (n != ARGS) return PyErr_Format(PyExc_TypeError, "expected %d arguments", ARGS);
+    Block p;
+    memset(&p, 0, sizeof p);
+    try {
+        const int dev = fill(p);
+        PyObject *bytes = PyBytes_FromStringAndSize(reinterpret_cast<const char *>(&p), sizeof p);
+        return bytes ? Py_BuildValue("(Ni)", bytes, dev) : nullptr;
+    } catch (const Refused &) {
+    } catch (const std::exception &e) {
+        PyErr_SetString(PyExc_RuntimeError, e.what());
+    }
+    return nullptr;
+}
+
+PyObject *kv8_append(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    return block<flb_kv8_append_params, 16>(n, [a](flb_kv8_append_params &p) {
+        const int dev = cache_of(a, p.cache);
+        const int64_t B = p.cache.batch_size, H = p.cache.kv_head_num, d = p.cache.size_per_head;
+        const at::Tensor &k = tensor(a[5], "k", dev);
+        if (k.dim() != 4) refuse("k must be [B,S,heads,d]");
+        const int64_t S = k.size(1);
+        p.seq_len = as_int(S, "the number of tokens");
+        p.input_mode = input_mode(k);
+        p.kv_row_stride = kv_rows(a[5], a[6], {B, S, H, d}, k.scalar_type(), dev, p.k, p.v);
+        p.start_pos = integer(a[7], "start_pos");
+        p.past_lens = opt<int>(a[8], "past_lens", {B}, at::kInt, dev);
+        p.new_lens = opt<int>(a[9], "new_lens", {B}, at::kInt, dev);
+        p.token_pos = opt<int>(a[10], "token_pos", {B}, at::kInt, dev);
+        if (p.input_mode == FLB_IN_INT32) {
+            p.act_scale = act_scale(a[11], B * S, dev);
+            p.k_w_scale = w_scale(a[12], "k_w_scale", H * d, dev);
+            p.v_w_scale = w_scale(a[13], "v_w_scale", H * d, dev);
+        }
+        p.freq_cis = rope(a[14], d, dev, p.freq_rows);
+        size_t bytes;
+        p.status = static_cast<unsigned *>(scratch(a[15], dev, bytes));
+        if (a[15] != Py_None && bytes < sizeof(unsigned)) refuse("scratch must hold the status word");
+        return dev;
+    });
+}
+
+PyObject *kv8_decode(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    return block<flb_kv8_decode_params, 27>(n, [a](flb_kv8_decode_params &p) {
+        const int dev = cache_of(a, p.cache);
+        const int64_t B = p.cache.batch_size, Hkv = p.cache.kv_head_num, T = p.cache.total_len, d = p.cache.size_per_head;
+        const at::Tensor &q = tensor(a[5], "q", dev), &out = tensor(a[8], "out", dev);
+        if (q.dim() != 4) refuse("q must be [B,1,heads,d]");
+        if (out.scalar_type() != at::kFloat && out.scalar_type() != at::kHalf) refuse("out must be float32 or float16");
+        const int64_t Hq = q.size(2);
+        int64_t row;
+        p.head_num = as_int(Hq, "the number of heads");
+        p.input_mode = input_mode(q);
+        p.q = rows(a[5], "q", {B, 1, Hq, d}, q.scalar_type(), dev, row);
+        p.q_row_stride = as_int(row, "the stride of q");
+        p.kv_row_stride = kv_rows(a[6], a[7], {B, 1, Hkv, d}, q.scalar_type(), dev, p.k, p.v);
+        p.out = dense(a[8], "out", {B, Hq, 1, d}, out.scalar_type(), dev);
+        p.out_dtype = out.scalar_type() == at::kFloat ? FLB_F32 : FLB_F16;
+        p.start_pos = integer(a[9], "start_pos");
+        p.past_lens = opt<int>(a[10], "past_lens", {B}, at::kInt, dev);
+        p.max_past_len = integer(a[11], "max_past_len");
+        p.token_pos = opt<int>(a[12], "token_pos", {B}, at::kInt, dev);
+        if (p.input_mode == FLB_IN_INT32) {
+            p.act_scale = act_scale(a[13], B, dev);
+            p.q_w_scale = w_scale(a[14], "q_w_scale", Hq * d, dev);
+            p.k_w_scale = w_scale(a[15], "k_w_scale", Hkv * d, dev);
+            p.v_w_scale = w_scale(a[16], "v_w_scale", Hkv * d, dev);
+        }
+        p.freq_cis = rope(a[17], d, dev, p.freq_rows);
+        p.softmax_scale = a[18] == Py_None ? (float)(1.0 / std::sqrt((double)d)) : number(a[18]);
+        p.softcap = number(a[19]);
+        p.alibi_slopes = opt<float>(a[20], "alibi_slopes", {Hq}, at::kFloat, dev);
+        p.key_begin = opt<int>(a[21], "key_begin", {B}, at::kInt, dev);
+        p.weight_in = opt<float>(a[22], "weight_in", {B, Hkv, T}, at::kFloat, dev);
+        p.weight_out = opt<float>(a[23], "weight_out", {B, Hkv, T}, at::kFloat, dev);
+        p.scratch = scratch(a[24], dev, p.scratch_bytes);
+        p.scratch_zeroed = PyObject_IsTrue(a[25]) == 1;
+        p.split_len = integer(a[26], "split_len");
+        return dev;
+    });
+}
+
+PyObject *kv8_evict(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    return block<flb_kv8_evict_params, 16>(n, [a](flb_kv8_evict_params &p) {
+        const int dev = cache_of(a, p.cache);
+        const int64_t B = p.cache.batch_size, H = p.cache.kv_head_num, T = p.cache.total_len;
+        p.start_pos = integer(a[5], "start_pos");
+        p.past_lens = opt<int>(a[6], "past_lens", {B}, at::kInt, dev);
+        p.len_out = static_cast<int *>(dense(a[7], "len_out", {B}, at::kInt, dev));
+        p.budget = integer(a[8], "budget");
+        p.recent = integer(a[9], "recent");
+        p.sinks = integer(a[10], "sinks");
+        p.next_pos = opt<int>(a[11], "next_pos", {B}, at::kInt, dev);
+        p.weight = static_cast<const float *>(dense(a[12], "weight", {B, H, T}, at::kFloat, dev));
+        p.weight_out = static_cast<float *>(dense(a[13], "weight_out", {B, H, T}, at::kFloat, dev));
+        p.pos_out = static_cast<int *>(dense(a[14], "pos_out", {B, H, T}, at::kInt, dev));
+        p.scratch = scratch(a[15], dev, p.scratch_bytes);
+        return dev;
+    });
+}
+
+// ---- single tensors, for blocks that Python fills: (tensor, name, shape, dtype or None, device index or None)
+template <typename F> PyObject *one(PyObject *const *a, Py_ssize_t n, F f) {
+    if (n != 5 || !PyUnicode_Check(a[1]) || !PyTuple_Check(a[2])) return PyErr_Format(PyExc_TypeError, "expected (tensor, name, shape, dtype, device)");
+    try {
+        c10::SmallVector<int64_t, 6> shape;
+        for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(a[2]); ++i) shape.push_back(integer(PyTuple_GET_ITEM(a[2], i), "a size"));
+        if (a[3] != Py_None && !THPDtype_Check(a[3])) refuse("%s: the type must be torch's", PyUnicode_AsUTF8(a[1]));
+        return f(PyUnicode_AsUTF8(a[1]), shape, a[3] == Py_None ? kAnyType : reinterpret_cast<THPDtype *>(a[3])->scalar_type,
+                 a[4] == Py_None ? kAnyDevice : integer(a[4], "the device"));
+    } catch (const Refused &) {
+    } catch (const std::exception &e) {
+        PyErr_SetString(PyExc_RuntimeError, e.what());
+    }
+    return nullptr;
+}
+PyObject *py_dense(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    return one(a, n, [&](const char *name, at::IntArrayRef shape, at::ScalarType type, int dev) { return PyLong_FromVoidPtr(dense(a[0], name, shape, type, dev)); });
+}
+PyObject *py_opt(PyObject *self, PyObject *const *a, Py_ssize_t n) {
     if (n > 0 && a[0] == Py_None) return PyLong_FromLong(0);
-    return dense(self, a, n);
+    return py_dense(self, a, n);
+}
+PyObject *py_rows(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    return one(a, n, [&](const char *name, at::IntArrayRef shape, at::ScalarType type, int dev) {
+        int64_t row;
+        void *p = rows(a[0], name, shape, type, dev, row);
+        return Py_BuildValue("(NL)", PyLong_FromVoidPtr(p), (long long)row);
+    });
 }
 
-// (address, elements between two tokens' rows) of q, k or v [B,S,heads,d]: dense heads, one stride between tokens.
-PyObject *rows(PyObject *, PyObject *const *a, Py_ssize_t n) {
-    const at::Tensor *t = checked(a, n, "token-row");
-    if (!t) return nullptr;
-    if (t->dim() != 4) return PyErr_Format(PyExc_ValueError, "%U must be [B,S,heads,d]", a[1]);
-    const int64_t B = t->size(0), S = t->size(1), H = t->size(2), d = t->size(3);
-    int64_t row = H * d;
-    if (!t->is_contiguous()) {
-        row = S > 1 ? t->stride(1) : (B > 1 ? t->stride(0) : H * d);
-        if (t->stride(3) != 1 || (H > 1 && t->stride(2) != d) || (S > 1 && t->stride(1) != row) || (B > 1 && t->stride(0) != S * row) || row < H * d)
-            return PyErr_Format(PyExc_ValueError, "%U must be [B,S,heads,d] with unit element stride, head stride d and one stride between tokens", a[1]);
-    }
-    return Py_BuildValue("(NL)", PyLong_FromVoidPtr(t->data_ptr()), (long long)row);
-}
+using Fast = PyObject *(*)(PyObject *, PyObject *const *, Py_ssize_t);
+PyCFunction fast(Fast f) { return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)); }
 
 PyMethodDef methods[] = {
-    {"dense", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(dense)), METH_FASTCALL, "address of a dense tensor"},
-    {"opt", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(opt)), METH_FASTCALL, "the same, 0 for None"},
-    {"rows", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rows)), METH_FASTCALL, "address and token-row stride"},
+    {"kv8_append", fast(kv8_append), METH_FASTCALL, "parameter block of an append, and its device"},
+    {"kv8_decode", fast(kv8_decode), METH_FASTCALL, "parameter block of a decode, and its device"},
+    {"kv8_evict", fast(kv8_evict), METH_FASTCALL, "parameter block of an eviction, and its device"},
+    {"dense", fast(py_dense), METH_FASTCALL, "address of a dense tensor"},
+    {"opt", fast(py_opt), METH_FASTCALL, "the same, 0 for None"},
+    {"rows", fast(py_rows), METH_FASTCALL, "address and token-row stride"},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensor_args", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -8,21 +8,15 @@ current stream unless one is given."""
 from __future__ import annotations
 
 import ctypes as C
-import math
 from dataclasses import dataclass
 from typing import Any
 
 import torch
 
 from . import _lib, _tensor_args
-from ._lib import FLB_F16, FLB_F32, FLB_IN_F16, FLB_IN_F32, FLB_IN_INT32  # noqa: F401
 
 FLB_KV8_I8, FLB_KV8_E4M3 = 0, 1
 STATUS_BAD_LEN, STATUS_BAD_POS = 4, 32
-
-_IN_MODE = {torch.int32: FLB_IN_INT32, torch.float32: FLB_IN_F32, torch.float16: FLB_IN_F16}
-_OUT = {torch.float32: FLB_F32, torch.float16: FLB_F16}
-_CODE = {torch.int8: FLB_KV8_I8, torch.float8_e4m3fn: FLB_KV8_E4M3}
 
 
 class FlbKv8Cache(C.Structure):
@@ -65,8 +59,6 @@ class FlbKv8Evict(C.Structure):
         ("pos_out", C.c_void_p), ("scratch", C.c_void_p), ("scratch_bytes", C.c_size_t),
     ]
 
-
-_PACK_APPEND, _PACK_DECODE, _PACK_EVICT = (_lib.packer(c) for c in (FlbKv8Append, FlbKv8Decode, FlbKv8Evict))
 
 # every symbol include/flb_kv8.h declares: name -> (restype, argtypes)
 _SIZE = C.POINTER(C.c_size_t)
@@ -139,62 +131,6 @@ def empty_cache(batch_size: int, kv_head_num: int, total_len: int, size_per_head
     return Cache(*codes, *scales, row_pos=pos)
 
 
-# (tensor, name, shape, dtype, device index) -> address of a dense tensor, 0 for None, (address, token-row stride) of q, k or v
-_dense, _opt, _rows = _tensor_args.dense, _tensor_args.opt, _tensor_args.rows
-
-
-def _cache(c: Cache) -> tuple:
-    """The values of a flb_kv8_cache, and the device's index (-1: host memory, for the checks alone)."""
-    k = c.k
-    code = _CODE.get(k.dtype)
-    if code is None or k.dim() != 4:
-        raise ValueError("cache codes must be int8 or float8_e4m3fn tensors [B,Hkv,T,d]")
-    shape = k.shape
-    B, H, T, d = shape
-    n = c.k_scale.shape[-1]
-    if n <= 0 or T % n:
-        raise ValueError("cache scales must be [B,Hkv,T/block_len]")
-    dev, scales = k.get_device(), (B, H, n)
-    return (B, H, d, T, T // n, code, _dense(k, "k", shape, k.dtype, dev), _dense(c.v, "v", shape, k.dtype, dev),
-            _dense(c.k_scale, "k_scale", scales, torch.float32, dev), _dense(c.v_scale, "v_scale", scales, torch.float32, dev),
-            _opt(c.row_pos, "row_pos", (B, H, T), torch.int32, dev)), dev
-
-
-def _kv_rows(k, v, shape, dtype, dev):
-    kp, ks = _rows(k, "k", shape, dtype, dev)
-    vp, vs = _rows(v, "v", shape, dtype, dev)
-    if ks != vs:
-        raise ValueError("k and v must share one token-row stride")
-    return kp, vp, ks
-
-
-def _scales(act, n, named, dev):
-    """Addresses of the activation scale (one per token) and of the weight scales (name, tensor, heads * d) of int32 inputs."""
-    if act is None or any(t is None for _, t, _ in named):
-        raise ValueError("int32 inputs need act_scale and the weight scales")
-    if act.numel() != n:
-        raise ValueError("act_scale must hold one value per token")
-    return [_dense(act, "act_scale", act.shape, torch.float32, dev)] + [_dense(t, name, (w,), torch.float32, dev) for name, t, w in named]
-
-
-def _rope(freq_cis, d, dev):
-    if freq_cis is None:
-        return 0, 0
-    n = freq_cis.shape[0]
-    if not n:
-        raise ValueError("freq_cis must have a row for every position")
-    return _dense(freq_cis, "freq_cis", (n, d), torch.float32, dev), n
-
-
-def _scratch(scratch, dev):
-    """Address and bytes."""
-    if scratch is None:
-        return 0, 0
-    if scratch.get_device() != dev or not scratch.is_contiguous():
-        raise ValueError("scratch must be a dense tensor on the cache's device")
-    return scratch.data_ptr(), scratch.nbytes
-
-
 def _call(fn, block: bytes, dev: int, stream) -> None:
     if dev < 0:
         raise ValueError("the 8-bit cache lives on a CUDA device")
@@ -210,25 +146,11 @@ def _call(fn, block: bytes, dev: int, stream) -> None:
         _lib.check(st)
 
 
-def _append_block(cache: Cache, k, v, *, start_pos: int = 0, past_lens=None, new_lens=None, token_pos=None, act_scale=None, k_w_scale=None,
+def _append_block(c: Cache, k, v, *, start_pos: int = 0, past_lens=None, new_lens=None, token_pos=None, act_scale=None, k_w_scale=None,
                   v_w_scale=None, freq_cis=None, scratch=None) -> tuple[bytes, int]:
-    c, dev = _cache(cache)
-    B, H, d = c[:3]
-    S, dt, lens = k.shape[1], k.dtype, (B,)
-    mode = _IN_MODE.get(dt)
-    if mode is None:
-        raise ValueError("k and v must be int32, float32 or float16")
-    kp, vp, row = _kv_rows(k, v, (B, S, H, d), dt, dev)
-    act = kw = vw = 0
-    if mode == FLB_IN_INT32:
-        act, kw, vw = _scales(act_scale, B * S, (("k_w_scale", k_w_scale, H * d), ("v_w_scale", v_w_scale, H * d)), dev)
-    i32 = torch.int32
-    word, size = _scratch(scratch, dev)
-    if scratch is not None and size < 4:
-        raise ValueError("scratch must hold the status word")
-    return _PACK_APPEND.pack(*c, S, start_pos, _opt(past_lens, "past_lens", lens, i32, dev), _opt(new_lens, "new_lens", lens, i32, dev),
-                             _opt(token_pos, "token_pos", lens, i32, dev), mode, kp, vp, row, act, kw, vw, *_rope(freq_cis, d, dev),
-                             word), dev
+    """The parameter block as bytes, and the index of the device (-1: host memory, for the checks alone)."""
+    return _tensor_args.kv8_append(c.k, c.v, c.k_scale, c.v_scale, c.row_pos, k, v, start_pos, past_lens, new_lens, token_pos, act_scale, k_w_scale,
+                                   v_w_scale, freq_cis, scratch)
 
 
 def append_params(cache: Cache, k, v, **kw) -> FlbKv8Append:
@@ -244,30 +166,13 @@ def append(cache: Cache, k, v, *, stream=None, **kw) -> None:
     _call(load_library().flb_kv8_append, *_append_block(cache, k, v, **kw), stream)
 
 
-def _decode_block(cache: Cache, q, k, v, out, *, start_pos: int = 0, past_lens=None, max_past_len: int = 0, token_pos=None, act_scale=None,
+def _decode_block(c: Cache, q, k, v, out, *, start_pos: int = 0, past_lens=None, max_past_len: int = 0, token_pos=None, act_scale=None,
                   q_w_scale=None, k_w_scale=None, v_w_scale=None, freq_cis=None, softmax_scale: float | None = None, softcap: float = 0.0,
                   alibi_slopes=None, key_begin=None, weight_in=None, weight_out=None, scratch=None, scratch_zeroed: bool = False,
                   split_len: int = 0) -> tuple[bytes, int]:
-    c, dev = _cache(cache)
-    B, Hkv, d, T = c[:4]
-    Hq, dt, lens = q.shape[2], q.dtype, (B,)
-    mode, od = _IN_MODE.get(dt), _OUT.get(out.dtype)
-    if mode is None or od is None:
-        raise ValueError("q, k and v must be int32, float32 or float16, out float32 or float16")
-    qp, qrow = _rows(q, "q", (B, 1, Hq, d), dt, dev)
-    kp, vp, row = _kv_rows(k, v, (B, 1, Hkv, d), dt, dev)
-    act = qw = kw = vw = 0
-    if mode == FLB_IN_INT32:
-        act, qw, kw, vw = _scales(act_scale, B, (("q_w_scale", q_w_scale, Hq * d), ("k_w_scale", k_w_scale, Hkv * d), ("v_w_scale", v_w_scale, Hkv * d)), dev)
-    i32, f32 = torch.int32, torch.float32
-    wi = wo = 0
-    if weight_in is not None or weight_out is not None:
-        wi, wo = _opt(weight_in, "weight_in", (B, Hkv, T), f32, dev), _opt(weight_out, "weight_out", (B, Hkv, T), f32, dev)
-    return _PACK_DECODE.pack(
-        *c, Hq, start_pos, _opt(past_lens, "past_lens", lens, i32, dev), max_past_len, _opt(token_pos, "token_pos", lens, i32, dev), mode, qp, kp, vp,
-        qrow, row, act, qw, kw, vw, *_rope(freq_cis, d, dev), softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(d), softcap,
-        _opt(alibi_slopes, "alibi_slopes", (Hq,), f32, dev), _opt(key_begin, "key_begin", lens, i32, dev), wi, wo,
-        _dense(out, "out", (B, Hq, 1, d), out.dtype, dev), od, *_scratch(scratch, dev), 1 if scratch_zeroed else 0, split_len), dev
+    return _tensor_args.kv8_decode(c.k, c.v, c.k_scale, c.v_scale, c.row_pos, q, k, v, out, start_pos, past_lens, max_past_len, token_pos, act_scale,
+                                   q_w_scale, k_w_scale, v_w_scale, freq_cis, softmax_scale, softcap, alibi_slopes, key_begin, weight_in, weight_out,
+                                   scratch, scratch_zeroed, split_len)
 
 
 def decode_params(cache: Cache, q, k, v, out, **kw) -> FlbKv8Decode:
@@ -284,18 +189,12 @@ def decode(cache: Cache, q, k, v, out, *, stream=None, **kw) -> None:
     _call(load_library().flb_kv8_decode, *_decode_block(cache, q, k, v, out, **kw), stream)
 
 
-def _evict_block(cache: Cache, *, len_out, budget: int, weight, start_pos: int = 0, past_lens=None, recent: int = 0, sinks: int = 0, next_pos=None,
+def _evict_block(c: Cache, *, len_out, budget: int, weight, start_pos: int = 0, past_lens=None, recent: int = 0, sinks: int = 0, next_pos=None,
                  weight_out=None, pos_out=None, scratch=None) -> tuple[bytes, int]:
-    if cache.row_pos is None:
+    if c.row_pos is None:
         raise ValueError("eviction needs a cache with row_pos")
-    c, dev = _cache(cache)
-    B, H, _, T = c[:4]
-    i32, f32, lens, rows = torch.int32, torch.float32, (B,), (B, H, T)
-    return _PACK_EVICT.pack(
-        *c, start_pos, _opt(past_lens, "past_lens", lens, i32, dev), _dense(len_out, "len_out", lens, i32, dev), budget, recent, sinks,
-        _opt(next_pos, "next_pos", lens, i32, dev), _dense(weight, "weight", rows, f32, dev),
-        _dense(weight if weight_out is None else weight_out, "weight_out", rows, f32, dev),
-        _dense(cache.row_pos if pos_out is None else pos_out, "pos_out", rows, i32, dev), *_scratch(scratch, dev)), dev
+    return _tensor_args.kv8_evict(c.k, c.v, c.k_scale, c.v_scale, c.row_pos, start_pos, past_lens, len_out, budget, recent, sinks, next_pos, weight,
+                                  weight if weight_out is None else weight_out, c.row_pos if pos_out is None else pos_out, scratch)
 
 
 def evict_params(cache: Cache, **kw) -> FlbKv8Evict:
