@@ -1,6 +1,7 @@
 // kv8_append.cu — fresh K/V rows into the 8-bit cache: dequantise, rotate (RoPE), one scale per block of rows and head.
 //
-// HBM-bound streaming pass: a token row and head costs 2 d (e_in + 1) bytes.  One CTA takes one block of rows of one head, K or V:
+// A streaming pass: a token row and head costs 2 d (e_in + 1) bytes.  Bound by instruction issue, about 150 per eight values at 2.9 a clock (8 x 32 heads of
+// 0-1024 fp16 tokens to int8: 32 us, 3.6 TB/s, 0.55 of the copy bandwidth).  One CTA takes one block of rows of one head, K or V:
 // block_len * d values, 32 per thread held in registers between the two halves of the work (largest magnitude, then
 // codes), so every value is read once.  Blocks of the K/V heads of the same tokens are neighbours in the grid: together
 // they read whole rows of the [B,S,Hkv,d] input.

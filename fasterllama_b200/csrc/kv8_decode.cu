@@ -1,7 +1,8 @@
 // kv8_decode.cu — single-token attention over the 8-bit cache, the new token's append included.
 //
 // For one K/V head and its G q heads:  x_r = c q.(code_r scale_r),  out = sum_r p_r code_r scale_r / sum_r p_r.
-// HBM-bound: 2 d bytes per cached row and K/V head, read once for all G heads.
+// HBM-bound: 2 d bytes per cached row and K/V head, read once for all G heads.  16 x 32 heads of 1024-2047 rows: 41 us, 4.9 TB/s; batches of 16, 32, 48 take
+// 9.5 us (launch, ramp, drain, joining) + bytes / 6.3 TB/s.
 //   * grid = K/V heads x splits of `split_len` rows; four warps per CTA, warp w takes the 16-row steps w, w + 4, ... of its
 //     split.  Every warp copies its own steps (cp.async, 16 bytes a lane) into a ring of its own in shared memory, three and more
 //     steps ahead: 192 KB per SM under way, no barrier between warps.  The first copies leave before q is looked at.
@@ -660,7 +661,7 @@ __global__ void __launch_bounds__(kWarps * 32, D == 128 ? (NT == 1 ? 4 : 3) : 1)
 constexpr int kHeadsAtOnce = 8;
 
 // weight_out = weight_in + sum over the group of 2^(score - max) / sum.  A thread takes four rows of one K/V head; HBM-bound, 4 (G + 2) bytes a
-// row and head (100001 rows, 8 heads of 4 q heads, from L2: 4 us).
+// row and head (100001 rows, 8 heads of 4 q heads, scores from L2: 7.6 us, 1.2 TB/s of scores and weights; latency).
 __global__ void __launch_bounds__(256) flb_kv8_weights_kernel(const __grid_constant__ Kv8DecodeArgs a, int blocks_per_unit) {
     const size_t unit = blockIdx.x / (unsigned)blocks_per_unit;
     const int r = ((int)(blockIdx.x % (unsigned)blocks_per_unit) * 256 + threadIdx.x) * 4;
