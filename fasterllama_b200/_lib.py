@@ -7,7 +7,6 @@ from __future__ import annotations
 
 import ctypes as C
 import os
-import struct
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(PKG_DIR, "libflb_attn.so")
@@ -136,28 +135,6 @@ EXPORTS = {
     "flb_attn_peer_exchange": (C.c_int, [C.POINTER(FlbPeerExchange), C.c_void_p]),
     "flb_attn_quantize": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p]),
 }
-
-_CODE_OF = {C.c_int: "i", C.c_uint: "I", C.c_float: "f", C.c_void_p: "P", C.c_size_t: "N"}
-
-
-def packer(cls) -> "struct.Struct":
-    """A struct.Struct that packs a parameter block from its fields' values in order (0 for a null pointer; nested blocks and arrays flat).
-    Filling a block of forty fields this way takes a microsecond, field by field through ctypes ten."""
-
-    def codes(c) -> str:
-        out = ""
-        for _, t in c._fields_:
-            if issubclass(t, C.Structure):
-                out += codes(t) + "0P"
-            elif issubclass(t, C.Array):
-                out += _CODE_OF[t._type_] * t._length_
-            else:
-                out += _CODE_OF[t]
-        return out
-
-    st = struct.Struct("@" + codes(cls) + "0P")
-    assert st.size == C.sizeof(cls), (cls, st.size, C.sizeof(cls))
-    return st
 
 
 _lib = None

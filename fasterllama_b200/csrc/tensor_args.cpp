@@ -1,8 +1,7 @@
 // tensor_args.cpp — the Python binding's view of torch tensors, in C++: shape, type, device and layout of a tensor and its address in about a tenth of
-// a microsecond, and the parameter blocks of flb_kv8.h filled from them.  From Python every attribute of a tensor costs that much, and a decode call
+// a microsecond, and the parameter blocks of flb_kv8.h and of scored attention calls filled from them.  From Python every attribute of a tensor costs that much, and a decode call
 // names a dozen tensors: its host time would be that of three kernel launches (8-bit decode: 4.2 us from Python, 1.2 us from here).  Python
 // module `_tensor_args`.
-#include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <climits>
@@ -10,6 +9,7 @@
 #include <cstring>
 #include <string>
 
+#include "../../include/flb_attn.h"
 #include "../../include/flb_kv8.h"
 
 namespace {
@@ -120,7 +120,7 @@ void *scratch(PyObject *o, int dev, size_t &bytes) {
     bytes = 0;
     if (o == Py_None) return nullptr;
     const at::Tensor &t = tensor(o, "scratch", dev);
-    if (!t.is_contiguous()) refuse("scratch must be a dense tensor on the cache's device");
+    if (!t.is_contiguous()) refuse("scratch must be a dense tensor");
     bytes = t.nbytes();
     return t.data_ptr();
 }
@@ -249,34 +249,77 @@ PyObject *kv8_evict(PyObject *, PyObject *const *a, Py_ssize_t n) {
     });
 }
 
-// ---- single tensors, for blocks that Python fills: (tensor, name, shape, dtype or None, device index or None)
-template <typename F> PyObject *one(PyObject *const *a, Py_ssize_t n, F f) {
-    if (n != 5 || !PyUnicode_Check(a[1]) || !PyTuple_Check(a[2])) return PyErr_Format(PyExc_TypeError, "expected (tensor, name, shape, dtype, device)");
-    try {
-        c10::SmallVector<int64_t, 6> shape;
-        for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(a[2]); ++i) shape.push_back(integer(PyTuple_GET_ITEM(a[2], i), "a size"));
-        if (a[3] != Py_None && !THPDtype_Check(a[3])) refuse("%s: the type must be torch's", PyUnicode_AsUTF8(a[1]));
-        return f(PyUnicode_AsUTF8(a[1]), shape, a[3] == Py_None ? kAnyType : reinterpret_cast<THPDtype *>(a[3])->scalar_type,
-                 a[4] == Py_None ? kAnyDevice : integer(a[4], "the device"));
-    } catch (const Refused &) {
-    } catch (const std::exception &e) {
-        PyErr_SetString(PyExc_RuntimeError, e.what());
-    }
-    return nullptr;
+// A tensor of which only type and layout are known here; null for None
+template <typename P> P *loose(PyObject *o, const char *name, at::ScalarType type) {
+    if (o == Py_None) return nullptr;
+    const at::Tensor &t = tensor(o, name, kAnyDevice);
+    if (t.scalar_type() != type || !t.is_contiguous()) refuse("%s must be a dense %s tensor", name, c10::toString(type));
+    return static_cast<P *>(t.data_ptr());
 }
-PyObject *py_dense(PyObject *, PyObject *const *a, Py_ssize_t n) {
-    return one(a, n, [&](const char *name, at::IntArrayRef shape, at::ScalarType type, int dev) { return PyLong_FromVoidPtr(dense(a[0], name, shape, type, dev)); });
+int dtype_of(const at::Tensor &t) {
+    if (t.scalar_type() != at::kFloat && t.scalar_type() != at::kHalf) refuse("caches and out must be float32 or float16");
+    return t.scalar_type() == at::kFloat ? FLB_F32 : FLB_F16;
 }
-PyObject *py_opt(PyObject *self, PyObject *const *a, Py_ssize_t n) {
-    if (n > 0 && a[0] == Py_None) return PyLong_FromLong(0);
-    return py_dense(self, a, n);
-}
-PyObject *py_rows(PyObject *, PyObject *const *a, Py_ssize_t n) {
-    return one(a, n, [&](const char *name, at::IntArrayRef shape, at::ScalarType type, int dev) {
+
+// The blocks of flb_attn.h with a score form.  Devices are not compared: the inputs of a decode may lie in pinned host memory.
+PyObject *scored(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    flb_score_form f;
+    memset(&f, 0, sizeof f);
+    PyObject *first = block<flb_attn_params, 30>(n, [a, &f](flb_attn_params &p) {
+        const at::Tensor &q = tensor(a[0], "q", kAnyDevice), &k = tensor(a[1], "k", kAnyDevice), &kc = tensor(a[3], "k_cache", kAnyDevice), &out = tensor(a[5], "out", kAnyDevice);
+        if (q.dim() != 4 || k.dim() != 4 || kc.dim() != 4) refuse("q and k must be [B,S,heads,d], k_cache [B,Hkv,T,d]");
+        const int64_t B = q.size(0), S = q.size(1), H = q.size(2), d = q.size(3), Hkv = k.size(2), T = kc.size(2);
+        if (Hkv <= 0 || H % Hkv) refuse("the number of K/V heads must divide that of the q heads");
+        p.batch_size = as_int(B, "the batch");
+        p.head_num = as_int(H, "the number of heads");
+        p.size_per_head = as_int(d, "the head size");
+        p.seq_len = as_int(S, "the number of tokens");
+        p.total_len = as_int(T, "the cache's length");
+        p.input_mode = input_mode(q);
         int64_t row;
-        void *p = rows(a[0], name, shape, type, dev, row);
-        return Py_BuildValue("(NL)", PyLong_FromVoidPtr(p), (long long)row);
+        p.q = rows(a[0], "q", q.sizes(), q.scalar_type(), kAnyDevice, row);
+        p.qkv_row_stride = row == H * d ? 0 : as_int(row, "the stride of q");
+        f.kv_head_num = as_int(Hkv, "the number of K/V heads");
+        f.kv_row_stride = kv_rows(a[1], a[2], {B, S, Hkv, d}, q.scalar_type(), kAnyDevice, p.k, p.v);
+        p.cache_dtype = dtype_of(kc);
+        p.k_cache = dense(a[3], "k_cache", {B, Hkv, T, d}, kc.scalar_type(), kAnyDevice);
+        p.v_cache = dense(a[4], "v_cache", {B, Hkv, T, d}, kc.scalar_type(), kAnyDevice);
+        p.out_dtype = dtype_of(out);
+        p.out = dense(a[5], "out", {B, H, S, d}, out.scalar_type(), kAnyDevice);
+        f.softcap = number(a[6]);
+        f.alibi_slopes = opt<float>(a[7], "alibi_slopes", {H}, at::kFloat, kAnyDevice);
+        const int64_t bounds[2] = {B, S};
+        const at::IntArrayRef bound_shape(bounds, S == 1 ? 1 : 2);
+        f.key_begin = opt<int>(a[8], "key_begin", bound_shape, at::kInt, kAnyDevice);
+        f.key_end = opt<int>(a[9], "key_end", bound_shape, at::kInt, kAnyDevice);
+        p.scratch = scratch(a[10], kAnyDevice, p.scratch_bytes);
+        p.start_pos = integer(a[11], "start_pos");
+        p.past_lens = opt<int>(a[12], "past_lens", {B}, at::kInt, kAnyDevice);
+        p.max_past_len = integer(a[13], "max_past_len");
+        p.act_scale = loose<float>(a[14], "act_scale", at::kFloat);
+        p.q_w_scale = loose<float>(a[15], "q_w_scale", at::kFloat);
+        p.k_w_scale = loose<float>(a[16], "k_w_scale", at::kFloat);
+        p.v_w_scale = loose<float>(a[17], "v_w_scale", at::kFloat);
+        p.freq_cis = loose<float>(a[18], "freq_cis", at::kFloat);
+        p.rope_pos0 = integer(a[19], "rope_pos0");
+        p.rope_add_past = PyObject_IsTrue(a[20]) == 1;
+        p.mask_mode = integer(a[21], "mask_mode");
+        p.attn_mask = loose<float>(a[22], "attn_mask", at::kFloat);
+        p.mask_row_stride = integer(a[23], "mask_row_stride");
+        if (p.attn_mask && !p.mask_row_stride) p.mask_row_stride = as_int(THPVariable_Unpack(a[22]).size(-1), "the mask's row");
+        p.softmax_scale = a[24] == Py_None ? (float)(1.0 / std::sqrt((double)d)) : number(a[24]);
+        p.scratch_zeroed = PyObject_IsTrue(a[25]) == 1;
+        p.split_len = integer(a[26], "split_len");
+        p.out_q8 = loose<int8_t>(a[27], "out_q8", at::kChar);
+        p.out_q8_scale = loose<float>(a[28], "out_q8_scale", at::kFloat);
+        p.early_start = integer(a[29], "early_start");
+        return 0;
     });
+    if (!first) return nullptr;
+    PyObject *p = PyTuple_GET_ITEM(first, 0), *bytes = PyBytes_FromStringAndSize(reinterpret_cast<const char *>(&f), sizeof f);
+    PyObject *both = bytes ? Py_BuildValue("(ON)", p, bytes) : nullptr;
+    Py_DECREF(first);
+    return both;
 }
 
 using Fast = PyObject *(*)(PyObject *, PyObject *const *, Py_ssize_t);
@@ -286,9 +329,7 @@ PyMethodDef methods[] = {
     {"kv8_append", fast(kv8_append), METH_FASTCALL, "parameter block of an append, and its device"},
     {"kv8_decode", fast(kv8_decode), METH_FASTCALL, "parameter block of a decode, and its device"},
     {"kv8_evict", fast(kv8_evict), METH_FASTCALL, "parameter block of an eviction, and its device"},
-    {"dense", fast(py_dense), METH_FASTCALL, "address of a dense tensor"},
-    {"opt", fast(py_opt), METH_FASTCALL, "the same, 0 for None"},
-    {"rows", fast(py_rows), METH_FASTCALL, "address and token-row stride"},
+    {"scored", fast(scored), METH_FASTCALL, "parameter block and score form of an attention call"},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensor_args", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

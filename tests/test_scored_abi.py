@@ -3,6 +3,7 @@ import ctypes as C
 
 import numpy as np
 import pytest
+import torch
 
 from fasterllama_b200 import _lib
 from fasterllama_b200 import attention as A
@@ -72,6 +73,37 @@ def test_key_bounds_of_a_prefill_need_their_scratch():
     assert A.validate_scored(p, f) == _lib.FLB_OK
     p.scratch_bytes = A.scored_workspace_bytes(p, None)
     assert A.validate_scored(p, f) == _lib.FLB_ERR_SCRATCH_TOO_SMALL
+
+
+@pytest.mark.parametrize("S", [1, 6])
+def test_tensors_and_arrays_fill_the_same_blocks(S):
+    B, H, T, d = 2, 8, 64, 128
+    kw = dict(alibi_slopes=np.ones(H, np.float32), key_begin=np.zeros((B,) if S == 1 else (B, S), np.int32), freq_cis=np.zeros((T, d), np.float32), softcap=7.5,
+              past_lens=np.zeros(B, np.int32), max_past_len=33, rope_pos0=2, rope_add_past=True, mask_mode=A.FLB_MASK_GENERIC, attn_mask=np.zeros((T, T), np.float32),
+              scratch_zeroed=True, split_len=256, early_start=1, start_pos=3, act_scale=np.ones(B * S, np.float32), out_q8=np.zeros((B, S, H * d), np.int8),
+              out_q8_scale=np.zeros(B * S, np.float32))
+    merged = np.zeros((B, S, (H + 4 + 4) * d), np.float16)  # q, k and v as columns of one projection
+    for name, at, heads in (("q", 0, H), ("k", H, 4), ("v", H + 4, 4)):
+        kw[name] = np.lib.stride_tricks.as_strided(merged[:, :, at * d:], (B, S, heads, d), (merged.strides[0], merged.strides[1], 2 * d, 2))
+    p, f, arrays = _call(S=S, T=T, **kw)
+    pt, ft = A.make_scored_params(**{n: torch.from_numpy(x) if isinstance(x, np.ndarray) else x for n, x in arrays.items()})
+    assert bytes(p) == bytes(pt) and bytes(f) == bytes(ft)
+    assert p.qkv_row_stride == 16 * d == f.kv_row_stride and f.kv_head_num == 4
+
+
+def test_tensors_are_refused_like_arrays():
+    def t(**kw):
+        a = dict(q=torch.zeros(2, 1, 8, 128), k=torch.zeros(2, 1, 4, 128), v=torch.zeros(2, 1, 4, 128), k_cache=torch.zeros(2, 4, 64, 128), v_cache=torch.zeros(2, 4, 64, 128),
+                 out=torch.zeros(2, 8, 1, 128), scratch=torch.zeros(1 << 20, dtype=torch.uint8))
+        return A.make_scored_params(**{**a, **kw})
+
+    assert A.validate_scored(*t()) == _lib.FLB_OK
+    for bad in (dict(alibi_slopes=torch.zeros(7)), dict(key_begin=torch.zeros(3, dtype=torch.int32)), dict(key_begin=torch.zeros(2, dtype=torch.int64)), dict(k=torch.zeros(2, 1, 3, 128)),
+                dict(v=torch.zeros(2, 1, 4, 128).half()), dict(k_cache=torch.zeros(2, 8, 64, 128)), dict(k_cache=torch.zeros(2, 4, 64, 256)[..., ::2]), dict(q=torch.zeros(2, 8, 128)),
+                dict(out=torch.zeros(2, 8, 1, 128, dtype=torch.bfloat16)), dict(freq_cis=torch.zeros(64, 128).double()), dict(freq_cis=torch.zeros(128, 64).T), dict(q=np.zeros(3)),
+                dict(start_pos=1 << 40), dict(act_scale="x")):
+        with pytest.raises((ValueError, AttributeError, IndexError)):
+            t(**bad)
 
 
 def test_binding_refuses_shapes_and_types():
