@@ -66,6 +66,11 @@ float number(PyObject *o) {
     if (x == -1.0 && PyErr_Occurred()) throw Refused();
     return (float)x;
 }
+int truth(PyObject *o) {
+    const int x = PyObject_IsTrue(o);
+    if (x < 0) throw Refused();
+    return x;
+}
 
 // q, k or v [B,S,heads,d]: dense heads, one stride between tokens
 void *rows(PyObject *o, const char *name, at::IntArrayRef shape, at::ScalarType type, int dev, int64_t &row) {
@@ -224,7 +229,7 @@ PyObject *kv8_decode(PyObject *, PyObject *const *a, Py_ssize_t n) {
         p.weight_in = opt<float>(a[22], "weight_in", {B, Hkv, T}, at::kFloat, dev);
         p.weight_out = opt<float>(a[23], "weight_out", {B, Hkv, T}, at::kFloat, dev);
         p.scratch = scratch(a[24], dev, p.scratch_bytes);
-        p.scratch_zeroed = PyObject_IsTrue(a[25]) == 1;
+        p.scratch_zeroed = truth(a[25]);
         p.split_len = integer(a[26], "split_len");
         return dev;
     });
@@ -302,13 +307,13 @@ PyObject *scored(PyObject *, PyObject *const *a, Py_ssize_t n) {
         p.v_w_scale = loose<float>(a[17], "v_w_scale", at::kFloat);
         p.freq_cis = loose<float>(a[18], "freq_cis", at::kFloat);
         p.rope_pos0 = integer(a[19], "rope_pos0");
-        p.rope_add_past = PyObject_IsTrue(a[20]) == 1;
+        p.rope_add_past = truth(a[20]);
         p.mask_mode = integer(a[21], "mask_mode");
         p.attn_mask = loose<float>(a[22], "attn_mask", at::kFloat);
         p.mask_row_stride = integer(a[23], "mask_row_stride");
         if (p.attn_mask && !p.mask_row_stride) p.mask_row_stride = as_int(THPVariable_Unpack(a[22]).size(-1), "the mask's row");
         p.softmax_scale = a[24] == Py_None ? (float)(1.0 / std::sqrt((double)d)) : number(a[24]);
-        p.scratch_zeroed = PyObject_IsTrue(a[25]) == 1;
+        p.scratch_zeroed = truth(a[25]);
         p.split_len = integer(a[26], "split_len");
         p.out_q8 = loose<int8_t>(a[27], "out_q8", at::kChar);
         p.out_q8_scale = loose<float>(a[28], "out_q8_scale", at::kFloat);

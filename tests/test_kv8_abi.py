@@ -186,6 +186,16 @@ def test_binding_refuses_shapes_types_and_hosts():
         kv8.append_params(bad, k, k.clone())
 
 
+def test_binding_passes_on_what_python_raises():
+    c = _cache()
+    q = torch.zeros(2, 1, 4, 128, dtype=torch.float16)
+    out = torch.zeros(2, 4, 1, 128)
+    for bad in (dict(scratch_zeroed=torch.zeros(2)), dict(softcap="1"), dict(split_len=1.5), dict(start_pos=1 << 40), dict(max_past_len=None), dict(past_lens=[1, 2])):
+        with pytest.raises((TypeError, ValueError, RuntimeError)):
+            kv8.decode_params(c, q, q.clone(), q.clone(), out, **bad)
+    kv8.decode_params(c, q, q.clone(), q.clone(), out)  # and nothing of it stays behind
+
+
 def test_merged_projection_columns_share_a_stride():
     c = _cache()
     buf = torch.zeros(2, 3, (8 + 4 + 4) * 128, dtype=torch.float16)
