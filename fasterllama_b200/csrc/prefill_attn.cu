@@ -116,7 +116,7 @@ struct PrefillArgs {
     int Hkv, G;        // K/V heads, q heads per K/V head
     int kv_row_stride; // of k and v
     float cap_log2e, cap_in; // softcap * log2(e); what a raw score is multiplied by to become the tanh's argument
-    float cap_c[3];           // polynomial of the capped score over the raw one, in the raw one's square, highest power first
+    float cap_c[3];           // the cap's polynomial, highest power first (see cap_chunk and chunk_exp_cap)
     int backwards;            // key tiles from the last to the first
     const float *slopes;
     const int *key_begin, *key_end; // [B,S]
@@ -466,17 +466,22 @@ __device__ __forceinline__ uint32_t bit_range(int lo, int hi) {
 // the weight) on packed FMAs; it costs no special-function result, of which the exponentials already take half the pipe.
 constexpr float kTanhPoly[3] = {0.11942387f, -0.33225426f, 0.99997884f}; // u^4, u^2, 1
 constexpr float kTanhReach = 0.4f;
-constexpr float kTiny = 1.1754944e-38f; // smallest normal number: the leading coefficient stays positive however large the cap
+constexpr float kTiny = 1.1754944e-38f; // smallest normal number
+// Where the cap goes into the exponent's argument (chunk_exp_cap) a hidden key is an infinite raw score and needs a leading coefficient above 0.  For
+// finished scores that is kTiny, and kTiny x^4 vanishes beside 1 up to this: larger caps, and coefficients that are no normal numbers, take the
+// kernel that caps before it hides.
+constexpr float kMaxCapInExp = 33554432.f; // 2^25, in units of log2
 __device__ __forceinline__ float chunk_abs_max(const uint32_t (&r)[32]) {
     float big = 0.f;
 #pragma unroll
     for (int i = 0; i < 32; i += 2) big = max3(big, fabsf(__uint_as_float(r[i])), fabsf(__uint_as_float(r[i + 1])));
     return big;
 }
+// (a.cap_c: the polynomial in u^2 times the cap.  Powers of cap_in in the coefficients would save a multiplication and underflow for large caps.)
 __device__ __forceinline__ void cap_chunk(uint32_t (&r)[32], const PrefillArgs &a) {
 #pragma unroll
     for (int i = 0; i < 32; i += 2) {
-        const float2 x = make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), y = __fmul2_rn(x, x);
+        const float2 x = __fmul2_rn(make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), make_float2(a.cap_in, a.cap_in)), y = __fmul2_rn(x, x);
         float2 p = __ffma2_rn(y, make_float2(a.cap_c[0], a.cap_c[0]), make_float2(a.cap_c[1], a.cap_c[1]));
         p = __ffma2_rn(p, y, make_float2(a.cap_c[2], a.cap_c[2]));
         p = __fmul2_rn(p, x);
@@ -542,7 +547,7 @@ __device__ __forceinline__ void chunk_exp(const uint32_t (&r)[32], float scale, 
 }
 
 // The same on raw scores whose cap goes into the exponent's argument: the polynomial's last multiplication and the subtraction of the maximum
-// are one operation.  c[0] > 0, so that a hidden key's -inf comes out as -inf.
+// are one operation.  k: the polynomial in the raw score's square, cap and powers of cap_in in its coefficients.  k[0] > 0, so that a hidden key's -inf comes out as -inf.
 __device__ __forceinline__ void chunk_exp_cap(const uint32_t (&r)[32], const float (&k)[3], float neg_m, float2 &l2, uint32_t (&packed)[16]) {
 #pragma unroll
     for (int i = 0; i < 32; i += 2) {
@@ -1004,7 +1009,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                             tmem_ld32(ts, ra);
                             tmem_ld32(ts + 32, rb);
                             tmem_wait_ld(ra, rb);
-                            kc[0] = kTiny; // x = x for every finite score
+                            kc[0] = kTiny; // x = x for every score up to kMaxCapInExp
                             kc[1] = 0.f;
                             kc[2] = 1.f;
                         } else if (!CAP_IN_EXP) {
@@ -1303,7 +1308,9 @@ template <int D> int launch_prefill_hd(const flb_attn_params *p, const flb_score
         for (int k = 0; k < 5 - 2 * i; ++k) c *= a.cap_in;
         a.cap_c[i] = (float)c;
     }
-    if (a.cap_c[0] < kTiny) a.cap_c[0] = kTiny;
+    const bool cap = a.cap_log2e > 0.f, cap_in_exp = cap && !a.slopes && p->mask_mode != FLB_MASK_GENERIC && a.cap_log2e <= kMaxCapInExp && a.cap_c[0] >= kTiny;
+    if (!cap_in_exp)
+        for (int i = 0; i < 3; ++i) a.cap_c[i] = kTanhPoly[i] * a.cap_log2e;
     // A distance bias grows towards the diagonal: from the last tile to the first a row's maximum is found at once, the other way round it
     // passes the rescaling threshold at nearly every tile (4001 tokens, 32 heads: 225 us forwards, 186 us backwards).
     a.backwards = a.slopes != nullptr;
@@ -1366,7 +1373,7 @@ template <int D> int launch_prefill_hd(const flb_attn_params *p, const flb_score
     pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     pdl[0].val.programmaticStreamSerializationAllowed = 1;
     const bool generic_mask = (a.mask_mode == FLB_MASK_GENERIC);
-    const int form = scored ? kFormBounds | (a.cap_log2e > 0.f ? kFormCap : 0) | (a.slopes ? kFormBias : 0) : 0;
+    const int form = scored ? kFormBounds | (cap ? kFormCap : 0) | (a.slopes || (cap && !cap_in_exp) ? kFormBias : 0) : 0;
     auto kern = attn_kernel_of<D>(generic_mask, a.out_f16, form);
     constexpr size_t smem_bytes = prefill_smem(D);
     // the shared-memory opt-in is a property of (kernel, device): set once per device, not on every call

@@ -360,3 +360,60 @@ def test_scored_prefill_and_decode_in_a_graph(cuda_device):
     graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(x, y) for x, y in zip(want, (o, o1, kc)))
+
+
+# ------------------------------------------------------------------------------------------------ large caps and scores
+def two_keys(less, *, cap, scale, mask_b=0.0, alibi=False, d=64):
+    """One query row whose keys have raw scores of 0 but for key 3 (2^30) and key 9 (2^30 - less * 181; less = None: 0); the other rows see
+    nothing -> the weight of key 9.  mask_b: an additive mask lets the row see these two only and adds this to the second's score."""
+    S, row = 70, 66
+    q, k, v = (torch.zeros(1, S, 1, d, dtype=torch.float16, device=DEV) for _ in range(3))
+    q[0, row, 0, 0], q[0, row, 0, 1] = 32768.0, 181.0
+    k[0, 3, 0, 0] = 32768.0
+    if less is not None:
+        k[0, 9, 0, 0], k[0, 9, 0, 1] = 32768.0, -float(less)
+    v[0, 9] = 1.0
+    begin = torch.full((1, S), S, dtype=torch.int32, device=DEV)
+    begin[0, row] = 0
+    mask = None
+    if mask_b:
+        mask = torch.full((S, S), -torch.finfo(torch.float32).max, device=DEV)
+        mask[row, 3], mask[row, 9] = 0.0, mask_b
+    kc, vc = (torch.zeros(1, 1, S, d, dtype=torch.float16, device=DEV) for _ in range(2))
+    o = torch.empty(1, 1, S, d, device=DEV)
+    scratch = torch.zeros(A.workspace_bytes(1, 1, S, S, size_per_head=d) + 65536, dtype=torch.uint8, device=DEV)
+    p, f = A.make_scored_params(q=q, k=k, v=v, k_cache=kc, v_cache=vc, out=o, scratch=scratch, softcap=cap, softmax_scale=scale, key_begin=begin,
+                                mask_mode=A.FLB_MASK_NONE if mask is None else A.FLB_MASK_GENERIC, attn_mask=mask,
+                                alibi_slopes=torch.full((1,), 2.0 ** -20, device=DEV) if alibi else None)
+    A.forward_scored(p, f)
+    torch.cuda.synchronize()
+    assert A.scratch_status(scratch) == 0
+    assert float(o[0, 0, :row].abs().max()) == 0
+    return float(o[0, 0, row, 5])
+
+
+@pytest.mark.parametrize("alibi", [False, True])
+@pytest.mark.parametrize("log_cap", [18, 20, 24, 25, 28, 30, 40])
+def test_prefill_large_caps_keep_the_distance_of_large_scores(cuda_device, log_cap, alibi):
+    """Raw scores of 2^30 and 181^2 less, 65536 and 2 less after the scale, below a quarter of the cap.  Tolerance: a score of 2^16.5 in units of log2 is rounded to 2^-8
+    at each of five operations on either side and the fit's error changes the difference by less than 2^-10 of it, so the exponent is off by at most 0.03."""
+    raw, scale, cap = 2.0 ** 30, 2.0 ** -14, 2.0 ** log_cap
+    gap = cap * (math.tanh(raw * scale / cap) - math.tanh((raw - 181.0 ** 2) * scale / cap)) - (6 * 2.0 ** -20 if alibi else 0.0)
+    got = two_keys(181, cap=cap, scale=scale, alibi=alibi)
+    assert 0 < got < 1
+    assert abs(math.log(got / (1 - got)) + gap) <= 0.03 + 2.0 ** -9, (got, gap)  # (weights are fp16)
+
+
+@pytest.mark.parametrize("log_cap", [28, 30, 35, 40])
+def test_prefill_large_capped_scores_against_a_mask(cuda_device, log_cap):
+    """A raw score of 2^30 comes to 8.7e7 (or what the cap leaves of it), and loses to a mask that lifts the other key 4 % above it."""
+    scale, cap = 0.08125, 2.0 ** log_cap
+    x = cap * math.tanh(2.0 ** 30 * scale / cap)
+    assert two_keys(None, cap=cap, scale=scale, mask_b=1.04 * x) == 1.0
+    assert two_keys(None, cap=cap, scale=scale, mask_b=0.96 * x) == 0.0
+
+
+@pytest.mark.parametrize("log_cap", [20, 28, 40])
+def test_prefill_saturated_caps_share_the_weight(cuda_device, log_cap):
+    """Two scores far beyond the cap are both the cap."""
+    assert two_keys(0, cap=2.0 ** log_cap, scale=2.0 ** (log_cap - 26)) == pytest.approx(0.5, abs=2.0 ** -11)
