@@ -7,6 +7,7 @@
 // they read whole rows of the [B,S,Hkv,d] input.
 #include "kv8.cuh"
 
+#include <climits>
 #include <type_traits>
 
 namespace flb {
@@ -35,7 +36,7 @@ template <int D, int CODE, int MODE> __global__ void __launch_bounds__(1024) flb
     const size_t unit = (size_t)b * a.c.H + h;
     uint8_t *codes = a.c.codes[kv] + (unit * a.c.T + row0) * D;
     float *scale_p = a.c.scale[kv] + unit * a.c.nblk + blk;
-    const int pos0 = (a.token_pos ? __ldg(a.token_pos + b) : past) - past; // position = row + pos0
+    const long long pos_lo = (a.token_pos ? __ldg(a.token_pos + b) : past) + (long long)(lo - past); // position of row lo: any int, and the tokens behind it further
 
     const int col = (int)(threadIdx.x % CPR) * 8, step = (int)(blockDim.x / CPR), r0 = row0 + (int)(threadIdx.x / CPR); // rows r0, r0 + step, ...
     // All loads first: the rows, then the table's.  What is not a new row of this block is read as the nearest that is, and not used.  FULL: every
@@ -46,15 +47,15 @@ template <int D, int CODE, int MODE> __global__ void __launch_bounds__(1024) flb
         Kv8Raw raw[kChunks];
         float4 f0[kChunks], f1[kChunks];
         const bool turn = kv == 0 && a.freq_cis;
-        const int tab0 = pos0, tab1 = a.freq_rows - 1;
-        if (turn && threadIdx.x == 0 && (lo + tab0 < 0 || hi - 1 + tab0 > tab1) && a.status) atomicOr(a.status, kKv8BadPos);
+        const int tab1 = a.freq_rows - 1, tab_lo = (int)min(max(pos_lo, -128ll), INT_MAX - 128ll); // (a block holds 128 rows or fewer)
+        if (turn && threadIdx.x == 0 && (pos_lo < 0 || pos_lo + (hi - 1 - lo) > tab1) && a.status) atomicOr(a.status, kKv8BadPos);
         const size_t tok0 = (size_t)b * a.S + (lo - past);
 #pragma unroll
         for (int i = 0; i < kChunks; ++i) {
             const int row = row_of(i);
             raw[i] = kv8_raw8<MODE>(a.in[kv], tok0 + (row - lo), h * D + col);
             if (turn) {
-                const float4 *f = reinterpret_cast<const float4 *>(a.freq_cis + (size_t)min(max(row + tab0, 0), tab1) * D + col);
+                const float4 *f = reinterpret_cast<const float4 *>(a.freq_cis + (size_t)min(max(tab_lo + (row - lo), 0), tab1) * D + col);
                 f0[i] = __ldg(f);
                 f1[i] = __ldg(f + 1);
             }
@@ -89,7 +90,7 @@ template <int D, int CODE, int MODE> __global__ void __launch_bounds__(1024) flb
     else
         work(std::false_type());
     if (kv == 0 && a.c.row_pos)
-        for (int r = lo + (int)threadIdx.x; r < hi; r += blockDim.x) a.c.row_pos[unit * a.c.T + r] = r + pos0;
+        for (int r = lo + (int)threadIdx.x; r < hi; r += blockDim.x) a.c.row_pos[unit * a.c.T + r] = (int)min(pos_lo + (r - lo), (long long)INT_MAX);
 }
 
 template <int D, int CODE> cudaError_t launch_t(const Kv8AppendArgs &a, int input_mode, cudaStream_t stream) {

@@ -55,7 +55,8 @@ typedef struct flb_kv8_append_params {
     const int *past_lens;   /* device int[B] or NULL                                    */
     const int *new_lens;    /* device int[B] or NULL: tokens of sequence b that count (0..S; the rest of a padded
                                batch is not stored); NULL = S                            */
-    const int *token_pos;   /* device int[B] or NULL: position of the first new token; NULL = the cached rows */
+    const int *token_pos;   /* device int[B] or NULL: position of the first new token; NULL = the cached rows.  Positions that pass
+                               INT_MAX are kept as INT_MAX in row_pos                     */
     int input_mode;         /* flb_input_mode                                           */
     const void *k;          /* [B,S,Hkv,d]                                              */
     const void *v;

@@ -780,3 +780,26 @@ def test_empty_cache_and_dequantize(cuda_device):
     step = c.k_scale.repeat_interleave(64, 2)[:, :, :100, None]
     assert bool(((kd[:, :, :100] - k.transpose(1, 2)).abs() <= step * (0.5 + 127 * 2.0 ** -22)).all())
     assert torch.equal(kd, vd)
+
+
+# ------------------------------------------------------------------------------------------------ positions at the ends of their type
+def test_append_positions_at_the_ends_of_int(cuda_device):
+    """Positions outside the table are flagged and take the nearest row of it, however far outside; those that pass INT_MAX are kept as that."""
+    g = gen(90)
+    top, d, S = 2147483647, 64, 20
+    tab = table(50, d)
+    k, _ = tokens(g, "float32", 1, S, 2, d)
+    for first, past in ((top, 0), (top - 1, 3), (top - 18, 5), (-top - 1, 7), (-top - 1, 0), (-3, 9), (45, 2)):
+        c = kv8.empty_cache(1, 2, 48, d, block_len=16, row_pos=True, device=DEV)
+        st = torch.zeros(4, dtype=torch.int32, device=DEV)
+        want = clone(c)
+        pos = [min(first + i, top) for i in range(S)]
+        kr = R.rotate(k, tab, torch.tensor([[min(max(p, 0), 49) for p in pos]], device=DEV))
+        for h in range(2):
+            R.put_rows(want.k[0, h], want.k_scale[0, h], kr[0, :, h], list(range(past, past + S)), past, past, 16)
+            R.put_rows(want.v[0, h], want.v_scale[0, h], k[0, :, h], list(range(past, past + S)), past, past, 16)
+            want.row_pos[0, h, past:past + S] = i32(pos)
+        kv8.append(c, k, k, start_pos=past, token_pos=i32([first]), freq_cis=tab, scratch=st)
+        torch.cuda.synchronize()
+        assert int(st[0]) == kv8.STATUS_BAD_POS
+        same(c, want)
