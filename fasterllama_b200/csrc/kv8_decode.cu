@@ -440,7 +440,7 @@ __global__ void __launch_bounds__(kWarps * 32, D == 128 ? (NT == 1 ? 4 : 3) : 1)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 if (FORM && a.cap_log2e > 0.f) x[n][i] = cap_score(x[n][i], a.cap_log2e, inv_cap);
-                if (FORM) x[n][i] = fmaf(-slope[n], fabsf((float)(pos - kpos[i])), x[n][i]);
+                if (FORM) x[n][i] = fmaf(-slope[n], (float)__sad(pos, kpos[i], 0u), x[n][i]);
                 x[n][i] = vis[i] ? x[n][i] : -INFINITY;
             }
             if (a.scores && 4 * n + t < nheads) {

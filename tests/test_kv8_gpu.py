@@ -803,3 +803,17 @@ def test_append_positions_at_the_ends_of_int(cuda_device):
         torch.cuda.synchronize()
         assert int(st[0]) == kv8.STATUS_BAD_POS
         same(c, want)
+
+
+def test_decode_distances_beyond_31_bits(cuda_device):
+    """Rows and token at opposite ends of int: the distance is 2^32 - 1 and not 1.  k = 0, so the weights are those of the bias."""
+    d, top = 64, 2147483647
+    for token, row in ((top, -top - 1), (-top - 1, top), (5, -top), (top, top - 7)):
+        c = kv8.empty_cache(1, 1, 16, d, block_len=16, row_pos=True, device=DEV)
+        one, zero = torch.ones(1, 1, 1, d, device=DEV), torch.zeros(1, 1, 1, d, device=DEV)
+        kv8.append(c, zero, zero, token_pos=i32([row]))
+        o = torch.empty(1, 1, 1, d, device=DEV)
+        s = torch.zeros(kv8.decode_workspace_bytes(1, 1, 1, 16, d, block_len=16), dtype=torch.uint8, device=DEV)
+        kv8.decode(c, zero, zero, one, o, start_pos=1, token_pos=i32([token]), alibi_slopes=torch.full((1,), 2.0 ** -32, device=DEV), scratch=s)
+        want = 1.0 / (1.0 + math.exp(-abs(token - row) * 2.0 ** -32))
+        assert float((o - want).abs().max()) <= 2.0 ** -20  # v = 1 is coded as 127 * fp32(1 / 127); exponent and quotient a few roundings of 2^-23
