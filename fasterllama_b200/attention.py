@@ -166,20 +166,11 @@ def make_params(
     return p
 
 
-def _np_dense(t, name, shape, dtype):
-    if t.shape != shape or t.dtype != dtype or not _is_contiguous(t):
-        raise ValueError(f"{name} must be a dense {dtype} array of shape {shape}")
-    return _ptr(t)
+def _tensor(x):
+    """numpy arrays (host memory, for the checks alone) as tensors over the same memory."""
+    import torch
 
-
-def _np_opt(t, name, shape, dtype):
-    return None if t is None else _np_dense(t, name, shape, dtype)
-
-
-def _np_rows(t, name, shape, dtype):
-    if t.shape != shape or t.dtype != dtype:
-        raise ValueError(f"{name} must be {dtype} of shape {shape}")
-    return _ptr(t), _token_row_stride(t, *shape)
+    return torch.from_numpy(x) if hasattr(x, "__array_interface__") else x
 
 
 def make_scored_params(
@@ -217,39 +208,14 @@ def make_scored_params(
 ) -> tuple[FlbAttnParams, FlbScoreForm]:
     """A parameter block as from `make_params` and the score form beside it (see flb_score_form): capped scores, distance bias (float32 [H]),
     per-row key bounds (int32, decode [B], prefill [B,S]), and k, v [B,S,Hkv,d] with caches [B,Hkv,T,d] of fewer heads than q."""
-    if hasattr(q, "data_ptr"):
-        from . import _tensor_args
+    from . import _tensor_args
 
-        blocks = _tensor_args.scored(q, k, v, k_cache, v_cache, out, softcap, alibi_slopes, key_begin, key_end, scratch, start_pos, past_lens, max_past_len,
-                                     act_scale, q_w_scale, k_w_scale, v_w_scale, freq_cis, rope_pos0, rope_add_past, mask_mode, attn_mask, mask_row_stride,
-                                     softmax_scale, scratch_zeroed, split_len, out_q8, out_q8_scale, early_start)
-        p, f = FlbAttnParams.from_buffer_copy(blocks[0]), FlbScoreForm.from_buffer_copy(blocks[1])
-    else:  # numpy arrays: host memory, for the checks alone
-        B, S, H, d = q.shape
-        Hkv, T, dt = k.shape[2], k_cache.shape[2], q.dtype
-        mode, cdt, odt = _IN_MODE.get(_dtype_name(q)), _DT.get(_dtype_name(k_cache)), _DT.get(_dtype_name(out))
-        if mode is None or cdt is None or odt is None:
-            raise ValueError("q, k and v must be int32, float32 or float16, caches and out float32 or float16")
-        if H % Hkv:
-            raise ValueError("the number of K/V heads must divide that of the q heads")
-        kv_shape, cache_shape = (B, S, Hkv, d), (B, Hkv, T, d)
-        (qp, row), (kp, krow), (vp, vrow) = _np_rows(q, "q", (B, S, H, d), dt), _np_rows(k, "k", kv_shape, dt), _np_rows(v, "v", kv_shape, dt)
-        if krow != vrow:
-            raise ValueError("k and v must share one token-row stride")
-        bounds = (B,) if S == 1 else (B, S)
-        if attn_mask is not None and not mask_row_stride:
-            mask_row_stride = attn_mask.shape[-1]
-        p = FlbAttnParams(
-            batch_size=B, head_num=H, size_per_head=d, seq_len=S, start_pos=start_pos, total_len=T, past_lens=_np_opt(past_lens, "past_lens", (B,), "int32"),
-            max_past_len=max_past_len, input_mode=mode, q=qp, k=kp, v=vp, act_scale=_ptr(act_scale), q_w_scale=_ptr(q_w_scale), k_w_scale=_ptr(k_w_scale),
-            v_w_scale=_ptr(v_w_scale), freq_cis=_ptr(freq_cis), rope_pos0=rope_pos0, rope_add_past=1 if rope_add_past else 0, mask_mode=mask_mode,
-            attn_mask=_ptr(attn_mask), mask_row_stride=mask_row_stride, k_cache=_np_dense(k_cache, "k_cache", cache_shape, k_cache.dtype),
-            v_cache=_np_dense(v_cache, "v_cache", cache_shape, k_cache.dtype), cache_dtype=cdt, out=_np_dense(out, "out", (B, H, S, d), out.dtype), out_dtype=odt,
-            softmax_scale=softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(d), scratch=_ptr(scratch), scratch_bytes=0 if scratch is None else scratch.nbytes,
-            scratch_zeroed=1 if scratch_zeroed else 0, split_len=split_len, out_q8=_ptr(out_q8), out_q8_scale=_ptr(out_q8_scale), early_start=early_start,
-            qkv_row_stride=0 if row == H * d else row)
-        f = FlbScoreForm(kv_head_num=Hkv, kv_row_stride=krow, softcap=softcap, alibi_slopes=_np_opt(alibi_slopes, "alibi_slopes", (H,), "float32"),
-                         key_begin=_np_opt(key_begin, "key_begin", bounds, "int32"), key_end=_np_opt(key_end, "key_end", bounds, "int32"))
+    args = (q, k, v, k_cache, v_cache, out, softcap, alibi_slopes, key_begin, key_end, scratch, start_pos, past_lens, max_past_len, act_scale, q_w_scale, k_w_scale, v_w_scale,
+            freq_cis, rope_pos0, rope_add_past, mask_mode, attn_mask, mask_row_stride, softmax_scale, scratch_zeroed, split_len, out_q8, out_q8_scale, early_start)
+    if not hasattr(q, "data_ptr"):
+        args = tuple(_tensor(x) for x in args)
+    blocks = _tensor_args.scored(*args)
+    p, f = FlbAttnParams.from_buffer_copy(blocks[0]), FlbScoreForm.from_buffer_copy(blocks[1])
     # keep the tensors alive as long as the blocks
     p._keep = (q, k, v, k_cache, v_cache, out, scratch, past_lens, act_scale, q_w_scale, k_w_scale, v_w_scale, freq_cis, attn_mask, out_q8, out_q8_scale)
     f._keep = (alibi_slopes, key_begin, key_end)
