@@ -207,7 +207,9 @@ def make_scored_params(
     early_start: int = 0,
 ) -> tuple[FlbAttnParams, FlbScoreForm]:
     """A parameter block as from `make_params` and the score form beside it (see flb_score_form): capped scores, distance bias (float32 [H]),
-    per-row key bounds (int32, decode [B], prefill [B,S]), and k, v [B,S,Hkv,d] with caches [B,Hkv,T,d] of fewer heads than q."""
+    per-row key bounds (int32, decode [B], prefill [B,S]), and k, v [B,S,Hkv,d] with caches [B,Hkv,T,d] of fewer heads than q.
+    Every tensor lies on the device of the caches and covers what the call can reach: RoPE table and additive mask every position up to
+    max_past_len (0 = T - 1), start_pos, or the prompt's last.  What a decode call reads or writes once may be pinned host memory."""
     from . import _tensor_args
 
     args = (q, k, v, k_cache, v_cache, out, softcap, alibi_slopes, key_begin, key_end, scratch, start_pos, past_lens, max_past_len, act_scale, q_w_scale, k_w_scale, v_w_scale,
@@ -216,6 +218,7 @@ def make_scored_params(
         args = tuple(_tensor(x) for x in args)
     blocks = _tensor_args.scored(*args)
     p, f = FlbAttnParams.from_buffer_copy(blocks[0]), FlbScoreForm.from_buffer_copy(blocks[1])
+    p._device = blocks[2]  # -1: host memory
     # keep the tensors alive as long as the blocks
     p._keep = (q, k, v, k_cache, v_cache, out, scratch, past_lens, act_scale, q_w_scale, k_w_scale, v_w_scale, freq_cis, attn_mask, out_q8, out_q8_scale)
     f._keep = (alibi_slopes, key_begin, key_end)
@@ -271,17 +274,30 @@ def validate_scored(p: FlbAttnParams, f: FlbScoreForm | None) -> int:
     return int(_lib.load_library().flb_attn_validate_scored(C.byref(p), _form(f)))
 
 
+def _scored(fn, p: FlbAttnParams, f: FlbScoreForm | None, stream) -> None:
+    import torch
+
+    dev = getattr(p, "_device", None)  # None: a block that was filled by hand, on the current device
+    if dev is not None:
+        if dev < 0:
+            raise ValueError("a scored call runs on tensors of a CUDA device")
+        if torch.cuda.current_device() != dev:
+            with torch.cuda.device(dev):
+                return _scored(fn, p, f, stream)
+    _lib.check(fn(C.byref(p), _form(f), torch._C._cuda_getCurrentRawStream(dev) if stream is None and dev is not None else _stream_handle(stream)))
+
+
 def forward_scored(p: FlbAttnParams, f: FlbScoreForm | None, stream=None) -> None:
-    """`forward` with a score form (both from `make_scored_params`)."""
-    _lib.check(_lib.load_library().flb_attn_forward_scored(C.byref(p), _form(f), _stream_handle(stream)))
+    """`forward` with a score form (both from `make_scored_params`), on the device of its tensors."""
+    _scored(_lib.load_library().flb_attn_forward_scored, p, f, stream)
 
 
 def decode_scored(p: FlbAttnParams, f: FlbScoreForm | None, stream=None) -> None:
-    _lib.check(_lib.load_library().flb_attn_decode_scored(C.byref(p), _form(f), _stream_handle(stream)))
+    _scored(_lib.load_library().flb_attn_decode_scored, p, f, stream)
 
 
 def prefill_scored(p: FlbAttnParams, f: FlbScoreForm | None, stream=None) -> None:
-    _lib.check(_lib.load_library().flb_attn_prefill_scored(C.byref(p), _form(f), _stream_handle(stream)))
+    _scored(_lib.load_library().flb_attn_prefill_scored, p, f, stream)
 
 
 def forward(p: FlbAttnParams, stream=None) -> None:

@@ -24,15 +24,23 @@ template <typename... A> [[noreturn]] void refuse(const char *format, A... a) {
     throw Refused();
 }
 
-const at::Tensor &tensor(PyObject *o, const char *name, int dev) {
+// Where a tensor has to be: on this device; `pinned`: or in pinned host memory.
+struct Place {
+    int dev;
+    bool pinned;
+    Place(int d, bool p = false) : dev(d), pinned(p) {}
+};
+const at::Tensor &tensor(PyObject *o, const char *name, Place at) {
     if (!THPVariable_Check(o)) refuse("%s must be a torch tensor", name);
     const at::Tensor &t = THPVariable_Unpack(o);
-    if (dev != kAnyDevice && t.get_device() != dev) refuse("%s is on another device (%d) than the cache (%d)", name, (int)t.get_device(), dev);
+    if (!t.device().is_cuda() && !t.device().is_cpu()) refuse("%s must lie in CUDA or host memory", name);
+    if (at.dev != kAnyDevice && t.get_device() != at.dev && !(at.pinned && t.device().is_cpu() && t.is_pinned()))
+        refuse("%s is on another device (%d) than the cache (%d)", name, (int)t.get_device(), at.dev);
     if (t.layout() != at::kStrided) refuse("%s must be a strided tensor", name);
     return t;
 }
 
-const at::Tensor &shaped(PyObject *o, const char *name, at::IntArrayRef shape, at::ScalarType type, int dev) {
+const at::Tensor &shaped(PyObject *o, const char *name, at::IntArrayRef shape, at::ScalarType type, Place dev) {
     const at::Tensor &t = tensor(o, name, dev);
     if (t.sizes() != shape || (type != kAnyType && t.scalar_type() != type)) {
         std::string want;
@@ -43,12 +51,12 @@ const at::Tensor &shaped(PyObject *o, const char *name, at::IntArrayRef shape, a
 }
 
 // address of a dense tensor
-void *dense(PyObject *o, const char *name, at::IntArrayRef shape, at::ScalarType type, int dev) {
+void *dense(PyObject *o, const char *name, at::IntArrayRef shape, at::ScalarType type, Place dev) {
     const at::Tensor &t = shaped(o, name, shape, type, dev);
     if (!t.is_contiguous()) refuse("%s must be a dense tensor", name);
     return t.data_ptr();
 }
-template <typename P> P *opt(PyObject *o, const char *name, at::IntArrayRef shape, at::ScalarType type, int dev) {
+template <typename P> P *opt(PyObject *o, const char *name, at::IntArrayRef shape, at::ScalarType type, Place dev) {
     return o == Py_None ? nullptr : static_cast<P *>(dense(o, name, shape, type, dev));
 }
 
@@ -73,7 +81,7 @@ int truth(PyObject *o) {
 }
 
 // q, k or v [B,S,heads,d]: dense heads, one stride between tokens
-void *rows(PyObject *o, const char *name, at::IntArrayRef shape, at::ScalarType type, int dev, int64_t &row) {
+void *rows(PyObject *o, const char *name, at::IntArrayRef shape, at::ScalarType type, Place dev, int64_t &row) {
     const at::Tensor &t = shaped(o, name, shape, type, dev);
     if (t.dim() != 4) refuse("%s must be [B,S,heads,d]", name);
     const int64_t B = t.size(0), S = t.size(1), H = t.size(2), d = t.size(3);
@@ -86,7 +94,7 @@ void *rows(PyObject *o, const char *name, at::IntArrayRef shape, at::ScalarType 
     return t.data_ptr();
 }
 // k and v of the tokens; their stride
-int kv_rows(PyObject *ko, PyObject *vo, at::IntArrayRef shape, at::ScalarType type, int dev, const void *&k, const void *&v) {
+int kv_rows(PyObject *ko, PyObject *vo, at::IntArrayRef shape, at::ScalarType type, Place dev, const void *&k, const void *&v) {
     int64_t rk, rv;
     k = rows(ko, "k", shape, type, dev, rk);
     v = rows(vo, "v", shape, type, dev, rv);
@@ -254,11 +262,12 @@ PyObject *kv8_evict(PyObject *, PyObject *const *a, Py_ssize_t n) {
     });
 }
 
-// A tensor of which only type and layout are known here; null for None
-template <typename P> P *loose(PyObject *o, const char *name, at::ScalarType type) {
+// A dense tensor of so many elements, in whatever shape; null for None
+template <typename P> P *flat(PyObject *o, const char *name, at::ScalarType type, int64_t n, Place dev) {
     if (o == Py_None) return nullptr;
-    const at::Tensor &t = tensor(o, name, kAnyDevice);
+    const at::Tensor &t = tensor(o, name, dev);
     if (t.scalar_type() != type || !t.is_contiguous()) refuse("%s must be a dense %s tensor", name, c10::toString(type));
+    if (n >= 0 && t.numel() != n) refuse("%s must hold %lld elements", name, (long long)n);
     return static_cast<P *>(t.data_ptr());
 }
 int dtype_of(const at::Tensor &t) {
@@ -266,14 +275,18 @@ int dtype_of(const at::Tensor &t) {
     return t.scalar_type() == at::kFloat ? FLB_F32 : FLB_F16;
 }
 
-// The blocks of flb_attn.h with a score form.  Devices are not compared: the inputs of a decode may lie in pinned host memory.
+// The blocks of flb_attn.h with a score form.  What a call can read and write has to be there: host memory is left for the checks alone (the
+// cache there too), or, pinned, for what a decode call may read from and write to it.
 PyObject *scored(PyObject *, PyObject *const *a, Py_ssize_t n) {
     flb_score_form f;
     memset(&f, 0, sizeof f);
     PyObject *first = block<flb_attn_params, 30>(n, [a, &f](flb_attn_params &p) {
-        const at::Tensor &q = tensor(a[0], "q", kAnyDevice), &k = tensor(a[1], "k", kAnyDevice), &kc = tensor(a[3], "k_cache", kAnyDevice), &out = tensor(a[5], "out", kAnyDevice);
+        const at::Tensor &kc = tensor(a[3], "k_cache", kAnyDevice);
+        const int dev = (int)kc.get_device();
+        const at::Tensor &q = tensor(a[0], "q", kAnyDevice), &k = tensor(a[1], "k", kAnyDevice), &out = tensor(a[5], "out", kAnyDevice);
         if (q.dim() != 4 || k.dim() != 4 || kc.dim() != 4) refuse("q and k must be [B,S,heads,d], k_cache [B,Hkv,T,d]");
         const int64_t B = q.size(0), S = q.size(1), H = q.size(2), d = q.size(3), Hkv = k.size(2), T = kc.size(2);
+        const Place near(dev, S == 1);
         if (Hkv <= 0 || H % Hkv) refuse("the number of K/V heads must divide that of the q heads");
         p.batch_size = as_int(B, "the batch");
         p.head_num = as_int(H, "the number of heads");
@@ -282,47 +295,54 @@ PyObject *scored(PyObject *, PyObject *const *a, Py_ssize_t n) {
         p.total_len = as_int(T, "the cache's length");
         p.input_mode = input_mode(q);
         int64_t row;
-        p.q = rows(a[0], "q", q.sizes(), q.scalar_type(), kAnyDevice, row);
+        p.q = rows(a[0], "q", q.sizes(), q.scalar_type(), near, row);
         p.qkv_row_stride = row == H * d ? 0 : as_int(row, "the stride of q");
         f.kv_head_num = as_int(Hkv, "the number of K/V heads");
-        f.kv_row_stride = kv_rows(a[1], a[2], {B, S, Hkv, d}, q.scalar_type(), kAnyDevice, p.k, p.v);
+        f.kv_row_stride = kv_rows(a[1], a[2], {B, S, Hkv, d}, q.scalar_type(), near, p.k, p.v);
         p.cache_dtype = dtype_of(kc);
-        p.k_cache = dense(a[3], "k_cache", {B, Hkv, T, d}, kc.scalar_type(), kAnyDevice);
-        p.v_cache = dense(a[4], "v_cache", {B, Hkv, T, d}, kc.scalar_type(), kAnyDevice);
+        p.k_cache = dense(a[3], "k_cache", {B, Hkv, T, d}, kc.scalar_type(), dev);
+        p.v_cache = dense(a[4], "v_cache", {B, Hkv, T, d}, kc.scalar_type(), dev);
         p.out_dtype = dtype_of(out);
-        p.out = dense(a[5], "out", {B, H, S, d}, out.scalar_type(), kAnyDevice);
+        p.out = dense(a[5], "out", {B, H, S, d}, out.scalar_type(), near);
         f.softcap = number(a[6]);
-        f.alibi_slopes = opt<float>(a[7], "alibi_slopes", {H}, at::kFloat, kAnyDevice);
+        f.alibi_slopes = opt<float>(a[7], "alibi_slopes", {H}, at::kFloat, near);
         const int64_t bounds[2] = {B, S};
         const at::IntArrayRef bound_shape(bounds, S == 1 ? 1 : 2);
-        f.key_begin = opt<int>(a[8], "key_begin", bound_shape, at::kInt, kAnyDevice);
-        f.key_end = opt<int>(a[9], "key_end", bound_shape, at::kInt, kAnyDevice);
-        p.scratch = scratch(a[10], kAnyDevice, p.scratch_bytes);
+        f.key_begin = opt<int>(a[8], "key_begin", bound_shape, at::kInt, near);
+        f.key_end = opt<int>(a[9], "key_end", bound_shape, at::kInt, near);
+        p.scratch = scratch(a[10], dev, p.scratch_bytes);
         p.start_pos = integer(a[11], "start_pos");
-        p.past_lens = opt<int>(a[12], "past_lens", {B}, at::kInt, kAnyDevice);
+        p.past_lens = opt<int>(a[12], "past_lens", {B}, at::kInt, near);
         p.max_past_len = integer(a[13], "max_past_len");
-        p.act_scale = loose<float>(a[14], "act_scale", at::kFloat);
-        p.q_w_scale = loose<float>(a[15], "q_w_scale", at::kFloat);
-        p.k_w_scale = loose<float>(a[16], "k_w_scale", at::kFloat);
-        p.v_w_scale = loose<float>(a[17], "v_w_scale", at::kFloat);
-        p.freq_cis = loose<float>(a[18], "freq_cis", at::kFloat);
+        const bool scaled = p.input_mode == FLB_IN_INT32; // the scales are read
+        p.act_scale = flat<float>(a[14], "act_scale", at::kFloat, scaled ? B * S : -1, near);
+        p.q_w_scale = flat<float>(a[15], "q_w_scale", at::kFloat, scaled ? H * d : -1, near);
+        p.k_w_scale = flat<float>(a[16], "k_w_scale", at::kFloat, scaled ? Hkv * d : -1, near);
+        p.v_w_scale = flat<float>(a[17], "v_w_scale", at::kFloat, scaled ? Hkv * d : -1, near);
+        p.freq_cis = flat<float>(a[18], "freq_cis", at::kFloat, -1, near);
         p.rope_pos0 = integer(a[19], "rope_pos0");
         p.rope_add_past = truth(a[20]);
+        // rows that the call can reach: of a prompt its own, else up to the host's bound on the cached ones
+        const int64_t most = S > 1 ? S - 1 : !p.past_lens ? p.start_pos : p.max_past_len > 0 ? p.max_past_len : T - 1;
+        const int64_t last = (int64_t)p.rope_pos0 + (S > 1 || p.rope_add_past ? most : 0);
+        if (a[18] != Py_None && d > 0 && THPVariable_Unpack(a[18]).numel() / d <= last) refuse("freq_cis must have a row of the head size for every position up to %lld", (long long)last);
         p.mask_mode = integer(a[21], "mask_mode");
-        p.attn_mask = loose<float>(a[22], "attn_mask", at::kFloat);
+        p.attn_mask = flat<float>(a[22], "attn_mask", at::kFloat, -1, near);
         p.mask_row_stride = integer(a[23], "mask_row_stride");
-        if (p.attn_mask && !p.mask_row_stride) p.mask_row_stride = as_int(THPVariable_Unpack(a[22]).size(-1), "the mask's row");
+        if (a[22] != Py_None && !p.mask_row_stride) p.mask_row_stride = as_int(THPVariable_Unpack(a[22]).size(-1), "the mask's row");
+        if (a[22] != Py_None && p.mask_mode == FLB_MASK_GENERIC && THPVariable_Unpack(a[22]).numel() <= most * p.mask_row_stride + most)
+            refuse("attn_mask must have rows and columns for every position up to %lld", (long long)most);
         p.softmax_scale = a[24] == Py_None ? (float)(1.0 / std::sqrt((double)d)) : number(a[24]);
         p.scratch_zeroed = truth(a[25]);
         p.split_len = integer(a[26], "split_len");
-        p.out_q8 = loose<int8_t>(a[27], "out_q8", at::kChar);
-        p.out_q8_scale = loose<float>(a[28], "out_q8_scale", at::kFloat);
+        p.out_q8 = flat<int8_t>(a[27], "out_q8", at::kChar, B * S * H * d, near);
+        p.out_q8_scale = flat<float>(a[28], "out_q8_scale", at::kFloat, B * S, near);
         p.early_start = integer(a[29], "early_start");
-        return 0;
+        return dev;
     });
     if (!first) return nullptr;
-    PyObject *p = PyTuple_GET_ITEM(first, 0), *bytes = PyBytes_FromStringAndSize(reinterpret_cast<const char *>(&f), sizeof f);
-    PyObject *both = bytes ? Py_BuildValue("(ON)", p, bytes) : nullptr;
+    PyObject *bytes = PyBytes_FromStringAndSize(reinterpret_cast<const char *>(&f), sizeof f);
+    PyObject *both = bytes ? Py_BuildValue("(ONO)", PyTuple_GET_ITEM(first, 0), bytes, PyTuple_GET_ITEM(first, 1)) : nullptr;
     Py_DECREF(first);
     return both;
 }
@@ -334,7 +354,7 @@ PyMethodDef methods[] = {
     {"kv8_append", fast(kv8_append), METH_FASTCALL, "parameter block of an append, and its device"},
     {"kv8_decode", fast(kv8_decode), METH_FASTCALL, "parameter block of a decode, and its device"},
     {"kv8_evict", fast(kv8_evict), METH_FASTCALL, "parameter block of an eviction, and its device"},
-    {"scored", fast(scored), METH_FASTCALL, "parameter block and score form of an attention call"},
+    {"scored", fast(scored), METH_FASTCALL, "parameter block and score form of an attention call, and their device"},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensor_args", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

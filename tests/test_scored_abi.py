@@ -112,3 +112,67 @@ def test_binding_refuses_shapes_and_types():
                 dict(k_cache=np.zeros((2, 8, 64, 128), np.float16)), dict(k_cache=np.zeros((2, 4, 64, 128), np.float16)[:, :, ::2], v_cache=np.zeros((2, 4, 32, 128), np.float16))):
         with pytest.raises(ValueError):
             _call(**bad)
+
+
+def _tensors(S=1, dtype=torch.float16, **kw):
+    B, H, Hkv, T, d = 2, 8, 4, 64, 128
+    a = dict(q=torch.zeros(B, S, H, d, dtype=dtype), k=torch.zeros(B, S, Hkv, d, dtype=dtype), v=torch.zeros(B, S, Hkv, d, dtype=dtype),
+             k_cache=torch.zeros(B, Hkv, T, d, dtype=torch.float16), v_cache=torch.zeros(B, Hkv, T, d, dtype=torch.float16), out=torch.zeros(B, H, S, d),
+             scratch=torch.zeros(A.workspace_bytes(B, H, T, S, size_per_head=d) + 65536, dtype=torch.uint8))
+    return A.make_scored_params(**{**a, **kw})
+
+
+SCALES = dict(act_scale=2 * 5, q_w_scale=8 * 128, k_w_scale=4 * 128, v_w_scale=4 * 128)
+
+
+@pytest.mark.parametrize("name", list(SCALES))
+def test_scales_of_int32_inputs_have_their_lengths(name):
+    good = {n: torch.ones(k) for n, k in SCALES.items()}
+    assert A.validate_scored(*_tensors(5, torch.int32, **good)) == _lib.FLB_OK
+    for n in (SCALES[name] - 1, SCALES[name] + 1, 0):
+        with pytest.raises(ValueError, match=name):
+            _tensors(5, torch.int32, **{**good, name: torch.ones(n)})
+
+
+@pytest.mark.parametrize("kw,rows", [
+    (dict(S=5), 5), (dict(S=5, rope_pos0=3), 8), (dict(start_pos=9, rope_add_past=True), 10), (dict(start_pos=9), 1), (dict(start_pos=9, rope_pos0=7), 8),
+    (dict(past_lens=torch.zeros(2, dtype=torch.int32), max_past_len=20, rope_add_past=True), 21),
+    (dict(past_lens=torch.zeros(2, dtype=torch.int32), rope_add_past=True, rope_pos0=2), 66)])
+def test_rope_tables_reach_every_position(kw, rows):
+    assert A.validate_scored(*_tensors(freq_cis=torch.zeros(rows, 128), **kw)) == _lib.FLB_OK
+    with pytest.raises(ValueError, match="freq_cis"):
+        _tensors(freq_cis=torch.zeros(rows - 1, 128), **kw)
+    if rows > 1:
+        with pytest.raises(ValueError, match="freq_cis"):
+            _tensors(freq_cis=torch.zeros(rows, 64), **kw)
+
+
+@pytest.mark.parametrize("kw,n", [(dict(S=5), 5), (dict(start_pos=9), 10), (dict(past_lens=torch.zeros(2, dtype=torch.int32), max_past_len=20), 21),
+                                  (dict(past_lens=torch.zeros(2, dtype=torch.int32)), 64)])
+def test_additive_masks_reach_every_position(kw, n):
+    kw = dict(kw, mask_mode=A.FLB_MASK_GENERIC)
+    assert A.validate_scored(*_tensors(attn_mask=torch.zeros(n, n), **kw)) == _lib.FLB_OK
+    assert A.validate_scored(*_tensors(attn_mask=torch.zeros(n, n + 3), **kw)) == _lib.FLB_OK
+    assert A.validate_scored(*_tensors(attn_mask=torch.zeros(n * n), mask_row_stride=n, **kw)) == _lib.FLB_OK
+    for bad in (dict(attn_mask=torch.zeros(n - 1, n)), dict(attn_mask=torch.zeros(n, n), mask_row_stride=n + 1)):
+        with pytest.raises(ValueError, match="attn_mask"):
+            _tensors(**bad, **kw)
+
+
+@pytest.mark.parametrize("S", [1, 5])
+def test_quantised_outputs_have_their_sizes(S):
+    good = dict(out_q8=torch.zeros(2, S, 1024, dtype=torch.int8), out_q8_scale=torch.zeros(2 * S))
+    assert A.validate_scored(*_tensors(S, **good)) == _lib.FLB_OK
+    for bad in (dict(out_q8=torch.zeros(2, S, 1023, dtype=torch.int8)), dict(out_q8_scale=torch.zeros(2 * S - 1))):
+        with pytest.raises(ValueError, match="out_q8"):
+            _tensors(S, **{**good, **bad})
+
+
+@pytest.mark.parametrize("S", [1, 5])
+def test_host_memory_is_not_launched_on(S):
+    p, f = _tensors(S)
+    for call in (A.forward_scored, A.decode_scored if S == 1 else A.prefill_scored):
+        with pytest.raises(ValueError, match="CUDA device"):
+            call(p, f)
+    with pytest.raises(ValueError, match="memory"):
+        _tensors(S, alibi_slopes=torch.zeros(8, device="meta"))

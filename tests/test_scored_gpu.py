@@ -417,3 +417,34 @@ def test_prefill_large_capped_scores_against_a_mask(cuda_device, log_cap):
 def test_prefill_saturated_caps_share_the_weight(cuda_device, log_cap):
     """Two scores far beyond the cap are both the cap."""
     assert two_keys(0, cap=2.0 ** log_cap, scale=2.0 ** (log_cap - 26)) == pytest.approx(0.5, abs=2.0 ** -11)
+
+
+# ------------------------------------------------------------------------------------------------ devices
+@pytest.mark.parametrize("S", [1, 5])
+def test_tensors_in_host_memory_are_refused(cuda_device, S):
+    """Refused while the blocks are filled, so no kernel sees their addresses; a decode call may read pinned ones."""
+    B, H, Hkv, T, d = 2, 8, 4, 64, 128
+    good = dict(q=torch.zeros(B, S, H, d).half(), k=torch.zeros(B, S, Hkv, d).half(), v=torch.zeros(B, S, Hkv, d).half(), k_cache=torch.zeros(B, Hkv, T, d), v_cache=torch.zeros(B, Hkv, T, d),
+                out=torch.zeros(B, H, S, d), scratch=torch.zeros(A.workspace_bytes(B, H, T, S) + 65536, dtype=torch.uint8), alibi_slopes=torch.zeros(H),
+                key_begin=torch.zeros((B,) if S == 1 else (B, S), dtype=torch.int32), freq_cis=torch.zeros(T, d), out_q8=torch.zeros(B, S, H * d, dtype=torch.int8),
+                out_q8_scale=torch.zeros(B * S))
+    dev = {n: t.to(DEV) for n, t in good.items()}
+    A.make_scored_params(**dev)
+    for name, t in good.items():
+        with pytest.raises(ValueError, match="another device"):
+            A.make_scored_params(**{**dev, name: t})
+        pinned = {**dev, name: t.pin_memory()}
+        if S == 1 and name not in ("k_cache", "v_cache", "scratch"):
+            A.make_scored_params(**pinned)
+        else:
+            with pytest.raises(ValueError, match="another device"):
+                A.make_scored_params(**pinned)
+
+
+def test_decode_reads_and_writes_pinned_memory(cuda_device):
+    (q, k, v, kc, vc), o = run_decode(60, B=2, H=4, Hkv=2, T=256, d=128, past=[255, 17], cap=10.0, rope=False)
+    host = {n: t.cpu().pin_memory() for n, t in (("q", q), ("k", k), ("v", v), ("out", torch.zeros_like(o)), ("past_lens", torch.tensor([255, 17], dtype=torch.int32)))}
+    scratch = torch.zeros(A.workspace_bytes(2, 4, 256), dtype=torch.uint8, device=DEV)
+    A.forward_scored(*A.make_scored_params(**host, k_cache=kc, v_cache=vc, scratch=scratch, max_past_len=255, softcap=10.0))
+    torch.cuda.synchronize()
+    assert torch.equal(host["out"], o.cpu())
