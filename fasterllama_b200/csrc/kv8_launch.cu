@@ -8,6 +8,7 @@ namespace {
 inline size_t round_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline bool aligned4(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+template <typename... P> inline bool aligned4(const void *p, P... more) { return aligned4(p) && aligned4(more...); }
 
 int check_sizes(const flb_kv8_cache &c) {
     if (c.batch_size <= 0 || c.kv_head_num <= 0 || c.size_per_head <= 0 || c.total_len <= 0) return FLB_ERR_BAD_SHAPE;
@@ -25,7 +26,7 @@ int check_cache(const flb_kv8_cache &c) {
     if (c.code_type != FLB_KV8_I8 && c.code_type != FLB_KV8_E4M3) return FLB_ERR_BAD_ENUM;
     if (!c.k_codes || !c.v_codes || !c.k_scale || !c.v_scale) return FLB_ERR_NULL_POINTER;
     if (!aligned16(c.k_codes) || !aligned16(c.v_codes)) return FLB_ERR_MISALIGNED;
-    if (!aligned4(c.k_scale) || !aligned4(c.v_scale) || !aligned4(c.row_pos)) return FLB_ERR_MISALIGNED;
+    if (!aligned4(c.k_scale, c.v_scale, c.row_pos)) return FLB_ERR_MISALIGNED;
     return FLB_OK;
 }
 // one of q, k, v: pointer, scale, stride (elements; 0 = dense)
@@ -142,6 +143,7 @@ int flb_kv8_validate_append(const flb_kv8_append_params *p) {
     if ((st = check_input(p->input_mode, p->k, p->k_w_scale, p->kv_row_stride, dense)) != FLB_OK) return st;
     if ((st = check_input(p->input_mode, p->v, p->v_w_scale, p->kv_row_stride, dense)) != FLB_OK) return st;
     if ((st = check_rope(p->freq_cis, p->freq_rows)) != FLB_OK) return st;
+    if (!aligned4(p->past_lens, p->new_lens, p->token_pos, p->act_scale, p->status)) return FLB_ERR_MISALIGNED;
     if (!p->past_lens && (p->start_pos < 0 || p->start_pos > p->cache.total_len - p->seq_len)) return FLB_ERR_BAD_SHAPE;
     // one CTA per block that a call can touch: the grid's second and third extents hold 65535
     if (p->cache.batch_size > 65535 || window_blocks(p->cache, p->seq_len, p->past_lens != nullptr, p->start_pos) > 65535) return FLB_ERR_TOO_LARGE;
@@ -166,6 +168,7 @@ int flb_kv8_validate_decode(const flb_kv8_decode_params *p) {
     if (!aligned16(p->out)) return FLB_ERR_MISALIGNED;
     if ((p->weight_in != nullptr) != (p->weight_out != nullptr)) return FLB_ERR_NULL_POINTER;
     if (!aligned16(p->weight_in) || !aligned16(p->weight_out)) return FLB_ERR_MISALIGNED;
+    if (!aligned4(p->past_lens, p->token_pos, p->act_scale, p->alibi_slopes, p->key_begin)) return FLB_ERR_MISALIGNED;
     const int mp = max_past_of(p);
     if (mp < 0 || mp >= p->cache.total_len) return FLB_ERR_BAD_SHAPE;
     if (!p->scratch) return FLB_ERR_NULL_POINTER;
@@ -186,7 +189,7 @@ int flb_kv8_validate_evict(const flb_kv8_evict_params *p) {
     if (p->recent > 0 && !p->next_pos) return FLB_ERR_NULL_POINTER;
     if (p->budget <= 0 || p->recent < 0 || p->sinks < 0 || p->recent > p->budget || p->sinks > p->budget - p->recent) return FLB_ERR_BAD_SHAPE;
     if (!p->past_lens && (p->start_pos < 0 || p->start_pos > p->cache.total_len)) return FLB_ERR_BAD_SHAPE;
-    if (!aligned16(p->scratch)) return FLB_ERR_MISALIGNED;
+    if (!aligned16(p->scratch) || !aligned4(p->past_lens, p->len_out, p->next_pos)) return FLB_ERR_MISALIGNED;
     if (!aligned16(p->weight) || !aligned16(p->cache.row_pos) || !aligned16(p->weight_out) || !aligned16(p->pos_out)) return FLB_ERR_MISALIGNED;
     if (8ull * p->cache.batch_size * p->cache.kv_head_num * (p->cache.total_len / p->cache.block_len + 1) > 0x7fffffffull) return FLB_ERR_TOO_LARGE;
     if (p->scratch_bytes < evict_bytes(p->cache)) return FLB_ERR_SCRATCH_TOO_SMALL;

@@ -275,6 +275,7 @@ int flb_attn_validate_scored(const flb_attn_params *p, const flb_score_form *f) 
         if (((size_t)f->kv_row_stride * (p->input_mode == FLB_IN_F16 ? 2 : 4)) % 16u) return FLB_ERR_MISALIGNED;
     }
     if (!flb::cap_ok(f->softcap)) return FLB_ERR_BAD_SHAPE;
+    if ((reinterpret_cast<uintptr_t>(f->alibi_slopes) | reinterpret_cast<uintptr_t>(f->key_begin) | reinterpret_cast<uintptr_t>(f->key_end)) & 3u) return FLB_ERR_MISALIGNED;
     if (p->seq_len == 1) return f->key_end ? FLB_ERR_UNSUPPORTED : FLB_OK; // a decode call sees what is cached
     if (!(p->softmax_scale > 0.f) || p->softmax_scale > 3.402823466e38f) return FLB_ERR_BAD_SHAPE; // maxima are taken before the scale
     if (f->softcap > 0.f && p->softmax_scale > 65536.f * f->softcap) return FLB_ERR_BAD_SHAPE; // its fifth power is a coefficient

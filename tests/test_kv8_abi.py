@@ -210,3 +210,18 @@ def test_workspaces_cover_shorter_calls_and_grow():
     assert kv8.decode_workspace_bytes(2, 8, 4, 4096) > a >= kv8.counter_bytes(2, 8, 4)
     assert kv8.decode_workspace_bytes(2, 8, 4, 1024, weights=True) >= a + 2 * 8 * 1024 * 4
     assert kv8.evict_workspace_bytes(2, 4, 2048) > kv8.evict_workspace_bytes(2, 4, 1024)
+
+
+def test_words_at_odd_addresses_are_refused():
+    p, keep = _append()
+    for field in ("past_lens", "new_lens", "token_pos", "act_scale", "status"):
+        _refused(p, field, 4098, _lib.FLB_ERR_MISALIGNED)
+    p, keep = _decode()
+    for field in ("past_lens", "token_pos", "act_scale", "alibi_slopes", "key_begin"):
+        _refused(p, field, 4097, _lib.FLB_ERR_MISALIGNED)
+    p, keep = _evict()
+    for field in ("past_lens", "len_out", "next_pos"):
+        _refused(p, field, 4099, _lib.FLB_ERR_MISALIGNED)
+    c = _cache()
+    k = torch.zeros(2, 1, 4, 128, dtype=torch.float16)
+    assert kv8.validate(kv8.append_params(c, k, k.clone(), scratch=torch.zeros(9, dtype=torch.uint8)[1:])) == _lib.FLB_ERR_MISALIGNED

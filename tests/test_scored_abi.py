@@ -176,3 +176,10 @@ def test_host_memory_is_not_launched_on(S):
             call(p, f)
     with pytest.raises(ValueError, match="memory"):
         _tensors(S, alibi_slopes=torch.zeros(8, device="meta"))
+
+
+@pytest.mark.parametrize("S,field", [(1, "alibi_slopes"), (1, "key_begin"), (5, "alibi_slopes"), (5, "key_begin"), (5, "key_end")])
+def test_words_at_odd_addresses_are_refused(S, field):
+    p, f, keep = _call(S=S)
+    setattr(f, field, 4098)
+    assert A.validate_scored(p, f) == _lib.FLB_ERR_MISALIGNED
