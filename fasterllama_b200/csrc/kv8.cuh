@@ -13,6 +13,8 @@ namespace flb {
 // Every kernel of this family is launched with programmatic stream serialisation: its CTAs may become resident while the kernel in front
 // drains.  They touch nothing before that kernel, and with it everything before, has completed, and let the next one go after that
 // only: for a caller a launch is as ordered as any, it merely starts sooner.  All threads call it first.
+// What the kernel in front may write (inputs, lengths, positions) is read by plain loads: the read-only path is for data that nobody writes while a
+// kernel is resident, and loads through it may be moved in front of the wait.
 __device__ __forceinline__ void kv8_begin() {
     grid_dependency_wait();
     grid_launch_dependents();
@@ -120,12 +122,12 @@ template <int MODE> __device__ __forceinline__ Kv8Raw kv8_raw8(const Kv8Input &i
     const size_t off = token * in.row_stride + col;
     Kv8Raw r;
     if (MODE == 2) {
-        r.lo = __ldg(reinterpret_cast<const uint4 *>((const __half *)in.p + off));
+        r.lo = *reinterpret_cast<const uint4 *>((const __half *)in.p + off);
         r.hi = make_uint4(0u, 0u, 0u, 0u);
     } else {
         const uint4 *p = reinterpret_cast<const uint4 *>((const uint32_t *)in.p + off);
-        r.lo = __ldg(p);
-        r.hi = __ldg(p + 1);
+        r.lo = p[0];
+        r.hi = p[1];
     }
     return r;
 }
@@ -144,9 +146,9 @@ template <int MODE> __device__ __forceinline__ void kv8_values8(const Kv8Raw &r,
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(u[i]);
         } else {
-            const float as = __ldg(act_scale + token);
+            const float as = act_scale[token];
             const float4 *w = reinterpret_cast<const float4 *>(in.w_scale + col);
-            const float4 w0 = __ldg(w), w1 = __ldg(w + 1);
+            const float4 w0 = w[0], w1 = w[1];
             const float ws[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(__fmul_rn((float)(int)u[i], as), ws[i]);
@@ -170,7 +172,8 @@ __device__ __forceinline__ void kv8_rotate8(const float4 &f0, const float4 &f1, 
     }
 }
 __device__ __forceinline__ void kv8_rotate8(const float *row, float (&x)[8]) {
-    kv8_rotate8(__ldg(reinterpret_cast<const float4 *>(row)), __ldg(reinterpret_cast<const float4 *>(row) + 1), x);
+    const float4 *f = reinterpret_cast<const float4 *>(row);
+    kv8_rotate8(f[0], f[1], x);
 }
 
 // table row of a position; one outside the table is flagged and the nearest row taken

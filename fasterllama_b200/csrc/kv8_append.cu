@@ -22,8 +22,8 @@ template <int D, int CODE, int MODE> __global__ void __launch_bounds__(1024) flb
     kv8_begin();
     const int kv = (int)(blockIdx.x & 1u), h = (int)(blockIdx.x >> 1), j = (int)blockIdx.y, b = (int)blockIdx.z;
 
-    const int past = a.past_lens ? __ldg(a.past_lens + b) : a.start_pos;
-    const int n = a.new_lens ? __ldg(a.new_lens + b) : a.S;
+    const int past = a.past_lens ? a.past_lens[b] : a.start_pos;
+    const int n = a.new_lens ? a.new_lens[b] : a.S;
     if (past < 0 || n < 0 || n > a.S || past > min(a.c.T - n, a.max_past)) { // nothing of this sequence is touched
         if (threadIdx.x == 0 && a.status) atomicOr(a.status, kKv8BadLen);
         return;
@@ -36,7 +36,7 @@ template <int D, int CODE, int MODE> __global__ void __launch_bounds__(1024) flb
     const size_t unit = (size_t)b * a.c.H + h;
     uint8_t *codes = a.c.codes[kv] + (unit * a.c.T + row0) * D;
     float *scale_p = a.c.scale[kv] + unit * a.c.nblk + blk;
-    const long long pos_lo = (a.token_pos ? __ldg(a.token_pos + b) : past) + (long long)(lo - past); // position of row lo: any int, and the tokens behind it further
+    const long long pos_lo = (a.token_pos ? a.token_pos[b] : past) + (long long)(lo - past); // position of row lo: any int, and the tokens behind it further
 
     const int col = (int)(threadIdx.x % CPR) * 8, step = (int)(blockDim.x / CPR), r0 = row0 + (int)(threadIdx.x / CPR); // rows r0, r0 + step, ...
     // All loads first: the rows, then the table's.  What is not a new row of this block is read as the nearest that is, and not used.  FULL: every
@@ -56,8 +56,8 @@ template <int D, int CODE, int MODE> __global__ void __launch_bounds__(1024) flb
             raw[i] = kv8_raw8<MODE>(a.in[kv], tok0 + (row - lo), h * D + col);
             if (turn) {
                 const float4 *f = reinterpret_cast<const float4 *>(a.freq_cis + (size_t)min(max(tab_lo + (row - lo), 0), tab1) * D + col);
-                f0[i] = __ldg(f);
-                f1[i] = __ldg(f + 1);
+                f0[i] = f[0];
+                f1[i] = f[1];
             }
         }
         const float old = (FULL || row0 >= past) ? 0.f : *scale_p;

@@ -186,8 +186,8 @@ __global__ void __launch_bounds__(kWarps * 32, D == 128 ? (NT == 1 ? 4 : 3) : 1)
     const int head0 = h * a.G + chunk * HEADS, nheads = min(HEADS, a.G - chunk * HEADS);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
 
-    const int past = a.past_lens ? __ldg(a.past_lens + b) : a.start_pos;
-    const int pos = a.token_pos ? __ldg(a.token_pos + b) : past;
+    const int past = a.past_lens ? a.past_lens[b] : a.start_pos;
+    const int pos = a.token_pos ? a.token_pos[b] : past;
     float qx[QH][8];
     static_assert(D <= 256, "a warp holds a row, eight dims to a lane");
 #pragma unroll
@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(kWarps * 32, D == 128 ? (NT == 1 ? 4 : 3) : 1)
     const int row0 = split * a.split_len, row1 = min(row0 + a.split_len, past + 1);
     const bool is_last = split == nsplit - 1;
     const int prow = a.freq_cis ? kv8_table_row(pos, a.freq_rows, a.status) : 0;
-    const int begin = (FORM && a.key_begin) ? __ldg(a.key_begin + b) : INT_MIN;
+    const int begin = (FORM && a.key_begin) ? a.key_begin[b] : INT_MIN;
 
     // ---- the warp's steps: rows r, r + 64, ...
     using R = Ring<D>;
@@ -356,7 +356,7 @@ __global__ void __launch_bounds__(kWarps * 32, D == 128 ? (NT == 1 ? 4 : 3) : 1)
         qu[n] = q_unit[4 * n + t];
         m_run[n] = kNoMax;
         l_run[n] = 0.f;
-        slope[n] = (FORM && a.slopes && 4 * n + t < nheads) ? __ldg(a.slopes + head0 + 4 * n + t) * kLog2e : 0.f;
+        slope[n] = (FORM && a.slopes && 4 * n + t < nheads) ? a.slopes[head0 + 4 * n + t] * kLog2e : 0.f;
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -667,14 +667,14 @@ __global__ void __launch_bounds__(256) flb_kv8_weights_kernel(const __grid_const
     const int r = ((int)(blockIdx.x % (unsigned)blocks_per_unit) * 256 + threadIdx.x) * 4;
     const int b = (int)(unit / a.c.H), h = (int)(unit - (size_t)b * a.c.H);
     // The kernel in front is the attention kernel, which lets this one start only after everything before it has completed, and writes neither
-    // lengths nor weights: they are read while it runs.
-    const int past = a.past_lens ? __ldg(a.past_lens + b) : a.start_pos;
+    // lengths nor weights: they are read while it runs (from L2: this SM's L1 may be older than what came before).
+    const int past = a.past_lens ? __ldcg(a.past_lens + b) : a.start_pos;
     const bool on = past >= 0 && past <= a.max_past && r <= past;
     const size_t i = unit * a.c.T + r; // T is a multiple of 16: four rows never leave the slab
-    const int begin = a.key_begin && !a.c.row_pos ? __ldg(a.key_begin + b) : INT_MIN; // no score was left below it
+    const int begin = a.key_begin && !a.c.row_pos ? __ldcg(a.key_begin + b) : INT_MIN; // no score was left below it
     float w[4] = {0.f, 0.f, 0.f, 0.f};
     if (on) {
-        const float4 in = *reinterpret_cast<const float4 *>(a.weight_in + i);
+        const float4 in = __ldcg(reinterpret_cast<const float4 *>(a.weight_in + i));
         w[0] = in.x;
         w[1] = in.y;
         w[2] = in.z;

@@ -225,3 +225,12 @@ def test_words_at_odd_addresses_are_refused():
     c = _cache()
     k = torch.zeros(2, 1, 4, 128, dtype=torch.float16)
     assert kv8.validate(kv8.append_params(c, k, k.clone(), scratch=torch.zeros(9, dtype=torch.uint8)[1:])) == _lib.FLB_ERR_MISALIGNED
+
+
+def test_kernels_of_the_cache_use_no_read_only_loads():
+    """They are resident while the kernel in front still writes what they read."""
+    src = os.path.join(ROOT, "fasterllama_b200", "csrc")
+    for name in sorted(os.listdir(src)):
+        if name.startswith("kv8"):
+            text = open(os.path.join(src, name)).read()
+            assert "__ldg(" not in text and "global.nc" not in text and "__restrict__" not in text, name
