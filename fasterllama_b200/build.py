@@ -50,14 +50,18 @@ def build_cuda(force: bool = False, verbose: bool = False) -> str:
     return LIB_PATH
 
 
-def build_tensor_args(force: bool = False) -> str:
-    """The binding's tensor checks and parameter blocks (csrc/tensor_args.cpp), a Python extension module against this interpreter and torch."""
+def build_tensor_args(force: bool = False) -> str | None:
+    """The binding's tensor checks and parameter blocks (csrc/tensor_args.cpp), a Python extension module against this interpreter and torch.  Without
+    torch there is nothing to bind: None."""
+    try:
+        import torch
+    except ImportError:
+        print("torch is not installed: the Python binding's module is left out", file=sys.stderr)
+        return None
     src = os.path.join(CSRC, "tensor_args.cpp")
     if not force and _newer(ARGS_PATH, [src, *(os.path.join(ROOT, "include", f) for f in ("flb_attn.h", "flb_kv8.h"))]):
         return ARGS_PATH
     import sysconfig
-
-    import torch
 
     root = os.path.dirname(torch.__file__)
     inc = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include")]
@@ -123,10 +127,10 @@ def build_e2e_variants(force: bool = False) -> list[str]:
 
 def build_all(force: bool = False, verbose: bool = False) -> None:
     build_cuda(force, verbose)
-    build_tensor_args(force)
     build_oracle(force)
     build_reference(force)
     build_e2e_variants(force)
+    build_tensor_args(force)  # last: the others need no torch
 
 
 if __name__ == "__main__":
