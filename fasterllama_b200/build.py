@@ -7,12 +7,14 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG_DIR)
 CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_PATH = os.path.join(PKG_DIR, "libflb_attn.so")
-ARGS_PATH = os.path.join(PKG_DIR, "_tensor_args.so")
+ARGS_PATH = os.path.join(PKG_DIR, "_tensor_args" + sysconfig.get_config_var("EXT_SUFFIX"))  # this interpreter's
+ARGS_STAMP = os.path.join(PKG_DIR, "_tensor_args.built_for")  # the torch it was built against
 ORACLE_DIR = os.path.join(ROOT, "oracle")
 ORACLE_LIB = os.path.join(ORACLE_DIR, "libflb_oracle.so")
 
@@ -51,24 +53,28 @@ def build_cuda(force: bool = False, verbose: bool = False) -> str:
 
 
 def build_tensor_args(force: bool = False) -> str | None:
-    """The binding's tensor checks and parameter blocks (csrc/tensor_args.cpp), a Python extension module against this interpreter and torch.  Without
-    torch there is nothing to bind: None."""
+    """The binding's tensor checks and parameter blocks (csrc/tensor_args.cpp), a Python extension module against this interpreter and torch, whose
+    version it checks when it is imported.  Without torch there is nothing to bind: None."""
     try:
         import torch
     except ImportError:
         print("torch is not installed: the Python binding's module is left out", file=sys.stderr)
         return None
     src = os.path.join(CSRC, "tensor_args.cpp")
-    if not force and _newer(ARGS_PATH, [src, *(os.path.join(ROOT, "include", f) for f in ("flb_attn.h", "flb_kv8.h"))]):
+    built_for = open(ARGS_STAMP).read() if os.path.exists(ARGS_STAMP) else None
+    if not force and built_for == str(torch.__version__) and _newer(ARGS_PATH, [src, *(os.path.join(ROOT, "include", f) for f in ("flb_attn.h", "flb_kv8.h"))]):
         return ARGS_PATH
-    import sysconfig
-
     root = os.path.dirname(torch.__file__)
     inc = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include")]
     cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           *(a for p in inc for a in ("-isystem", p)), "-I" + sysconfig.get_paths()["include"], src, "-o", ARGS_PATH,
+           f'-DFLB_BUILT_FOR_TORCH="{torch.__version__}"', *(a for p in inc for a in ("-isystem", p)), "-I" + sysconfig.get_paths()["include"], src, "-o", ARGS_PATH,
            "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10"]
     subprocess.run(cmd, check=True)
+    untagged = os.path.join(PKG_DIR, "_tensor_args.so")  # its name before it carried the interpreter's
+    if os.path.exists(untagged):
+        os.remove(untagged)
+    with open(ARGS_STAMP, "w") as f:
+        f.write(torch.__version__)
     return ARGS_PATH
 
 

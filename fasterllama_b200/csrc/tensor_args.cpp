@@ -361,4 +361,14 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensor_args", nullptr, -1, method
 
 } // namespace
 
-PyMODINIT_FUNC PyInit__tensor_args(void) { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__tensor_args(void) {
+    // what a tensor looks like in memory is torch's own affair, of one version
+    PyObject *torch = PyImport_ImportModule("torch"), *version = torch ? PyObject_GetAttrString(torch, "__version__") : nullptr, *text = version ? PyObject_Str(version) : nullptr;
+    const char *is = text ? PyUnicode_AsUTF8(text) : nullptr;
+    const bool same = is && !strcmp(is, FLB_BUILT_FOR_TORCH);
+    if (is && !same) PyErr_Format(PyExc_ImportError, "_tensor_args was built for torch " FLB_BUILT_FOR_TORCH ", this is %s: run python -m fasterllama_b200.build", is);
+    Py_XDECREF(text);
+    Py_XDECREF(version);
+    Py_XDECREF(torch);
+    return same ? PyModule_Create(&module) : nullptr;
+}
