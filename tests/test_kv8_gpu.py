@@ -817,3 +817,21 @@ def test_decode_distances_beyond_31_bits(cuda_device):
         kv8.decode(c, zero, zero, one, o, start_pos=1, token_pos=i32([token]), alibi_slopes=torch.full((1,), 2.0 ** -32, device=DEV), scratch=s)
         want = 1.0 / (1.0 + math.exp(-abs(token - row) * 2.0 ** -32))
         assert float((o - want).abs().max()) <= 2.0 ** -20  # v = 1 is coded as 127 * fp32(1 / 127); exponent and quotient a few roundings of 2^-23
+
+
+# ------------------------------------------------------------------------------------------------ joins of many splits
+@pytest.mark.parametrize("past", [[8191], [8192], [20000, 8200]])
+@pytest.mark.parametrize("dtype,d,G", [(I8, 64, 1), (E4, 64, 3), (I8, 128, 8), (E4, 128, 1), (I8, 256, 4), (I8, 128, 9)])
+@pytest.mark.parametrize("weights", [None, "apart"])
+def test_decode_joins_more_than_64_splits(cuda_device, past, dtype, d, G, weights):
+    """64, 65 and 157 splits of 128 rows: the join's weights are worked out 64 splits at a time; with few heads its threads share a column's splits, with many they take
+    several columns each."""
+    run_decode(21 + G + d, B=len(past), Hq=G, Hkv=1, T=20096, d=d, block=32, dtype=dtype, past=past, split=128, weights=weights, cap=30.0 if G == 8 else 0.0)
+
+
+def test_decode_of_many_splits_is_repeatable(cuda_device):
+    c, (q, k, v, o), args = run_decode(22, B=1, Hq=16, Hkv=2, T=20096, d=128, block=64, dtype=I8, past=[20000], split=128)
+    for _ in range(5):
+        again = torch.empty_like(o)
+        kv8.decode(c, q, k, v, again, **args)
+        assert torch.equal(o, again)
