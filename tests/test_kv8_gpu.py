@@ -835,3 +835,74 @@ def test_decode_of_many_splits_is_repeatable(cuda_device):
         again = torch.empty_like(o)
         kv8.decode(c, q, k, v, again, **args)
         assert torch.equal(o, again)
+
+
+# ------------------------------------------------------------------------------------------------ captures with several branches
+def test_captured_calls_wait_for_every_branch(cuda_device):
+    """Inputs and lengths are made on two other streams, by kernels of this family and by others, and the results are used on a third: as graph nodes
+    the calls have several predecessors and successors."""
+    g = gen(95)
+    B, Hq, Hkv, T, d, block, S = 2, 8, 2, 4096, 128, 32, 1500
+    raw = [tokens(g, "float16", B, n, h, d)[0] for n, h in ((S, Hkv), (S, Hkv), (1, Hq), (1, Hkv), (1, Hkv))]
+    tab = table(T, d)
+    c, other = (kv8.empty_cache(B, Hkv, T, d, block_len=block, row_pos=True, device=DEV) for _ in range(2))
+    src = [torch.empty_like(t) for t in raw]
+    ins = [torch.empty_like(t) for t in raw]
+    past, nxt, w = i32([0] * B), i32([S + 1] * B), torch.zeros(B, Hkv, T, device=DEV)
+    out, twice = torch.empty(B, Hq, 1, d, device=DEV), torch.empty(B, Hq, 1, d, device=DEV)
+    ds, es = (torch.zeros(n, dtype=torch.uint8, device=DEV) for n in (kv8.decode_workspace_bytes(B, Hq, Hkv, T, d, block_len=block, weights=True),
+                                                                      kv8.evict_workspace_bytes(B, Hkv, T, d, block_len=block)))
+    left, right = torch.cuda.Stream(), torch.cuda.Stream()
+
+    def run():
+        main = torch.cuda.current_stream()
+        past.zero_()
+        w.zero_()
+        left.wait_stream(main)
+        right.wait_stream(main)
+        with torch.cuda.stream(left):  # k, q: other kernels, with some work in front of them
+            for _ in range(8):
+                ins[0].copy_(src[0])
+                ins[2].copy_(src[2])
+                ins[3].copy_(src[3])
+        with torch.cuda.stream(right):  # v: behind a call of this family on another cache
+            for _ in range(8):
+                ins[1].copy_(src[1])
+                ins[4].copy_(src[4])
+            kv8.append(other, ins[1], ins[1])
+        main.wait_stream(left)
+        main.wait_stream(right)
+        kv8.append(c, ins[0], ins[1], past_lens=past, freq_cis=tab)
+        right.wait_stream(main)
+        with torch.cuda.stream(right):
+            past.add_(S)
+        main.wait_stream(right)
+        kv8.decode(c, ins[2], ins[3], ins[4], out, past_lens=past, freq_cis=tab, weight_in=w, weight_out=w, scratch=ds)
+        past.add_(1)
+        left.wait_stream(main)
+        with torch.cuda.stream(left):
+            torch.mul(out, 2, out=twice)
+        kv8.evict(c, past_lens=past, len_out=past, budget=1000, recent=16, sinks=4, next_pos=nxt, weight=w, scratch=es)
+        main.wait_stream(left)
+
+    def result():
+        torch.cuda.synchronize()
+        return [t.clone() for t in (out, twice, past, w[..., :1000], c.k.view(I8)[:, :, :1000], c.v.view(I8)[:, :, :1000], c.row_pos[:, :, :1000], other.v.view(I8))]
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for turn in range(4):
+        for t, r in zip(src, raw):
+            t.copy_(r * (1 + 0.25 * turn))
+        torch.cuda.synchronize()
+        run()
+        want = result()
+        for t in (*ins, out, twice):
+            t.fill_(7)
+        for x in (c.k, c.v, c.k_scale, c.v_scale, c.row_pos):
+            x.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(want, result())), turn
+    assert torch.equal(out * 2, twice)
