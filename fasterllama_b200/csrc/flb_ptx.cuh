@@ -84,7 +84,8 @@ __device__ __forceinline__ float ex2_fma(float x) {
     p = fmaf(p, f, 1.0f);
     return __int_as_float(__float_as_int(p) + (__float_as_int(t) << 23));
 }
-// cap * tanh(x / cap), in any unit; inv_cap = 1 / cap.  Up to |u| = 1 tanh(u) / u is a polynomial in u^2 (own minimax fit, 2e-8 of tanh), beyond
+// cap * tanh(x / cap), in any unit; inv_cap = 1 / cap.  Up to |u| = 1 tanh(u) / u is a polynomial in u^2 (own minimax fit, within 3.5e-8 and
+// 3.0e-7 of itself), beyond
 // tanh |u| = 1 - 2 / (1 + e^2|u|), where the difference cancels nothing: within 2^-22 of the cap everywhere.
 __device__ __forceinline__ float cap_score(float x, float cap, float inv_cap) {
     const float u = x * inv_cap;

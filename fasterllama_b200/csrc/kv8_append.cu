@@ -1,7 +1,7 @@
 // kv8_append.cu — fresh K/V rows into the 8-bit cache: dequantise, rotate (RoPE), one scale per block of rows and head.
 //
 // A streaming pass: a token row and head costs 2 d (e_in + 1) bytes.  Bound by instruction issue, about 100 per eight values at 2.6 a clock (8 x 32 heads of
-// 0-1024 fp16 tokens to int8: 32 us, 3.6 TB/s, 0.55 of the copy bandwidth).  One CTA takes one block of rows of one head, K or V:
+// 0-1024 fp16 tokens to int8: 33-36 us by the lengths drawn, 3.2-3.5 TB/s, 0.50-0.54 of the copy bandwidth).  One CTA takes one block of rows of one head, K or V:
 // block_len * d values, 32 per thread held in registers between the two halves of the work (largest magnitude, then
 // codes), so every value is read once.  Blocks of the K/V heads of the same tokens are neighbours in the grid: together
 // they read whole rows of the [B,S,Hkv,d] input.
@@ -14,7 +14,7 @@ namespace flb {
 
 namespace {
 
-constexpr int kChunks = 4; // 8-value chunks per thread (the call above: 2: 40.0 us, 4: 32.0, 8: 39.0)
+constexpr int kChunks = 4; // 8-value chunks per thread (the call above, same lengths: 2: 40.0 us, 4: 32.0, 8: 39.0)
 
 template <int D, int CODE, int MODE> __global__ void __launch_bounds__(1024) flb_kv8_append_kernel(const __grid_constant__ Kv8AppendArgs a) {
     constexpr int CPR = D / 8; // chunks per row

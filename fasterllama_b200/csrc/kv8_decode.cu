@@ -1,8 +1,8 @@
 // kv8_decode.cu — single-token attention over the 8-bit cache, the new token's append included.
 //
 // For one K/V head and its G q heads:  x_r = c q.(code_r scale_r),  out = sum_r p_r code_r scale_r / sum_r p_r.
-// HBM-bound: 2 d bytes per cached row and K/V head, read once for all G heads.  16 x 32 heads of 1024-2047 rows: 41 us, 4.9 TB/s; batches of 16, 32, 48 take
-// 9.5 us (launch, ramp, drain, joining) + bytes / 6.3 TB/s.
+// HBM-bound: 2 d bytes per cached row and K/V head, read once for all G heads.  16 x 32 heads of 1024-2047 rows: 43-45 us, 4.5-4.8 TB/s (41-42
+// us from a replayed graph); batches of 16, 32, 48 x 1535 rows take 40, 68, 98 us: 11 us (launch, ramp, drain, joining) + bytes / 7.0 TB/s.
 //   * grid = K/V heads x splits of `split_len` rows; four warps per CTA, warp w takes the 16-row steps w, w + 4, ... of its
 //     split.  Every warp copies its own steps (cp.async, 16 bytes a lane) into a ring of its own in shared memory, three and more
 //     steps ahead: 192 KB per SM under way, no barrier between warps.  The first copies leave before q is looked at.

@@ -73,8 +73,8 @@ __device__ __forceinline__ void all_sync(cg::cluster_group &cluster, int ranks) 
 }
 
 // A cluster of CTAs (one, for short slabs) per K/V head; every thread has `per` neighbouring rows.  ROWS: so many of them at most, whose keys stay in
-// registers over the passes; 0: any number, read again.  With 32 warps on an SM every instruction per row is eight clocks: code for 16 rows where 8 do
-// took 5000 clocks instead of 2100 to bring the keys into registers.
+// registers over the passes; 0: any number, read again.  With 32 warps on an SM every instruction per row is eight clocks, so code
+// for 16 rows does not serve where 8 do.
 template <int ROWS> __global__ void __launch_bounds__(kSelThreads) flb_kv8_select_kernel(const __grid_constant__ Kv8EvictArgs a) {
     constexpr bool REGS = ROWS > 0;
     constexpr int K = REGS ? ROWS : 4, V = K / 4;
@@ -202,8 +202,8 @@ template <int ROWS> __global__ void __launch_bounds__(kSelThreads) flb_kv8_selec
     auto to_all = [&](auto *p, auto value) { // into the same word of every CTA
         for (int c = 0; c < ranks; ++c) *(ranks == 1 ? p : cluster.map_shared_rank(p, c)) = value;
     };
-    // The leading digit at which the count from above reaches `want`.  Bins are summed over the cluster, by each CTA an eighth of them (every CTA all of them:
-    // 12000 clocks instead of 4000); four bins per thread in a CTA alone.
+    // The leading digit at which the count from above reaches `want`.  Bins are summed over the cluster, by each CTA an eighth of them; four bins per thread
+    // in a CTA alone.
     auto find = [&](int want) {
         if (ranks == 1) {
             const int top = kBins - 4 * (tid + 1);
@@ -368,8 +368,8 @@ template <int ROWS> __global__ void __launch_bounds__(kSelThreads) flb_kv8_selec
     int *hole_list = a.holes + unit * room, *move_list = a.moves + unit * room;
     const int in_block = (1 << a.c.block_shift) - 1;
     int e = (int)(before >> 32), kept = kept_of(before); // in front of the row
-    // The lists are gathered in shared memory, from where they leave in order (straight from the threads, 4 bytes here and there, they took 10000 clocks instead
-    // of 5000): rows of this CTA's stretch, holes from the front, sources up to the end.
+    // The lists are gathered in shared memory, from where they leave in order (not straight from the threads, 4 bytes
+    // here and there): rows of this CTA's stretch, holes from the front, sources up to the end.
     uint16_t *const list = reinterpret_cast<uint16_t *>(pool);
     constexpr int kList = ROWS * kSelThreads;
     const int c0 = rank * kSelThreads * per, c1 = min(n, c0 + kSelThreads * per); // the stretch
@@ -618,7 +618,10 @@ template <int D, int CODE> __global__ void __launch_bounds__(1024) flb_kv8_move_
 
 template <int D, int CODE> cudaError_t launch_t(const Kv8EvictArgs &a, cudaStream_t stream) {
     const unsigned units = (unsigned)a.c.B * (unsigned)a.c.H;
-    // One CTA per head up to 8192 rows, eight beyond (a portable cluster); up to 16 rows per thread keys stay in registers.
+    // One CTA per head up to 8192 rows, eight beyond (a portable cluster); up to 16 rows per thread keys stay in registers.  Measured (us, whole eviction to a
+    // quarter, replayed graph, one CTA against eight): 8 heads of 1024 rows 18.0 and 23.5, 2048 18.1 and 23.7, 4096 18.8 and 24.2, 8192 19.9 and 26.2, 16384 27.9 and 32.9
+    // (by a sixteenth: 28.1 and 26.3); 128 heads of 1024 rows 26 and 143, 8192 63 and 185, 16384 117 and 246.  Longer slabs would leave a CTA's threads more rows
+    // than registers.  (So a CTA alone would serve many heads of up to 16384 rows better; clusters are for few heads of long slabs.)
     const int ranks = a.c.T <= 8192 ? 1 : kRanks, per = rows_per_thread(a.c.T, ranks);
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

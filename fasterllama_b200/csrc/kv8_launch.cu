@@ -71,8 +71,8 @@ inline int window_blocks(const flb_kv8_cache &c, int S, bool any_past, int start
 
 // Rows of one split when the caller names none: a function of the slab's capacity alone, so results stay the same under any sharding of
 // the batch and the heads.  A CTA costs about 3 us besides its rows, of which four per SM overlap, and every split a partial result.  Measured
-// (us; 16 x 32 heads of 1024-2047 rows): 256 rows 51.6, 512 42.7, 1024 44.6, 2048 39.8; (1 x 32 heads, 1000 rows) 9.1, 10.5, 10.1; (1 x 8
-// heads of 4 q heads, 8000 rows) 11.2, 10.9, 13.5, 19.7; (the same, 100001 rows) 79, 57, 51, 46.
+// (us, replayed graph; 16 x 32 heads of 1024-2047 rows): 256 rows 48.2, 512 41.3, 1024 43.4, 2048 39.8; (1 x 32 heads, 1000 rows) 8.5, 9.5, 9.8; (1 x 8
+// heads of 4 q heads, 8000 rows) 9.9, 9.9, 13.8, 18.7; (the same, 100001 rows) 72, 55, 51, 42.
 inline int split_len_of(const flb_kv8_decode_params *p) {
     if (p->split_len > 0) return p->split_len;
     const int T = p->cache.total_len;

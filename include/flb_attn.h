@@ -238,9 +238,12 @@ typedef struct flb_peer_exchange {
  * then the mask of flb_attn_params is added.  A key is seen only if the mask mode lets it and key_begin <= key < key_end of its
  * query row: documents packed into one prompt (key_begin = first token of the row's document), windows
  * (key_begin = row - width + 1), a prefix that every row sees (mask mode NONE and key_end = max(row + 1, prefix)), prompts padded on the
- * right (key_end = 0 behind the prompt).  Bounds outside 0..S (a decode call: 0..past) act like the nearest one.  A row
- * that sees no key returns zeros.  Values of k and v have to be finite in all rows of a prefill call, unseen ones included (a
- * masked key has weight 0, and 0 times infinity is NaN); rows that a decode call does not see are not read into its result. */
+ * right (key_end = 0 behind the prompt).  Bounds outside 0..S (a decode call: 0..past + 1, where key_begin = past + 1 hides the
+ * new token too) act like the nearest one.  A row that sees no key returns zeros.  Values of k and v have to be finite in all rows of a prefill call, unseen ones included (a
+ * masked key has weight 0, and 0 times infinity is NaN); rows that a decode call does not see are not read into its result.
+ * Precision: a prefill call multiplies q, k, v and the weights as fp16, whatever the types of inputs, caches and out (as the plain call does: 4e-4
+ * to 6e-4 of the result against exact arithmetic), and its capped scores are off by up to 2.1e-5 of themselves, 1.2e-6 of the cap where they come near it.  A
+ * decode call computes in fp32; its capped scores are within 2^-22 of the cap. */
 typedef struct flb_score_form {
     int kv_head_num;           /* Hkv: k, v are [B,S,Hkv,d] and the caches [B,Hkv,T,d]; q head h reads K/V head
                                   h / (head_num / Hkv).  0 = head_num                              */

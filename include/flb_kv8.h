@@ -3,8 +3,8 @@
  * one scale per block of rows and K/V head, single-token attention reads the codes, and rows that drew little
  * attention are evicted.  It stands beside the fp32/fp16 cache of flb_attn.h and follows its manners: plain C, device
  * pointers, sizes as ints / size_t, the stream a cudaStream_t passed as void*; the library allocates nothing, never
- * synchronises, never exits and never throws; every entry point returns a flb_status.  The reference has no
- * counterpart (its cache is fp32, open_decoder.h:72-77).
+ * synchronises, never exits and never throws; every entry point returns a flb_status.  Calls that can run at the same
+ * time need scratch of their own.  The reference has no counterpart (its cache is fp32, open_decoder.h:72-77).
  */
 #ifndef FLB_KV8_H
 #define FLB_KV8_H
@@ -27,8 +27,8 @@ typedef enum flb_kv8_code {
  * How rows get in (append, decode and evict alike): per block and head, K and V apart, amax = the largest magnitude of
  * the rows that come in, need = amax / top (top = 127 for int8, 448 for e4m3), and
  *     scale' = need               for a block whose first row is new,
- *     scale' = max(scale, need)   for a block that holds rows already; if it grew, the codes it held become
- *                                 rne(code * (scale / scale')),
+ *     scale' = max(scale, need)   for a block that holds rows already (an eviction fills holes, so always this); if it grew,
+ *                                 the codes it held become rne(code * (scale / scale')),
  *     new code = rne(x / scale')  (0 where scale' is 0 or not finite; held to -top..top, which matters for subnormal scales),
  * each operation one IEEE fp32 operation, so two calls that store the same rows store the same bits.  A block
  * into which an infinity or NaN was stored has an infinite or NaN scale from then on: its rows read as NaN. */
@@ -47,7 +47,8 @@ typedef struct flb_kv8_cache {
                           Needed once rows have been evicted and a distance bias or key_begin is used */
 } flb_kv8_cache;
 
-/* Appends seq_len tokens (1 or more) behind the rows that are there. */
+/* Appends seq_len tokens (1 or more) behind the rows that are there.  Accumulated attention (weight_in, weight_out below) is the caller's: what stands in
+ * its buffer for the new rows, left from rows that an eviction dropped for instance, is to be zeroed before the next decode. */
 typedef struct flb_kv8_append_params {
     flb_kv8_cache cache;
     int seq_len;            /* S                                                        */
@@ -108,8 +109,9 @@ typedef struct flb_kv8_decode_params {
     size_t scratch_bytes;
     int scratch_zeroed;      /* promise: the first flb_kv8_counter_bytes() bytes are zero on entry.  They are left zero; a call of
                                 other sizes in between may write there */
-    int split_len;           /* rows of one split of a sequence, a multiple of 128 up to 2048; 0 = default.  Results
-                                depend on it and on each sequence alone, never on the batch or the grid */
+    int split_len;           /* rows of one split of a sequence, a multiple of 128 up to 2048; 0 = default, by total_len.  Results
+                                depend on it and on each sequence alone, never on the batch or the grid.  Where total_len is far
+                                above the lengths in use, name that of a slab of those (512 up to 8192 rows) */
 } flb_kv8_decode_params;
 
 /* Cuts every sequence down to `budget` rows per head.  Of the n cached rows, those at a position below `sinks` or at or
