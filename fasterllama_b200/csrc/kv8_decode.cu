@@ -688,6 +688,7 @@ __global__ void __launch_bounds__(256) flb_kv8_weights_kernel(const __grid_const
     const size_t hq0 = (size_t)b * a.Hq + h * a.G;
     const float *scores = a.scores + hq0 * a.c.T + r;
     const float2 *ml = reinterpret_cast<const float2 *>(a.ml) + hq0;
+    float sum[4] = {0.f, 0.f, 0.f, 0.f}; // over the group, apart from what has accumulated: that is rounded once per step and not once per head
     for (int j0 = 0; j0 < a.G; j0 += kHeadsAtOnce) {
         const int nj = min(kHeadsAtOnce, a.G - j0);
         // Maximum and reciprocal sum, read once per block: read by every thread, the few words they are in held the kernel up for 5 us.
@@ -707,10 +708,12 @@ __global__ void __launch_bounds__(256) flb_kv8_weights_kernel(const __grid_const
             const float s[4] = {s4[j].x, s4[j].y, s4[j].z, s4[j].w};
             const float2 m = ml_s[j];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) w[e] += m.y != 0.f && r + e >= begin ? ex2(s[e] - m.x) * m.y : 0.f;
+            for (int e = 0; e < 4; ++e) sum[e] += m.y != 0.f && r + e >= begin ? ex2(s[e] - m.x) * m.y : 0.f;
         }
     }
     if (!on) return;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] += sum[e];
     if (r + 3 <= past) {
         *reinterpret_cast<float4 *>(a.weight_out + i) = make_float4(w[0], w[1], w[2], w[3]);
     } else {

@@ -906,3 +906,25 @@ def test_captured_calls_wait_for_every_branch(cuda_device):
         graph.replay()
         assert all(torch.equal(a, b) for a, b in zip(want, result())), turn
     assert torch.equal(out * 2, twice)
+
+
+# ------------------------------------------------------------------------------------------------ accumulated weights
+@pytest.mark.parametrize("G", [1, 6, 8, 11])
+def test_accumulated_weights_are_rounded_once_per_step(cuda_device, G):
+    """Weights of 2^-11 or less join accumulated ones between 1/2 and 1: the group's sum is below 2^-7 and off by 2^-20 of itself at most, so the result is off
+    by its own rounding, 2^-25, and 2^-27."""
+    g = gen(96)
+    T, d, n = 4096, 64, 4095
+    c = used_cache(g, 1, 1, T, d, 64, I8)
+    q, _ = tokens(g, "float32", 1, 1, G, d, 0.01)
+    k, _ = tokens(g, "float32", 1, 1, 1, d)
+    w = torch.rand(1, 1, T, generator=g, device=DEV) * 0.49 + 0.5
+    w_out, o = torch.empty_like(w), torch.empty(1, G, 1, d, device=DEV)
+    s = torch.zeros(kv8.decode_workspace_bytes(1, G, 1, T, d, weights=True), dtype=torch.uint8, device=DEV)
+    kv8.decode(c, q, k, k, o, start_pos=n, weight_in=w, weight_out=w_out, scratch=s)
+    kd = R.dequant(c.k[0, 0], c.k_scale[0, 0], 64)
+    p = torch.softmax(q[0, 0].double() @ kd.T / math.sqrt(d), -1)
+    assert float(p.max()) < 2.0 ** -11
+    want = w[0, 0].double() + p.sum(0)
+    want[n] -= w[0, 0, n].double()
+    assert float((w_out[0, 0].double() - want).abs().max()) <= 2.0 ** -25 + 2.0 ** -27
