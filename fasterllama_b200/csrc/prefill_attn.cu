@@ -1312,7 +1312,7 @@ template <int D> int launch_prefill_hd(const flb_attn_params *p, const flb_score
     if (!cap_in_exp)
         for (int i = 0; i < 3; ++i) a.cap_c[i] = kTanhPoly[i] * a.cap_log2e;
     // A distance bias grows towards the diagonal: from the last tile to the first a row's maximum is found at once, the other way round it
-    // passes the rescaling threshold at nearly every tile (4001 tokens, 32 heads, on one box: 225 us forwards, 186 us backwards).
+    // passes the rescaling threshold at nearly every tile (4001 tokens, 32 heads, measured in turn: 225 us forwards, 186 us backwards).
     a.backwards = a.slopes != nullptr;
     // The larger the group, the closer the list is to heaviest-first over everything (measured at batch 8 x 32 heads x 1024
     // tokens: 142 us with groups of 32 units, 138 us with 64, 139 us with 128, 141 us with all 256 in one group; at
